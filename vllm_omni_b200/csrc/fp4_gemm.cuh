@@ -11,7 +11,8 @@
 // tensor memory (columns of their own per stage, free again when the stage is) and issues the MMAs that read them.
 //
 //   fp4_kernel<FMT, XR, GATED, PAIR>
-//     XR = 64, 128      single CTAs, two accumulators, so that the drain of a tile overlaps the next one's products
+//     XR = 16, 64       single CTAs, two per SM, two accumulators, so that the drain of a tile overlaps the next one's products
+//     XR = 128          the same, one per SM
 //     XR = 256, pairs   (cta_group::2) 256 x 256 tiles: each CTA brings 128 rows of W and half of the rows of X, and an MMA reads both: half the
 //                       L2 traffic per product, which is what bounds 4-bit tiles (128 x 128: 32 KB per 8.4 Mflop).
 //                       One accumulator: the scales take the rest of tensor memory; sixteen warps drain it into registers at once
@@ -19,12 +20,11 @@
 //     few tiles         a cluster of 2 to 8 CTAs shares a tile along K: partial sums meet in shared memory, added in the order of the ranks
 //
 // All waits are bounded (ptx_sm100.cuh).  No load is a multicast.
+#pragma once
 #include "host_util.h"
 #include "lowbit.cuh"
 
 namespace omni {
-
-typedef __nv_bfloat16 bf16;
 
 struct Fp4Args {
   CUtensorMap tmW, tmWS, tmX, tmXS;
@@ -47,31 +47,34 @@ struct Fp4Cfg {
   static constexpr int X_TILES = XR > 128 ? 2 : 1;                             // scale tiles of 128 rows of X: a pair's CTAs both hold them all
   static constexpr int W_BYTES = 128 * 128, X_BYTES = X_ROWS * 128, WS_BYTES = WORDS * 512, XS_BYTES = X_TILES * WORDS * 512;
   static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + WS_BYTES + XS_BYTES;
-  static constexpr int BOX = PAIR ? 32 : 64;                                   // rows of X per load
+  static constexpr int BOX = PAIR ? 32 : XR < 64 ? XR : 64;                    // rows of X per load
   static constexpr int ACCS = PAIR ? 1 : 2, SCALE_COLS = 4 * WORDS * (1 + X_TILES);
-  static constexpr int DRAIN_WARPS = PAIR ? 16 : 8, THREADS = 64 + 32 * DRAIN_WARPS;
+  static constexpr int CTAS = XR <= 64 ? 2 : 1;                                // per SM
+  static constexpr int PARTS = XR == 16 ? 1 : PAIR ? 4 : 2;                    // draining warps per quadrant of tensor memory
+  static constexpr int CHUNKS = XR / 16 / PARTS;                               // of 16 rows of X, per draining warp
+  static constexpr int DRAIN_WARPS = 4 * PARTS, THREADS = 64 + 32 * DRAIN_WARPS;
   static constexpr int TURN_BYTES = DRAIN_WARPS * 2048;                        // 16 x 32 fp32 per draining warp
-  static constexpr int BY_SMEM = (226 * 1024 - 1024 - TURN_BYTES) / ((STAGE_BYTES + 1023) / 1024 * 1024), BY_TMEM = (512 - ACCS * XR) / SCALE_COLS;
-  static constexpr int STAGES = BY_SMEM < BY_TMEM ? BY_SMEM : BY_TMEM;
   static constexpr int STAGE_PITCH = (STAGE_BYTES + 1023) / 1024 * 1024;       // codes begin on 1024 bytes (swizzle)
+  static constexpr int TMEM_COLS = 512 / CTAS;
+  static constexpr int BY_SMEM = (226 * 1024 / CTAS - 1024 - TURN_BYTES) / STAGE_PITCH, BY_TMEM = (TMEM_COLS - ACCS * XR) / SCALE_COLS;
+  static constexpr int STAGES = BY_SMEM < BY_TMEM ? BY_SMEM : BY_TMEM;
   static constexpr int SMEM_BYTES = STAGES * STAGE_PITCH + TURN_BYTES + 1024;
 };
 
 enum Fp4Act : int { FP4_NONE = 0, FP4_GELU_TANH = 1, FP4_SILU = 2 };
 
-__device__ __forceinline__ float silu_exact(float x) { return x / (1.0f + __expf(-x)); }
-__device__ __forceinline__ float fp4_act(float x, int act) {
-  if (act == FP4_GELU_TANH) {
-    const float u = 0.7978845608028654f * x * fmaf(0.044715f * x, x, 1.0f);
-    return x / (1.0f + __expf(-2.0f * u));                                     // 0.5 x (1 + tanh u)
-  }
-  return act == FP4_SILU ? silu_exact(x) : x;
+// x / (1 + e^-x); the quotient is good to 2 steps of fp32
+__device__ __forceinline__ float silu_of(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
+// 0.5 x (1 + tanh u) = x / (1 + e^-2u)
+__device__ __forceinline__ float gelu_of(float x) {
+  const float u = 0.7978845608028654f * x * fmaf(0.044715f * x, x, 1.0f);
+  return __fdividef(x, 1.0f + __expf(-2.0f * u));
 }
 
 // One result of row m of X: weight row n of the matrix (already times both factors).
 __device__ __forceinline__ float fp4_finish(const Fp4Args& a, float v, long m, int n) {
   if (a.bias) v += __bfloat162float(a.bias[n]);
-  v = fp4_act(v, a.act);
+  v = a.act == FP4_SILU ? silu_of(v) : a.act == FP4_GELU_TANH ? gelu_of(v) : v;
   if (a.gate) v *= __bfloat162float(a.gate[m / a.rows_per_gate * a.gate_stride + n]);
   if (a.residual) v += __bfloat162float(a.residual[m * a.ldr + n]);
   return v;
@@ -91,22 +94,34 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 
 // 16 rows of X by 32 rows of W, as a warp's accumulator lanes hold them (a lane per weight row), out to memory: turned in 2 KB of the
 // warp's own, so that a lane gets eight neighbouring outputs of a row and loads and stores go in 16 bytes.  m0: the first row of X, n0: the
-// warp's first weight row; rows: how many of the 16 there are; wf: the factor of this lane's weight row.
+// warp's first weight row; rows: how many of the 16 there are; wf: the factor of this lane's weight row, xf: of row lane % 16 of X.  The
+// factors were loaded before the tile was waited for, bias and residual are before the turn: a load where it is used costs its latency per
+// chunk (768 -> 2048 for 2463 tokens of 128 experts 103 us, FIXME).
 template <bool GATED>
-__device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v, float* turned, long m0, int rows, int n0, float wf, int lane) {
+__device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v, float* turned, long m0, int rows, int n0, float wf, float xf,
+                                          int lane) {
+  const int n = n0 + (lane & 3) * 8;
+  uint4 res[2], bias8;
+  if (!GATED && a.bias && a.by16 && n < a.N) bias8 = *reinterpret_cast<const uint4*>(a.bias + n);
+  if (!GATED && a.residual && a.by16) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = i * 8 + (lane >> 2);
+      if (r < rows && n < a.N) res[i] = *reinterpret_cast<const uint4*>(a.residual + (m0 + r) * a.ldr + n);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 16; ++i) turned[i * 32 + lane] = __uint_as_float(v[i]) * wf;
   __syncwarp();
   if (GATED) {
-    const int r = lane >> 1, g = (lane & 1) * 16, o = (n0 + g) / 2, cols = a.N / 2 - o;
-    if (r < rows && cols > 0) {
-      const long m = m0 + r;
-      const float f = a.xf ? a.xf[m] : 1.0f;
+    const int r = lane >> 1, g = (lane & 1) * 16, o = (n0 + g) / 2;
+    const float f = __shfl_sync(0xffffffffu, xf, r);
+    if (r < rows && o < a.N / 2) {
       const float* p = turned + r * 32 + g;
       float w[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = silu_exact(p[e] * f) * (p[8 + e] * f);
-      bf16* out = a.y + m * a.ldy + o;
+      for (int e = 0; e < 8; ++e) w[e] = silu_of(p[e] * f) * (p[8 + e] * f);
+      bf16* out = a.y + (m0 + r) * a.ldy + o;
       if (a.by16) *reinterpret_cast<uint4*>(out) = pack8(w);                   // N / 2 is a multiple of 8
       else
         for (int e = 0; e < 8; ++e) out[e] = __float2bfloat16(w[e]);
@@ -114,21 +129,25 @@ __device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v, f
   } else {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = i * 8 + (lane >> 2), n = n0 + (lane & 3) * 8;
+      const int r = i * 8 + (lane >> 2);
+      const float f = __shfl_sync(0xffffffffu, xf, r);
       if (r < rows && n < a.N) {
         const long m = m0 + r;
-        const float f = a.xf ? a.xf[m] : 1.0f;
         const float4* p = reinterpret_cast<const float4*>(turned + r * 32 + (lane & 3) * 8);
         const float4 lo = p[0], hi = p[1];
         float w[8] = {lo.x * f, lo.y * f, lo.z * f, lo.w * f, hi.x * f, hi.y * f, hi.z * f, hi.w * f};
         bf16* out = a.y + m * a.ldy + n;
         if (a.by16) {
-          if (a.bias) add8(w, *reinterpret_cast<const uint4*>(a.bias + n));
-          if (a.act != FP4_NONE)
+          if (a.bias) add8(w, bias8);
+          if (a.act == FP4_SILU) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = fp4_act(w[e], a.act);
+            for (int e = 0; e < 8; ++e) w[e] = silu_of(w[e]);
+          } else if (a.act == FP4_GELU_TANH) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = gelu_of(w[e]);
+          }
           if (a.gate) mul8(w, *reinterpret_cast<const uint4*>(a.gate + m / a.rows_per_gate * a.gate_stride + n));
-          if (a.residual) add8(w, *reinterpret_cast<const uint4*>(a.residual + m * a.ldr + n));
+          if (a.residual) add8(w, res[i]);
           *reinterpret_cast<uint4*>(out) = pack8(w);
         } else {
           for (int e = 0; e < 8 && n + e < a.N; ++e) out[e] = __float2bfloat16(fp4_finish(a, w[e], m, n + e));
@@ -139,10 +158,14 @@ __device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v, f
   __syncwarp();
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
+}
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* tmap, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
 }
 
 // a tile of rows: which expert, its first row in X and y, how many rows, and where its scales begin
@@ -168,7 +191,7 @@ __device__ __forceinline__ bool row_tile(const Fp4Args& a, int t, RowTile& r) {
 }
 
 template <int FMT, int XR, bool GATED, bool PAIR>
-__global__ void __launch_bounds__(Fp4Cfg<FMT, XR, PAIR>::THREADS, 1)
+__global__ void __launch_bounds__(Fp4Cfg<FMT, XR, PAIR>::THREADS, Fp4Cfg<FMT, XR, PAIR>::CTAS)
 fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
   using Cfg = Fp4Cfg<FMT, XR, PAIR>;
   constexpr int STAGES = Cfg::STAGES, ACCS = Cfg::ACCS, STEP = PAIR ? 32 : 16;         // steps of an MMA's N
@@ -208,10 +231,10 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
   }
   if (warp == 1) {
     if (PAIR) {
-      tmem_alloc_pair(smem_u32(&tmem_base_s), 512);
+      tmem_alloc_pair(smem_u32(&tmem_base_s), Cfg::TMEM_COLS);
       tmem_relinquish_pair();
     } else {
-      tmem_alloc(smem_u32(&tmem_base_s), 512);
+      tmem_alloc(smem_u32(&tmem_base_s), Cfg::TMEM_COLS);
       tmem_relinquish();
     }
   }
@@ -220,13 +243,17 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
   if (PAIR || a.split > 1) cluster_sync_all();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_base_s, tmem_scales = tmem_base + ACCS * XR;
-  pdl_begin();
-
   // item -> (block of weight rows, tile of rows).  One matrix: tiles of rows first, so that neighbours share the weights and all of X, which is small in 4
   // bits, stays in L2.  Experts: blocks of weight rows first; the tiles of an expert follow one another and share its weights.
   const bool experts = a.tile_expert != nullptr;
   auto tile_of = [&](int it) { return experts ? it / num_n : it % a.max_tiles; };
   auto block_of = [&](int it) { return (experts ? it % num_n : it / a.max_tiles) * (PAIR ? 2 : 1) + rank; };
+
+  // the first stages' weights into L2 while the kernel before (the rows' quantiser) runs out
+  if (!experts && warp == 0 && first < num_items && elect_one())
+    for (int kb = kb0; kb < kb1 && kb < kb0 + STAGES; ++kb) tma_prefetch_3d(&a.tmW, kb * 128, block_of(first) * 128, 0);
+  __syncwarp();
+  pdl_begin();
 
   if (warp == 0) {
     if (elect_one()) {
@@ -320,47 +347,51 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
     for (int it = first; it < num_items; it += step) {
       RowTile t;
       if (!row_tile<XR>(a, tile_of(it), t)) break;
-      const int n0 = block_of(it) * 128 + q * 32;
+      const int n0 = block_of(it) * 128 + q * 32, c0 = part * 16 * Cfg::CHUNKS;
       const float wf = a.wf && n0 + lane < a.N ? a.wf[(long)t.expert * a.N + n0 + lane] : 1.0f;
+      float xf[Cfg::CHUNKS];
+#pragma unroll
+      for (int i = 0; i < Cfg::CHUNKS; ++i) {
+        const int r = c0 + i * 16 + (lane & 15);
+        xf[i] = a.xf && r < t.rows ? a.xf[t.row0 + r] : 1.0f;
+      }
       mbar_wait(smem_u32(&tfull_bar[acc]), acc_phase, &s_abort, status, ERR_WAIT_TMEM_FULL);
       tc_fence_after_sync();
-      const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + acc * XR;
+      const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + acc * XR + c0;
       if (PAIR) {
         // 64 of the 256 rows per warp, into registers; then the accumulator is free
-        uint32_t v[4][16];
+        uint32_t v[Cfg::CHUNKS][16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld_32x16(at + part * 64 + i * 16, v[i]);
+        for (int i = 0; i < Cfg::CHUNKS; ++i) tmem_ld_32x16(at + i * 16, v[i]);
         tmem_wait_ld();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[acc]), 0));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = part * 64 + i * 16;
-          if (c < t.rows) fp4_store<GATED>(a, v[i], turned, t.row0 + c, t.rows - c, n0, wf, lane);
+        for (int i = 0; i < Cfg::CHUNKS; ++i) {
+          const int c = c0 + i * 16;
+          if (c < t.rows) fp4_store<GATED>(a, v[i], turned, t.row0 + c, t.rows - c, n0, wf, xf[i], lane);
         }
-      } else if (a.split == 1) {
-#pragma unroll 1
-        for (int c = part * 16; c < t.rows; c += 32) {
+      } else {
+        // split: this CTA's sums [row of X][128] to its ring, which nothing reads any more
+        float* sums = reinterpret_cast<float*>(smem) + q * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < Cfg::CHUNKS; ++i) {
+          const int c = c0 + i * 16;
+          if (c >= t.rows) break;
           uint32_t v[16];
-          tmem_ld_32x16(at + c, v);
+          tmem_ld_32x16(at + i * 16, v);
           tmem_wait_ld();
-          fp4_store<GATED>(a, v, turned, t.row0 + c, t.rows - c, n0, wf, lane);
+          if (a.split == 1) {
+            fp4_store<GATED>(a, v, turned, t.row0 + c, t.rows - c, n0, wf, xf[i], lane);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[(c + j) * 128] = __uint_as_float(v[j]) * wf;
+          }
         }
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
-      } else {
-        // this CTA's sums [row of X][128] to its ring, which nothing reads any more
-        float* sums = reinterpret_cast<float*>(smem) + q * 32 + lane;
-#pragma unroll 1
-        for (int c = part * 16; c < t.rows; c += 32) {
-          uint32_t v[16];
-          tmem_ld_32x16(at + c, v);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sums[(c + i) * 128] = __uint_as_float(v[i]) * wf;
-        }
       }
       if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
     }
@@ -371,22 +402,35 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
     cluster_sync_all();
     RowTile t;
     if (first < num_items && row_tile<XR>(a, tile_of(first), t)) {
-      // every CTA finishes 128 / split of the weight rows (at least 16: a gate group and its lift rows), all rows of X
-      const int width = 128 / a.split, base = share * width, n0 = block_of(first) * 128 + base, outs = GATED ? width / 2 : width;
-      auto sum = [&](int r, int n) {
-        float s = 0.f;
-        for (int c = 0; c < a.split; ++c) s += ld_cluster_f32(mapa_shared(smem_base + (r * 128 + base + n) * 4, c));
-        return s;
+      // every CTA finishes 128 / split of the weight rows (at least 16: a gate group and its lift rows), all rows of X, four at a time
+      const int width = 128 / a.split, base = share * width, n0 = block_of(first) * 128 + base, outs = GATED ? width / 2 : width, quads = outs / 4;
+      auto sum = [&](int r, int n, float (&s)[4]) {
+        float4 v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (c < a.split) v[c] = ld_cluster_f32x4(mapa_shared(smem_base + (r * 128 + base + n) * 4, c));
+        s[0] = v[0].x; s[1] = v[0].y; s[2] = v[0].z; s[3] = v[0].w;
+#pragma unroll
+        for (int c = 1; c < 8; ++c)
+          if (c < a.split) { s[0] += v[c].x; s[1] += v[c].y; s[2] += v[c].z; s[3] += v[c].w; }
       };
-      for (int i = threadIdx.x; i < t.rows * outs; i += blockDim.x) {
-        const int r = i / outs, o = i - r * outs;
+      for (int i = threadIdx.x; i < t.rows * quads; i += blockDim.x) {
+        const int r = i / quads, o = (i - r * quads) * 4;
         const long m = t.row0 + r;
         const float f = a.xf ? a.xf[m] : 1.0f;
+        float s0[4], s1[4];
         if (GATED) {
           const int n = o / 8 * 16 + o % 8;
-          if (n0 + n < a.N) a.y[m * a.ldy + n0 / 2 + o] = __float2bfloat16(silu_exact(sum(r, n) * f) * (sum(r, n + 8) * f));
-        } else if (n0 + o < a.N) {
-          a.y[m * a.ldy + n0 + o] = __float2bfloat16(fp4_finish(a, sum(r, o) * f, m, n0 + o));
+          sum(r, n, s0);
+          sum(r, n + 8, s1);
+          if (n0 + n < a.N)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a.y[m * a.ldy + n0 / 2 + o + e] = __float2bfloat16(silu_of(s0[e] * f) * (s1[e] * f));
+        } else {
+          sum(r, o, s0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n0 + o + e < a.N) a.y[m * a.ldy + n0 + o + e] = __float2bfloat16(fp4_finish(a, s0[e] * f, m, n0 + o + e));
         }
       }
     }
@@ -402,8 +446,8 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
   if (PAIR || a.split > 1) cluster_sync_all();   // nobody leaves while another may still signal it or read its sums
   if (warp == 1) {
     tc_fence_after_sync();
-    if (PAIR) tmem_dealloc_pair(tmem_base, 512);
-    else tmem_dealloc(tmem_base, 512);
+    if (PAIR) tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
+    else tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
   }
 }
 
@@ -433,6 +477,25 @@ struct Fp4Operands {
   long x_rows, xs_tiles;         // rows of X, its scale tiles of 128 rows
 };
 
+// How many pairs run at once: a persistent kernel of more would leave its last ones to a round of their own.
+static int resident_pairs(const void* kernel, int threads, int smem) {
+  static int cached = 0;
+  if (cached) return cached;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sm_count() & ~1);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+  (void)cudaGetLastError();
+  return cached = n <= 0 || n > sm_count() / 2 ? sm_count() / 2 : n;
+}
+
 template <int FMT, int XR, bool GATED, bool PAIR>
 static int launch_fp4(Fp4Args& a, const Fp4Operands& o, int* status, cudaStream_t stream) {
   using Cfg = Fp4Cfg<FMT, XR, PAIR>;
@@ -454,7 +517,7 @@ static int launch_fp4(Fp4Args& a, const Fp4Operands& o, int* status, cudaStream_
   auto* kernel = fp4_kernel<FMT, XR, GATED, PAIR>;
   if (int e = ensure_dynamic_smem((const void*)kernel, Cfg::SMEM_BYTES, prepared)) return e;
   const long items = (long)a.max_tiles * ((a.N + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128));
-  const int group = PAIR ? 2 : a.split, most = sm_count() / group;
+  const int group = PAIR ? 2 : a.split, most = PAIR ? resident_pairs((const void*)kernel, Cfg::THREADS, Cfg::SMEM_BYTES) : Cfg::CTAS * sm_count();
   const long run = a.split > 1 ? items : items < most ? items : most;
   if (run <= 0 || run * group > 0x7fffffffL) return RC_BAD_ARG;
   return launch_with(true, group, kernel, (unsigned)(run * group), Cfg::THREADS, Cfg::SMEM_BYTES, stream, a, status);
@@ -463,6 +526,7 @@ static int launch_fp4(Fp4Args& a, const Fp4Operands& o, int* status, cudaStream_
 template <int FMT, bool GATED>
 static int launch_rows_of(Fp4Args& a, const Fp4Operands& o, int tile, int* status, cudaStream_t s) {
   switch (tile) {
+    case 16: return launch_fp4<FMT, 16, GATED, false>(a, o, status, s);
     case 64: return launch_fp4<FMT, 64, GATED, false>(a, o, status, s);
     case 128: return launch_fp4<FMT, 128, GATED, false>(a, o, status, s);
     case 256: return launch_fp4<FMT, 256, GATED, true>(a, o, status, s);
@@ -476,55 +540,20 @@ static int launch_any(Fp4Args& a, const Fp4Operands& o, int fmt, bool gated, int
   return RC_BAD_ARG;
 }
 
-static bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Tile and split of a linear layer: the tile's rows, or a negative code.
+static int pick_tiles(Fp4Args& a, int force_tile, int force_split) {
+  const int tile = force_tile ? force_tile : a.M <= 16 ? 16 : a.M <= 64 ? 64 : a.M <= 128 ? 128 : 256;
+  if ((tile != 16 && tile != 64 && tile != 128 && tile != 256) || (tile <= 64 && a.M > tile)) return RC_BAD_ARG;
+  a.max_tiles = (int)(((long)a.M + tile - 1) / tile);
+  a.split = 1;
+  if (tile == 256) return force_split > 1 ? RC_BAD_ARG : tile;
+  const long items = (long)a.max_tiles * ((a.N + 127) / 128), slots = (tile <= 64 ? 2 : 1) * sm_count();
+  const int kb = (a.K + 255) / 256;
+  if (force_split) a.split = force_split;
+  else
+    while (a.split < 8 && items * a.split * 2 <= slots && kb >= a.split * 4) a.split *= 2;
+  if (a.split < 1 || a.split > 8 || (a.split & (a.split - 1)) || a.split > kb) return RC_BAD_ARG;
+  return tile;
+}
 
 }  // namespace omni
-
-using namespace omni;
-
-// y [M, N] (gated: [M, N / 2]) of x [M, K] and w [N, K]; force_tile 0: by the rule below, 64 / 128 / 256; force_split 0: by the rule, 1 / 2 / 4 / 8.
-extern "C" int omni_fp4_linear(const void* x, const void* xs, const float* xf, const void* w, const void* ws, const float* wf, void* y, long ldy, long M,
-                               int N, int K, int fmt, int gated, const void* bias, int act, const void* gate, long gate_stride, int rows_per_gate,
-                               const void* residual, long ldr, int force_tile, int force_split, int* status, void* stream) {
-  if (M <= 0 || N <= 0 || K <= 0) return RC_OK;
-  if (M > 0x7fffff00L || K % 32 || (gated && (N % 16 || bias || act || gate || residual)) || act < 0 || act > 2) return RC_BAD_ARG;
-  if (gate && rows_per_gate < 1) return RC_BAD_ARG;
-  Fp4Args a = {};
-  a.y = (bf16*)y; a.ldy = ldy; a.wf = wf; a.xf = xf;
-  a.bias = (const bf16*)bias; a.residual = (const bf16*)residual; a.gate = (const bf16*)gate;
-  a.ldr = ldr; a.gate_stride = gate_stride; a.rows_per_gate = rows_per_gate; a.act = act;
-  a.M = (int)M; a.N = N; a.K = K;
-  a.by16 = (gated ? N % 16 == 0 : N % 8 == 0) && ldy % 8 == 0 && ldr % 8 == 0 && gate_stride % 8 == 0 && on16(y) && on16(bias) && on16(gate) && on16(residual);
-  const Fp4Operands o = {w, ws, x, xs, 1, M, (M + 127) / 128};
-  int tile = force_tile ? force_tile : M <= 64 ? 64 : 128;
-  if (tile == 64 && M > 64) return RC_BAD_ARG;
-  a.max_tiles = (int)((M + tile - 1) / tile);
-  a.split = 1;
-  if (tile != 256) {
-    const long items = (long)a.max_tiles * ((N + 127) / 128);
-    const int kb = (K + 255) / 256;
-    if (force_split) a.split = force_split;
-    else
-      while (a.split < 8 && items * a.split * 2 <= sm_count() && kb >= a.split * 4) a.split *= 2;
-    if (a.split < 1 || a.split > 8 || (a.split & (a.split - 1)) || a.split > kb) return RC_BAD_ARG;
-  }
-  return launch_any(a, o, fmt, gated != 0, tile, status, (cudaStream_t)stream);
-}
-
-// Rows of all experts, by the tables of a plan (moe.cu): y[r] of x[r] for the rows of every tile; w [experts, N, K].  Scales of a tile's rows begin at row
-// t * (tile > 128 ? 256 : 128) of xs.  `rows`: rows of x; tile: the most rows a tile has, 64 / 128 / 256.
-extern "C" int omni_fp4_experts(const void* x, const void* xs, const float* xf, const void* w, const void* ws, const float* wf, int experts, void* y,
-                                long ldy, long rows, int N, int K, int fmt, int gated, const int* tile_expert, const int* tile_row0, const int* tile_rows,
-                                int max_tiles, int tile, int* status, void* stream) {
-  if (rows <= 0 || N <= 0 || K <= 0 || max_tiles <= 0) return RC_OK;
-  if (rows > 0x7fffff00L || K % 32 || (gated && N % 16) || experts < 1 || !tile_expert || !tile_row0 || !tile_rows) return RC_BAD_ARG;
-  Fp4Args a = {};
-  a.y = (bf16*)y; a.ldy = ldy; a.wf = wf; a.xf = xf;
-  a.M = (int)rows; a.N = N; a.K = K;
-  a.rows_per_gate = 1;
-  a.by16 = (gated ? N % 16 == 0 : N % 8 == 0) && ldy % 8 == 0 && on16(y);
-  a.tile_expert = tile_expert; a.tile_row0 = tile_row0; a.tile_rows = tile_rows; a.max_tiles = max_tiles;
-  a.split = 1;
-  const Fp4Operands o = {w, ws, x, xs, experts, rows, (long)max_tiles * (tile > 128 ? 2 : 1)};
-  return launch_any(a, o, fmt, gated != 0, tile, status, (cudaStream_t)stream);
-}

@@ -12,6 +12,10 @@
 
 namespace omni {
 
+typedef __nv_bfloat16 bf16;
+
+inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 enum LowFmt : int { FMT_MXFP4 = 0, FMT_NVFP4 = 1, FMT_FP8 = 2 };
 
 template <int FMT> struct LowCfg {

@@ -10,6 +10,7 @@ that runs on CPU tensors.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -43,41 +44,90 @@ class QuantRows:
     ``codes`` uint8 [.., R, K / 2] (fp8: [R, K]), element 2 i in the low half of byte i; ``scales`` as ``scale_shape`` says; ``row_scale`` fp32
     [.., R] for nvfp4.  ``gated``: the rows of a SwiGLU weight, 8 gate rows, their 8 lift rows, the next 8 gate rows and so on."""
 
-    __slots__ = ("codes", "scales", "row_scale", "fmt", "gated", "rows", "cols", "experts")
+    __slots__ = ("fmt", "gated", "rows", "cols", "experts", "index", "_codes", "_scales", "_row", "_buf", "_at")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, row_scale: torch.Tensor | None = None, gated: bool = False):
         if fmt not in FORMATS:
             raise ValueError(f"format {fmt!r}: one of {', '.join(FORMATS)}")
         if codes.dtype != torch.uint8 or codes.dim() not in (2, 3) or not codes.is_contiguous() or not scales.is_contiguous():
             raise ValueError("codes: contiguous uint8 [rows, cols] or [experts, rows, cols], scales contiguous")
-        rows, cols = codes.shape[-2], codes.shape[-1] * (1 if fmt == "fp8" else 2)
+        shape = tuple(codes.shape)
+        lead, rows, cols = shape[:-2], shape[-2], shape[-1] * (1 if fmt == "fp8" else 2)
         step = 128 if fmt == "fp8" else 32
         if cols % step or cols == 0:
             raise ValueError(f"{fmt}: columns ({cols}) must be a multiple of {step}")
-        lead = codes.shape[:-2]
         if fmt == "fp8" and lead:
             raise ValueError("fp8: rows of one matrix only")
-        want = lead + scale_shape(fmt, rows, cols)
-        if tuple(scales.shape) != want or scales.dtype != (torch.float32 if fmt == "fp8" else torch.uint8) or scales.device != codes.device:
-            raise ValueError(f"{fmt} scales of {tuple(codes.shape)} codes: {want} expected on {codes.device}, got {scales.dtype} {tuple(scales.shape)} on {scales.device}")
+        want, index = lead + scale_shape(fmt, rows, cols), codes.get_device()
+        if tuple(scales.shape) != want or scales.dtype != (torch.float32 if fmt == "fp8" else torch.uint8) or scales.get_device() != index:
+            raise ValueError(f"{fmt} scales of {shape} codes: {want} expected on {codes.device}, got {scales.dtype} {tuple(scales.shape)} on {scales.device}")
         if fmt == "nvfp4":
             if row_scale is None or row_scale.dtype != torch.float32 or tuple(row_scale.shape) != lead + (rows,) or not row_scale.is_contiguous() \
-                    or row_scale.device != codes.device:
+                    or row_scale.get_device() != index:
                 raise ValueError(f"nvfp4 needs fp32 row scales {lead + (rows,)} on {codes.device}")
         elif row_scale is not None:
             raise ValueError(f"{fmt} has no row scales")
         if gated and rows % 16:
             raise ValueError(f"gated weight: rows ({rows}) must be a multiple of 16")
-        self.codes, self.scales, self.row_scale, self.fmt, self.gated = codes, scales, row_scale, fmt, gated
-        self.rows, self.cols, self.experts = rows, cols, lead[0] if lead else None
+        if index >= 0 and (codes.data_ptr() % 16 or scales.data_ptr() % 16):
+            raise ValueError("codes and scales must begin on 16 bytes")
+        self._codes, self._scales, self._row, self._buf = codes, scales, row_scale, None
+        self._at = (codes.data_ptr(), scales.data_ptr(), None if row_scale is None else row_scale.data_ptr())
+        self.fmt, self.gated, self.rows, self.cols, self.experts, self.index = fmt, gated, rows, cols, lead[0] if lead else None, index
+
+    @classmethod
+    def _on_buffer(cls, buf: torch.Tensor, fmt: str, rows: int, cols: int, experts: int | None = None, gated: bool = False) -> "QuantRows":
+        """Rows that a kernel writes into one allocation (``_sizes``); the three tensors are made when somebody asks for them."""
+        q = cls.__new__(cls)
+        q._codes = q._scales = q._row = None
+        q._buf, q.fmt, q.gated, q.rows, q.cols, q.experts, q.index = buf, fmt, gated, rows, cols, experts, buf.get_device()
+        n, m, r = _sizes(fmt, rows, cols, experts or 1)
+        p = buf.data_ptr()
+        q._at = (p, p + n, p + n + m if r else None)
+        return q
+
+    def _part(self, which: int) -> torch.Tensor:
+        n, m, r = _sizes(self.fmt, self.rows, self.cols, self.experts or 1)
+        lead = () if self.experts is None else (self.experts,)
+        if which == 0:
+            shape = (*lead, self.rows, self.cols if self.fmt == "fp8" else self.cols // 2)
+            return self._buf[:math.prod(shape)].view(shape)
+        if which == 1:
+            shape = (*lead, *scale_shape(self.fmt, self.rows, self.cols))
+            size = math.prod(shape) * (4 if self.fmt == "fp8" else 1)
+            part = self._buf[n:n + size]
+            return (part.view(torch.float32) if self.fmt == "fp8" else part).view(shape)
+        return self._buf[n + m:n + m + 4 * self.rows * (self.experts or 1)].view(torch.float32).view(*lead, self.rows)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._part(0)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._part(1)
+        return self._scales
+
+    @property
+    def row_scale(self) -> torch.Tensor | None:
+        if self._row is None and self.fmt == "nvfp4":
+            self._row = self._part(2)
+        return self._row
 
     @property
     def shape(self) -> tuple[int, ...]:
-        return (*self.codes.shape[:-1], self.cols)
+        return (self.rows, self.cols) if self.experts is None else (self.experts, self.rows, self.cols)
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return (self._codes if self._buf is None else self._buf).device
+
+    @property
+    def is_cuda(self) -> bool:
+        return self.index >= 0
 
     @property
     def out_features(self) -> int:
@@ -90,28 +140,65 @@ class QuantRows:
         return f"QuantRows({self.fmt}, {list(self.shape)}{', gated' if self.gated else ''}, {self.device})"
 
 
-class _on:
-    """Makes a tensor's device the current one where it is not: kernels go to the current device's stream."""
+def _sizes(fmt: str, rows: int, cols: int, experts: int = 1) -> tuple[int, int, int]:
+    """Bytes of codes, scales and row factors in one allocation, each a multiple of 256."""
+    if fmt == "fp8":
+        n, m, r = rows * cols, rows * cols // 32, 0
+    else:
+        n, m, r = rows * cols // 2, -(-rows // 128) * scale_words(fmt, cols) * 512, 4 * rows if fmt == "nvfp4" else 0
+    return tuple(-(-experts * v // 256) * 256 for v in (n, m, r))
 
-    def __init__(self, t):
-        self.idx = t.device.index
+
+def _allocate(fmt: str, rows: int, cols: int, index: int, experts: int = 1) -> torch.Tensor:
+    return torch.empty(sum(_sizes(fmt, rows, cols, experts)), dtype=torch.uint8, device=_device(index))
+
+
+@functools.lru_cache(maxsize=None)
+def _device(index: int) -> torch.device:
+    return torch.device("cuda", index)
+
+
+class _on:
+    """Makes a device the current one where it is not: kernels go to the current device's stream."""
+
+    __slots__ = ("idx", "prev")
+
+    def __init__(self, index: int):
+        self.idx = index
 
     def __enter__(self):
         self.prev = torch._C._cuda_getDevice()
         if self.prev != self.idx:
             torch._C._cuda_setDevice(self.idx)
+        return torch._C._cuda_getCurrentRawStream(self.idx)
 
     def __exit__(self, *exc):
         if self.prev != self.idx:
             torch._C._cuda_setDevice(self.prev)
 
 
+_KINDS = {"p": ctypes.c_void_p, "l": ctypes.c_long, "i": ctypes.c_int, "f": ctypes.c_float}
+_ENTRIES = {"omni_lowbit_rows": "pllilipl" "pfplpl" "pppp", "omni_lowbit_dequantize": "ppplilii" "pp",
+            "omni_lowbit_linear": "plppp" "pppplliiii" "pipllpliipp", "omni_lowbit_experts": "plilii" "pppp" "pppp" "iipp"}
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    """An entry point that takes plain Python numbers: converting them by declared types is half the cost of wrapping each."""
+    lib = nv.lib("lowbit")
+    raw = getattr(lib._cdll, name)
+    raw.argtypes = [_KINDS[k] for k in _ENTRIES[name]]
+    return getattr(lib, name)
+
+
 def _rows16(t: torch.Tensor, name: str) -> torch.Tensor:
     """[rows, cols] bf16 whose rows begin on 16 bytes (a copy where they do not)."""
-    if t.dtype != torch.bfloat16:
+    if t.dtype is not torch.bfloat16:
         raise ValueError(f"{name}: bf16 expected, got {t.dtype}")
-    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    (rows, cols), (ld, one) = t.shape, t.stride()
+    if one != 1 or ld % 8 or t.data_ptr() % 16 or (rows > 1 and ld < cols):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
@@ -124,12 +211,6 @@ def _check_cols(fmt: str, cols: int) -> None:
     step = 128 if fmt == "fp8" else 32
     if cols % step or not 0 < cols <= MAX_COLS:
         raise ValueError(f"{fmt}: columns ({cols}) must be a multiple of {step} and at most {MAX_COLS}")
-
-
-def _empty(fmt: str, rows: int, cols: int, device, lead=()) -> tuple:
-    codes = torch.empty(*lead, rows, cols if fmt == "fp8" else cols // 2, dtype=torch.uint8, device=device)
-    scales = torch.empty(*lead, *scale_shape(fmt, rows, cols), dtype=torch.float32 if fmt == "fp8" else torch.uint8, device=device)
-    return codes, scales, torch.empty(*lead, rows, dtype=torch.float32, device=device) if fmt == "nvfp4" else None
 
 
 # ------------------------------------------------------------------ restatements in PyTorch
@@ -192,16 +273,18 @@ def _swiglu_torch(y):
 
 
 # ------------------------------------------------------------------ quantisation
-def _rows(x, fmt, *, residual=None, gain=None, eps=0.0, total=None, normed=None, group=0, lead=()):
+def _rows(x, fmt, *, residual=None, gain=None, eps=0.0, total=None, normed=None, experts=None, gated=False) -> QuantRows:
     rows, cols = x.shape
-    codes, scales, row = _empty(fmt, rows if not lead else rows // lead[0], cols, x.device, lead)
-    ld = lambda t: c_long(0 if t is None else t.stride(0))
-    with _on(x):
-        rc = nv.lib("lowbit").omni_lowbit_rows(
-            nv.ptr(x), ld(x), c_long(rows), c_int(cols), c_long(group or rows), c_int(FORMATS[fmt]), nv.ptr(residual), ld(residual), nv.ptr(gain),
-            c_float(eps), nv.ptr(total), ld(total), nv.ptr(normed), ld(normed), nv.ptr(codes), nv.ptr(scales), nv.ptr(row), nv.stream_ptr())
-    nv.check_rc(rc, "omni_lowbit_rows")
-    return codes, scales, row
+    per = rows // experts if experts else rows
+    q = QuantRows._on_buffer(_allocate(fmt, per, cols, x.get_device(), experts or 1), fmt, per, cols, experts, gated)
+    at = q._at
+    at_ld = lambda t: (None, 0) if t is None else (t.data_ptr(), t.stride(0))
+    with _on(q.index) as stream:
+        rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], *at_ld(residual), None if gain is None else gain.data_ptr(), eps,
+                                        *at_ld(total), *at_ld(normed), at[0], at[1], at[2], stream)
+    if rc:
+        nv.check_rc(rc, "omni_lowbit_rows")
+    return q
 
 
 def quantize(x: torch.Tensor, fmt: str) -> QuantRows:
@@ -212,8 +295,7 @@ def quantize(x: torch.Tensor, fmt: str) -> QuantRows:
     x2 = _rows16(x, "x")
     if not x.is_cuda:
         return _quantize_torch(x2, fmt)
-    codes, scales, row = _rows(x2, fmt)
-    return QuantRows(codes, scales, fmt, row)
+    return _rows(x2, fmt)
 
 
 def interleave_gated(w: torch.Tensor) -> torch.Tensor:
@@ -234,27 +316,26 @@ def pack_weight(w: torch.Tensor, fmt: str, gated: bool = False) -> QuantRows:
     _check_cols(fmt, w.shape[-1])
     if gated:
         w = interleave_gated(w)
-    lead = w.shape[:-2]
     if not w.is_cuda:
         if w.dtype != torch.bfloat16:
             raise ValueError(f"w: bf16 expected, got {w.dtype}")
         return _quantize_torch(w, fmt, gated)
-    codes, scales, row = _rows(_rows16(w, "w"), fmt, group=w.shape[-2], lead=tuple(lead))
-    return QuantRows(codes, scales, fmt, row, gated)
+    return _rows(_rows16(w, "w"), fmt, experts=w.shape[0] if w.dim() == 3 else None, gated=gated)
 
 
 def dequantize(q: QuantRows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of ``q`` as bf16 or fp32 (4-bit formats quantised here: exactly in either)."""
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"dequantize: bf16 or fp32, got {dtype}")
-    if not q.codes.is_cuda:
+    if not q.is_cuda:
         return _values_torch(q).to(dtype)
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
-    with _on(out):
-        rc = nv.lib("lowbit").omni_lowbit_dequantize(
-            nv.ptr(q.codes), nv.ptr(q.scales), nv.ptr(q.row_scale), c_long(q.rows * (q.experts or 1)), c_int(q.cols), c_long(q.rows),
-            c_int(FORMATS[q.fmt]), c_int(int(dtype == torch.float32)), nv.ptr(out), nv.stream_ptr())
-    nv.check_rc(rc, "omni_lowbit_dequantize")
+    out = torch.empty(q.shape, dtype=dtype, device=_device(q.index))
+    at = q._at
+    with _on(q.index) as stream:
+        rc = _entry("omni_lowbit_dequantize")(at[0], at[1], at[2], q.rows * (q.experts or 1), q.cols, q.rows, FORMATS[q.fmt], int(dtype is torch.float32),
+                                              out.data_ptr(), stream)
+    if rc:
+        nv.check_rc(rc, "omni_lowbit_dequantize")
     return out
 
 
@@ -293,14 +374,12 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, fmt: str, eps: floa
         return t2
 
     x2 = _rows16(x, "x")
-    codes, scales, row = _rows(x2, fmt, residual=None if residual is None else _rows16(residual, "residual"), gain=_aligned(weight), eps=eps,
-                               total=None if total is None else out_rows(total, "total"),
-                               normed=None if normed is None else out_rows(normed, "normed"))
-    return QuantRows(codes, scales, fmt, row)
+    return _rows(x2, fmt, residual=None if residual is None else _rows16(residual, "residual"), gain=_aligned(weight), eps=eps,
+                 total=None if total is None else out_rows(total, "total"), normed=None if normed is None else out_rows(normed, "normed"))
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
+    t = t if t.is_contiguous() else t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
 
@@ -320,20 +399,20 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
     if isinstance(x, QuantRows):
         if x.fmt != w.fmt or x.experts is not None or x.gated:
             raise ValueError(f"x is {x!r}, w {w!r}: rows of the same format expected")
-        lead, q = (x.rows,), x
+        lead, q, M, cols, index = (x.rows,), x, x.rows, x.cols, x.index
     else:
-        lead, q = tuple(x.shape[:-1]), None
-    cols = x.shape[-1]
-    if cols != w.cols or x.device != w.device:
+        lead, q, cols, index = x.shape[:-1], None, x.shape[-1], x.get_device()
+        M = lead[0] if len(lead) == 1 else math.prod(lead)
+    if cols != w.cols or index != w.index:
         raise ValueError(f"x {list(x.shape)} on {x.device} does not fit w {w!r}")
-    N, M = w.out_features, math.prod(lead)
+    N = w.out_features
     for name, t, shape in (("bias", bias, (w.rows,)), ("residual", residual, (*lead, N)), ("out", out, (*lead, N))):
-        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.bfloat16 or t.device != w.device):
-            raise ValueError(f"{name}: bf16 {shape} on {w.device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if t is not None and (t.shape != shape or t.dtype is not torch.bfloat16 or t.get_device() != index):
+            raise ValueError(f"{name}: bf16 {tuple(shape)} on {w.device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if gate is not None and (gate.dim() != 2 or gate.shape[1] != N or gate.shape[0] == 0 or M % gate.shape[0] or gate.stride(1) != 1
-                             or gate.dtype != torch.bfloat16 or gate.device != w.device):
+                             or gate.dtype is not torch.bfloat16 or gate.get_device() != index):
         raise ValueError(f"gate: bf16 [B, {N}] with B dividing {M} rows expected, got {gate.dtype} {tuple(gate.shape)}")
-    if not w.codes.is_cuda:
+    if index < 0:
         y = _values_torch(q if q is not None else quantize(x, w.fmt)) @ _values_torch(w).t()
         if w.gated:
             y = _swiglu_torch(y)
@@ -346,24 +425,39 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
             y = y + residual.reshape(M, N).float()
         y = y.to(torch.bfloat16).view(*lead, N)
         return y if out is None else out.copy_(y)
+    raw, ldx = None, 0
     if q is None:
-        q = quantize(x, w.fmt)
+        _check_cols(w.fmt, cols)
+        x = _rows16(x, "x")
+        raw, ldx = x.data_ptr(), x.stride(0)
+        q = QuantRows._on_buffer(_allocate(w.fmt, M, cols, index), w.fmt, M, cols)
     if out is None:
-        out = torch.empty(*lead, N, dtype=torch.bfloat16, device=w.device)
-    o2 = out.view(M, N)
-    r2 = None if residual is None else residual.reshape(M, N)
-    if (M > 1 or N > 1) and (o2.stride(1) != 1 or (r2 is not None and r2.stride(1) != 1)):
+        o2 = torch.empty(M, N, dtype=torch.bfloat16, device=_device(index))
+        out = o2 if len(lead) == 1 else o2.view(*lead, N)
+    else:
+        o2 = out if out.dim() == 2 else out.view(M, N)
+    r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(M, N)
+    if N > 1 and (o2.stride(1) != 1 or (r2 is not None and r2.stride(1) != 1)):
         raise ValueError("out and residual: the last dimension must be contiguous")
-    if bias is not None:
+    if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    with _on(out):
-        rc = nv.lib("gemm_fp4_sm100").omni_fp4_linear(
-            nv.ptr(q.codes), nv.ptr(q.scales), nv.ptr(q.row_scale), nv.ptr(w.codes), nv.ptr(w.scales), nv.ptr(w.row_scale), nv.ptr(o2),
-            c_long(o2.stride(0)), c_long(M), c_int(w.rows), c_int(cols), c_int(FORMATS[w.fmt]), c_int(int(w.gated)), nv.ptr(bias), c_int(ACT[act]),
-            nv.ptr(gate), c_long(0 if gate is None or gate.shape[0] == 1 else gate.stride(0)), c_int(0 if gate is None else max(1, M // gate.shape[0])),
-            nv.ptr(r2), c_long(0 if r2 is None else r2.stride(0)), c_int(force_tile), c_int(force_split), nv.ptr(nv.status_word(w.device)), nv.stream_ptr())
-    nv.check_rc(rc, "omni_fp4_linear")
+    B = 0 if gate is None else gate.shape[0]
+    (xc, xs, xf), (wc, ws, wf) = q._at, w._at
+    with _on(index) as stream:
+        rc = _entry("omni_lowbit_linear")(
+            raw, ldx, xc, xs, xf, wc, ws, wf, o2.data_ptr(), o2.stride(0), M, w.rows, cols, FORMATS[w.fmt], int(w.gated),
+            None if bias is None else bias.data_ptr(), ACT[act], None if gate is None else gate.data_ptr(), gate.stride(0) if B > 1 else 0,
+            max(1, M // B) if B else 0, None if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0), force_tile, force_split,
+            nv.status_word(o2.device).data_ptr(), stream)
+    if rc:
+        nv.check_rc(rc, "omni_lowbit_linear")
+    if raw is not None:
+        nv.count_launches(1)
     return out
+
+
+class _ExpertOperand(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("codes", "scales", "row_scale", "w", "ws", "wf")] + [("N", c_int), ("K", c_int)]
 
 
 def _tile_rows(pairs: int, experts: int) -> int:
@@ -413,40 +507,29 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
     x2, ids, weights = _rows16(x, "x"), ids.contiguous(), weights.contiguous()
     res = None if residual is None else _rows16(residual, "residual")
     o2 = out if out.stride(1) == 1 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0 else torch.empty_like(out, memory_format=torch.contiguous_format)
-    pairs = T * k
+    pairs, dev = T * k, x.device
     tile = _tile_rows(pairs, E)
-    max_tiles, pitch = min(E, pairs) + pairs // tile, 256 if tile > 128 else 128
-    dev = x.device
-    plan = torch.empty(pairs + 3 * max_tiles + 1, dtype=torch.int32, device=dev)
-    row_of_pair, te, tr, tn, n_rows = plan.split([pairs, max_tiles, max_tiles, max_tiles, 1])
-
-    def operand(cols):
-        codes = torch.empty(pairs, cols // 2, dtype=torch.uint8, device=dev)
-        scales = torch.empty(max_tiles * pitch // 128, scale_words(fmt, cols), 32, 4, 4, dtype=torch.uint8, device=dev)
-        return codes, scales, torch.empty(pairs, dtype=torch.float32, device=dev) if fmt == "nvfp4" else None
-
-    h = torch.empty(pairs, Fd, dtype=x.dtype, device=dev)
-    y = torch.empty(pairs, D, dtype=x.dtype, device=dev)
-    moe, low, g, fc = nv.lib("moe"), nv.lib("lowbit"), nv.lib("gemm_fp4_sm100"), c_int(FORMATS[fmt])
-    with _on(x):
-        st, status = nv.stream_ptr(), nv.ptr(nv.status_word(dev))
+    max_tiles = min(E, pairs) + pairs // tile
+    scale_rows = max_tiles * (256 if tile > 128 else 128)
+    # one workspace: the plan, both products' rows, what is between them, the experts' results
+    parts, at = [], 0
+    for size in (4 * pairs, 4 * max_tiles, 4 * max_tiles, 4 * max_tiles, 4, pairs * Fd * 2, pairs * D * 2,
+                 *(v for cols in (D, Fd) for v in (pairs * cols // 2, _sizes(fmt, scale_rows, cols)[1], 4 * pairs))):
+        parts.append(at)
+        at += -(-size // 256) * 256
+    work = torch.empty(at, dtype=torch.uint8, device=dev)
+    row_of_pair, te, tr, tn, n_rows, h, y, *ops = (work.data_ptr() + p for p in parts)
+    half = [_ExpertOperand(*ops[3 * i:3 * i + 2], ops[3 * i + 2] if fmt == "nvfp4" else None, *w._at, w.rows, w.cols) for i, w in enumerate((up, down))]
+    moe = nv.lib("moe")
+    p = ctypes.c_void_p
+    with _on(up.index) as stream:
+        status = nv.status_word(dev).data_ptr()
         if nv.bounds_check_enabled():
-            moe.omni_moe_set_bounds(c_long(pairs), status)
-        nv.check_rc(moe.omni_moe_plan_tiles(nv.ptr(ids), c_int(pairs), c_int(E), c_int(0), c_int(E), c_int(tile), c_int(max_tiles), nv.ptr(row_of_pair),
-                                            nv.ptr(te), nv.ptr(tr), nv.ptr(tn), nv.ptr(n_rows), st), "omni_moe_plan_tiles")
-
-        def product(src, per, pair_rows, w, dst):
-            (codes, scales, row) = op = operand(w.cols)
-            nv.check_rc(low.omni_lowbit_dispatch(nv.ptr(src), c_long(src.stride(0)), c_long(pairs), c_int(per), c_int(w.cols), fc, nv.ptr(pair_rows), nv.ptr(te),
-                                                 nv.ptr(tr), nv.ptr(tn), c_int(max_tiles), c_int(pitch), nv.ptr(codes), nv.ptr(scales), nv.ptr(row), st),
-                        "omni_lowbit_dispatch")
-            nv.check_rc(g.omni_fp4_experts(nv.ptr(codes), nv.ptr(scales), nv.ptr(row), nv.ptr(w.codes), nv.ptr(w.scales), nv.ptr(w.row_scale), c_int(E),
-                                           nv.ptr(dst), c_long(dst.stride(0)), c_long(pairs), c_int(w.rows), c_int(w.cols), fc, c_int(int(w.gated)),
-                                           nv.ptr(te), nv.ptr(tr), nv.ptr(tn), c_int(max_tiles), c_int(tile), status, st), "omni_fp4_experts")
-            return op
-
-        product(x2, k, row_of_pair, up, h)
-        product(h, 1, None, down, y)
-        nv.check_rc(moe.omni_moe_combine(nv.ptr(y), nv.ptr(row_of_pair), nv.ptr(weights), c_int(T), c_int(k), c_int(D), nv.ptr(res),
-                                         c_long(0 if res is None else res.stride(0)), nv.ptr(o2), c_long(o2.stride(0)), st), "omni_moe_combine")
+            moe.omni_moe_set_bounds(c_long(pairs), p(status))
+        nv.check_rc(moe.omni_moe_plan_tiles(p(ids.data_ptr()), c_int(pairs), c_int(E), c_int(0), c_int(E), c_int(tile), c_int(max_tiles), p(row_of_pair), p(te), p(tr),
+                                            p(tn), p(n_rows), p(stream)), "omni_moe_plan_tiles")
+        nv.check_rc(_entry("omni_lowbit_experts")(x2.data_ptr(), x2.stride(0), k, pairs, E, FORMATS[fmt], ctypes.addressof(half[0]), ctypes.addressof(half[1]), h, y,
+                                                  row_of_pair, te, tr, tn, max_tiles, tile, status, stream), "omni_lowbit_experts")
+        nv.check_rc(moe.omni_moe_combine(p(y), p(row_of_pair), p(weights.data_ptr()), c_int(T), c_int(k), c_int(D), p(0 if res is None else res.data_ptr()),
+                                         c_long(0 if res is None else res.stride(0)), p(o2.data_ptr()), c_long(o2.stride(0)), p(stream)), "omni_moe_combine")
     return out if o2 is out else out.copy_(o2)
