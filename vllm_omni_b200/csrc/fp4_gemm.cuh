@@ -10,7 +10,7 @@
 // elements of K (one 128-byte swizzle row of codes) of both operands and their scale tiles; the issuing thread copies the scales to
 // tensor memory (columns of their own per stage, free again when the stage is) and issues the MMAs that read them.
 //
-//   fp4_kernel<FMT, XR, GATED, PAIR>
+//   fp4_kernel<FMT, XR, EPI, PAIR>
 //     XR = 16, 64       single CTAs, two per SM, two accumulators, so that the drain of a tile overlaps the next one's products
 //     XR = 128          the same, one per SM
 //     XR = 256, pairs   (cta_group::2) 256 x 256 tiles: each CTA brings 128 rows of W and half of the rows of X, and an MMA reads both: half the
@@ -53,22 +53,29 @@ struct Fp4Cfg {
   static constexpr int PARTS = XR == 16 ? 1 : PAIR ? 4 : 2;                    // draining warps per quadrant of tensor memory
   static constexpr int CHUNKS = XR / 16 / PARTS;                               // of 16 rows of X, per draining warp
   static constexpr int DRAIN_WARPS = 4 * PARTS, THREADS = 64 + 32 * DRAIN_WARPS;
-  static constexpr int TURN_BYTES = DRAIN_WARPS * 2048;                        // 16 x 32 fp32 per draining warp
+  static constexpr int TURN_BYTES = DRAIN_WARPS * 1024;                        // 16 x 32 bf16 per draining warp
   static constexpr int STAGE_PITCH = (STAGE_BYTES + 1023) / 1024 * 1024;       // codes begin on 1024 bytes (swizzle)
   static constexpr int TMEM_COLS = 512 / CTAS;
-  static constexpr int BY_SMEM = (226 * 1024 / CTAS - 1024 - TURN_BYTES) / STAGE_PITCH, BY_TMEM = (TMEM_COLS - ACCS * XR) / SCALE_COLS;
+  // an SM has 228 KB, of which every CTA takes 1 KB, up to 1 KB to begin on 1024 bytes and its barriers
+  static constexpr int BY_SMEM = (228 * 1024 / CTAS - 2560 - TURN_BYTES) / STAGE_PITCH, BY_TMEM = (TMEM_COLS - ACCS * XR) / SCALE_COLS;
   static constexpr int STAGES = BY_SMEM < BY_TMEM ? BY_SMEM : BY_TMEM;
   static constexpr int SMEM_BYTES = STAGES * STAGE_PITCH + TURN_BYTES + 1024;
 };
 
 enum Fp4Act : int { FP4_NONE = 0, FP4_GELU_TANH = 1, FP4_SILU = 2 };
+enum Fp4Epilogue : int { EPI_PLAIN = 0, EPI_GATED = 1, EPI_ANY = 2 };         // the sums; silu(gate) * lift; bias, activation, gate and residual where given
 
-// x / (1 + e^-x); the quotient is good to 2 steps of fp32
-__device__ __forceinline__ float silu_of(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// x / (1 + e^-x), by a reciprocal good to a step of fp32
+__device__ __forceinline__ float silu_of(float x) { return x * rcp_approx(1.0f + __expf(-x)); }
 // 0.5 x (1 + tanh u) = x / (1 + e^-2u)
 __device__ __forceinline__ float gelu_of(float x) {
   const float u = 0.7978845608028654f * x * fmaf(0.044715f * x, x, 1.0f);
-  return __fdividef(x, 1.0f + __expf(-2.0f * u));
+  return x * rcp_approx(1.0f + __expf(-2.0f * u));
 }
 
 // One result of row m of X: weight row n of the matrix (already times both factors).
@@ -80,88 +87,153 @@ __device__ __forceinline__ float fp4_finish(const Fp4Args& a, float v, long m, i
   return v;
 }
 
-__device__ __forceinline__ void add8(float (&v)[8], const uint4& u) {
-  const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), d = unpack_bf16(u.w);
-  v[0] += a.x; v[1] += a.y; v[2] += b.x; v[3] += b.y; v[4] += c.x; v[5] += c.y; v[6] += d.x; v[7] += d.y;
+// eight neighbouring values of which n exist, where they do not begin on 16 bytes
+__device__ __forceinline__ void store_some(bf16* p, const uint4& u, int n) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n) p[e] = __ushort_as_bfloat16((unsigned short)(w[e >> 1] >> (16 * (e & 1))));
 }
-__device__ __forceinline__ void mul8(float (&v)[8], const uint4& u) {
-  const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), d = unpack_bf16(u.w);
-  v[0] *= a.x; v[1] *= a.y; v[2] *= b.x; v[3] *= b.y; v[4] *= c.x; v[5] *= c.y; v[6] *= d.x; v[7] *= d.y;
-}
-__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
-  return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+__device__ __forceinline__ uint4 load_some(const bf16* p, int n) {
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n) w[e >> 1] |= (uint32_t)__bfloat16_as_ushort(p[e]) << (16 * (e & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 16 rows of X by 32 rows of W, as a warp's accumulator lanes hold them (a lane per weight row), out to memory: turned in 2 KB of the
-// warp's own, so that a lane gets eight neighbouring outputs of a row and loads and stores go in 16 bytes.  m0: the first row of X, n0: the
-// warp's first weight row; rows: how many of the 16 there are; wf: the factor of this lane's weight row, xf: of row lane % 16 of X.  The
-// factors were loaded before the tile was waited for, bias and residual are before the turn: a load where it is used costs its latency per
-// chunk (768 -> 2048 for 2463 tokens of 128 experts 103 us, FIXME).
-template <bool GATED>
-__device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v, float* turned, long m0, int rows, int n0, float wf, float xf,
-                                          int lane) {
-  const int n = n0 + (lane & 3) * 8;
-  uint4 res[2], bias8;
-  if (!GATED && a.bias && a.by16 && n < a.N) bias8 = *reinterpret_cast<const uint4*>(a.bias + n);
-  if (!GATED && a.residual && a.by16) {
+// What a draining lane keeps of a tile, loaded while the tile is waited for: factors and biases of weight rows n0 + 8 i + lane / 4 of its warp's 32.
+template <int EPI> struct Fp4Lane {
+  float wf[4], bias[EPI == EPI_ANY ? 4 : 1];
+  __device__ __forceinline__ void load(const Fp4Args& a, long wf0, int n0, int lane) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = i * 8 + (lane >> 2);
-      if (r < rows && n < a.N) res[i] = *reinterpret_cast<const uint4*>(a.residual + (m0 + r) * a.ldr + n);
+    for (int i = 0; i < 4; ++i) {
+      const int n = n0 + 8 * i + (lane >> 2);
+      wf[i] = a.wf && n < a.N ? a.wf[wf0 + n] : 1.0f;
+      if (EPI == EPI_ANY) bias[i] = a.bias && n < a.N ? __bfloat162float(a.bias[n]) : 0.0f;
     }
   }
+};
+
+// 16 rows of X by 32 rows of W out to memory.  v0, v1: the accumulator as fragments, for either half of the weight rows [8 rows of X][4], so that a lane holds
+// for rows 2 (lane % 4) and the next of either eight the weight rows lane / 4 + 0, 8, 16, 24: the gate and the lift of an output are its own, factors and biases of
+// weight rows stay for the tile, and the transposing matrix stores turn rounded results in 1 KB of the warp's own, from where they leave in pieces of 16
+// bytes.  Residuals come in the same way.  m0: the first row, rows: how many there are; n0: the warp's first weight row; xf: the factor of row lane % 16.
+// (A lane per weight row and a turn of fp32 took 500 instructions per 16 x 32: 2390 x 8192 x 2048 with GELU 59 us, FIXME.)
+template <int EPI>
+__device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v0, const uint32_t* v1, uint32_t turned, long m0, int rows, int n0,
+                                          const Fp4Lane<EPI>& keep, float xf, int lane) {
+  float f[4];                                                                  // factors of this lane's rows of X: eight g, column c at 2 g + c
 #pragma unroll
-  for (int i = 0; i < 16; ++i) turned[i * 32 + lane] = __uint_as_float(v[i]) * wf;
-  __syncwarp();
-  if (GATED) {
-    const int r = lane >> 1, g = (lane & 1) * 16, o = (n0 + g) / 2;
-    const float f = __shfl_sync(0xffffffffu, xf, r);
-    if (r < rows && o < a.N / 2) {
-      const float* p = turned + r * 32 + g;
-      float w[8];
+  for (int i = 0; i < 4; ++i) f[i] = __shfl_sync(0xffffffffu, xf, (i >> 1) * 8 + 2 * (lane & 3) + (i & 1));
+  if (EPI == EPI_GATED) {
+    uint32_t o[4];                                                             // [half][eight rows]
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = silu_of(p[e] * f) * (p[8 + e] * f);
-      bf16* out = a.y + (m0 + r) * a.ldy + o;
-      if (a.by16) *reinterpret_cast<uint4*>(out) = pack8(w);                   // N / 2 is a multiple of 8
-      else
-        for (int e = 0; e < 8; ++e) out[e] = __float2bfloat16(w[e]);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const uint32_t* v = (h ? v1 : v0) + 4 * g;
+        float r[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          r[c] = silu_of(__uint_as_float(v[c]) * keep.wf[2 * h] * f[2 * g + c]) * (__uint_as_float(v[2 + c]) * keep.wf[2 * h + 1] * f[2 * g + c]);
+        o[2 * h + g] = pack_bf16(r[0], r[1]);
+      }
+    // 32 bytes per row of X; matrix (h, g) = (lane / 16, lane / 8 % 2)
+    const int m = ((lane >> 3) & 1) * 8 + (lane & 7);
+    stmatrix_x4_trans(turned + m * 32 + (((lane >> 4) ^ (m >> 2)) & 1) * 16, o[0], o[1], o[2], o[3]);
+    __syncwarp();
+    const int r = lane >> 1, h = lane & 1, col = n0 / 2 + h * 8;
+    if (r < rows && col < a.N / 2) {
+      const uint4 u = ld_shared_v4(turned + r * 32 + ((h ^ (r >> 2)) & 1) * 16);
+      bf16* out = a.y + (m0 + r) * a.ldy + col;
+      if (a.by16) *reinterpret_cast<uint4*>(out) = u;                          // N / 2 is a multiple of 8
+      else store_some(out, u, 8);
     }
   } else {
+    const int sm = ((lane >> 3) & 1) * 8 + (lane & 7), sn = lane >> 4;         // matrix (sn, eight) of a half: which row of 16 bytes this lane names
+    const int rr = lane >> 2, rn = lane & 3, n = n0 + rn * 8;                  // what it moves: rows rr and rr + 8, outputs n ..
+    auto at = [&](int m, int n8) { return turned + m * 64 + ((n8 ^ (m >> 1)) & 3) * 16; };
+    if (EPI == EPI_ANY && a.residual) {
+      uint4 u[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = i * 8 + (lane >> 2);
-      const float f = __shfl_sync(0xffffffffu, xf, r);
-      if (r < rows && n < a.N) {
-        const long m = m0 + r;
-        const float4* p = reinterpret_cast<const float4*>(turned + r * 32 + (lane & 3) * 8);
-        const float4 lo = p[0], hi = p[1];
-        float w[8] = {lo.x * f, lo.y * f, lo.z * f, lo.w * f, hi.x * f, hi.y * f, hi.z * f, hi.w * f};
-        bf16* out = a.y + m * a.ldy + n;
-        if (a.by16) {
-          if (a.bias) add8(w, bias8);
-          if (a.act == FP4_SILU) {
+      for (int i = 0; i < 2; ++i) {
+        const bf16* p = a.residual + (m0 + rr + 8 * i) * a.ldr + n;
+        u[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (rr + 8 * i < rows && n < a.N) {
+          if (a.by16) u[i] = *reinterpret_cast<const uint4*>(p);
+          else u[i] = load_some(p, a.N - n);
+        }
+      }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = silu_of(w[e]);
-          } else if (a.act == FP4_GELU_TANH) {
+      for (int i = 0; i < 2; ++i) st_shared_v4(at(rr + 8 * i, rn), u[i]);
+      __syncwarp();
+    }
+    float r[2][8];                                                             // [half][2 (2 s + g) + c]
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = gelu_of(w[e]);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int s = i >> 2, g = (i >> 1) & 1, c = i & 1;
+        r[h][i] = __uint_as_float((h ? v1 : v0)[4 * g + 2 * s + c]) * keep.wf[2 * h + s] * f[2 * g + c];
+        if (EPI == EPI_ANY) r[h][i] += keep.bias[2 * h + s];
+      }
+    if (EPI == EPI_ANY) {
+      // a step for all sixteen values at a time: they do not depend on one another, and the branches are the same for all
+      if (a.act == FP4_SILU) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[i >> 3][i & 7] = silu_of(r[i >> 3][i & 7]);
+      } else if (a.act == FP4_GELU_TANH) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[i >> 3][i & 7] = gelu_of(r[i >> 3][i & 7]);
+      }
+      if (a.gate) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int h = i >> 3, s = (i >> 2) & 1, g = (i >> 1) & 1, c = i & 1;
+          const int row = min(8 * g + 2 * (lane & 3) + c, rows - 1), col = min(n0 + 16 * h + 8 * s + (lane >> 2), a.N - 1);
+          r[h][i & 7] *= __bfloat162float(a.gate[(m0 + row) / a.rows_per_gate * a.gate_stride + col]);
+        }
+      }
+      if (a.residual) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t res[4];
+          ldmatrix_x4_trans(at(sm, 2 * h + sn), res);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 t = unpack_bf16(res[i]);
+            r[h][2 * i] += t.x;
+            r[h][2 * i + 1] += t.y;
           }
-          if (a.gate) mul8(w, *reinterpret_cast<const uint4*>(a.gate + m / a.rows_per_gate * a.gate_stride + n));
-          if (a.residual) add8(w, res[i]);
-          *reinterpret_cast<uint4*>(out) = pack8(w);
-        } else {
-          for (int e = 0; e < 8 && n + e < a.N; ++e) out[e] = __float2bfloat16(fp4_finish(a, w[e], m, n + e));
         }
       }
     }
+    uint32_t o[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[h][i] = pack_bf16(r[h][2 * i], r[h][2 * i + 1]);
+    if (EPI == EPI_ANY && a.residual) __syncwarp();                            // everybody has read what they write over
+#pragma unroll
+    for (int h = 0; h < 2; ++h) stmatrix_x4_trans(at(sm, 2 * h + sn), o[h][0], o[h][1], o[h][2], o[h][3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = rr + 8 * i;
+      if (r < rows && n < a.N) {
+        const uint4 u = ld_shared_v4(at(r, rn));
+        bf16* out = a.y + (m0 + r) * a.ldy + n;
+        if (a.by16) *reinterpret_cast<uint4*>(out) = u;                        // N is a multiple of 8
+        else store_some(out, u, a.N - n);
+      }
+    }
   }
-  __syncwarp();
+  __syncwarp();                                                                // the next 16 rows are turned in the same place
 }
 
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* tmap, int c0, int c1, int c2) {
   asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2)
@@ -190,10 +262,11 @@ __device__ __forceinline__ bool row_tile(const Fp4Args& a, int t, RowTile& r) {
   return true;
 }
 
-template <int FMT, int XR, bool GATED, bool PAIR>
+template <int FMT, int XR, int EPI, bool PAIR>
 __global__ void __launch_bounds__(Fp4Cfg<FMT, XR, PAIR>::THREADS, Fp4Cfg<FMT, XR, PAIR>::CTAS)
 fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
   using Cfg = Fp4Cfg<FMT, XR, PAIR>;
+  constexpr bool GATED = EPI == EPI_GATED;
   constexpr int STAGES = Cfg::STAGES, ACCS = Cfg::ACCS, STEP = PAIR ? 32 : 16;         // steps of an MMA's N
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[STAGES];               // pairs: in the even CTA, the bytes of both
@@ -255,6 +328,8 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
   __syncwarp();
   pdl_begin();
 
+  uint32_t part_sums[PAIR ? 1 : Cfg::CHUNKS][16];                  // split: of the draining warps
+  float wf = 1.0f;
   if (warp == 0) {
     if (elect_one()) {
       int stage = 0;
@@ -341,14 +416,15 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
     }
   } else {
     const int q = warp & 3, part = (warp - 2) >> 2;                // quadrant of tensor memory; which share of the tile's rows of X
-    float* turned = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_PITCH + (warp - 2) * 2048);
+    const uint32_t turned = smem_base + STAGES * Cfg::STAGE_PITCH + (warp - 2) * 1024;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int it = first; it < num_items; it += step) {
       RowTile t;
       if (!row_tile<XR>(a, tile_of(it), t)) break;
       const int n0 = block_of(it) * 128 + q * 32, c0 = part * 16 * Cfg::CHUNKS;
-      const float wf = a.wf && n0 + lane < a.N ? a.wf[(long)t.expert * a.N + n0 + lane] : 1.0f;
+      Fp4Lane<EPI> keep;
+      keep.load(a, (long)t.expert * a.N, n0, lane);
       float xf[Cfg::CHUNKS];
 #pragma unroll
       for (int i = 0; i < Cfg::CHUNKS; ++i) {
@@ -357,62 +433,84 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
       }
       mbar_wait(smem_u32(&tfull_bar[acc]), acc_phase, &s_abort, status, ERR_WAIT_TMEM_FULL);
       tc_fence_after_sync();
-      const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + acc * XR + c0;
-      if (PAIR) {
-        // 64 of the 256 rows per warp, into registers; then the accumulator is free
-        uint32_t v[Cfg::CHUNKS][16];
+      const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + acc * XR + c0, half = 16u << 16;
+      if constexpr (PAIR) {
+        // 64 of the 256 rows per warp, into registers (with operands in the epilogue in two steps, for want of registers); then the accumulator is free
+        constexpr int STEPS = EPI == EPI_ANY ? 2 : 1, PER = Cfg::CHUNKS / STEPS;
 #pragma unroll
-        for (int i = 0; i < Cfg::CHUNKS; ++i) tmem_ld_32x16(at + i * 16, v[i]);
-        tmem_wait_ld();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[acc]), 0));
+        for (int j = 0; j < STEPS; ++j) {
+          uint32_t v[2][8 * PER];
 #pragma unroll
-        for (int i = 0; i < Cfg::CHUNKS; ++i) {
-          const int c = c0 + i * 16;
-          if (c < t.rows) fp4_store<GATED>(a, v[i], turned, t.row0 + c, t.rows - c, n0, wf, xf[i], lane);
+          for (int h = 0; h < 2; ++h)
+            if (PER == 4) tmem_ld_16x256_x8(at + h * half, v[h]);
+            else tmem_ld_16x256_x4(at + h * half + j * 16 * PER, v[h]);
+          tmem_wait_ld();
+          if (j == STEPS - 1) {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[acc]), 0));
+          }
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const int c = c0 + (j * PER + i) * 16;
+            if (c < t.rows) fp4_store<EPI>(a, v[0] + 8 * i, v[1] + 8 * i, turned, t.row0 + c, t.rows - c, n0, keep, xf[j * PER + i], lane);
+          }
         }
-      } else {
-        // split: this CTA's sums [row of X][128] to its ring, which nothing reads any more
-        float* sums = reinterpret_cast<float*>(smem) + q * 32 + lane;
+      } else if (a.split == 1) {
 #pragma unroll
         for (int i = 0; i < Cfg::CHUNKS; ++i) {
           const int c = c0 + i * 16;
           if (c >= t.rows) break;
-          uint32_t v[16];
-          tmem_ld_32x16(at + i * 16, v);
+          uint32_t v[2][8];
+          tmem_ld_16x256_x2(at + i * 16, v[0]);
+          tmem_ld_16x256_x2(at + i * 16 + half, v[1]);
           tmem_wait_ld();
-          if (a.split == 1) {
-            fp4_store<GATED>(a, v, turned, t.row0 + c, t.rows - c, n0, wf, xf[i], lane);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sums[(c + j) * 128] = __uint_as_float(v[j]) * wf;
-          }
+          fp4_store<EPI>(a, v[0], v[1], turned, t.row0 + c, t.rows - c, n0, keep, xf[i], lane);
         }
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
+      } else {
+        // this CTA's sums stay in registers until everybody's ring is free
+        wf = a.wf && n0 + lane < a.N ? a.wf[(long)t.expert * a.N + n0 + lane] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < Cfg::CHUNKS; ++i)
+          if (c0 + i * 16 < t.rows) tmem_ld_32x16(at + i * 16, part_sums[i]);
+        tmem_wait_ld();
       }
       if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
     }
   }
 
   if (!PAIR && a.split > 1) {
+    // Every CTA finishes 128 / split of the weight rows (at least 16: a gate group and its lift rows), all rows of X: the others' sums come to it as [their
+    // share][row of X][width], in its ring, and are added in the order of the shares.
+    RowTile t;
+    const bool any = first < num_items && row_tile<XR>(a, tile_of(first), t);
+    const int width = 128 / a.split;
     __syncwarp();
     cluster_sync_all();
-    RowTile t;
-    if (first < num_items && row_tile<XR>(a, tile_of(first), t)) {
-      // every CTA finishes 128 / split of the weight rows (at least 16: a gate group and its lift rows), all rows of X, four at a time
-      const int width = 128 / a.split, base = share * width, n0 = block_of(first) * 128 + base, outs = GATED ? width / 2 : width, quads = outs / 4;
+    if (any && warp >= 2) {
+      const int n = (warp & 3) * 32 + lane, owner = n / width, c0 = ((warp - 2) >> 2) * 16 * Cfg::CHUNKS;
+      const uint32_t to = mapa_shared(smem_base + ((share * t.rows + c0) * width + n % width) * 4, owner);
+#pragma unroll
+      for (int i = 0; i < (PAIR ? 1 : Cfg::CHUNKS); ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c0 + i * 16 + j < t.rows) st_cluster_f32(to + (i * 16 + j) * width * 4, __uint_as_float(part_sums[i][j]) * wf);
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (any) {
+      const int base = share * width, n0 = block_of(first) * 128 + base, outs = GATED ? width / 2 : width, quads = outs / 4;
       auto sum = [&](int r, int n, float (&s)[4]) {
-        float4 v[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          if (c < a.split) v[c] = ld_cluster_f32x4(mapa_shared(smem_base + (r * 128 + base + n) * 4, c));
-        s[0] = v[0].x; s[1] = v[0].y; s[2] = v[0].z; s[3] = v[0].w;
-#pragma unroll
-        for (int c = 1; c < 8; ++c)
-          if (c < a.split) { s[0] += v[c].x; s[1] += v[c].y; s[2] += v[c].z; s[3] += v[c].w; }
+        const uint32_t at = smem_base + (r * width + n) * 4;
+        const uint4 f = ld_shared_v4(at);
+        s[0] = __uint_as_float(f.x); s[1] = __uint_as_float(f.y); s[2] = __uint_as_float(f.z); s[3] = __uint_as_float(f.w);
+        for (int c = 1; c < a.split; ++c) {
+          const uint4 g = ld_shared_v4(at + c * t.rows * width * 4);
+          s[0] += __uint_as_float(g.x); s[1] += __uint_as_float(g.y); s[2] += __uint_as_float(g.z); s[3] += __uint_as_float(g.w);
+        }
       };
       for (int i = threadIdx.x; i < t.rows * quads; i += blockDim.x) {
         const int r = i / quads, o = (i - r * quads) * 4;
@@ -421,16 +519,25 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
         float s0[4], s1[4];
         if (GATED) {
           const int n = o / 8 * 16 + o % 8;
+          if (n0 + n >= a.N) continue;
           sum(r, n, s0);
           sum(r, n + 8, s1);
-          if (n0 + n < a.N)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) a.y[m * a.ldy + n0 / 2 + o + e] = __float2bfloat16(silu_of(s0[e] * f) * (s1[e] * f));
+          for (int e = 0; e < 4; ++e) s0[e] = silu_of(s0[e] * f) * (s1[e] * f);
+          bf16* out = a.y + m * a.ldy + n0 / 2 + o;
+          if (a.by16) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(s0[0], s0[1]), pack_bf16(s0[2], s0[3]));
+          else
+            for (int e = 0; e < 4; ++e) out[e] = __float2bfloat16(s0[e]);
         } else {
+          const int n = n0 + o;
+          if (n >= a.N) continue;
           sum(r, o, s0);
+          bf16* out = a.y + m * a.ldy + n;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n0 + o + e < a.N) a.y[m * a.ldy + n0 + o + e] = __float2bfloat16(fp4_finish(a, s0[e] * f, m, n0 + o + e));
+          for (int e = 0; e < 4; ++e) s0[e] = EPI == EPI_ANY ? (n + e < a.N ? fp4_finish(a, s0[e] * f, m, n + e) : 0.f) : s0[e] * f;
+          if (a.by16) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(s0[0], s0[1]), pack_bf16(s0[2], s0[3]));
+          else
+            for (int e = 0; e < 4 && n + e < a.N; ++e) out[e] = __float2bfloat16(s0[e]);
         }
       }
     }
@@ -443,7 +550,7 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
     while (globaltimer_ns() - t0 < 200000ull) {
     }
   }
-  if (PAIR || a.split > 1) cluster_sync_all();   // nobody leaves while another may still signal it or read its sums
+  if (PAIR) cluster_sync_all();                 // neither CTA leaves while its partner may still signal it
   if (warp == 1) {
     tc_fence_after_sync();
     if (PAIR) tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
@@ -496,7 +603,7 @@ static int resident_pairs(const void* kernel, int threads, int smem) {
   return cached = n <= 0 || n > sm_count() / 2 ? sm_count() / 2 : n;
 }
 
-template <int FMT, int XR, bool GATED, bool PAIR>
+template <int FMT, int XR, int EPI, bool PAIR>
 static int launch_fp4(Fp4Args& a, const Fp4Operands& o, int* status, cudaStream_t stream) {
   using Cfg = Fp4Cfg<FMT, XR, PAIR>;
   const uint64_t K2 = a.K / 2, words = scale_words(FMT, a.K), blocks = (a.N + 127) / 128;
@@ -514,7 +621,7 @@ static int launch_fp4(Fp4Args& a, const Fp4Operands& o, int* status, cudaStream_
   if (int rc = make_map(&a.tmXS, o.xs, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, xsd, xsp, xsb, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
 
   static unsigned long long prepared = 0;
-  auto* kernel = fp4_kernel<FMT, XR, GATED, PAIR>;
+  auto* kernel = fp4_kernel<FMT, XR, EPI, PAIR>;
   if (int e = ensure_dynamic_smem((const void*)kernel, Cfg::SMEM_BYTES, prepared)) return e;
   const long items = (long)a.max_tiles * ((a.N + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128));
   const int group = PAIR ? 2 : a.split, most = PAIR ? resident_pairs((const void*)kernel, Cfg::THREADS, Cfg::SMEM_BYTES) : Cfg::CTAS * sm_count();
@@ -523,20 +630,26 @@ static int launch_fp4(Fp4Args& a, const Fp4Operands& o, int* status, cudaStream_
   return launch_with(true, group, kernel, (unsigned)(run * group), Cfg::THREADS, Cfg::SMEM_BYTES, stream, a, status);
 }
 
-template <int FMT, bool GATED>
+template <int FMT, int EPI>
 static int launch_rows_of(Fp4Args& a, const Fp4Operands& o, int tile, int* status, cudaStream_t s) {
   switch (tile) {
-    case 16: return launch_fp4<FMT, 16, GATED, false>(a, o, status, s);
-    case 64: return launch_fp4<FMT, 64, GATED, false>(a, o, status, s);
-    case 128: return launch_fp4<FMT, 128, GATED, false>(a, o, status, s);
-    case 256: return launch_fp4<FMT, 256, GATED, true>(a, o, status, s);
+    case 16: return launch_fp4<FMT, 16, EPI, false>(a, o, status, s);
+    case 64: return launch_fp4<FMT, 64, EPI, false>(a, o, status, s);
+    case 128: return launch_fp4<FMT, 128, EPI, false>(a, o, status, s);
+    case 256: return launch_fp4<FMT, 256, EPI, true>(a, o, status, s);
     default: return RC_BAD_ARG;
   }
 }
 
+template <int FMT>
+static int launch_epi(Fp4Args& a, const Fp4Operands& o, bool gated, int tile, int* status, cudaStream_t s) {
+  if (gated) return launch_rows_of<FMT, EPI_GATED>(a, o, tile, status, s);
+  const bool any = a.bias || a.act || a.gate || a.residual;
+  return any ? launch_rows_of<FMT, EPI_ANY>(a, o, tile, status, s) : launch_rows_of<FMT, EPI_PLAIN>(a, o, tile, status, s);
+}
 static int launch_any(Fp4Args& a, const Fp4Operands& o, int fmt, bool gated, int tile, int* status, cudaStream_t s) {
-  if (fmt == FMT_MXFP4) return gated ? launch_rows_of<FMT_MXFP4, true>(a, o, tile, status, s) : launch_rows_of<FMT_MXFP4, false>(a, o, tile, status, s);
-  if (fmt == FMT_NVFP4) return gated ? launch_rows_of<FMT_NVFP4, true>(a, o, tile, status, s) : launch_rows_of<FMT_NVFP4, false>(a, o, tile, status, s);
+  if (fmt == FMT_MXFP4) return launch_epi<FMT_MXFP4>(a, o, gated, tile, status, s);
+  if (fmt == FMT_NVFP4) return launch_epi<FMT_NVFP4>(a, o, gated, tile, status, s);
   return RC_BAD_ARG;
 }
 

@@ -55,13 +55,14 @@ struct ExpertOperand {           // one product's rows in a workspace, and its w
   int N, K;
 };
 
-// Rows of x (pair p reads row p / per) through `up` (gated, N = 2 F) to h [pairs, F] and through `down` to y [pairs, D], both in the plan's order of rows;
-// tile: the most rows a tile has, 64 / 128 / 256.
+// Rows of x (pair p reads row p / per, pairs a multiple of per) through `up` (gated, N = 2 F) to h [pairs, F] and through `down` to y [pairs, D], both in the plan's order of rows;
+// tile: the most rows a tile has, 64 / 128 / 256; n_rows: how many rows the
+// plan has; place_of_row [pairs]: scratch.
 extern "C" int omni_lowbit_experts(const void* x, long ldx, int per, long pairs, int experts, int fmt, const ExpertOperand* up, const ExpertOperand* down, void* h,
                                    void* y, const int* row_of_pair, const int* tile_expert, const int* tile_row0, const int* tile_rows, int max_tiles,
-                                   int tile, void* status, void* stream) {
+                                   int tile, const int* n_rows, int* place_of_row, void* status, void* stream) {
   if (pairs <= 0 || max_tiles <= 0) return RC_OK;
-  if (pairs > 0x7fffff00L || per < 1 || experts < 1 || !row_of_pair || !tile_expert || !tile_row0 || !tile_rows || up->N % 16 || up->N != 2 * down->K ||
+  if (pairs > 0x7fffff00L || per < 1 || experts < 1 || !row_of_pair || !n_rows || !place_of_row || pairs % per || !tile_expert || !tile_row0 || !tile_rows || up->N % 16 || up->N != 2 * down->K ||
       up->K % 32 || down->K % 32 || fmt == FMT_FP8)
     return RC_BAD_ARG;
   cudaStream_t s = (cudaStream_t)stream;
@@ -69,9 +70,9 @@ extern "C" int omni_lowbit_experts(const void* x, long ldx, int per, long pairs,
   for (int half = 0; half < 2; ++half) {
     const ExpertOperand& o = half ? *down : *up;
     RowsArgs r = {};
-    r.x = (const bf16*)(half ? h : x); r.ldx = half ? o.K : ldx; r.rows = pairs; r.K = o.K;
+    r.x = (const bf16*)(half ? h : x); r.ldx = half ? o.K : ldx; r.rows = half ? pairs : pairs / per; r.K = o.K;
     r.codes = (uint8_t*)o.codes; r.scales = o.scales; r.row_scale = (float*)o.row_scale;
-    r.place = {1, half ? nullptr : row_of_pair, tile_expert, tile_row0, tile_rows, per, max_tiles, pitch};
+    r.place = {1, half ? nullptr : row_of_pair, tile_expert, tile_row0, tile_rows, n_rows, place_of_row, per, max_tiles, pitch};
     if (int e = rows_any(r, fmt, s)) return e;
     Fp4Args a = {};
     a.y = (bf16*)(half ? y : h); a.ldy = half ? o.N : o.N / 2; a.wf = (const float*)o.wf; a.xf = (const float*)o.row_scale;

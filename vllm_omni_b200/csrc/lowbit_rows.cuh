@@ -12,12 +12,14 @@
 
 namespace omni {
 
-// Where a launch's rows come from and go to.  `tiles` null: row r of x to row r, scales by groups of `group` rows (the experts of a weight), each from
-// a new tile of 128 on.  Else expert rows: with `row_of_pair`, item p is pair p, whose source is row p / per; without, source and
-// place are the item's own index.  Scales of row i of tile t stand at t * pitch + i; rows of no tile are left out.
+// Where a launch's rows go.  ROWS: row r of x to row r, scales by groups of `group` rows (the experts of a weight), each from a new tile of 128 on.
+// GATHER: item t is a token, its row goes to the rows row_of_pair[t * per ..] of its choices, and scales to the place of the tile those lie in: row i of
+// tile t at t * pitch + i; place_of_row keeps that.  PLACED: row r to row r, scales to place_of_row[r] (rows that no choice has are left out).
+enum RowMode : int { ROWS = 0, GATHER = 1, PLACED = 2 };
 struct RowPlace {
   long group;
-  const int *row_of_pair, *tile_expert, *tile_row0, *tile_rows;
+  const int *row_of_pair, *tile_expert, *tile_row0, *tile_rows, *n_rows;
+  int* place_of_row;
   int per, max_tiles, pitch;
 };
 
@@ -60,12 +62,22 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
   v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
 }
 
-// One chunk of eight elements per lane; `row_inv` (nvfp4) the reciprocal of the row's factor.  Writes the codes and, from the first lane of a
-// word, the scales.
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Codes of a chunk (4-bit: x; fp8: x and y) and its scale: the whole word on every lane of its four blocks (4-bit), an fp32 (fp8).
+struct Chunk {
+  uint2 code;
+  uint32_t scale;
+};
+// Eight elements per lane; `row_inv` (nvfp4) the reciprocal of the row's factor; `in`: the chunk exists (else its bytes of the word are zero).
 template <int FMT>
-__device__ __forceinline__ void quantize_chunk(const RowsArgs& a, const uint4& u, int chunk, long code_row, long scale_row, float row_inv, bool live) {
+__device__ __forceinline__ Chunk quantize_chunk(const uint4& u, float row_inv, bool in) {
   const int lane = threadIdx.x & 31;
-  const bool in = live && chunk * 8 < a.K;
+  Chunk out;
   float v[8];
   unpack8(u, v);
   if (FMT == FMT_FP8) {
@@ -80,30 +92,29 @@ __device__ __forceinline__ void quantize_chunk(const RowsArgs& a, const uint4& u
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       w[i >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * inv, v[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3) << (16 * (i & 1));
-    if (in) {
-      *reinterpret_cast<uint2*>(a.codes + code_row * a.K + chunk * 8) = make_uint2(w[0], w[1]);
-      if ((lane & 15) == 0) reinterpret_cast<float*>(a.scales)[scale_row * (a.K / 128) + chunk / 16] = scale;
-    }
-    return;
+    out.code = make_uint2(w[0], w[1]);
+    out.scale = __float_as_uint(scale);
+    return out;
   }
-  const uint32_t top = group_max<FMT == FMT_MXFP4 ? 4 : 2>(max_pattern(u));
+  constexpr int PER = FMT == FMT_MXFP4 ? 4 : 2;                 // lanes of a block; a word is four blocks
+  const uint32_t top = group_max<PER>(max_pattern(u));
   uint32_t byte;
   float q[8];
   if (FMT == FMT_MXFP4) {
     // the power of two two below the largest magnitude's (6 = 1.5 * 2^2 is the largest code): dividing by it is exact
     const uint32_t e = top >> 7;
     byte = e == 255 ? 255 : e > 2 ? e - 2 : 0;
-    const float inv = __uint_as_float(byte == 254 ? 1u << 22 : (254u - byte) << 23);       // 2^-(byte - 127); no scale is above 253
+    const float inv = __uint_as_float((254u - byte) << 23);     // 2^-(byte - 127); no finite block's byte is above 252
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = v[i] * inv;
   } else {
-    // s = e4m3(max / 6).  The quotient is formed by one rounded reciprocal, then rounded to fp16: x / s of an 8-bit by a 4-bit mantissa is
-    // either exactly halfway between two codes or off by 2^-9 of itself, so that the 11 bits of fp16 restore what the reciprocal's last
-    // bit would make of a tie.
-    const float s_want = __fdiv_rn(__uint_as_float(top << 16) * row_inv, 6.0f);
-    byte = __nv_cvt_float_to_fp8(s_want, __NV_SATFINITE, __NV_E4M3);
+    // s = e4m3(max / 6), code = e2m1(x / s).  Both quotients are products with a reciprocal, off by a few steps of fp32, rounded to fp16 before they are
+    // rounded to the format: max / 6 (8-bit mantissas) is either exactly halfway between two e4m3 values or 2^-9 of itself away, and so is x / s (8 by
+    // 4 bits) for e2m1, so that the 11 bits of fp16 keep what is no tie from becoming one and restore what is.
+    const __half want = __float2half_rn(__uint_as_float(top << 16) * row_inv * (1.0f / 6.0f));
+    byte = __nv_cvt_halfraw_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
     const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
-    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+    const float inv = s > 0.f ? rcp_fast(s) : 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 f = __half22float2(__floats2half2_rn(v[2 * i] * row_inv * inv, v[2 * i + 1] * row_inv * inv));
@@ -112,77 +123,82 @@ __device__ __forceinline__ void quantize_chunk(const RowsArgs& a, const uint4& u
     }
     if (top >= 0x7f80u) byte = 0x7f;
   }
-  if (in) *reinterpret_cast<uint32_t*>(a.codes + code_row * (a.K / 2) + chunk * 4) = e2m1x8(q);
-  constexpr int PER = FMT == FMT_MXFP4 ? 4 : 2;                 // lanes of a block; a word is four blocks
-  uint32_t word = (lane % PER) == 0 && chunk * 8 < a.K ? byte << (8 * ((lane / PER) & 3)) : 0u;
+  out.code = make_uint2(e2m1x8(q), 0u);
+  uint32_t word = in ? byte << (8 * ((lane / PER) & 3)) : 0u;
   word |= __shfl_xor_sync(0xffffffffu, word, PER);
-  word |= __shfl_xor_sync(0xffffffffu, word, 2 * PER);
-  const int words = scale_words(FMT, a.K), at = chunk / (4 * PER);
-  if (live && lane % (4 * PER) == 0 && at < words)
-    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.scales) + scale_word_at(scale_row, at, words)) = word;
+  out.scale = word | __shfl_xor_sync(0xffffffffu, word, 2 * PER);
+  return out;
 }
 
+template <int FMT>
+__device__ __forceinline__ void store_chunk(const RowsArgs& a, const Chunk& c, int chunk, long code_row, long scale_row) {
+  const int lane = threadIdx.x & 31;
+  if (FMT == FMT_FP8) {
+    if (chunk * 8 < a.K) {
+      *reinterpret_cast<uint2*>(a.codes + code_row * a.K + chunk * 8) = c.code;
+      if ((lane & 15) == 0) static_cast<uint32_t*>(a.scales)[scale_row * (a.K / 128) + chunk / 16] = c.scale;
+    }
+  } else {
+    constexpr int PER = FMT == FMT_MXFP4 ? 4 : 2;
+    if (chunk * 8 < a.K) *reinterpret_cast<uint32_t*>(a.codes + code_row * (a.K / 2) + chunk * 4) = c.code.x;
+    const int words = scale_words(FMT, a.K), at = chunk / (4 * PER);
+    if (lane % (4 * PER) == 0 && at < words)
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.scales) + scale_word_at(scale_row, at, words)) = c.scale;
+  }
+}
+
+constexpr int GATHER_MOST = 8;   // choices placed at a time
+
 // NV chunks per thread, a.tpr threads per row, blockDim / tpr rows per block.
-template <int FMT, bool NORM, int NV>
+template <int FMT, bool NORM, int MODE, int NV>
 __global__ void __launch_bounds__(1024)
 lowbit_rows_kernel(const RowsArgs a) {
   __shared__ uint32_t red[32];
-  __shared__ int found[32];
   const int sub = threadIdx.x / a.tpr, tid = threadIdx.x - sub * a.tpr, lane = threadIdx.x & 31;
   const int warps = a.tpr >> 5, warp0 = sub * warps;
   const long item = (long)blockIdx.x * (blockDim.x / a.tpr) + sub;
+  const RowPlace& pl = a.place;
   bool live = item < a.rows;
   pdl_begin();
-  const RowPlace& pl = a.place;
-  const bool tiled = pl.tile_expert != nullptr;
-  long src = item, code_row = item, scale_row = 0;
-  if (tiled) {
-    if (pl.row_of_pair) {
-      code_row = live ? pl.row_of_pair[item] : -1;
-      src = item / pl.per;
-    }
-    live = live && code_row >= 0;
-  } else {
-    const long g = item / pl.group;
-    scale_row = g * ((pl.group + 127) / 128 * 128) + (item - g * pl.group);
-  }
   uint4 u[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = tid + i * a.tpr;
-    u[i] = live && c * 8 < a.K ? *reinterpret_cast<const uint4*>(a.x + src * a.ldx + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+    u[i] = live && c * 8 < a.K ? *reinterpret_cast<const uint4*>(a.x + item * a.ldx + c * 8) : make_uint4(0u, 0u, 0u, 0u);
   }
-  if (tiled) {
-    if (tid == 0) found[sub] = -1;
-    __syncthreads();
-    for (int t = tid; t < pl.max_tiles; t += a.tpr) {
-      const int i = (int)code_row - pl.tile_row0[t];
-      if (live && pl.tile_expert[t] >= 0 && i >= 0 && i < pl.tile_rows[t]) found[sub] = t * pl.pitch + i;
-    }
-    __syncthreads();
-    scale_row = found[sub];
-    live = live && scale_row >= 0;
+  long scale_row = item;
+  if (MODE == PLACED) {
+    live = live && item < *pl.n_rows;
+    scale_row = live ? pl.place_of_row[item] : 0;
+  } else if (MODE == ROWS && pl.group != a.rows) {
+    const long g = item / pl.group;
+    scale_row = g * ((pl.group + 127) / 128 * 128) + (item - g * pl.group);
   }
   if (NORM) {
     float ss = 0.f;
     if (a.residual) {
+      uint4 r[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = tid + i * a.tpr;
-        if (live && c * 8 < a.K) {
-          const uint4 r = *reinterpret_cast<const uint4*>(a.residual + src * a.ldr + c * 8);
-          float v[8], w[8];
-          unpack8(u[i], v);
-          unpack8(r, w);
-          u[i] = make_uint4(pack_bf16(v[0] + w[0], v[1] + w[1]), pack_bf16(v[2] + w[2], v[3] + w[3]), pack_bf16(v[4] + w[4], v[5] + w[5]),
-                            pack_bf16(v[6] + w[6], v[7] + w[7]));
-        }
+        r[i] = live && c * 8 < a.K ? *reinterpret_cast<const uint4*>(a.residual + item * a.ldr + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float v[8], w[8];
+        unpack8(u[i], v);
+        unpack8(r[i], w);
+        u[i] = make_uint4(pack_bf16(v[0] + w[0], v[1] + w[1]), pack_bf16(v[2] + w[2], v[3] + w[3]), pack_bf16(v[4] + w[4], v[5] + w[5]),
+                          pack_bf16(v[6] + w[6], v[7] + w[7]));
       }
     }
+    uint4 gain[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = tid + i * a.tpr;
-      if (a.total && live && c * 8 < a.K) *reinterpret_cast<uint4*>(a.total + src * a.ldt + c * 8) = u[i];
+      const bool in = live && c * 8 < a.K;
+      gain[i] = in ? *reinterpret_cast<const uint4*>(a.gain + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+      if (a.total && in) *reinterpret_cast<uint4*>(a.total + item * a.ldt + c * 8) = u[i];
       float v[8];
       unpack8(u[i], v);
 #pragma unroll
@@ -195,24 +211,22 @@ lowbit_rows_kernel(const RowsArgs a) {
       __syncthreads();
       ss = 0.f;
       for (int w = 0; w < warps; ++w) ss += __uint_as_float(red[warp0 + w]);
-      __syncthreads();
+      if (FMT == FMT_NVFP4) __syncthreads();
     }
     const float r = 1.0f / sqrtf(ss / (float)a.K + a.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = tid + i * a.tpr;
-      if (live && c * 8 < a.K) {
-        float v[8], g[8];
-        unpack8(u[i], v);
-        unpack8(*reinterpret_cast<const uint4*>(a.gain + c * 8), g);
-        // rounded to bf16 before the blocks' scales are taken: the values a norm of its own would have stored
-        u[i] = make_uint4(pack_bf16(v[0] * r * g[0], v[1] * r * g[1]), pack_bf16(v[2] * r * g[2], v[3] * r * g[3]),
-                          pack_bf16(v[4] * r * g[4], v[5] * r * g[5]), pack_bf16(v[6] * r * g[6], v[7] * r * g[7]));
-        if (a.normed) *reinterpret_cast<uint4*>(a.normed + src * a.ldn + c * 8) = u[i];
-      }
+      float v[8], g[8];
+      unpack8(u[i], v);
+      unpack8(gain[i], g);
+      // rounded to bf16 before the blocks' scales are taken: the values a norm of its own would have stored
+      u[i] = make_uint4(pack_bf16(v[0] * r * g[0], v[1] * r * g[1]), pack_bf16(v[2] * r * g[2], v[3] * r * g[3]),
+                        pack_bf16(v[4] * r * g[4], v[5] * r * g[5]), pack_bf16(v[6] * r * g[6], v[7] * r * g[7]));
+      if (a.normed && live && c * 8 < a.K) *reinterpret_cast<uint4*>(a.normed + item * a.ldn + c * 8) = u[i];
     }
   }
-  float row_inv = 1.f;
+  float row_inv = 1.f, factor = 1.f;
   if (FMT == FMT_NVFP4) {
     // the row's factor: the power of two that puts the row's largest magnitude into [2^10, 2^11), its block's scale into [170, 342)
     uint32_t top = 0;
@@ -226,10 +240,47 @@ lowbit_rows_kernel(const RowsArgs a) {
     }
     const int e = (int)(top >> 7), field = top == 0 ? 127 : e > 11 ? e - 10 : 1;
     row_inv = __uint_as_float((uint32_t)(254 - field) << 23);
-    if (live && tid == 0) a.row_scale[code_row] = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)field << 23);
+    factor = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)field << 23);
   }
+  Chunk c[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) quantize_chunk<FMT>(a, u[i], tid + i * a.tpr, code_row, scale_row, row_inv, live);
+  for (int i = 0; i < NV; ++i) c[i] = quantize_chunk<FMT>(u[i], row_inv, (tid + i * a.tpr) * 8 < a.K);
+  if (MODE != GATHER) {
+    if (!live) return;
+    if (FMT == FMT_NVFP4 && tid == 0) a.row_scale[item] = factor;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) store_chunk<FMT>(a, c[i], tid + i * a.tpr, item, scale_row);
+  } else {
+    // quantised once, written once per choice; the tiles of up to eight choices are looked for together, a tile per thread
+    __shared__ int found[32][GATHER_MOST];
+    for (int j0 = 0; j0 < pl.per; j0 += GATHER_MOST) {
+      int row[GATHER_MOST];
+#pragma unroll
+      for (int j = 0; j < GATHER_MOST; ++j) row[j] = live && j0 + j < pl.per ? pl.row_of_pair[item * pl.per + j0 + j] : -1;
+      __syncthreads();
+      if (tid < GATHER_MOST) found[sub][tid] = -1;
+      __syncthreads();
+      for (int t = tid; t < pl.max_tiles; t += a.tpr) {
+        const int first = pl.tile_row0[t], n = pl.tile_expert[t] >= 0 ? pl.tile_rows[t] : 0;
+#pragma unroll
+        for (int j = 0; j < GATHER_MOST; ++j)
+          if (row[j] >= first && row[j] < first + n) found[sub][j] = t * pl.pitch + (row[j] - first);
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int j = 0; j < GATHER_MOST; ++j) {
+        const int r = __shfl_sync(0xffffffffu, live && j0 + j < pl.per ? pl.row_of_pair[item * pl.per + j0 + j] : -1, 0);
+        const int at = found[sub][j];
+        if (r < 0 || at < 0) continue;
+        if (tid == 0) {
+          pl.place_of_row[r] = at;
+          if (FMT == FMT_NVFP4) a.row_scale[r] = factor;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store_chunk<FMT>(a, c[i], tid + i * a.tpr, r, at);
+      }
+    }
+  }
 }
 
 struct DequantArgs {
@@ -241,70 +292,95 @@ struct DequantArgs {
   int K, f32;
 };
 
-// Eight elements per thread.
+// Eight elements per thread, four rows on their way at a time; blockDim.x chunks by blockDim.y rows per block.
 template <int FMT>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const DequantArgs a) {
   pdl_begin();
-  const int chunks = a.K / 8;
-  const long total = a.rows * chunks;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long)gridDim.x * blockDim.x) {
-    const long row = i / chunks;
-    const int c = (int)(i - row * chunks);
-    float v[8];
-    if (FMT == FMT_FP8) {
-      const uint2 u = *reinterpret_cast<const uint2*>(a.codes + row * a.K + c * 8);
-      const float s = reinterpret_cast<const float*>(a.scales)[row * (a.K / 128) + c / 16];
+  constexpr int PER = FMT == FMT_MXFP4 ? 4 : 2, DEPTH = 4;
+  const int chunks = a.K / 8, words = scale_words(FMT, a.K);
+  const long step = (long)gridDim.y * blockDim.y;
+  for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < chunks; c += gridDim.x * blockDim.x) {
+    const int block = c / PER;
+    for (long row0 = (long)blockIdx.y * blockDim.y + threadIdx.y; row0 < a.rows; row0 += DEPTH * step) {
+      uint2 code[DEPTH];
+      float s[DEPTH];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[e] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)((e < 4 ? u.x : u.y) >> (8 * (e & 3))), __NV_E4M3))) * s;
-    } else {
-      constexpr int PER = FMT == FMT_MXFP4 ? 4 : 2;
-      const uint32_t u = *reinterpret_cast<const uint32_t*>(a.codes + row * (a.K / 2) + c * 4);
-      const long g = row / a.group, scale_row = g * ((a.group + 127) / 128 * 128) + (row - g * a.group);
-      const int block = c / PER;
-      const uint32_t byte = static_cast<const uint8_t*>(a.scales)[scale_word_at(scale_row, block >> 2, scale_words(FMT, a.K)) + (block & 3)];
-      float s;
-      if (FMT == FMT_MXFP4) s = __uint_as_float(byte == 255 ? 0x7fc00000u : byte == 0 ? 1u << 22 : byte << 23);
-      else s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3))) * a.row_scale[row];
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float2 f = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(u >> (8 * p)), __NV_E2M1)));
-        v[2 * p] = f.x * s;
-        v[2 * p + 1] = f.y * s;
+      for (int d = 0; d < DEPTH; ++d) {
+        const long row = row0 + d * step;
+        code[d] = make_uint2(0u, 0u);
+        s[d] = 0.f;
+        if (row < a.rows) {
+          if (FMT == FMT_FP8) {
+            code[d] = *reinterpret_cast<const uint2*>(a.codes + row * a.K + c * 8);
+            s[d] = static_cast<const float*>(a.scales)[row * (a.K / 128) + c / 16];
+          } else {
+            code[d].x = *reinterpret_cast<const uint32_t*>(a.codes + row * (a.K / 2) + c * 4);
+            long scale_row = row;
+            if (a.group != a.rows) {
+              const long g = row / a.group;
+              scale_row = g * ((a.group + 127) / 128 * 128) + (row - g * a.group);
+            }
+            const uint32_t byte = static_cast<const uint8_t*>(a.scales)[scale_word_at(scale_row, block >> 2, words) + (block & 3)];
+            if (FMT == FMT_MXFP4) s[d] = __uint_as_float(byte == 255 ? 0x7fc00000u : byte == 0 ? 1u << 22 : byte << 23);
+            else s[d] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3))) * a.row_scale[row];
+          }
+        }
       }
-    }
-    if (a.f32) {
-      float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * a.K + c * 8);
-      o[0] = make_float4(v[0], v[1], v[2], v[3]);
-      o[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      *reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + row * a.K + c * 8) =
-          make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        const long row = row0 + d * step;
+        if (row >= a.rows) break;
+        float v[8];
+        if (FMT == FMT_FP8) {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((p < 2 ? code[d].x : code[d].y) >> (16 * (p & 1))), __NV_E4M3));
+            const float2 f = __half22float2(h);
+            v[2 * p] = f.x * s[d];
+            v[2 * p + 1] = f.y * s[d];
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const float2 f = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(code[d].x >> (8 * p)), __NV_E2M1)));
+            v[2 * p] = f.x * s[d];
+            v[2 * p + 1] = f.y * s[d];
+          }
+        }
+        if (a.f32) {
+          float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * a.K + c * 8);
+          o[0] = make_float4(v[0], v[1], v[2], v[3]);
+          o[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          *reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + row * a.K + c * 8) =
+              make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+        }
+      }
     }
   }
 }
 
 // Threads per row and chunks per thread: up to two rows per SM a lane per chunk (one round trip); for more, four chunks per lane.
-static void row_threads(int K, long rows, int& tpr, int& nv) {
+static void row_threads(int K, long rows, bool norm, int& tpr, int& nv) {
   const int chunks = K / 8;
-  nv = rows <= 2L * sm_count() ? 1 : 4;
+  nv = rows <= 2L * sm_count() ? 1 : norm ? 2 : 4;
   while (nv < 4 && chunks > 1024 * nv) nv *= 2;
   while (nv > 1 && chunks <= 32 * (nv / 2)) nv /= 2;
   tpr = (chunks + 32 * nv - 1) / (32 * nv) * 32;
 }
 
-template <int FMT, bool NORM>
+template <int FMT, bool NORM, int MODE>
 static int launch_rows(RowsArgs& a, cudaStream_t s) {
   int nv;
-  row_threads(a.K, a.rows, a.tpr, nv);
+  row_threads(a.K, a.rows, NORM, a.tpr, nv);
   if (a.tpr > 1024) return RC_TOO_LARGE;
   const int per = a.tpr >= 256 ? 1 : 256 / a.tpr, threads = per * a.tpr;
   const unsigned grid = (unsigned)((a.rows + per - 1) / per);
   switch (nv) {
-    case 1: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, 1>, grid, threads, 0, s, a);
-    case 2: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, 2>, grid, threads, 0, s, a);
-    default: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, 4>, grid, threads, 0, s, a);
+    case 1: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 1>, grid, threads, 0, s, a);
+    case 2: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 2>, grid, threads, 0, s, a);
+    default: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 4>, grid, threads, 0, s, a);
   }
 }
 
@@ -317,15 +393,20 @@ static int rows_any(RowsArgs& a, int fmt, cudaStream_t s) {
   if (fmt == FMT_NVFP4 && !a.row_scale) return RC_BAD_ARG;
   if (a.gain) {
     switch (fmt) {
-      case FMT_MXFP4: return launch_rows<FMT_MXFP4, true>(a, s);
-      case FMT_NVFP4: return launch_rows<FMT_NVFP4, true>(a, s);
-      case FMT_FP8: return launch_rows<FMT_FP8, true>(a, s);
+      case FMT_MXFP4: return launch_rows<FMT_MXFP4, true, ROWS>(a, s);
+      case FMT_NVFP4: return launch_rows<FMT_NVFP4, true, ROWS>(a, s);
+      case FMT_FP8: return launch_rows<FMT_FP8, true, ROWS>(a, s);
       default: return RC_BAD_ARG;
     }
   }
-  switch (fmt) {
-    case FMT_MXFP4: return launch_rows<FMT_MXFP4, false>(a, s);
-    case FMT_NVFP4: return launch_rows<FMT_NVFP4, false>(a, s);
+  const int mode = a.place.row_of_pair ? GATHER : a.place.place_of_row ? PLACED : ROWS;
+  switch (fmt * 3 + mode) {
+    case FMT_MXFP4 * 3 + ROWS: return launch_rows<FMT_MXFP4, false, ROWS>(a, s);
+    case FMT_MXFP4 * 3 + GATHER: return launch_rows<FMT_MXFP4, false, GATHER>(a, s);
+    case FMT_MXFP4 * 3 + PLACED: return launch_rows<FMT_MXFP4, false, PLACED>(a, s);
+    case FMT_NVFP4 * 3 + ROWS: return launch_rows<FMT_NVFP4, false, ROWS>(a, s);
+    case FMT_NVFP4 * 3 + GATHER: return launch_rows<FMT_NVFP4, false, GATHER>(a, s);
+    case FMT_NVFP4 * 3 + PLACED: return launch_rows<FMT_NVFP4, false, PLACED>(a, s);
     default: return RC_BAD_ARG;
   }
 }
@@ -333,12 +414,16 @@ static int rows_any(RowsArgs& a, int fmt, cudaStream_t s) {
 static int dequantize_any(const DequantArgs& a, int fmt, cudaStream_t s) {
   if (a.rows <= 0 || a.K <= 0) return RC_OK;
   if (a.K % (fmt == FMT_FP8 ? 128 : 32) || !on16(a.codes) || !on16(a.out) || (fmt == FMT_NVFP4 && !a.row_scale)) return RC_BAD_ARG;
-  const long blocks = (a.rows * (a.K / 8) + 255) / 256, most = (long)sm_count() * 16;
-  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+  int x = 32;
+  while (x < 256 && x < a.K / 8) x *= 2;
+  const int y = 256 / x;
+  const long gx = (a.K / 8 + x - 1) / x, want = (a.rows + 4 * y - 1) / (4 * y), most = (16L * sm_count() + gx - 1) / gx;
+  const long gy = want < most ? want : most;
+  const dim3 grid((unsigned)gx, (unsigned)(gy > 65535 ? 65535 : gy)), block(x, y);
   switch (fmt) {
-    case FMT_MXFP4: return launch_overlapped(dequantize_kernel<FMT_MXFP4>, grid, 256, 0, s, a);
-    case FMT_NVFP4: return launch_overlapped(dequantize_kernel<FMT_NVFP4>, grid, 256, 0, s, a);
-    case FMT_FP8: return launch_overlapped(dequantize_kernel<FMT_FP8>, grid, 256, 0, s, a);
+    case FMT_MXFP4: return launch_overlapped(dequantize_kernel<FMT_MXFP4>, grid, block, 0, s, a);
+    case FMT_NVFP4: return launch_overlapped(dequantize_kernel<FMT_NVFP4>, grid, block, 0, s, a);
+    case FMT_FP8: return launch_overlapped(dequantize_kernel<FMT_FP8>, grid, block, 0, s, a);
     default: return RC_BAD_ARG;
   }
 }

@@ -18,7 +18,7 @@ import torch.nn.functional as F
 
 from . import _native as nv
 
-c_int, c_long, c_float = ctypes.c_int, ctypes.c_long, ctypes.c_float
+c_int, c_long = ctypes.c_int, ctypes.c_long
 
 FORMATS = {"mxfp4": 0, "nvfp4": 1, "fp8": 2}
 BLOCK = {"mxfp4": 32, "nvfp4": 16, "fp8": 128}
@@ -76,18 +76,19 @@ class QuantRows:
         self.fmt, self.gated, self.rows, self.cols, self.experts, self.index = fmt, gated, rows, cols, lead[0] if lead else None, index
 
     @classmethod
-    def _on_buffer(cls, buf: torch.Tensor, fmt: str, rows: int, cols: int, experts: int | None = None, gated: bool = False) -> "QuantRows":
-        """Rows that a kernel writes into one allocation (``_sizes``); the three tensors are made when somebody asks for them."""
+    def _empty(cls, fmt: str, rows: int, cols: int, index: int, experts: int | None = None, gated: bool = False) -> "QuantRows":
+        """Rows that a kernel is to write, in one allocation; the three tensors are made when somebody asks for them."""
         q = cls.__new__(cls)
         q._codes = q._scales = q._row = None
-        q._buf, q.fmt, q.gated, q.rows, q.cols, q.experts, q.index = buf, fmt, gated, rows, cols, experts, buf.get_device()
-        n, m, r = _sizes(fmt, rows, cols, experts or 1)
+        size, scales, row = _layout(fmt, rows, cols, experts or 1)
+        q._buf = buf = torch.empty(size, dtype=torch.uint8, device=_device(index))
+        q.fmt, q.gated, q.rows, q.cols, q.experts, q.index = fmt, gated, rows, cols, experts, index
         p = buf.data_ptr()
-        q._at = (p, p + n, p + n + m if r else None)
+        q._at = (p, p + scales, p + row if fmt == "nvfp4" else None)
         return q
 
     def _part(self, which: int) -> torch.Tensor:
-        n, m, r = _sizes(self.fmt, self.rows, self.cols, self.experts or 1)
+        _, scales, row = _layout(self.fmt, self.rows, self.cols, self.experts or 1)
         lead = () if self.experts is None else (self.experts,)
         if which == 0:
             shape = (*lead, self.rows, self.cols if self.fmt == "fp8" else self.cols // 2)
@@ -95,9 +96,9 @@ class QuantRows:
         if which == 1:
             shape = (*lead, *scale_shape(self.fmt, self.rows, self.cols))
             size = math.prod(shape) * (4 if self.fmt == "fp8" else 1)
-            part = self._buf[n:n + size]
+            part = self._buf[scales:scales + size]
             return (part.view(torch.float32) if self.fmt == "fp8" else part).view(shape)
-        return self._buf[n + m:n + m + 4 * self.rows * (self.experts or 1)].view(torch.float32).view(*lead, self.rows)
+        return self._buf[row:row + 4 * self.rows * (self.experts or 1)].view(torch.float32).view(*lead, self.rows)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -140,17 +141,15 @@ class QuantRows:
         return f"QuantRows({self.fmt}, {list(self.shape)}{', gated' if self.gated else ''}, {self.device})"
 
 
-def _sizes(fmt: str, rows: int, cols: int, experts: int = 1) -> tuple[int, int, int]:
-    """Bytes of codes, scales and row factors in one allocation, each a multiple of 256."""
+@functools.lru_cache(maxsize=4096)
+def _layout(fmt: str, rows: int, cols: int, experts: int = 1) -> tuple[int, int, int]:
+    """Bytes of one allocation for codes, scales and row factors, and where the scales and the factors begin (each on 256 bytes)."""
     if fmt == "fp8":
         n, m, r = rows * cols, rows * cols // 32, 0
     else:
         n, m, r = rows * cols // 2, -(-rows // 128) * scale_words(fmt, cols) * 512, 4 * rows if fmt == "nvfp4" else 0
-    return tuple(-(-experts * v // 256) * 256 for v in (n, m, r))
-
-
-def _allocate(fmt: str, rows: int, cols: int, index: int, experts: int = 1) -> torch.Tensor:
-    return torch.empty(sum(_sizes(fmt, rows, cols, experts)), dtype=torch.uint8, device=_device(index))
+    n, m, r = (-(-experts * v // 256) * 256 for v in (n, m, r))
+    return n + m + r, n, n + m
 
 
 @functools.lru_cache(maxsize=None)
@@ -158,34 +157,24 @@ def _device(index: int) -> torch.device:
     return torch.device("cuda", index)
 
 
-class _on:
-    """Makes a device the current one where it is not: kernels go to the current device's stream."""
+@functools.lru_cache(maxsize=None)
+def _status(index: int) -> int:
+    return nv.status_word(_device(index)).data_ptr()
 
-    __slots__ = ("idx", "prev")
 
-    def __init__(self, index: int):
-        self.idx = index
-
-    def __enter__(self):
-        self.prev = torch._C._cuda_getDevice()
-        if self.prev != self.idx:
-            torch._C._cuda_setDevice(self.idx)
-        return torch._C._cuda_getCurrentRawStream(self.idx)
-
-    def __exit__(self, *exc):
-        if self.prev != self.idx:
-            torch._C._cuda_setDevice(self.prev)
+_current, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 _KINDS = {"p": ctypes.c_void_p, "l": ctypes.c_long, "i": ctypes.c_int, "f": ctypes.c_float}
 _ENTRIES = {"omni_lowbit_rows": "pllilipl" "pfplpl" "pppp", "omni_lowbit_dequantize": "ppplilii" "pp",
-            "omni_lowbit_linear": "plppp" "pppplliiii" "pipllpliipp", "omni_lowbit_experts": "plilii" "pppp" "pppp" "iipp"}
+            "omni_moe_plan_tiles": "piiiiiipppppp", "omni_moe_combine": "pppiiiplplp",
+            "omni_lowbit_linear": "plppp" "pppplliiii" "pipllpliipp", "omni_lowbit_experts": "plilii" "pppp" "pppp" "iipppp"}
 
 
 @functools.lru_cache(maxsize=None)
 def _entry(name: str):
     """An entry point that takes plain Python numbers: converting them by declared types is half the cost of wrapping each."""
-    lib = nv.lib("lowbit")
+    lib = nv.lib("moe" if name.startswith("omni_moe") else "lowbit")
     raw = getattr(lib._cdll, name)
     raw.argtypes = [_KINDS[k] for k in _ENTRIES[name]]
     return getattr(lib, name)
@@ -274,14 +263,21 @@ def _swiglu_torch(y):
 
 # ------------------------------------------------------------------ quantisation
 def _rows(x, fmt, *, residual=None, gain=None, eps=0.0, total=None, normed=None, experts=None, gated=False) -> QuantRows:
+    index = x.get_device()
+    if _current() != index:                       # kernels go to the current device's stream
+        with torch.cuda.device(index):
+            return _rows(x, fmt, residual=residual, gain=gain, eps=eps, total=total, normed=normed, experts=experts, gated=gated)
     rows, cols = x.shape
     per = rows // experts if experts else rows
-    q = QuantRows._on_buffer(_allocate(fmt, per, cols, x.get_device(), experts or 1), fmt, per, cols, experts, gated)
-    at = q._at
-    at_ld = lambda t: (None, 0) if t is None else (t.data_ptr(), t.stride(0))
-    with _on(q.index) as stream:
-        rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], *at_ld(residual), None if gain is None else gain.data_ptr(), eps,
-                                        *at_ld(total), *at_ld(normed), at[0], at[1], at[2], stream)
+    q = QuantRows._empty(fmt, per, cols, index, experts, gated)
+    codes, scales, row = q._at
+    if gain is None:
+        rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], None, 0, None, 0.0, None, 0, None, 0, codes, scales, row,
+                                        _stream(index))
+    else:
+        at = lambda t: (None, 0) if t is None else (t.data_ptr(), t.stride(0))
+        rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], *at(residual), gain.data_ptr(), eps, *at(total), *at(normed),
+                                        codes, scales, row, _stream(index))
     if rc:
         nv.check_rc(rc, "omni_lowbit_rows")
     return q
@@ -329,11 +325,13 @@ def dequantize(q: QuantRows, dtype: torch.dtype = torch.bfloat16) -> torch.Tenso
         raise ValueError(f"dequantize: bf16 or fp32, got {dtype}")
     if not q.is_cuda:
         return _values_torch(q).to(dtype)
+    if _current() != q.index:
+        with torch.cuda.device(q.index):
+            return dequantize(q, dtype)
     out = torch.empty(q.shape, dtype=dtype, device=_device(q.index))
-    at = q._at
-    with _on(q.index) as stream:
-        rc = _entry("omni_lowbit_dequantize")(at[0], at[1], at[2], q.rows * (q.experts or 1), q.cols, q.rows, FORMATS[q.fmt], int(dtype is torch.float32),
-                                              out.data_ptr(), stream)
+    codes, scales, row = q._at
+    rc = _entry("omni_lowbit_dequantize")(codes, scales, row, q.rows * (q.experts or 1), q.cols, q.rows, FORMATS[q.fmt], int(dtype is torch.float32),
+                                          out.data_ptr(), _stream(q.index))
     if rc:
         nv.check_rc(rc, "omni_lowbit_dequantize")
     return out
@@ -390,14 +388,15 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
 
     x: bf16 [.., K], quantised here in w's format, or ``QuantRows`` of that format.  bias [N], residual [.., N] (may be ``out``), gate [B, N] where the
     rows split evenly into B batches."""
-    if not isinstance(w, QuantRows) or w.fmt not in ("mxfp4", "nvfp4") or w.experts is not None:
+    if not isinstance(w, QuantRows) or w.fmt == "fp8" or w.experts is not None:
         raise ValueError(f"w: a packed 4-bit matrix expected, got {w!r}")
+    fmt, gated, N = w.fmt, w.gated, w.rows // 2 if w.gated else w.rows
     if act not in ACT:
         raise ValueError(f"act {act!r}: None, 'gelu_tanh' or 'silu'")
-    if w.gated and not (bias is None and act is None and residual is None and gate is None):
+    if gated and not (bias is None and act is None and residual is None and gate is None):
         raise ValueError("a gated weight takes no bias, activation, gate or residual")
     if isinstance(x, QuantRows):
-        if x.fmt != w.fmt or x.experts is not None or x.gated:
+        if x.fmt != fmt or x.experts is not None or x.gated:
             raise ValueError(f"x is {x!r}, w {w!r}: rows of the same format expected")
         lead, q, M, cols, index = (x.rows,), x, x.rows, x.cols, x.index
     else:
@@ -405,10 +404,12 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
         M = lead[0] if len(lead) == 1 else math.prod(lead)
     if cols != w.cols or index != w.index:
         raise ValueError(f"x {list(x.shape)} on {x.device} does not fit w {w!r}")
-    N = w.out_features
-    for name, t, shape in (("bias", bias, (w.rows,)), ("residual", residual, (*lead, N)), ("out", out, (*lead, N))):
-        if t is not None and (t.shape != shape or t.dtype is not torch.bfloat16 or t.get_device() != index):
-            raise ValueError(f"{name}: bf16 {tuple(shape)} on {w.device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if bias is not None:
+        _check_operand("bias", bias, (w.rows,), index)
+    if residual is not None:
+        _check_operand("residual", residual, (*lead, N), index)
+    if out is not None:
+        _check_operand("out", out, (*lead, N), index)
     if gate is not None and (gate.dim() != 2 or gate.shape[1] != N or gate.shape[0] == 0 or M % gate.shape[0] or gate.stride(1) != 1
                              or gate.dtype is not torch.bfloat16 or gate.get_device() != index):
         raise ValueError(f"gate: bf16 [B, {N}] with B dividing {M} rows expected, got {gate.dtype} {tuple(gate.shape)}")
@@ -425,35 +426,57 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
             y = y + residual.reshape(M, N).float()
         y = y.to(torch.bfloat16).view(*lead, N)
         return y if out is None else out.copy_(y)
+    if _current() != index:
+        with torch.cuda.device(index):
+            return linear(x, w, bias, act, residual, gate, out, force_tile, force_split)
     raw, ldx = None, 0
     if q is None:
-        _check_cols(w.fmt, cols)
+        _check_cols(fmt, cols)
         x = _rows16(x, "x")
         raw, ldx = x.data_ptr(), x.stride(0)
-        q = QuantRows._on_buffer(_allocate(w.fmt, M, cols, index), w.fmt, M, cols)
+        q = QuantRows._empty(fmt, M, cols, index)
+        nv.count_launches(1)
     if out is None:
         o2 = torch.empty(M, N, dtype=torch.bfloat16, device=_device(index))
         out = o2 if len(lead) == 1 else o2.view(*lead, N)
     else:
         o2 = out if out.dim() == 2 else out.view(M, N)
-    r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(M, N)
-    if N > 1 and (o2.stride(1) != 1 or (r2 is not None and r2.stride(1) != 1)):
+    ldo, yp = o2.stride(), o2.data_ptr()
+    rp = bp = gp = None
+    ldr, lds, per = (0, 1), 0, 0
+    if residual is not None:
+        r2 = residual if residual.dim() == 2 else residual.reshape(M, N)
+        rp, ldr = r2.data_ptr(), r2.stride()
+    if N > 1 and (ldo[1] != 1 or ldr[1] != 1):
         raise ValueError("out and residual: the last dimension must be contiguous")
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
-    B = 0 if gate is None else gate.shape[0]
-    (xc, xs, xf), (wc, ws, wf) = q._at, w._at
-    with _on(index) as stream:
-        rc = _entry("omni_lowbit_linear")(
-            raw, ldx, xc, xs, xf, wc, ws, wf, o2.data_ptr(), o2.stride(0), M, w.rows, cols, FORMATS[w.fmt], int(w.gated),
-            None if bias is None else bias.data_ptr(), ACT[act], None if gate is None else gate.data_ptr(), gate.stride(0) if B > 1 else 0,
-            max(1, M // B) if B else 0, None if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0), force_tile, force_split,
-            nv.status_word(o2.device).data_ptr(), stream)
+    if bias is not None:
+        bias = bias if bias.is_contiguous() else bias.contiguous()
+        bp = bias.data_ptr()
+    if gate is not None:
+        gp, B = gate.data_ptr(), gate.shape[0]
+        lds, per = gate.stride(0) if B > 1 else 0, max(1, M // B)
+    rc = _entry("omni_lowbit_linear")(raw, ldx, *q._at, *w._at, yp, ldo[0], M, w.rows, cols, FORMATS[fmt], int(gated), bp, ACT[act], gp, lds, per, rp, ldr[0],
+                                      force_tile, force_split, _status(index), _stream(index))
     if rc:
         nv.check_rc(rc, "omni_lowbit_linear")
-    if raw is not None:
-        nv.count_launches(1)
     return out
+
+
+def _check_operand(name: str, t: torch.Tensor, shape: tuple, index: int) -> None:
+    if t.shape != shape or t.dtype is not torch.bfloat16 or t.get_device() != index:
+        raise ValueError(f"{name}: bf16 {tuple(shape)} on {'cpu' if index < 0 else _device(index)} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+@functools.lru_cache(maxsize=1024)
+def _expert_layout(fmt: str, pairs: int, max_tiles: int, scale_rows: int, D: int, Fd: int) -> tuple[int, list[int]]:
+    """Bytes of the workspace of ``experts`` and where its parts begin: pairs' rows, three tables of tiles, the number of rows, the rows' places, what lies between the
+    products, the results; codes, scales and factors of the rows of either product."""
+    at, end = [], 0
+    for size in (4 * pairs, 4 * max_tiles, 4 * max_tiles, 4 * max_tiles, 4, 4 * pairs, 2 * pairs * Fd, 2 * pairs * D,
+                 *(v for cols in (D, Fd) for v in (pairs * cols // 2, scale_rows * 4 * scale_words(fmt, cols), 4 * pairs))):
+        at.append(end)
+        end += -(-size // 256) * 256
+    return end, at
 
 
 class _ExpertOperand(ctypes.Structure):
@@ -504,6 +527,9 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
         out = torch.empty(T, D, dtype=x.dtype, device=x.device)
     if T == 0:
         return out
+    if _current() != up.index:
+        with torch.cuda.device(up.index):
+            return experts(x, ids, weights, up, down, residual, out)
     x2, ids, weights = _rows16(x, "x"), ids.contiguous(), weights.contiguous()
     res = None if residual is None else _rows16(residual, "residual")
     o2 = out if out.stride(1) == 1 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0 else torch.empty_like(out, memory_format=torch.contiguous_format)
@@ -512,24 +538,19 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
     max_tiles = min(E, pairs) + pairs // tile
     scale_rows = max_tiles * (256 if tile > 128 else 128)
     # one workspace: the plan, both products' rows, what is between them, the experts' results
-    parts, at = [], 0
-    for size in (4 * pairs, 4 * max_tiles, 4 * max_tiles, 4 * max_tiles, 4, pairs * Fd * 2, pairs * D * 2,
-                 *(v for cols in (D, Fd) for v in (pairs * cols // 2, _sizes(fmt, scale_rows, cols)[1], 4 * pairs))):
-        parts.append(at)
-        at += -(-size // 256) * 256
-    work = torch.empty(at, dtype=torch.uint8, device=dev)
-    row_of_pair, te, tr, tn, n_rows, h, y, *ops = (work.data_ptr() + p for p in parts)
-    half = [_ExpertOperand(*ops[3 * i:3 * i + 2], ops[3 * i + 2] if fmt == "nvfp4" else None, *w._at, w.rows, w.cols) for i, w in enumerate((up, down))]
-    moe = nv.lib("moe")
-    p = ctypes.c_void_p
-    with _on(up.index) as stream:
-        status = nv.status_word(dev).data_ptr()
-        if nv.bounds_check_enabled():
-            moe.omni_moe_set_bounds(c_long(pairs), p(status))
-        nv.check_rc(moe.omni_moe_plan_tiles(p(ids.data_ptr()), c_int(pairs), c_int(E), c_int(0), c_int(E), c_int(tile), c_int(max_tiles), p(row_of_pair), p(te), p(tr),
-                                            p(tn), p(n_rows), p(stream)), "omni_moe_plan_tiles")
-        nv.check_rc(_entry("omni_lowbit_experts")(x2.data_ptr(), x2.stride(0), k, pairs, E, FORMATS[fmt], ctypes.addressof(half[0]), ctypes.addressof(half[1]), h, y,
-                                                  row_of_pair, te, tr, tn, max_tiles, tile, status, stream), "omni_lowbit_experts")
-        nv.check_rc(moe.omni_moe_combine(p(y), p(row_of_pair), p(weights.data_ptr()), c_int(T), c_int(k), c_int(D), p(0 if res is None else res.data_ptr()),
-                                         c_long(0 if res is None else res.stride(0)), p(o2.data_ptr()), c_long(o2.stride(0)), p(stream)), "omni_moe_combine")
+    size, at = _expert_layout(fmt, pairs, max_tiles, scale_rows, D, Fd)
+    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    base = work.data_ptr()
+    row_of_pair, te, tr, tn, n_rows, place, h, y, *ops = [base + v for v in at]
+    up_op, down_op = (_ExpertOperand(*ops[i:i + 2], ops[i + 2] if fmt == "nvfp4" else None, *w._at, w.rows, w.cols) for i, w in ((0, up), (3, down)))
+    status, stream = _status(up.index), _stream(up.index)
+    if nv.bounds_check_enabled():
+        nv.lib("moe").omni_moe_set_bounds(c_long(pairs), ctypes.c_void_p(status))
+    rc = _entry("omni_moe_plan_tiles")(ids.data_ptr(), pairs, E, 0, E, tile, max_tiles, row_of_pair, te, tr, tn, n_rows, stream)
+    rc = rc or _entry("omni_lowbit_experts")(x2.data_ptr(), x2.stride(0), k, pairs, E, FORMATS[fmt], ctypes.addressof(up_op), ctypes.addressof(down_op), h, y, row_of_pair,
+                                             te, tr, tn, max_tiles, tile, n_rows, place, status, stream)
+    rc = rc or _entry("omni_moe_combine")(y, row_of_pair, weights.data_ptr(), T, k, D, None if res is None else res.data_ptr(), 0 if res is None else res.stride(0),
+                                          o2.data_ptr(), o2.stride(0), stream)
+    if rc:
+        nv.check_rc(rc, "experts")
     return out if o2 is out else out.copy_(o2)
