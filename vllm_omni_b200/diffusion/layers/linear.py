@@ -2,8 +2,8 @@
 
 The layer keeps the HF/diffusers parameter names (``weight`` [out, in], ``bias`` [out]) so
 checkpoints load unchanged.  Optional LoRA deltas (``y += scale * (x A^T) B^T``, the
-semantics of vllm_omni/diffusion/lora/layers/base_linear.py) and fp8 block-scaled weights
-attach to the same object.
+semantics of vllm_omni/diffusion/lora/layers/base_linear.py), fp8 block-scaled weights and 4-bit
+weights attach to the same object.
 """
 from __future__ import annotations
 
@@ -26,6 +26,7 @@ class FusedLinear(nn.Module):
         self.init_std = init_std
         self.lora = None      # set by the LoRA manager: list of (A [r, in], B [out, r], scale)
         self.fp8 = None       # set by the fp8 quantiser: (w_fp8, w_scale) block-scaled weights
+        self.fp4 = None       # set by ``to_fp4``: packed 4-bit weights (ops/lowbit.py)
         self.reset_parameters()
 
     @torch.no_grad()
@@ -36,7 +37,47 @@ class FusedLinear(nn.Module):
         if self.bias is not None:
             self.bias.zero_()
 
+    @property
+    def quantized(self) -> bool:
+        """The bf16 weight is gone: only the layer itself can compute its product."""
+        return self.fp8 is not None or self.fp4 is not None
+
+    @torch.no_grad()
+    def to_fp4(self, fmt: str, gated: bool = False) -> None:
+        """Replaces the weight by its ``mxfp4`` or ``nvfp4`` form.  ``gated``: its rows are [gate | lift], for layers that are used through ``swiglu``."""
+        from ...ops import lowbit
+        self.fp4 = lowbit.pack_weight(self.weight.data.to(torch.bfloat16), fmt, gated=gated)
+        self.weight.data = torch.empty(0, dtype=self.weight.dtype, device=self.weight.device)
+
+    def _forward_fp4(self, x, act, residual, gate, out, kw):
+        """As the bf16 layer; rows that peers are to receive or send cannot be quantised on the way and are refused."""
+        from ...ops import lowbit
+        if any(kw.get(k) is not None for k in ("scatter", "row_scatter", "sync")):
+            raise ValueError("4-bit weights: no fused exchange with peers (scatter, row_scatter, sync)")
+        rows = x.view(-1, x.shape[-1]) if isinstance(x, torch.Tensor) and x.dim() != 2 and x.is_contiguous() else x
+        lead = (x.rows,) if isinstance(x, lowbit.QuantRows) else tuple(x.shape[:-1])
+        bf16 = isinstance(x, lowbit.QuantRows) or x.dtype == torch.bfloat16
+        if not bf16:
+            rows = rows.to(torch.bfloat16)             # the CPU's fp32 models: products of 4-bit operands are bf16
+        N = self.out_features
+        if act in lowbit.ACT and bf16 and not self.lora and not self.fp4.gated:
+            return lowbit.linear(x, self.fp4, self.bias, act, residual=residual, gate=gate, out=out)
+        w = self.fp4
+        y = lowbit.linear(rows, lowbit.QuantRows(w.codes, w.scales, w.fmt, row_scale=w.row_scale) if w.gated else w)
+        if w.gated:                                    # asked for as [gate | lift] rows
+            y = y.unflatten(-1, (-1, 2, 8)).transpose(-3, -2).flatten(-3)
+        y = y.reshape(*lead, N)
+        if not bf16:
+            y = y.to(x.dtype)
+        if self.bias is not None:
+            y = y + self.bias
+        for (A, B, scale) in self.lora or ():
+            y = y + scale * gemm.linear(gemm.linear(x, A), B)
+        return _epilogue(y, act, residual, gate, out, kw.get("coef", (0.0, 0.0)))
+
     def forward(self, x, act=None, residual=None, gate=None, out=None, **kw):
+        if self.fp4 is not None:
+            return self._forward_fp4(x, act, residual, gate, out, kw)
         if self.fp8 is not None:
             from ..quantization.fp8 import fp8_linear
             y = fp8_linear(x, self.fp8, self.bias, act=act, residual=residual, gate=gate, out=out, **kw)
@@ -55,7 +96,13 @@ class FusedLinear(nn.Module):
         hooks, a forward of one's own."""
         hooked = self._forward_hooks or self._forward_pre_hooks or self._backward_hooks or self._backward_pre_hooks or _has_any_global_hook()
         if self.fp8 is None and not self.lora and self.bias is None and not hooked and getattr(self.forward, "__func__", None) is FusedLinear.forward:
-            return gemm.linear_swiglu(x, self.weight)
+            if self.fp4 is None:
+                return gemm.linear_swiglu(x, self.weight)
+            if self.fp4.gated:
+                from ...ops import lowbit
+                rows = x if isinstance(x, lowbit.QuantRows) or x.dtype == torch.bfloat16 else x.to(torch.bfloat16)
+                y = lowbit.linear(rows, self.fp4)
+                return y if rows is x else y.to(x.dtype)
         from ...ops import fused
         return fused.silu_mul(self(x))
 

@@ -33,10 +33,10 @@ from ...layers.linear import FusedLinear
 
 def _plain_pair(blk) -> bool:
     """True when the image and text linears of a block can share launches: plain bf16 weights
-    (no LoRA delta, no fp8 state) on both streams."""
+    (no LoRA delta, no quantised weights) on both streams."""
     for sp in (blk.img, blk.txt):
         for lin in (sp.to_qkv, sp.to_out, sp.mlp_up, sp.mlp_down):
-            if lin is None or lin.lora or lin.fp8 is not None:
+            if lin is None or lin.lora or lin.quantized:
                 return False
     return True
 

@@ -1,1 +1,1 @@
-from .fp8 import DiffusionFp8Config, fp8_linear, quantize_pipeline, quantize_weight_blockwise  # noqa: F401
+from .fp8 import DiffusionFp8Config, fp8_linear, quantize_layer, quantize_pipeline, quantize_weight_blockwise  # noqa: F401

@@ -18,6 +18,7 @@ import torch
 
 from ...ops import _native as nv
 from ...ops import gemm
+from ...ops.lowbit import QuantRows, dequantize
 
 FP8_MAX = 448.0
 
@@ -70,11 +71,14 @@ def fp8_linear_reference(x, w8, sw, bias=None, act=None, residual=None, gate=Non
     x2 = x.reshape(-1, K)
     q, sa = quantize_rows_reference(x2)
     xd = (q.float().view(x2.shape[0], K // 128, 128) * sa[..., None]).view_as(x2)
-    N = w8.shape[0]
-    wd = w8.float().view(N, K // 128, 128) * sw.repeat_interleave(128, 0)[:N, :, None]
-    y = xd @ wd.view(N, K).t()
-    y = y.reshape(*x.shape[:-1], N)
+    y = xd @ _weight_values(w8, sw).t()
+    y = y.reshape(*x.shape[:-1], w8.shape[0])
     return _epi(y, bias, act, residual, gate)
+
+
+def _weight_values(w8, sw):
+    N, K = w8.shape
+    return (w8.float().view(N, K // 128, 128) * sw.repeat_interleave(128, 0)[:N, :, None]).view(N, K)
 
 
 def _epi(y, bias, act, residual, gate):
@@ -94,24 +98,34 @@ def _epi(y, bias, act, residual, gate):
 
 
 def fp8_linear(x, fp8_state, bias=None, act=None, residual=None, gate=None, out=None, **_):
+    """``x``: rows of bf16, quantised here, or fp8 ``QuantRows`` that a norm left (ops/lowbit.py)."""
     w8, sw = fp8_state
     K, N = x.shape[-1], w8.shape[0]
+    ready = isinstance(x, QuantRows)
+    if ready and (x.fmt != "fp8" or K != w8.shape[1]):
+        raise ValueError(f"fp8 layer of {tuple(w8.shape)}: rows {x!r}")
     if not x.is_cuda:
-        y = fp8_linear_reference(x, w8, sw, bias, act, residual, gate).to(x.dtype)
+        if ready:
+            y = _epi(dequantize(x, torch.float32) @ _weight_values(w8, sw).t(), bias, act, residual, gate).to(torch.bfloat16)
+        else:
+            y = fp8_linear_reference(x, w8, sw, bias, act, residual, gate).to(x.dtype)
         if out is not None:
             out.copy_(y.reshape(out.shape))
             return out
         return y
-    x2 = x.reshape(-1, K)
-    M = x2.shape[0]
     lib = nv.lib("gemm_fp8_sm100")
-    xq = torch.empty(M, K, dtype=torch.uint8, device=x.device)
-    sa = torch.empty(M, K // 128, dtype=torch.float32, device=x.device)
-    nv.check_rc(lib.omni_quant_fp8_rows(nv.ptr(x2), ctypes.c_long(x2.stride(0)), nv.ptr(xq), ctypes.c_long(K), nv.ptr(sa),
-                                        ctypes.c_int(K // 128), ctypes.c_int(M), ctypes.c_int(K), nv.stream_ptr()),
-                "omni_quant_fp8_rows")
+    if ready:
+        M, xq, sa = x.rows, x.codes, x.scales
+    else:
+        x2 = x.reshape(-1, K)
+        M = x2.shape[0]
+        xq = torch.empty(M, K, dtype=torch.uint8, device=x.device)
+        sa = torch.empty(M, K // 128, dtype=torch.float32, device=x.device)
+        nv.check_rc(lib.omni_quant_fp8_rows(nv.ptr(x2), ctypes.c_long(x2.stride(0)), nv.ptr(xq), ctypes.c_long(K), nv.ptr(sa),
+                                            ctypes.c_int(K // 128), ctypes.c_int(M), ctypes.c_int(K), nv.stream_ptr()),
+                    "omni_quant_fp8_rows")
     if out is None:
-        out = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+        out = torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16 if ready else x.dtype, device=x.device)
     o2 = out.view(-1, N)
     res2 = residual.reshape(-1, N) if residual is not None else None
     gs, rpb = 0, 0
@@ -128,26 +142,39 @@ def fp8_linear(x, fp8_state, bias=None, act=None, residual=None, gate=None, out=
     return out
 
 
+def quantize_layer(m, fmt: str, gated: bool = False) -> None:
+    """Replaces the weight of a ``FusedLinear`` by its ``fp8``, ``mxfp4`` or ``nvfp4`` form (``gated``: see ``FusedLinear.to_fp4``)."""
+    if fmt in ("mxfp4", "nvfp4"):
+        m.to_fp4(fmt, gated=gated)
+        return
+    w8, sw = quantize_weight_blockwise(m.weight.data)
+    m.fp8 = (w8.view(torch.uint8) if w8.is_cuda else w8, sw)
+    m.weight.data = torch.empty(0, dtype=m.weight.dtype, device=m.weight.device)
+
+
 def quantize_pipeline(pipe, od_config) -> int:
-    """Quantise every eligible ``FusedLinear`` of the pipeline's transformer in place; returns
-    the number of layers converted."""
+    """Quantise every eligible ``FusedLinear`` of the pipeline's transformer in place (``quantization``: ``fp8``, or 4 bits as ``mxfp4`` /
+    ``nvfp4``, which take the same ``ignored_layers`` and ``min_features``); returns the number of layers converted."""
     from ..layers.linear import FusedLinear
-    qc = od_config.quantization_config
+    qc, fmt = od_config.quantization_config, od_config.quantization
     cfg = qc if isinstance(qc, DiffusionFp8Config) else DiffusionFp8Config.from_dict(qc if isinstance(qc, dict) else None)
-    if od_config.quantization not in ("fp8",):
-        raise ValueError(f"unsupported quantization {od_config.quantization!r}")
+    if fmt not in ("fp8", "mxfp4", "nvfp4"):
+        raise ValueError(f"unsupported quantization {fmt!r}")
+    if fmt != "fp8":
+        par = getattr(od_config, "parallel_config", None)
+        if par is not None and any(getattr(par, k, 1) > 1 for k in ("tensor_parallel_size", "ulysses_degree", "ring_degree")):
+            raise ValueError(f"quantization={fmt!r}: not with tensor or sequence parallelism, whose layers exchange bf16 rows in their products")
+    step = 128 if fmt == "fp8" else 32
     n = 0
     for name, m in pipe.transformer.named_modules():
         if not isinstance(m, FusedLinear):
             continue
-        if m.in_features % 128 or min(m.in_features, m.out_features) < cfg.min_features:
+        if m.in_features % step or min(m.in_features, m.out_features) < cfg.min_features:
             continue
         if any(fnmatch.fnmatch(name, pat) for pat in cfg.ignored_layers):
             continue
         if name in ("mod", "norm_out", "proj_out", "img_in", "txt_in") or name.startswith("time_embed"):
             continue
-        w8, sw = quantize_weight_blockwise(m.weight.data)
-        m.fp8 = (w8.view(torch.uint8) if w8.is_cuda else w8, sw)
-        m.weight.data = torch.empty(0, dtype=m.weight.dtype, device=m.weight.device)
+        quantize_layer(m, fmt)
         n += 1
     return n

@@ -44,7 +44,7 @@ def make_serve_parser(sub=None) -> argparse.ArgumentParser:
     p.add_argument("--flow-shift", type=float, default=None)
     p.add_argument("--default-sampling-params", type=json.loads, default=None, help="JSON dict")
     p.add_argument("--max-generated-image-size", type=int, default=None)
-    p.add_argument("--quantization", default=None, choices=[None, "fp8"])
+    p.add_argument("--quantization", default=None, choices=[None, "fp8", "mxfp4", "nvfp4"])
     p.add_argument("--enforce-eager", action="store_true")
     p.add_argument("--dtype", default="bfloat16")
     p.add_argument("--lora-path", default=None)

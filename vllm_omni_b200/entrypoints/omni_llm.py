@@ -56,6 +56,7 @@ class OmniEngineArgs:
     enable_expert_parallel: bool = False
     distributed_executor_backend: str | None = None
     load_format: str = "auto"
+    quantization: str | None = None       # weights of the stage's decoder after loading: fp8, mxfp4 or nvfp4
     async_scheduling: bool = False
     model_overrides: dict = field(default_factory=dict)     # e.g. {"tiny": True} for tests
 
@@ -121,6 +122,13 @@ class OmniLLM:
                     n += self.model.load_auxiliary(model)
                 logger.info("stage %d (%s): loaded %d tensors", stage_id, a.model_stage, n)
         self.model.eval()
+        if a.quantization:
+            dec = getattr(self.model, "decoder", None)
+            if dec is None or not hasattr(dec, "quantize"):
+                raise NotImplementedError(f"stage model {type(self.model).__name__} ({a.model_stage}) has no decoder whose weights can be quantised")
+            if tp > 1:
+                raise NotImplementedError("quantization needs tensor_parallel_size: 1 for this stage")
+            logger.info("stage %d (%s): %d matrices as %s", stage_id, a.model_stage, dec.quantize(a.quantization), a.quantization)
         if tp_group is not None:
             dec = getattr(self.model, "decoder", None)
             if dec is None or not hasattr(dec, "enable_tensor_parallel"):

@@ -20,9 +20,9 @@ import torch
 from torch import nn
 
 from ..diffusion.layers.linear import FusedLinear
-from ..ops import fused, kv_cache as KC
+from ..ops import fused, kv_cache as KC, lowbit
 from ..ops.attention import attention
-from ..ops.moe import MoEScratch, MoEWorkspace, moe_forward
+from ..ops.moe import MoEScratch, MoEWorkspace, moe_forward, route
 from ..ops.step_inputs import token_rows
 
 
@@ -163,6 +163,7 @@ class DecoderLayer(nn.Module):
             self.w2 = nn.Parameter(torch.empty(E, D, F_, dtype=dtype, device=device).normal_(0, 0.02),
                                    requires_grad=False)
             self.moe_ws = MoEWorkspace(moe_scratch)
+            self.w13_fp4 = self.w2_fp4 = None          # packed 4-bit experts, in place of w13 / w2
             Fs = cfg.shared_expert_intermediate_size
             if Fs:
                 self.shared_gate_up = FusedLinear(D, 2 * Fs, bias=False, dtype=dtype, device=device)
@@ -193,6 +194,55 @@ class QwenDecoderModel(nn.Module):
         self.tp_group = None          # tensor-parallel group: heads and MLP columns sharded
         self.tp_reduce = None
         self.local_heads = (cfg.num_attention_heads, cfg.num_key_value_heads)   # (q, kv) heads on this rank
+        self.quantization = None      # format of the layers' weights once ``quantize`` replaced them
+
+    @torch.no_grad()
+    def quantize(self, fmt: str) -> int:
+        """Weights of the layers in low precision, after loading: attention and MLP projections as ``fp8`` (block-scaled e4m3), ``mxfp4`` or ``nvfp4``, the
+        experts of a mixture in 4 bits with the latter two; embeddings, norms, routers and the LM head stay.  Norms then write quantised rows
+        (``rms_norm_quantize``) where nothing else reads them.  Returns the number of matrices converted."""
+        from ..diffusion.quantization.fp8 import quantize_layer
+        cfg = self.cfg
+        if fmt not in ("fp8", "mxfp4", "nvfp4"):
+            raise ValueError(f"unsupported quantization {fmt!r}: fp8, mxfp4 or nvfp4")
+        if self.quantization is not None:
+            raise ValueError(f"already quantised as {self.quantization}")
+        if self.tp_group is not None or self.ep_group is not None:
+            raise NotImplementedError("quantised weights with tensor or expert parallelism")
+        step = 128 if fmt == "fp8" else 32
+        experts = bool(cfg.num_experts) and fmt != "fp8"
+        widths = {"hidden_size": cfg.hidden_size, "num_attention_heads * head_dim": cfg.num_attention_heads * cfg.head_dim}
+        if not cfg.num_experts:
+            widths["intermediate_size"] = cfg.intermediate_size
+        if experts:
+            widths["moe_intermediate_size"] = cfg.moe_intermediate_size
+        if cfg.num_experts and cfg.shared_expert_intermediate_size:
+            widths["shared_expert_intermediate_size"] = cfg.shared_expert_intermediate_size
+        bad = [f"{k} ({v})" for k, v in widths.items() if v % step]
+        if bad:
+            raise ValueError(f"quantization={fmt!r} needs widths that are multiples of {step}: {', '.join(bad)}")
+        n = 0
+        for layer in self.layers:
+            names = ["qkv_proj", "o_proj"] + (["gate_up", "down"] if not cfg.num_experts else
+                                              ["shared_gate_up", "shared_down"] if cfg.shared_expert_intermediate_size else [])
+            for name in names:
+                quantize_layer(getattr(layer, name), fmt, gated=name == "gate_up")
+                n += 1
+            if experts:
+                layer.w13_fp4 = lowbit.pack_weight(layer.w13.data.to(torch.bfloat16), fmt, gated=True)
+                layer.w2_fp4 = lowbit.pack_weight(layer.w2.data.to(torch.bfloat16), fmt)
+                for p in (layer.w13, layer.w2):
+                    p.data = torch.empty(0, dtype=p.dtype, device=p.device)
+                n += 2
+        self.quantization = fmt
+        return n
+
+    def _norm_rows(self, x, gain, xn):
+        """The norm of ``x`` for a projection that is its only reader: rows in the projection's format, or bf16 rows in ``xn``."""
+        eps = self.cfg.rms_norm_eps
+        if self.quantization is not None and x.dtype == torch.bfloat16:
+            return lowbit.rms_norm_quantize(x, gain, self.quantization, eps=eps)
+        return fused.norm_modulate(x, weight=gain, rms=True, eps=eps, out=xn)
 
     def short_padding(self, n: int) -> bool:
         """Padding rows of a captured step of ``n`` sequences may see one key only (engine/graph_runner.py).  With experts they choose others than row 0 then:
@@ -221,6 +271,8 @@ class QwenDecoderModel(nn.Module):
         Row-parallel outputs are summed by ``RowParallelReduce`` (GEMM epilogue stores to the row
         owners + local reduce on the GPU, all-reduce on CPU / ``mode="nccl"``)."""
         from ..parallel.tensor_parallel import RowParallelReduce, shard_cols
+        if self.quantization is not None:
+            raise NotImplementedError("tensor parallelism of quantised weights")
         cfg = self.cfg
         P, r = group.world_size, group.rank_in_group
         if P == 1:
@@ -291,6 +343,8 @@ class QwenDecoderModel(nn.Module):
         P, r = group.world_size, group.rank_in_group
         if not cfg.num_experts or P == 1:
             return
+        if self.quantization is not None:
+            raise NotImplementedError("expert parallelism of quantised weights")
         if cfg.num_experts % P:
             raise ValueError(f"num_experts ({cfg.num_experts}) must be divisible by the expert-parallel size ({P})")
         per = cfg.num_experts // P
@@ -371,10 +425,9 @@ class QwenDecoderModel(nn.Module):
         tp_cap = max(64, 1 << (T - 1).bit_length())          # peer-buffer bucket of the row-parallel reduces
         normed = False                                       # xn already holds the norm that comes next
         for li, layer in enumerate(self.layers):
-            if not normed:
-                fused.norm_modulate(x, weight=layer.input_layernorm, rms=True, eps=cfg.rms_norm_eps, out=xn)
+            rows = xn if normed else self._norm_rows(x, layer.input_layernorm, xn)
             normed = False
-            qkv = layer.qkv_proj(xn)
+            qkv = layer.qkv_proj(rows)
             kc, vc = kv_caches[li] if kv_caches is not None else (None, None)
             fused.qk_norm_rope_(qkv.view(1, T, -1), H, Hkv, Dh, wq=layer.q_norm, wk=layer.k_norm, cos=cos, sin=sin,
                                 interleaved=False, eps=cfg.rms_norm_eps,
@@ -384,8 +437,8 @@ class QwenDecoderModel(nn.Module):
                 self.tp_reduce.linear(layer.o_proj, attn, residual=x, out=x, capacity=tp_cap)   # sum over ranks
             else:
                 layer.o_proj(attn, residual=x, out=x)
-            fused.norm_modulate(x, weight=layer.post_attention_layernorm, rms=True, eps=cfg.rms_norm_eps, out=xn)
             if cfg.num_experts:
+                fused.norm_modulate(x, weight=layer.post_attention_layernorm, rms=True, eps=cfg.rms_norm_eps, out=xn)
                 logits = layer.router(xn)
                 e_lo, e_hi = self.ep_range
                 shared = None
@@ -393,7 +446,13 @@ class QwenDecoderModel(nn.Module):
                     # replicated under expert parallelism: added once, after the routed experts
                     g = torch.sigmoid(xn.float() @ layer.shared_expert_gate.float().t())
                     shared = layer.shared_down(fused.silu_mul(layer.shared_gate_up(xn))).float().mul_(g)
-                if self.ep_group is None or self.ep_group.world_size == 1:
+                if layer.w13_fp4 is not None:
+                    ids, weights = route(logits, cfg.num_experts_per_tok, cfg.norm_topk_prob)
+                    if x.dtype == torch.bfloat16:
+                        lowbit.experts(xn, ids, weights, layer.w13_fp4, layer.w2_fp4, residual=x, out=x)
+                    else:                                  # the CPU's fp32 models
+                        x.add_(lowbit.experts(xn.to(torch.bfloat16), ids, weights, layer.w13_fp4, layer.w2_fp4))
+                elif self.ep_group is None or self.ep_group.world_size == 1:
                     # where nothing else is added to the rows, the next norm leaves the combining launch with them
                     normed = shared is None and (deepstack is None or li >= len(deepstack))
                     gain = self.layers[li + 1].input_layernorm if li + 1 < len(self.layers) else self.norm
@@ -417,7 +476,7 @@ class QwenDecoderModel(nn.Module):
                 if shared is not None:
                     x.add_(shared.to(x.dtype))
             else:
-                h = layer.gate_up.swiglu(xn)
+                h = layer.gate_up.swiglu(self._norm_rows(x, layer.post_attention_layernorm, xn))
                 if self.tp_reduce is not None:
                     self.tp_reduce.linear(layer.down, h, residual=x, out=x, capacity=tp_cap)
                 else:

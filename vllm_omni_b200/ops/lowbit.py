@@ -440,7 +440,10 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
         o2 = torch.empty(M, N, dtype=torch.bfloat16, device=_device(index))
         out = o2 if len(lead) == 1 else o2.view(*lead, N)
     else:
-        o2 = out if out.dim() == 2 else out.view(M, N)
+        try:
+            o2 = out if out.dim() == 2 else out.view(M, N)
+        except RuntimeError:                      # rows of several batches that no single pitch reaches
+            return out.copy_(linear(x if raw is None else x.view(*lead, cols), w, bias, act, residual, gate, None, force_tile, force_split))
     ldo, yp = o2.stride(), o2.data_ptr()
     rp = bp = gp = None
     ldr, lds, per = (0, 1), 0, 0

@@ -198,6 +198,22 @@ def _route(logits, T, E, k, renorm, ws):
                                              nv.ptr(ws.ids), nv.ptr(ws.weights), nv.stream_ptr()), "omni_moe_route")
 
 
+def route(logits, k: int, renorm: bool = True):
+    """(ids int32, weights fp32) [T, k]: the ``k`` largest of bf16 logits [T, E] and their softmax probabilities, among themselves with ``renorm``."""
+    T, E = logits.shape
+    if not 1 <= k <= min(E, 16) or E > 256:
+        raise ValueError(f"route: 1 to 16 of at most 256 experts, got {k} of {E}")
+    if not logits.is_cuda:
+        ids, w = moe_route_reference(logits, k, renorm)
+        return ids, w
+    assert logits.dtype == torch.bfloat16 and logits.stride(1) == 1
+    ids = torch.empty(T, k, dtype=torch.int32, device=logits.device)
+    w = torch.empty(T, k, dtype=torch.float32, device=logits.device)
+    nv.check_rc(nv.lib("moe").omni_moe_route(nv.ptr(logits), c_int(logits.stride(0)), c_int(T), c_int(E), c_int(k), c_int(1 if renorm else 0), nv.ptr(ids), nv.ptr(w),
+                                             nv.stream_ptr()), "omni_moe_route")
+    return ids, w
+
+
 def _few_plan(ws, T, E, e_lo, e_hi, k, logits=None, renorm=True):
     """Tiles of few tokens; with ``logits`` the choice (``ws.ids``, ``ws.weights``) is made as well, in the same launch (one block) for
     up to 16 tokens: 4 us for one token, 12 us for 64 against 3 + 4 us in two launches."""

@@ -92,7 +92,7 @@ class UlyssesJointAttention:
         G, B = self.Hp * self.Dh, self.B
         if self.mode == "fused":
             bs = self.S_tot * 3 * G
-            plain = all(l.fp8 is None and not l.lora for l in (img_lin, txt_lin))
+            plain = all(not l.quantized and not l.lora for l in (img_lin, txt_lin))
             # the block's other linears must be able to carry the wait as well (set by the model)
             self._flags_now = flags = self.use_flags and plain and getattr(self, "block_plain", True)
             sig = self.ch_qkv.signal() if flags else None
