@@ -282,7 +282,7 @@ def test_linear(fmt, M, N, K):
     want = want_linear(q, p)
     close(L.linear(x, p), want)
     kb = -(-K // 256)
-    for tile, split in [(16, s) for s in (1, 2, 4, 8)] + [(64, s) for s in (1, 2, 4, 8)] + [(128, s) for s in (1, 2, 4, 8)] + [(256, 0)]:
+    for tile, split in [(tile, s) for tile in (16, 64, 128) for s in (1, 2, 4)] + [(256, s) for s in (1, 2)]:
         if (tile <= 64 and M > tile) or split > kb:
             continue
         close(L.linear(q, p, force_tile=tile, force_split=split), want)
@@ -291,7 +291,7 @@ def test_linear(fmt, M, N, K):
 @gpu
 @pytest.mark.parametrize("fmt", FMT4)
 @pytest.mark.parametrize("M,N,K,tile,split", [(6, 136, 512, 16, 1), (6, 136, 512, 64, 1), (6, 1000, 512, 64, 2), (6, 77, 512, 0, 0), (130, 264, 512, 128, 1), (130, 264, 512, 128, 2), (260, 1000, 288, 256, 0),
-                                              (260, 333, 288, 256, 0), (4096, 256, 64, 0, 0)])
+                                              (260, 333, 288, 256, 0), (200, 333, 544, 256, 2), (260, 520, 1056, 256, 2), (4096, 256, 64, 0, 0)])
 @pytest.mark.parametrize("act", [None, "silu", "gelu_tanh"])
 def test_linear_epilogue(fmt, M, N, K, tile, split, act):
     x, w = rows_of(M, K, device="cuda"), weight_of(N, K, device="cuda")
@@ -313,8 +313,8 @@ def test_linear_epilogue(fmt, M, N, K, tile, split, act):
 
 @gpu
 @pytest.mark.parametrize("fmt", FMT4)
-@pytest.mark.parametrize("M,N,K,tile,split", [(1, 32, 64, 0, 0), (5, 272, 512, 16, 1), (5, 272, 512, 64, 1), (5, 272, 2080, 64, 8), (5, 272, 2080, 16, 2), (40, 4096, 512, 0, 0), (130, 528, 544, 128, 1), (100, 528, 1024, 128, 4),
-                                              (300, 1040, 288, 256, 0), (513, 512, 512, 256, 0)])
+@pytest.mark.parametrize("M,N,K,tile,split", [(1, 32, 64, 0, 0), (5, 272, 512, 16, 1), (5, 272, 512, 64, 1), (5, 272, 2080, 64, 4), (5, 272, 2080, 16, 2), (40, 4096, 512, 0, 0), (130, 528, 544, 128, 1), (100, 528, 1024, 128, 4),
+                                              (300, 1040, 288, 256, 1), (300, 1040, 1056, 256, 2), (513, 512, 512, 256, 0)])
 def test_linear_gated(fmt, M, N, K, tile, split):
     x, w = rows_of(M, K, device="cuda") / 4, weight_of(N, K, device="cuda")
     q, p = L.quantize(x, fmt), L.pack_weight(w, fmt, gated=True)
@@ -328,7 +328,7 @@ def test_linear_gated(fmt, M, N, K, tile, split):
 
 @gpu
 @pytest.mark.parametrize("fmt", FMT4)
-@pytest.mark.parametrize("tile,split,M", [(16, 1, 13), (16, 4, 13), (64, 1, 20), (64, 4, 20), (128, 1, 200), (256, 0, 300)])
+@pytest.mark.parametrize("tile,split,M", [(16, 1, 13), (16, 4, 13), (64, 1, 20), (64, 4, 20), (128, 1, 200), (256, 1, 300), (256, 2, 300)])
 def test_linear_nan_rows_stay_alone(fmt, tile, split, M):
     """A row or a weight row of NaN makes its own results NaN and no others."""
     x, w = rows_of(M, 1024, device="cuda"), weight_of(200, 1024, device="cuda")
@@ -570,7 +570,7 @@ def test_refusals_on_a_gpu():
         L.linear(x.cpu(), p)
     with pytest.raises(ValueError, match="contiguous"):
         L.linear(x, p, out=torch.empty(32, 4, dtype=BF, device="cuda").t())
-    for bad in (dict(force_tile=32), dict(force_split=3), dict(force_split=2)):        # one block of K only
+    for bad in (dict(force_tile=32), dict(force_split=3), dict(force_split=8), dict(force_split=2)):        # one block of K only
         with pytest.raises(nv.NativeError):
             L.linear(x, p, **bad)
     with pytest.raises(nv.NativeError):

@@ -113,11 +113,9 @@ def test_fp8_rows_of_a_norm_feed_the_fp8_layer(device):
     q = L.rms_norm_quantize(x, g, "fp8", normed=normed)
     a, b = fp8_linear(q, state), fp8_linear(normed, state)
     assert a.dtype == BF
-    if device == "cuda":
-        assert torch.equal(a, b)                                         # the same codes, scales and kernel
-    else:                                                                # scales of amax / 448 there, of amax * (1 / 448) here: a step of fp32, which tips no more than half a step of e4m3
-        S = L.dequantize(q, torch.float32).abs() @ (w8.float().abs() * sw.repeat_interleave(128, 0).repeat_interleave(128, 1)).t()
-        assert ((a.float() - b.float()).abs() <= 2 * U * b.float().abs() + S * 2.0 ** -4).all()
+    # the layer's own quantiser multiplies by a rounded reciprocal, the norm's restores ties: a code may be off by half a step of e4m3
+    S = L.dequantize(q, torch.float32).abs() @ (w8.float().abs() * sw.repeat_interleave(128, 0).repeat_interleave(128, 1)).t()
+    assert ((a.float() - b.float()).abs() <= 2 * U * b.float().abs() + S * 2.0 ** -4).all()
     with pytest.raises(ValueError, match="fp8 layer"):
         fp8_linear(L.quantize(x, "mxfp4"), state)
 

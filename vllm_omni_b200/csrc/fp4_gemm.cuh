@@ -11,13 +11,12 @@
 // tensor memory (columns of their own per stage, free again when the stage is) and issues the MMAs that read them.
 //
 //   fp4_kernel<FMT, XR, EPI, PAIR>
-//     XR = 16, 64       single CTAs, two per SM, two accumulators, so that the drain of a tile overlaps the next one's products
-//     XR = 128          the same, one per SM
+//     XR = 16, 64, 128  single CTAs, two accumulators, so that the drain of a tile overlaps the next one's products
 //     XR = 256, pairs   (cta_group::2) 256 x 256 tiles: each CTA brings 128 rows of W and half of the rows of X, and an MMA reads both: half the
 //                       L2 traffic per product, which is what bounds 4-bit tiles (128 x 128: 32 KB per 8.4 Mflop).
 //                       One accumulator: the scales take the rest of tensor memory; sixteen warps drain it into registers at once
 //                       and hand it back before they work on it.
-//     few tiles         a cluster of 2 to 8 CTAs shares a tile along K: partial sums meet in shared memory, added in the order of the ranks
+//     few tiles         2 or 4 CTAs (2 pairs) of a cluster share a tile along K; each finishes its part of the outputs from the sums of all
 //
 // All waits are bounded (ptx_sm100.cuh).  No load is a multicast.
 #pragma once
@@ -49,7 +48,7 @@ struct Fp4Cfg {
   static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + WS_BYTES + XS_BYTES;
   static constexpr int BOX = PAIR ? 32 : XR < 64 ? XR : 64;                    // rows of X per load
   static constexpr int ACCS = PAIR ? 1 : 2, SCALE_COLS = 4 * WORDS * (1 + X_TILES);
-  static constexpr int CTAS = XR <= 64 ? 2 : 1;                                // per SM
+  static constexpr int CTAS = XR <= 16 ? 2 : 1;                                // per SM
   static constexpr int PARTS = XR == 16 ? 1 : PAIR ? 4 : 2;                    // draining warps per quadrant of tensor memory
   static constexpr int CHUNKS = XR / 16 / PARTS;                               // of 16 rows of X, per draining warp
   static constexpr int DRAIN_WARPS = 4 * PARTS, THREADS = 64 + 32 * DRAIN_WARPS;
@@ -60,6 +59,7 @@ struct Fp4Cfg {
   static constexpr int BY_SMEM = (228 * 1024 / CTAS - 2560 - TURN_BYTES) / STAGE_PITCH, BY_TMEM = (TMEM_COLS - ACCS * XR) / SCALE_COLS;
   static constexpr int STAGES = BY_SMEM < BY_TMEM ? BY_SMEM : BY_TMEM;
   static constexpr int SMEM_BYTES = STAGES * STAGE_PITCH + TURN_BYTES + 1024;
+  static_assert(XR * 512 <= STAGES * STAGE_PITCH, "sums of a split tile lie in the ring");
 };
 
 enum Fp4Act : int { FP4_NONE = 0, FP4_GELU_TANH = 1, FP4_SILU = 2 };
@@ -79,11 +79,11 @@ __device__ __forceinline__ float gelu_of(float x) {
 }
 
 // One result of row m of X: weight row n of the matrix (already times both factors).
-__device__ __forceinline__ float fp4_finish(const Fp4Args& a, float v, long m, int n) {
+__device__ __forceinline__ float fp4_finish(const Fp4Args& a, float v, long m, int n, bool residual) {
   if (a.bias) v += __bfloat162float(a.bias[n]);
   v = a.act == FP4_SILU ? silu_of(v) : a.act == FP4_GELU_TANH ? gelu_of(v) : v;
   if (a.gate) v *= __bfloat162float(a.gate[m / a.rows_per_gate * a.gate_stride + n]);
-  if (a.residual) v += __bfloat162float(a.residual[m * a.ldr + n]);
+  if (residual && a.residual) v += __bfloat162float(a.residual[m * a.ldr + n]);
   return v;
 }
 
@@ -232,13 +232,24 @@ __device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v0, 
   __syncwarp();                                                                // the next 16 rows are turned in the same place
 }
 
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* tmap, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* tmap, int c0, int c1, int c2) {
   asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
+
+constexpr int SPLIT_MOST = 4;    // CTAs or pairs that share a tile
+// Stages of weights that a CTA asks for ahead of its first item.  One row of 24576 x 4096 with its quantisation: 14.2 us without, 13.8 with 4, 14.4 with 8,
+// 15.8 with 16 (asked for ahead of what other CTAs need first).
+constexpr int PREFETCH = 4;
 
 // a tile of rows: which expert, its first row in X and y, how many rows, and where its scales begin
 struct RowTile {
@@ -273,13 +284,14 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
   __shared__ __align__(8) uint64_t empty_bar[STAGES];
   __shared__ __align__(8) uint64_t tfull_bar[ACCS];
   __shared__ __align__(8) uint64_t tempty_bar[ACCS];               // pairs: in the even CTA, the warps of both
+  __shared__ float xf_s[XR];                                       // split: factors of the tile's rows of X
   __shared__ uint32_t tmem_base_s;
   __shared__ int s_abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = PAIR ? (int)cluster_ctarank() : 0;
-  const int share = !PAIR && a.split > 1 ? (int)cluster_ctarank() : 0;                 // this CTA's part of K
-  const int group = PAIR ? 2 : a.split;                                                // CTAs that work on an item
+  constexpr int SIZE = PAIR ? 2 : 1;
+  const int group = SIZE * a.split, in_group = group > 1 ? (int)cluster_ctarank() : 0;  // CTAs that work on an item
+  const int rank = in_group % SIZE, share = in_group / SIZE, even = share * SIZE;       // this CTA in its pair, its part of K, the pair's even CTA
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
   const int num_n = (a.N + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128), num_items = a.max_tiles * num_n;
@@ -313,7 +325,7 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (PAIR || a.split > 1) cluster_sync_all();
+  if (PAIR) cluster_sync_all();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_base_s, tmem_scales = tmem_base + ACCS * XR;
   // item -> (block of weight rows, tile of rows).  One matrix: tiles of rows first, so that neighbours share the weights and all of X, which is small in 4
@@ -322,14 +334,15 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
   auto tile_of = [&](int it) { return experts ? it / num_n : it % a.max_tiles; };
   auto block_of = [&](int it) { return (experts ? it % num_n : it / a.max_tiles) * (PAIR ? 2 : 1) + rank; };
 
-  // the first stages' weights into L2 while the kernel before (the rows' quantiser) runs out
+  // the first item's weights into L2 while the kernel before (the rows' quantiser) runs out
   if (!experts && warp == 0 && first < num_items && elect_one())
-    for (int kb = kb0; kb < kb1 && kb < kb0 + STAGES; ++kb) tma_prefetch_3d(&a.tmW, kb * 128, block_of(first) * 128, 0);
+    for (int kb = kb0; kb < kb1 && kb < kb0 + PREFETCH; ++kb) {
+      tma_prefetch_3d(&a.tmW, kb * 128, block_of(first) * 128, 0);
+      tma_prefetch_4d(&a.tmWS, 0, kb * Cfg::WORDS, block_of(first), 0);
+    }
   __syncwarp();
   pdl_begin();
 
-  uint32_t part_sums[PAIR ? 1 : Cfg::CHUNKS][16];                  // split: of the draining warps
-  float wf = 1.0f;
   if (warp == 0) {
     if (elect_one()) {
       int stage = 0;
@@ -345,7 +358,7 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
           const uint32_t s = smem_base + stage * Cfg::STAGE_PITCH, sx = s + Cfg::W_BYTES, sws = sx + Cfg::X_BYTES, sxs = sws + Cfg::WS_BYTES;
           if (PAIR) {
             if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[stage]), 2 * bytes);
-            const uint32_t fb = mapa_shared(smem_u32(&full_bar[stage]), 0);
+            const uint32_t fb = mapa_shared(smem_u32(&full_bar[stage]), even);
             tma_load_3d_pair(s, &a.tmW, fb, kb * 128, nb * 128, t.expert);
             tma_load_4d_pair(sws, &a.tmWS, fb, 0, kb * Cfg::WORDS, nb, t.expert);
             for (int b = 0; b < boxes; ++b) tma_load_2d_pair(sx + b * Cfg::BOX * 128, &a.tmX, fb, kb * 128, x0 + b * Cfg::BOX);
@@ -398,16 +411,16 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
                                   x_cols + 4 * Cfg::X_TILES * w, kb != kb0 || k != 0);
           }
           if (PAIR) {
-            tc_commit_pair(mapa_shared(smem_u32(&empty_bar[stage]), 0));
-            tc_commit_pair(mapa_shared(smem_u32(&empty_bar[stage]), 1));
+            tc_commit_pair(mapa_shared(smem_u32(&empty_bar[stage]), even));
+            tc_commit_pair(mapa_shared(smem_u32(&empty_bar[stage]), even + 1));
           } else {
             tc_commit(smem_u32(&empty_bar[stage]));
           }
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
         if (PAIR) {
-          tc_commit_pair(mapa_shared(smem_u32(&tfull_bar[acc]), 0));
-          tc_commit_pair(mapa_shared(smem_u32(&tfull_bar[acc]), 1));
+          tc_commit_pair(mapa_shared(smem_u32(&tfull_bar[acc]), even));
+          tc_commit_pair(mapa_shared(smem_u32(&tfull_bar[acc]), even + 1));
         } else {
           tc_commit(smem_u32(&tfull_bar[acc]));
         }
@@ -431,9 +444,30 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
         const int r = c0 + i * 16 + (lane & 15);
         xf[i] = a.xf && r < t.rows ? a.xf[t.row0 + r] : 1.0f;
       }
+      float wf = 1.0f;
+      if (a.split > 1) {                                           // what finishing will need, while the tile is waited for
+        if (a.wf && n0 + lane < a.N) wf = a.wf[n0 + lane];
+        if (q == 0)
+          for (int r = c0 + lane; r < min(t.rows, c0 + 16 * Cfg::CHUNKS); r += 32) xf_s[r] = a.xf ? a.xf[t.row0 + r] : 1.0f;
+      }
       mbar_wait(smem_u32(&tfull_bar[acc]), acc_phase, &s_abort, status, ERR_WAIT_TMEM_FULL);
       tc_fence_after_sync();
       const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + acc * XR + c0, half = 16u << 16;
+      if (a.split > 1) {
+        // this CTA's sums to its ring, which its products no longer read, as blocks [owner][row of X][width]
+        const int width = 128 / a.split, n = q * 32 + lane;
+        float* to = reinterpret_cast<float*>(smem) + (n / width * t.rows + c0) * width + n % width;
+#pragma unroll 1
+        for (int c = 0; c < 16 * Cfg::CHUNKS && c0 + c < t.rows; c += 16) {
+          uint32_t v[16];
+          tmem_ld_32x16(tmem_base + ((uint32_t)(q * 32) << 16) + c0 + c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + c + j < t.rows) to[(c + j) * width] = __uint_as_float(v[j]) * wf;
+        }
+        break;
+      }
       if constexpr (PAIR) {
         // 64 of the 256 rows per warp, into registers (with operands in the epilogue in two steps, for want of registers); then the accumulator is free
         constexpr int STEPS = EPI == EPI_ANY ? 2 : 1, PER = Cfg::CHUNKS / STEPS;
@@ -448,7 +482,7 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
           if (j == STEPS - 1) {
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[acc]), 0));
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[acc]), even));
           }
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
@@ -456,7 +490,7 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
             if (c < t.rows) fp4_store<EPI>(a, v[0] + 8 * i, v[1] + 8 * i, turned, t.row0 + c, t.rows - c, n0, keep, xf[j * PER + i], lane);
           }
         }
-      } else if (a.split == 1) {
+      } else {
 #pragma unroll
         for (int i = 0; i < Cfg::CHUNKS; ++i) {
           const int c = c0 + i * 16;
@@ -470,74 +504,66 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
-      } else {
-        // this CTA's sums stay in registers until everybody's ring is free
-        wf = a.wf && n0 + lane < a.N ? a.wf[(long)t.expert * a.N + n0 + lane] : 1.0f;
-#pragma unroll
-        for (int i = 0; i < Cfg::CHUNKS; ++i)
-          if (c0 + i * 16 < t.rows) tmem_ld_32x16(at + i * 16, part_sums[i]);
-        tmem_wait_ld();
       }
       if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
     }
   }
 
-  if (!PAIR && a.split > 1) {
-    // Every CTA finishes 128 / split of the weight rows (at least 16: a gate group and its lift rows), all rows of X: the others' sums come to it as [their
-    // share][row of X][width], in its ring, and are added in the order of the shares.
+  if (a.split > 1) {
+    // Every CTA finishes 128 / split of the weight rows (at least 16: a gate group and its lift rows), all rows of X.  Sums lie in the rings as blocks
+    // [owner][row of X][width]; the owner reads its block of every CTA where it lies and adds them in the order of the shares.
+    __syncwarp();
+    cluster_sync_all();
     RowTile t;
-    const bool any = first < num_items && row_tile<XR>(a, tile_of(first), t);
-    const int width = 128 / a.split;
-    __syncwarp();
-    cluster_sync_all();
-    if (any && warp >= 2) {
-      const int n = (warp & 3) * 32 + lane, owner = n / width, c0 = ((warp - 2) >> 2) * 16 * Cfg::CHUNKS;
-      const uint32_t to = mapa_shared(smem_base + ((share * t.rows + c0) * width + n % width) * 4, owner);
+    if (first < num_items && row_tile<XR>(a, tile_of(first), t)) {
+      const int width = 128 / a.split, n0 = block_of(first) * 128 + share * width, outs = GATED ? width / 2 : width, quads = outs / 4, total = t.rows * quads;
+      const uint32_t block = smem_base + share * t.rows * width * 4;
+      auto column = [&](int o) { return GATED ? o / 8 * 16 + o % 8 : o; };       // of the block, where output o (or its gate) stands
+      constexpr int COLS = GATED ? 2 : 1;                                        // gate and lift
+      for (int i0 = threadIdx.x; i0 < total; i0 += 2 * blockDim.x) {             // four outputs of two rows at a time
+        float sums[2][COLS][4];
+        uint2 res[2];
 #pragma unroll
-      for (int i = 0; i < (PAIR ? 1 : Cfg::CHUNKS); ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c0 + i * 16 + j < t.rows) st_cluster_f32(to + (i * 16 + j) * width * 4, __uint_as_float(part_sums[i][j]) * wf);
-    }
-    __syncwarp();
-    cluster_sync_all();
-    if (any) {
-      const int base = share * width, n0 = block_of(first) * 128 + base, outs = GATED ? width / 2 : width, quads = outs / 4;
-      auto sum = [&](int r, int n, float (&s)[4]) {
-        const uint32_t at = smem_base + (r * width + n) * 4;
-        const uint4 f = ld_shared_v4(at);
-        s[0] = __uint_as_float(f.x); s[1] = __uint_as_float(f.y); s[2] = __uint_as_float(f.z); s[3] = __uint_as_float(f.w);
-        for (int c = 1; c < a.split; ++c) {
-          const uint4 g = ld_shared_v4(at + c * t.rows * width * 4);
-          s[0] += __uint_as_float(g.x); s[1] += __uint_as_float(g.y); s[2] += __uint_as_float(g.z); s[3] += __uint_as_float(g.w);
+        for (int u = 0; u < 2; ++u) {
+          const int i = i0 + u * blockDim.x, r = i / quads, o = (i - r * quads) * 4;
+          if (EPI == EPI_ANY && a.residual && a.by16 && i < total && n0 + o < a.N) res[u] = *reinterpret_cast<const uint2*>(a.residual + (t.row0 + r) * a.ldr + n0 + o);
         }
-      };
-      for (int i = threadIdx.x; i < t.rows * quads; i += blockDim.x) {
-        const int r = i / quads, o = (i - r * quads) * 4;
-        const long m = t.row0 + r;
-        const float f = a.xf ? a.xf[m] : 1.0f;
-        float s0[4], s1[4];
-        if (GATED) {
-          const int n = o / 8 * 16 + o % 8;
-          if (n0 + n >= a.N) continue;
-          sum(r, n, s0);
-          sum(r, n + 8, s1);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s0[e] = silu_of(s0[e] * f) * (s1[e] * f);
-          bf16* out = a.y + m * a.ldy + n0 / 2 + o;
-          if (a.by16) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(s0[0], s0[1]), pack_bf16(s0[2], s0[3]));
-          else
-            for (int e = 0; e < 4; ++e) out[e] = __float2bfloat16(s0[e]);
-        } else {
-          const int n = n0 + o;
-          if (n >= a.N) continue;
-          sum(r, o, s0);
-          bf16* out = a.y + m * a.ldy + n;
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s0[e] = EPI == EPI_ANY ? (n + e < a.N ? fp4_finish(a, s0[e] * f, m, n + e) : 0.f) : s0[e] * f;
-          if (a.by16) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(s0[0], s0[1]), pack_bf16(s0[2], s0[3]));
+          for (int k = 0; k < COLS; ++k) {
+            const int i = i0 + u * blockDim.x, r = i / quads, o = (i - r * quads) * 4;
+            float4 v[SPLIT_MOST];
+#pragma unroll
+            for (int c = 0; c < SPLIT_MOST; ++c)
+              v[c] = c < a.split && i < total ? ld_cluster_f32x4(mapa_shared(block + (r * width + column(o) + 8 * k) * 4, c * SIZE + rank)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            float(&s)[4] = sums[u][k];
+            s[0] = v[0].x; s[1] = v[0].y; s[2] = v[0].z; s[3] = v[0].w;
+#pragma unroll
+            for (int c = 1; c < SPLIT_MOST; ++c) { s[0] += v[c].x; s[1] += v[c].y; s[2] += v[c].z; s[3] += v[c].w; }
+          }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int i = i0 + u * blockDim.x, r = i / quads, o = (i - r * quads) * 4;
+          if (i >= total || n0 + column(o) >= a.N) continue;
+          const long m = t.row0 + r;
+          const float f = xf_s[r];
+          bf16* out = a.y + m * a.ldy + (GATED ? n0 / 2 : n0) + o;
+          const int left = a.N - n0 - o;                                         // outputs that exist (gated: all)
+          float(&s)[4] = sums[u][0];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[e] *= f;
+            if (GATED) s[e] = silu_of(s[e]) * (sums[u][COLS - 1][e] * f);
+            else if (EPI == EPI_ANY && e < left) s[e] = fp4_finish(a, s[e], m, n0 + o + e, !a.by16);
+          }
+          if (EPI == EPI_ANY && a.residual && a.by16) {
+            const float2 lo = unpack_bf16(res[u].x), hi = unpack_bf16(res[u].y);
+            s[0] += lo.x; s[1] += lo.y; s[2] += hi.x; s[3] += hi.y;
+          }
+          if (a.by16) *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
           else
-            for (int e = 0; e < 4 && n + e < a.N; ++e) out[e] = __float2bfloat16(s0[e]);
+            for (int e = 0; e < 4 && (GATED || e < left); ++e) out[e] = __float2bfloat16(s[e]);
         }
       }
     }
@@ -550,7 +576,7 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
     while (globaltimer_ns() - t0 < 200000ull) {
     }
   }
-  if (PAIR) cluster_sync_all();                 // neither CTA leaves while its partner may still signal it
+  if (group > 1) cluster_sync_all();            // nobody leaves while another may still signal it or copy from it
   if (warp == 1) {
     tc_fence_after_sync();
     if (PAIR) tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
@@ -624,7 +650,7 @@ static int launch_fp4(Fp4Args& a, const Fp4Operands& o, int* status, cudaStream_
   auto* kernel = fp4_kernel<FMT, XR, EPI, PAIR>;
   if (int e = ensure_dynamic_smem((const void*)kernel, Cfg::SMEM_BYTES, prepared)) return e;
   const long items = (long)a.max_tiles * ((a.N + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128));
-  const int group = PAIR ? 2 : a.split, most = PAIR ? resident_pairs((const void*)kernel, Cfg::THREADS, Cfg::SMEM_BYTES) : Cfg::CTAS * sm_count();
+  const int group = (PAIR ? 2 : 1) * a.split, most = PAIR ? resident_pairs((const void*)kernel, Cfg::THREADS, Cfg::SMEM_BYTES) : Cfg::CTAS * sm_count();
   const long run = a.split > 1 ? items : items < most ? items : most;
   if (run <= 0 || run * group > 0x7fffffffL) return RC_BAD_ARG;
   return launch_with(true, group, kernel, (unsigned)(run * group), Cfg::THREADS, Cfg::SMEM_BYTES, stream, a, status);
@@ -654,18 +680,34 @@ static int launch_any(Fp4Args& a, const Fp4Operands& o, int fmt, bool gated, int
 }
 
 // Tile and split of a linear layer: the tile's rows, or a negative code.
+// More than 128 rows: 128-row tiles on single CTAs or 256-row tiles on pairs, by the rounds that each take.  In a full round a block of 256 of K costs 0.4 us
+// on single CTAs and 0.5 on pairs (what L2 delivers), in a last round that is not full 0.3 and 0.4.  N x K = 4096 x 4096, 512 rows 8.3 us on single
+// CTAs, 11 on pairs; 1000 rows 13.1 and 12.2; 24576 x 4096, 200 rows 19.2 and 18.4, 8192 rows 494 and 375.
+// Few tiles: a split saves blocks of K (0.28 us each) and costs an exchange of 1.4 us and 14 ns per row, 0.6 more in fours.  4096 x 12288, 33 rows: 15.2 us
+// whole, 12.9 in two, 10.1 in four; 4096 x 1024: 3.6, 4.8, 5.5.  (Clusters of 8 of these CTAs, one per SM, do not all find room: 22 us.)
 static int pick_tiles(Fp4Args& a, int force_tile, int force_split) {
-  const int tile = force_tile ? force_tile : a.M <= 16 ? 16 : a.M <= 64 ? 64 : a.M <= 128 ? 128 : 256;
+  const int sms = sm_count(), kb = (a.K + 255) / 256;
+  int tile = force_tile ? force_tile : a.M <= 16 ? 16 : a.M <= 64 ? 64 : 128;
+  if (!force_tile && a.M > 128) {
+    const long single = ((long)a.M + 127) / 128 * ((a.N + 127) / 128), pairs = ((long)a.M + 255) / 256 * ((a.N + 255) / 256), slots = sms / 2;
+    if (5 * (pairs / slots) + (pairs % slots ? 4 : 0) <= 4 * (single / sms) + (single % sms ? 3 : 0)) tile = 256;
+  }
   if ((tile != 16 && tile != 64 && tile != 128 && tile != 256) || (tile <= 64 && a.M > tile)) return RC_BAD_ARG;
+  const bool pair = tile == 256;
   a.max_tiles = (int)(((long)a.M + tile - 1) / tile);
+  const long items = (long)a.max_tiles * (pair ? (a.N + 255) / 256 : (a.N + 127) / 128);
+  const int most = pair ? 2 : SPLIT_MOST, rows = a.M < tile ? a.M : tile;
   a.split = 1;
-  if (tile == 256) return force_split > 1 ? RC_BAD_ARG : tile;
-  const long items = (long)a.max_tiles * ((a.N + 127) / 128), slots = (tile <= 64 ? 2 : 1) * sm_count();
-  const int kb = (a.K + 255) / 256;
-  if (force_split) a.split = force_split;
-  else
-    while (a.split < 8 && items * a.split * 2 <= slots && kb >= a.split * 4) a.split *= 2;
-  if (a.split < 1 || a.split > 8 || (a.split & (a.split - 1)) || a.split > kb) return RC_BAD_ARG;
+  if (force_split) {
+    a.split = force_split;
+  } else {
+    int least = 280 * kb;
+    for (int s = 2; s <= most && s <= kb && items * s <= (pair ? sms / 2 : sms); s *= 2) {
+      const int cost = 280 * ((kb + s - 1) / s) + 1400 + 14 * rows + (s > 2 ? 600 : 0);
+      if (cost < least) { least = cost; a.split = s; }
+    }
+  }
+  if (a.split < 1 || a.split > most || (a.split & (a.split - 1)) || a.split > kb) return RC_BAD_ARG;
   return tile;
 }
 

@@ -4,6 +4,8 @@
 //  omni_lowbit_dequantize  codes and scales -> bf16 or fp32
 //  omni_lowbit_linear      linear layer on a packed weight: rows as bf16 (quantised first, in the caller's workspace) or quantised  (fp4_gemm.cuh)
 //  omni_lowbit_experts     both products of a mixture of experts, by the tables of a plan (moe.cu)
+//
+// Each takes its operands as one block of 8-byte fields: a layer's 26 passed one by one cost a Python caller 3 us, of 6 for the whole call.
 #include "fp4_gemm.cuh"
 #include "lowbit_rows.cuh"
 
@@ -11,75 +13,119 @@ using namespace omni;
 
 // gain null: x is quantised as it is.  Else s = x + residual (rounded to bf16, stored in total where given), rows s / rms(s) * gain (bf16, stored in
 // normed where given) are.  group: rows of a weight's matrix (rows, for one).
-extern "C" int omni_lowbit_rows(const void* x, long ldx, long rows, int K, long group, int fmt, const void* residual, long ldr, const void* gain,
-                                float eps, void* total, long ldt, void* normed, long ldn, void* codes, void* scales, void* row_scale,
-                                void* stream) {
+struct LowbitRows {
+  const void* x;
+  long ldx, rows, K, group, fmt;
+  const void* residual;
+  long ldr;
+  const void* gain;
+  double eps;
+  void* total;
+  long ldt;
+  void* normed;
+  long ldn;
+  void *codes, *scales, *row_scale, *stream;
+};
+extern "C" int omni_lowbit_rows(const LowbitRows* c) {
   RowsArgs a = {};
-  a.x = (const bf16*)x; a.residual = (const bf16*)residual; a.gain = (const bf16*)gain; a.total = (bf16*)total; a.normed = (bf16*)normed;
-  a.ldx = ldx; a.ldr = ldr; a.ldt = ldt; a.ldn = ldn; a.rows = rows; a.K = K; a.eps = eps;
-  a.codes = (uint8_t*)codes; a.scales = scales; a.row_scale = (float*)row_scale;
-  a.place.group = group > 0 ? group : 1;
-  return rows_any(a, fmt, (cudaStream_t)stream);
+  a.x = (const bf16*)c->x; a.residual = (const bf16*)c->residual; a.gain = (const bf16*)c->gain; a.total = (bf16*)c->total; a.normed = (bf16*)c->normed;
+  a.ldx = c->ldx; a.ldr = c->ldr; a.ldt = c->ldt; a.ldn = c->ldn; a.rows = c->rows; a.K = (int)c->K; a.eps = (float)c->eps;
+  a.codes = (uint8_t*)c->codes; a.scales = c->scales; a.row_scale = (float*)c->row_scale;
+  a.place.group = c->group > 0 ? c->group : 1;
+  return rows_any(a, (int)c->fmt, (cudaStream_t)c->stream);
 }
 
-extern "C" int omni_lowbit_dequantize(const void* codes, const void* scales, const void* row_scale, long rows, int K, long group, int fmt,
-                                      int f32, void* out, void* stream) {
-  return dequantize_any({(const uint8_t*)codes, scales, (const float*)row_scale, out, rows, group > 0 ? group : 1, K, f32}, fmt, (cudaStream_t)stream);
+struct LowbitValues {
+  const void *codes, *scales, *row_scale;
+  long rows, K, group, fmt, f32;
+  void *out, *stream;
+};
+extern "C" int omni_lowbit_dequantize(const LowbitValues* c) {
+  return dequantize_any({(const uint8_t*)c->codes, c->scales, (const float*)c->row_scale, c->out, c->rows, c->group > 0 ? c->group : 1, (int)c->K, (int)c->f32},
+                        (int)c->fmt, (cudaStream_t)c->stream);
 }
 
 // y [M, N] (gated: [M, N / 2]) of x [M, K] and w [N, K].  raw (bf16 rows, pitch ldx) not null: quantised into x, xs, xf first.  force_tile 0: by the rules
-// of fp4_gemm.cuh, 16 / 64 / 128 / 256; force_split 0: by the rules, 1 / 2 / 4 / 8.
-extern "C" int omni_lowbit_linear(const void* raw, long ldx, void* x, void* xs, void* xf, const void* w, const void* ws, const void* wf, void* y, long ldy,
-                                  long M, int N, int K, int fmt, int gated, const void* bias, int act, const void* gate, long gate_stride,
-                                  long rows_per_gate, const void* residual, long ldr, int force_tile, int force_split, void* status, void* stream) {
-  if (M <= 0 || N <= 0 || K <= 0) return RC_OK;
-  if (M > 0x7fffff00L || K % 32 || (gated && (N % 16 || bias || act || gate || residual)) || act < 0 || act > 2) return RC_BAD_ARG;
-  if (gate && rows_per_gate < 1) return RC_BAD_ARG;
+// of fp4_gemm.cuh, 16 / 64 / 128 / 256; force_split 0: by the rules, 1 / 2 / 4 (256: 1 / 2).
+struct LowbitLinear {
+  const void* raw;
+  long ldx;
+  void *x, *xs, *xf;
+  const void *w, *ws, *wf;
+  void* y;
+  long ldy, M, N, K, fmt, gated;
+  const void* bias;
+  long act;
+  const void* gate;
+  long gate_stride, rows_per_gate;
+  const void* residual;
+  long ldr, force_tile, force_split;
+  void *status, *stream;
+};
+extern "C" int omni_lowbit_linear(const LowbitLinear* c) {
+  if (c->M <= 0 || c->N <= 0 || c->K <= 0) return RC_OK;
+  if (c->M > 0x7fffff00L || c->N > 0x7fffff00L || c->K > 0x7fffff00L || c->K % 32 || c->act < 0 || c->act > 2 || (c->gate && c->rows_per_gate < 1) ||
+      (c->gated && (c->N % 16 || c->bias || c->act || c->gate || c->residual)))
+    return RC_BAD_ARG;
   Fp4Args a = {};
-  a.y = (bf16*)y; a.ldy = ldy; a.wf = (const float*)wf; a.xf = (const float*)xf;
-  a.bias = (const bf16*)bias; a.residual = (const bf16*)residual; a.gate = (const bf16*)gate;
-  a.ldr = ldr; a.gate_stride = gate_stride; a.rows_per_gate = (int)rows_per_gate; a.act = act;
-  a.M = (int)M; a.N = N; a.K = K;
-  a.by16 = N % 8 == 0 && ldy % 8 == 0 && ldr % 8 == 0 && gate_stride % 8 == 0 && on16(y) && on16(bias) && on16(gate) && on16(residual);
-  const int rc = pick_tiles(a, force_tile, force_split);
-  if (rc < 0) return rc;
-  if (raw) {
-    if (int e = omni_lowbit_rows(raw, ldx, M, K, M, fmt, nullptr, 0, nullptr, 0.f, nullptr, 0, nullptr, 0, x, xs, xf, stream)) return e;
+  a.y = (bf16*)c->y; a.ldy = c->ldy; a.wf = (const float*)c->wf; a.xf = (const float*)c->xf;
+  a.bias = (const bf16*)c->bias; a.residual = (const bf16*)c->residual; a.gate = (const bf16*)c->gate;
+  a.ldr = c->ldr; a.gate_stride = c->gate_stride; a.rows_per_gate = c->gate ? (int)c->rows_per_gate : 1; a.act = (int)c->act;
+  a.M = (int)c->M; a.N = (int)c->N; a.K = (int)c->K;
+  a.by16 = a.N % 8 == 0 && a.ldy % 8 == 0 && a.ldr % 8 == 0 && a.gate_stride % 8 == 0 && on16(a.y) && on16(a.bias) && on16(a.gate) && on16(a.residual);
+  const int tile = pick_tiles(a, (int)c->force_tile, (int)c->force_split);
+  if (tile < 0) return tile;
+  if (c->raw) {
+    RowsArgs r = {};
+    r.x = (const bf16*)c->raw; r.ldx = c->ldx; r.rows = c->M; r.K = a.K;
+    r.codes = (uint8_t*)c->x; r.scales = c->xs; r.row_scale = (float*)c->xf;
+    r.place.group = c->M;
+    if (int e = rows_any(r, (int)c->fmt, (cudaStream_t)c->stream)) return e;
   }
-  return launch_any(a, {w, ws, x, xs, 1, M, (M + 127) / 128}, fmt, gated != 0, rc, (int*)status, (cudaStream_t)stream);
+  return launch_any(a, {c->w, c->ws, c->x, c->xs, 1, c->M, (c->M + 127) / 128}, (int)c->fmt, c->gated != 0, tile, (int*)c->status, (cudaStream_t)c->stream);
 }
 
+// Rows of x (pair p reads row p / per, pairs a multiple of per) through `up` (gated, N = 2 F) to h [pairs, F] and through `down` to y [pairs, D], both in the
+// plan's order of rows; tile: the most rows a tile has, 64 / 128 / 256; n_rows: how many rows the plan has; place_of_row [pairs]: scratch.
 struct ExpertOperand {           // one product's rows in a workspace, and its weights
   void *codes, *scales, *row_scale;
   const void *w, *ws, *wf;
-  int N, K;
+  long N, K;
 };
-
-// Rows of x (pair p reads row p / per, pairs a multiple of per) through `up` (gated, N = 2 F) to h [pairs, F] and through `down` to y [pairs, D], both in the plan's order of rows;
-// tile: the most rows a tile has, 64 / 128 / 256; n_rows: how many rows the
-// plan has; place_of_row [pairs]: scratch.
-extern "C" int omni_lowbit_experts(const void* x, long ldx, int per, long pairs, int experts, int fmt, const ExpertOperand* up, const ExpertOperand* down, void* h,
-                                   void* y, const int* row_of_pair, const int* tile_expert, const int* tile_row0, const int* tile_rows, int max_tiles,
-                                   int tile, const int* n_rows, int* place_of_row, void* status, void* stream) {
-  if (pairs <= 0 || max_tiles <= 0) return RC_OK;
-  if (pairs > 0x7fffff00L || per < 1 || experts < 1 || !row_of_pair || !n_rows || !place_of_row || pairs % per || !tile_expert || !tile_row0 || !tile_rows || up->N % 16 || up->N != 2 * down->K ||
-      up->K % 32 || down->K % 32 || fmt == FMT_FP8)
+struct LowbitExperts {
+  const void* x;
+  long ldx, per, pairs, experts, fmt;
+  void *h, *y;
+  const int *row_of_pair, *tile_expert, *tile_row0, *tile_rows;
+  long max_tiles, tile;
+  const int* n_rows;
+  int* place_of_row;
+  void *status, *stream;
+  ExpertOperand up, down;
+};
+extern "C" int omni_lowbit_experts(const LowbitExperts* c) {
+  const ExpertOperand &up = c->up, &down = c->down;
+  if (c->pairs <= 0 || c->max_tiles <= 0) return RC_OK;
+  if (c->pairs > 0x7fffff00L || c->per < 1 || c->pairs % c->per || c->experts < 1 || !c->row_of_pair || !c->n_rows || !c->place_of_row || !c->tile_expert ||
+      !c->tile_row0 || !c->tile_rows || up.N % 16 || up.N != 2 * down.K || up.K != down.N || up.K % 32 || down.K % 32 || c->fmt == FMT_FP8)
     return RC_BAD_ARG;
-  cudaStream_t s = (cudaStream_t)stream;
-  const int pitch = tile > 128 ? 256 : 128;
+  cudaStream_t s = (cudaStream_t)c->stream;
+  const int pitch = c->tile > 128 ? 256 : 128;
   for (int half = 0; half < 2; ++half) {
-    const ExpertOperand& o = half ? *down : *up;
+    const ExpertOperand& o = half ? down : up;
     RowsArgs r = {};
-    r.x = (const bf16*)(half ? h : x); r.ldx = half ? o.K : ldx; r.rows = half ? pairs : pairs / per; r.K = o.K;
+    r.x = (const bf16*)(half ? c->h : c->x); r.ldx = half ? o.K : c->ldx; r.rows = half ? c->pairs : c->pairs / c->per; r.K = (int)o.K;
     r.codes = (uint8_t*)o.codes; r.scales = o.scales; r.row_scale = (float*)o.row_scale;
-    r.place = {1, half ? nullptr : row_of_pair, tile_expert, tile_row0, tile_rows, n_rows, place_of_row, per, max_tiles, pitch};
-    if (int e = rows_any(r, fmt, s)) return e;
+    r.place = {1, half ? nullptr : c->row_of_pair, c->tile_expert, c->tile_row0, c->tile_rows, c->n_rows, c->place_of_row, (int)c->per, (int)c->max_tiles, pitch};
+    if (int e = rows_any(r, (int)c->fmt, s)) return e;
     Fp4Args a = {};
-    a.y = (bf16*)(half ? y : h); a.ldy = half ? o.N : o.N / 2; a.wf = (const float*)o.wf; a.xf = (const float*)o.row_scale;
-    a.M = (int)pairs; a.N = o.N; a.K = o.K; a.rows_per_gate = 1; a.split = 1;
+    a.y = (bf16*)(half ? c->y : c->h); a.ldy = half ? o.N : o.N / 2; a.wf = (const float*)o.wf; a.xf = (const float*)o.row_scale;
+    a.M = (int)c->pairs; a.N = (int)o.N; a.K = (int)o.K; a.rows_per_gate = 1; a.split = 1;
     a.by16 = a.N % 8 == 0 && a.ldy % 8 == 0 && on16(a.y);
-    a.tile_expert = tile_expert; a.tile_row0 = tile_row0; a.tile_rows = tile_rows; a.max_tiles = max_tiles;
-    if (int e = launch_any(a, {o.w, o.ws, o.codes, o.scales, experts, pairs, (long)max_tiles * (pitch / 128)}, fmt, half == 0, tile, (int*)status, s)) return e;
+    a.tile_expert = c->tile_expert; a.tile_row0 = c->tile_row0; a.tile_rows = c->tile_rows; a.max_tiles = (int)c->max_tiles;
+    if (int e = launch_any(a, {o.w, o.ws, o.codes, o.scales, (int)c->experts, c->pairs, c->max_tiles * (pitch / 128)}, (int)c->fmt, half == 0, (int)c->tile,
+                           (int*)c->status, s))
+      return e;
   }
   return RC_OK;
 }

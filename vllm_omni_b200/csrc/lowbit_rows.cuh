@@ -81,19 +81,18 @@ __device__ __forceinline__ Chunk quantize_chunk(const uint4& u, float row_inv, b
   float v[8];
   unpack8(u, v);
   if (FMT == FMT_FP8) {
-    // the arithmetic of the fp8 layers' own quantiser (gemm_fp8_sm100.cu)
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float scale = fmaxf(amax, 1e-8f) * (1.0f / 448.0f), inv = 1.0f / scale;
+    // s = max / 448, code = e4m3(448 x / max) from a product with a reciprocal, off by a few steps of fp32, rounded to 17 bits: 448 x (11 bits) over max (8)
+    // is either exactly halfway between two e4m3 values (5 bits) or 2^-14 of itself away, so that this restores ties and makes none.
+    const uint32_t top = group_max<16>(max_pattern(u));
+    const float amax = fmaxf(__uint_as_float(top << 16), 1e-8f), inv = rcp_fast(amax) * 448.0f;
     uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * inv, v[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3) << (16 * (i & 1));
+    for (int i = 0; i < 4; ++i) {
+      const float lo = __uint_as_float((__float_as_uint(v[2 * i] * inv) + 0x40u) & ~0x7fu), hi = __uint_as_float((__float_as_uint(v[2 * i + 1] * inv) + 0x40u) & ~0x7fu);
+      w[i >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3) << (16 * (i & 1));
+    }
     out.code = make_uint2(w[0], w[1]);
-    out.scale = __float_as_uint(scale);
+    out.scale = top >= 0x7f80u ? 0x7fc00000u : __float_as_uint(amax * (1.0f / 448.0f));
     return out;
   }
   constexpr int PER = FMT == FMT_MXFP4 ? 4 : 2;                 // lanes of a block; a word is four blocks

@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 
 import torch
 import torch.nn.functional as F
@@ -72,7 +73,7 @@ class QuantRows:
         if index >= 0 and (codes.data_ptr() % 16 or scales.data_ptr() % 16):
             raise ValueError("codes and scales must begin on 16 bytes")
         self._codes, self._scales, self._row, self._buf = codes, scales, row_scale, None
-        self._at = (codes.data_ptr(), scales.data_ptr(), None if row_scale is None else row_scale.data_ptr())
+        self._at = (codes.data_ptr(), scales.data_ptr(), 0 if row_scale is None else row_scale.data_ptr())
         self.fmt, self.gated, self.rows, self.cols, self.experts, self.index = fmt, gated, rows, cols, lead[0] if lead else None, index
 
     @classmethod
@@ -84,7 +85,7 @@ class QuantRows:
         q._buf = buf = torch.empty(size, dtype=torch.uint8, device=_device(index))
         q.fmt, q.gated, q.rows, q.cols, q.experts, q.index = fmt, gated, rows, cols, experts, index
         p = buf.data_ptr()
-        q._at = (p, p + scales, p + row if fmt == "nvfp4" else None)
+        q._at = (p, p + scales, p + row if fmt == "nvfp4" else 0)
         return q
 
     def _part(self, which: int) -> torch.Tensor:
@@ -165,18 +166,24 @@ def _status(index: int) -> int:
 _current, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-_KINDS = {"p": ctypes.c_void_p, "l": ctypes.c_long, "i": ctypes.c_int, "f": ctypes.c_float}
-_ENTRIES = {"omni_lowbit_rows": "pllilipl" "pfplpl" "pppp", "omni_lowbit_dequantize": "ppplilii" "pp",
-            "omni_moe_plan_tiles": "piiiiiipppppp", "omni_moe_combine": "pppiiiplplp",
-            "omni_lowbit_linear": "plppp" "pppplliiii" "pipllpliipp", "omni_lowbit_experts": "plilii" "pppp" "pppp" "iipppp"}
+# operands of an entry point as one block of 8-byte fields (csrc/lowbit.cu)
+_BLOCKS = {"omni_lowbit_rows": "9qd8q", "omni_lowbit_dequantize": "10q", "omni_lowbit_linear": "26q", "omni_lowbit_experts": "34q"}
 
 
 @functools.lru_cache(maxsize=None)
 def _entry(name: str):
-    """An entry point that takes plain Python numbers: converting them by declared types is half the cost of wrapping each."""
-    lib = nv.lib("moe" if name.startswith("omni_moe") else "lowbit")
-    raw = getattr(lib._cdll, name)
-    raw.argtypes = [_KINDS[k] for k in _ENTRIES[name]]
+    """``call(*numbers)`` of an entry point; pointers that are absent are 0."""
+    lib, pack = nv.lib("lowbit"), struct.Struct(_BLOCKS[name]).pack
+    getattr(lib._cdll, name).argtypes = [ctypes.c_char_p]
+    fn = getattr(lib, name)
+    return lambda *fields: fn(pack(*fields))
+
+
+@functools.lru_cache(maxsize=None)
+def _moe_entry(name: str, kinds: str):
+    """An entry point of the ``moe`` library that takes plain Python numbers."""
+    lib = nv.lib("moe")
+    getattr(lib._cdll, name).argtypes = [{"p": ctypes.c_void_p, "l": c_long, "i": c_int}[k] for k in kinds]
     return getattr(lib, name)
 
 
@@ -215,8 +222,9 @@ def _quantize_torch(x: torch.Tensor, fmt: str, gated: bool = False) -> QuantRows
     b = f.unflatten(-1, (-1, BLOCK[fmt]))
     size = b.abs().amax(-1)
     if fmt == "fp8":
-        scale = size.nan_to_num(0.0, float("inf")).clamp_min(1e-8) * torch.tensor(1.0 / 448.0, dtype=torch.float32)
-        q = (b * (1.0 / scale)[..., None]).clamp(-448.0, 448.0)
+        size = size.clamp_min(1e-8)
+        scale = torch.where(torch.isfinite(size), size * torch.tensor(1.0 / 448.0, dtype=torch.float32), float("nan"))
+        q = (b * 448.0 / size[..., None]).clamp(-448.0, 448.0)
         return QuantRows(q.flatten(-2).to(torch.float8_e4m3fn).view(torch.uint8), scale.contiguous(), fmt)
     fine = torch.isfinite(size)
     size = torch.where(fine, size, 0.0)
@@ -272,10 +280,10 @@ def _rows(x, fmt, *, residual=None, gain=None, eps=0.0, total=None, normed=None,
     q = QuantRows._empty(fmt, per, cols, index, experts, gated)
     codes, scales, row = q._at
     if gain is None:
-        rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], None, 0, None, 0.0, None, 0, None, 0, codes, scales, row,
+        rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], 0, 0, 0, 0.0, 0, 0, 0, 0, codes, scales, row,
                                         _stream(index))
     else:
-        at = lambda t: (None, 0) if t is None else (t.data_ptr(), t.stride(0))
+        at = lambda t: (0, 0) if t is None else (t.data_ptr(), t.stride(0))
         rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], *at(residual), gain.data_ptr(), eps, *at(total), *at(normed),
                                         codes, scales, row, _stream(index))
     if rc:
@@ -429,7 +437,7 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
     if _current() != index:
         with torch.cuda.device(index):
             return linear(x, w, bias, act, residual, gate, out, force_tile, force_split)
-    raw, ldx = None, 0
+    raw = ldx = 0
     if q is None:
         _check_cols(fmt, cols)
         x = _rows16(x, "x")
@@ -443,10 +451,10 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
         try:
             o2 = out if out.dim() == 2 else out.view(M, N)
         except RuntimeError:                      # rows of several batches that no single pitch reaches
-            return out.copy_(linear(x if raw is None else x.view(*lead, cols), w, bias, act, residual, gate, None, force_tile, force_split))
+            return out.copy_(linear(x.view(*lead, cols) if raw else x, w, bias, act, residual, gate, None, force_tile, force_split))
     ldo, yp = o2.stride(), o2.data_ptr()
-    rp = bp = gp = None
-    ldr, lds, per = (0, 1), 0, 0
+    rp = bp = gp = lds = per = 0
+    ldr = (0, 1)
     if residual is not None:
         r2 = residual if residual.dim() == 2 else residual.reshape(M, N)
         rp, ldr = r2.data_ptr(), r2.stride()
@@ -480,10 +488,6 @@ def _expert_layout(fmt: str, pairs: int, max_tiles: int, scale_rows: int, D: int
         at.append(end)
         end += -(-size // 256) * 256
     return end, at
-
-
-class _ExpertOperand(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("codes", "scales", "row_scale", "w", "ws", "wf")] + [("N", c_int), ("K", c_int)]
 
 
 def _tile_rows(pairs: int, experts: int) -> int:
@@ -545,15 +549,16 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
     work = torch.empty(size, dtype=torch.uint8, device=dev)
     base = work.data_ptr()
     row_of_pair, te, tr, tn, n_rows, place, h, y, *ops = [base + v for v in at]
-    up_op, down_op = (_ExpertOperand(*ops[i:i + 2], ops[i + 2] if fmt == "nvfp4" else None, *w._at, w.rows, w.cols) for i, w in ((0, up), (3, down)))
+    if fmt != "nvfp4":
+        ops[2] = ops[5] = 0
     status, stream = _status(up.index), _stream(up.index)
     if nv.bounds_check_enabled():
         nv.lib("moe").omni_moe_set_bounds(c_long(pairs), ctypes.c_void_p(status))
-    rc = _entry("omni_moe_plan_tiles")(ids.data_ptr(), pairs, E, 0, E, tile, max_tiles, row_of_pair, te, tr, tn, n_rows, stream)
-    rc = rc or _entry("omni_lowbit_experts")(x2.data_ptr(), x2.stride(0), k, pairs, E, FORMATS[fmt], ctypes.addressof(up_op), ctypes.addressof(down_op), h, y, row_of_pair,
-                                             te, tr, tn, max_tiles, tile, n_rows, place, status, stream)
-    rc = rc or _entry("omni_moe_combine")(y, row_of_pair, weights.data_ptr(), T, k, D, None if res is None else res.data_ptr(), 0 if res is None else res.stride(0),
-                                          o2.data_ptr(), o2.stride(0), stream)
+    rc = _moe_entry("omni_moe_plan_tiles", "piiiiiipppppp")(ids.data_ptr(), pairs, E, 0, E, tile, max_tiles, row_of_pair, te, tr, tn, n_rows, stream)
+    rc = rc or _entry("omni_lowbit_experts")(x2.data_ptr(), x2.stride(0), k, pairs, E, FORMATS[fmt], h, y, row_of_pair, te, tr, tn, max_tiles, tile, n_rows, place, status,
+                                             stream, *ops[:3], *up._at, up.rows, D, *ops[3:], *down._at, down.rows, Fd)
+    rc = rc or _moe_entry("omni_moe_combine", "pppiiiplplp")(y, row_of_pair, weights.data_ptr(), T, k, D, 0 if res is None else res.data_ptr(),
+                                                             0 if res is None else res.stride(0), o2.data_ptr(), o2.stride(0), stream)
     if rc:
         nv.check_rc(rc, "experts")
     return out if o2 is out else out.copy_(o2)
