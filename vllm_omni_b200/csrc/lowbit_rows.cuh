@@ -7,6 +7,7 @@
 #include <cuda_fp4.h>
 #include <cuda_fp8.h>
 
+#include "f32x2.cuh"
 #include "host_util.h"
 #include "lowbit.cuh"
 
@@ -30,30 +31,37 @@ struct RowsArgs {
   uint8_t* codes;
   void* scales;
   float* row_scale;
-  int K, tpr;                    // threads per row, a multiple of 32
-  float eps;
+  int K;
+  float eps, inv_k;              // 1 / K
   RowPlace place;
 };
 
-// largest magnitude of eight bf16, as a 15-bit pattern: ordered like the magnitudes, with infinity and NaN above all numbers
-__device__ __forceinline__ uint32_t max_pattern(const uint4& u) {
-  const uint32_t m = 0x7fff7fffu;
-  const uint32_t a = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
-  return max(a & 0xffffu, a >> 16);
+// The larger magnitudes of pairs of bf16, NaN above all: one instruction per pair of registers.
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("{\n\t.reg .b32 x, y;\n\tabs.bf16x2 x, %1;\n\tabs.bf16x2 y, %2;\n\tmax.NaN.bf16x2 %0, x, y;\n\t}" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
-
+// of eight bf16, two magnitudes side by side that hold the largest
+__device__ __forceinline__ uint32_t max_pair(const uint4& u) { return max_abs2(max_abs2(u.x, u.y), max_abs2(u.z, u.w)); }
+// Largest magnitude of LANES neighbouring lanes as a 15-bit pattern: ordered like the magnitudes, infinity and NaN from 0x7f80 on.
 template <int LANES>
-__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+__device__ __forceinline__ uint32_t group_top(uint32_t pair) {
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  for (int o = LANES / 2; o > 0; o >>= 1) pair = max_abs2(pair, __shfl_xor_sync(0xffffffffu, pair, o));
+  return max_abs2(pair, pair >> 16) & 0xffffu;
 }
 
+// eight values to e2m1, the first in the lowest half byte (the converted bytes merge into one register)
 __device__ __forceinline__ uint32_t e2m1x8(const float (&q)[8]) {
-  uint32_t out = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    out |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(q[2 * i], q[2 * i + 1]), __NV_E2M1, cudaRoundNearest) << (8 * i);
+  uint32_t out;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(out) : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
   return out;
 }
 
@@ -68,101 +76,119 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return y;
 }
 
-// Codes of a chunk (4-bit: x; fp8: x and y) and its scale: the whole word on every lane of its four blocks (4-bit), an fp32 (fp8).
+// Codes of a chunk (4-bit: x; fp8: x and y) and the scale of its block: a byte (4-bit), an fp32 (fp8).
 struct Chunk {
   uint2 code;
   uint32_t scale;
 };
-// Eight elements per lane; `row_inv` (nvfp4) the reciprocal of the row's factor; `in`: the chunk exists (else its bytes of the word are zero).
+// Eight elements per lane; `row_inv` (nvfp4) the reciprocal of the row's factor.  The integer pipe bounds this (8191 x 12288 to mxfp4: 78 % busy at 61 us with
+// integer maxima, shifts that assemble scale words and bytes), so maxima are taken on packed pairs, products and roundings on the floating-point pipe.
 template <int FMT>
-__device__ __forceinline__ Chunk quantize_chunk(const uint4& u, float row_inv, bool in) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ Chunk quantize_chunk(const uint4& u, float row_inv) {
   Chunk out;
   float v[8];
   unpack8(u, v);
   if (FMT == FMT_FP8) {
     // s = max / 448, code = e4m3(448 x / max) from a product with a reciprocal, off by a few steps of fp32, rounded to 17 bits: 448 x (11 bits) over max (8)
-    // is either exactly halfway between two e4m3 values (5 bits) or 2^-14 of itself away, so that this restores ties and makes none.
-    const uint32_t top = group_max<16>(max_pattern(u));
+    // is either exactly halfway between two e4m3 values (5 bits) or 2^-14 of itself away, so that this restores ties and makes none.  The
+    // rounding is Veltkamp's: c = (2^7 + 1) q, q' = c - (c - q).
+    const uint32_t top = group_top<16>(max_pair(u));
     const float amax = fmaxf(__uint_as_float(top << 16), 1e-8f), inv = rcp_fast(amax) * 448.0f;
+    const uint64_t inv2 = pack2(inv, inv), split = pack2(129.0f, 129.0f), minus = pack2(-1.0f, -1.0f);
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float lo = __uint_as_float((__float_as_uint(v[2 * i] * inv) + 0x40u) & ~0x7fu), hi = __uint_as_float((__float_as_uint(v[2 * i + 1] * inv) + 0x40u) & ~0x7fu);
+      const uint64_t q = mul2(pack2(v[2 * i], v[2 * i + 1]), inv2), c = mul2(q, split), d = fma2(q, minus, c), r = fma2(d, minus, c);
+      float lo, hi;
+      unpack2(r, lo, hi);
       w[i >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3) << (16 * (i & 1));
     }
     out.code = make_uint2(w[0], w[1]);
     out.scale = top >= 0x7f80u ? 0x7fc00000u : __float_as_uint(amax * (1.0f / 448.0f));
     return out;
   }
-  constexpr int PER = FMT == FMT_MXFP4 ? 4 : 2;                 // lanes of a block; a word is four blocks
-  const uint32_t top = group_max<PER>(max_pattern(u));
-  uint32_t byte;
+  const uint32_t top = group_top<FMT == FMT_MXFP4 ? 4 : 2>(max_pair(u));
   float q[8];
   if (FMT == FMT_MXFP4) {
     // the power of two two below the largest magnitude's (6 = 1.5 * 2^2 is the largest code): dividing by it is exact
     const uint32_t e = top >> 7;
-    byte = e == 255 ? 255 : e > 2 ? e - 2 : 0;
-    const float inv = __uint_as_float((254u - byte) << 23);     // 2^-(byte - 127); no finite block's byte is above 252
+    out.scale = e == 255 ? 255 : e > 2 ? e - 2 : 0;
+    const float inv = __uint_as_float((254u - out.scale) << 23);     // 2^-(byte - 127); no finite block's byte is above 252
+    const uint64_t inv2 = pack2(inv, inv);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = v[i] * inv;
+    for (int i = 0; i < 4; ++i) unpack2(mul2(pack2(v[2 * i], v[2 * i + 1]), inv2), q[2 * i], q[2 * i + 1]);
   } else {
     // s = e4m3(max / 6), code = e2m1(x / s).  Both quotients are products with a reciprocal, off by a few steps of fp32, rounded to fp16 before they are
     // rounded to the format: max / 6 (8-bit mantissas) is either exactly halfway between two e4m3 values or 2^-9 of itself away, and so is x / s (8 by
     // 4 bits) for e2m1, so that the 11 bits of fp16 keep what is no tie from becoming one and restore what is.
     const __half want = __float2half_rn(__uint_as_float(top << 16) * row_inv * (1.0f / 6.0f));
-    byte = __nv_cvt_halfraw_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
+    const uint32_t byte = __nv_cvt_halfraw_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
     const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
     const float inv = s > 0.f ? rcp_fast(s) : 0.f;
+    const uint64_t row2 = pack2(row_inv, row_inv), inv2 = pack2(inv, inv);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(__floats2half2_rn(v[2 * i] * row_inv * inv, v[2 * i + 1] * row_inv * inv));
+      float lo, hi;
+      unpack2(mul2(mul2(pack2(v[2 * i], v[2 * i + 1]), row2), inv2), lo, hi);
+      const float2 f = __half22float2(__floats2half2_rn(lo, hi));
       q[2 * i] = f.x;
       q[2 * i + 1] = f.y;
     }
-    if (top >= 0x7f80u) byte = 0x7f;
+    out.scale = top >= 0x7f80u ? 0x7f : byte;
   }
   out.code = make_uint2(e2m1x8(q), 0u);
-  uint32_t word = in ? byte << (8 * ((lane / PER) & 3)) : 0u;
-  word |= __shfl_xor_sync(0xffffffffu, word, PER);
-  out.scale = word | __shfl_xor_sync(0xffffffffu, word, 2 * PER);
   return out;
 }
 
-template <int FMT>
-__device__ __forceinline__ void store_chunk(const RowsArgs& a, const Chunk& c, int chunk, long code_row, long scale_row) {
-  const int lane = threadIdx.x & 31;
-  if (FMT == FMT_FP8) {
-    if (chunk * 8 < a.K) {
-      *reinterpret_cast<uint2*>(a.codes + code_row * a.K + chunk * 8) = c.code;
-      if ((lane & 15) == 0) static_cast<uint32_t*>(a.scales)[scale_row * (a.K / 128) + chunk / 16] = c.scale;
+// Where a thread's chunks go: chunk tid + i * tpr.  tpr is a multiple of 32, so that a block's first lane and its byte of the word are the same for all i.
+template <int FMT> struct ChunkPlace {
+  uint8_t *code, *scale;
+  int code_step, scale_step, left, scales_left;                 // chunks (and of them ones with a place for a scale) from this thread's first on
+  bool first;                                                   // of its block
+  __device__ __forceinline__ ChunkPlace(const RowsArgs& a, long code_row, long scale_row, int tid, int tpr) {
+    constexpr int PER = FMT == FMT_FP8 ? 16 : FMT == FMT_MXFP4 ? 4 : 2;
+    first = tid % PER == 0;
+    left = a.K / 8 - tid;
+    if (FMT == FMT_FP8) {
+      code = a.codes + code_row * a.K + tid * 8;
+      scale = static_cast<uint8_t*>(a.scales) + (scale_row * (a.K / 128) + tid / 16) * 4;
+      code_step = tpr * 8; scale_step = tpr / 16 * 4; scales_left = left;
+    } else {
+      const int words = scale_words(FMT, a.K);
+      code = a.codes + code_row * (a.K / 2) + tid * 4;
+      scale = static_cast<uint8_t*>(a.scales) + scale_word_at(scale_row, tid / (4 * PER), words) + tid / PER % 4;
+      code_step = tpr * 4; scale_step = tpr / (4 * PER) * 512; scales_left = words * 4 * PER - tid;      // blocks past K in a row's last word: zeros
     }
-  } else {
-    constexpr int PER = FMT == FMT_MXFP4 ? 4 : 2;
-    if (chunk * 8 < a.K) *reinterpret_cast<uint32_t*>(a.codes + code_row * (a.K / 2) + chunk * 4) = c.code.x;
-    const int words = scale_words(FMT, a.K), at = chunk / (4 * PER);
-    if (lane % (4 * PER) == 0 && at < words)
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.scales) + scale_word_at(scale_row, at, words)) = c.scale;
   }
-}
+  __device__ __forceinline__ void store(const Chunk& c, int i, int tpr) const {
+    if (i * tpr < left) {
+      if (FMT == FMT_FP8) *reinterpret_cast<uint2*>(code + (long)i * code_step) = c.code;
+      else *reinterpret_cast<uint32_t*>(code + (long)i * code_step) = c.code.x;
+    }
+    if (first && i * tpr < scales_left) {
+      if (FMT == FMT_FP8) *reinterpret_cast<uint32_t*>(scale + (long)i * scale_step) = c.scale;
+      else scale[(long)i * scale_step] = (uint8_t)c.scale;
+    }
+  }
+};
 
 constexpr int GATHER_MOST = 8;   // choices placed at a time
 
-// NV chunks per thread, a.tpr threads per row, blockDim / tpr rows per block.
-template <int FMT, bool NORM, int MODE, int NV>
-__global__ void __launch_bounds__(1024)
+// NV chunks per thread, blockDim.x threads (a multiple of 32) per row, blockDim.y rows per block.
+template <int FMT, bool NORM, int MODE, int NV, int MOST>
+__global__ void __launch_bounds__(MOST)
 lowbit_rows_kernel(const RowsArgs a) {
   __shared__ uint32_t red[32];
-  const int sub = threadIdx.x / a.tpr, tid = threadIdx.x - sub * a.tpr, lane = threadIdx.x & 31;
-  const int warps = a.tpr >> 5, warp0 = sub * warps;
-  const long item = (long)blockIdx.x * (blockDim.x / a.tpr) + sub;
+  const int tid = threadIdx.x, sub = threadIdx.y, tpr = blockDim.x, lane = tid & 31;
+  const int warps = tpr >> 5, warp0 = sub * warps, warp = warp0 + (tid >> 5);
+  const long item = (long)blockIdx.x * blockDim.y + sub;
   const RowPlace& pl = a.place;
   bool live = item < a.rows;
   pdl_begin();
   uint4 u[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = tid + i * a.tpr;
+    const int c = tid + i * tpr;
     u[i] = live && c * 8 < a.K ? *reinterpret_cast<const uint4*>(a.x + item * a.ldx + c * 8) : make_uint4(0u, 0u, 0u, 0u);
   }
   long scale_row = item;
@@ -179,7 +205,7 @@ lowbit_rows_kernel(const RowsArgs a) {
       uint4 r[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = tid + i * a.tpr;
+        const int c = tid + i * tpr;
         r[i] = live && c * 8 < a.K ? *reinterpret_cast<const uint4*>(a.residual + item * a.ldr + c * 8) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
@@ -194,7 +220,7 @@ lowbit_rows_kernel(const RowsArgs a) {
     uint4 gain[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = tid + i * a.tpr;
+      const int c = tid + i * tpr;
       const bool in = live && c * 8 < a.K;
       gain[i] = in ? *reinterpret_cast<const uint4*>(a.gain + c * 8) : make_uint4(0u, 0u, 0u, 0u);
       if (a.total && in) *reinterpret_cast<uint4*>(a.total + item * a.ldt + c * 8) = u[i];
@@ -206,16 +232,16 @@ lowbit_rows_kernel(const RowsArgs a) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (warps > 1) {
-      if (lane == 0) red[threadIdx.x >> 5] = __float_as_uint(ss);
+      if (lane == 0) red[warp] = __float_as_uint(ss);
       __syncthreads();
       ss = 0.f;
       for (int w = 0; w < warps; ++w) ss += __uint_as_float(red[warp0 + w]);
       if (FMT == FMT_NVFP4) __syncthreads();
     }
-    const float r = 1.0f / sqrtf(ss / (float)a.K + a.eps);
+    const float r = rsqrtf(ss * a.inv_k + a.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = tid + i * a.tpr;
+      const int c = tid + i * tpr;
       float v[8], g[8];
       unpack8(u[i], v);
       unpack8(gain[i], g);
@@ -230,10 +256,10 @@ lowbit_rows_kernel(const RowsArgs a) {
     // the row's factor: the power of two that puts the row's largest magnitude into [2^10, 2^11), its block's scale into [170, 342)
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) top = max(top, max_pattern(u[i]));
-    top = __reduce_max_sync(0xffffffffu, top);
+    for (int i = 0; i < NV; ++i) top = max_abs2(top, max_pair(u[i]));
+    top = __reduce_max_sync(0xffffffffu, max_abs2(top, top >> 16) & 0xffffu);
     if (warps > 1) {
-      if (lane == 0) red[threadIdx.x >> 5] = top;
+      if (lane == 0) red[warp] = top;
       __syncthreads();
       for (int w = 0; w < warps; ++w) top = max(top, red[warp0 + w]);
     }
@@ -243,12 +269,13 @@ lowbit_rows_kernel(const RowsArgs a) {
   }
   Chunk c[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) c[i] = quantize_chunk<FMT>(u[i], row_inv, (tid + i * a.tpr) * 8 < a.K);
+  for (int i = 0; i < NV; ++i) c[i] = quantize_chunk<FMT>(u[i], row_inv);
   if (MODE != GATHER) {
     if (!live) return;
     if (FMT == FMT_NVFP4 && tid == 0) a.row_scale[item] = factor;
+    const ChunkPlace<FMT> to(a, item, scale_row, tid, tpr);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) store_chunk<FMT>(a, c[i], tid + i * a.tpr, item, scale_row);
+    for (int i = 0; i < NV; ++i) to.store(c[i], i, tpr);
   } else {
     // quantised once, written once per choice; the tiles of up to eight choices are looked for together, a tile per thread
     __shared__ int found[32][GATHER_MOST];
@@ -259,7 +286,7 @@ lowbit_rows_kernel(const RowsArgs a) {
       __syncthreads();
       if (tid < GATHER_MOST) found[sub][tid] = -1;
       __syncthreads();
-      for (int t = tid; t < pl.max_tiles; t += a.tpr) {
+      for (int t = tid; t < pl.max_tiles; t += tpr) {
         const int first = pl.tile_row0[t], n = pl.tile_expert[t] >= 0 ? pl.tile_rows[t] : 0;
 #pragma unroll
         for (int j = 0; j < GATHER_MOST; ++j)
@@ -275,8 +302,9 @@ lowbit_rows_kernel(const RowsArgs a) {
           pl.place_of_row[r] = at;
           if (FMT == FMT_NVFP4) a.row_scale[r] = factor;
         }
+        const ChunkPlace<FMT> to(a, r, at, tid, tpr);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) store_chunk<FMT>(a, c[i], tid + i * a.tpr, r, at);
+        for (int i = 0; i < NV; ++i) to.store(c[i], i, tpr);
       }
     }
   }
@@ -360,26 +388,24 @@ dequantize_kernel(const DequantArgs a) {
   }
 }
 
-// Threads per row and chunks per thread: up to two rows per SM a lane per chunk (one round trip); for more, four chunks per lane.
-static void row_threads(int K, long rows, bool norm, int& tpr, int& nv) {
-  const int chunks = K / 8;
-  nv = rows <= 2L * sm_count() ? 1 : norm ? 2 : 4;
-  while (nv < 4 && chunks > 1024 * nv) nv *= 2;
-  while (nv > 1 && chunks <= 32 * (nv / 2)) nv /= 2;
-  tpr = (chunks + 32 * nv - 1) / (32 * nv) * 32;
-}
-
+// Threads per row and chunks per thread: up to two rows per SM a lane per chunk (one round trip); for more, up to four chunks per lane, which share what a
+// thread does once per row.
 template <int FMT, bool NORM, int MODE>
 static int launch_rows(RowsArgs& a, cudaStream_t s) {
-  int nv;
-  row_threads(a.K, a.rows, NORM, a.tpr, nv);
-  if (a.tpr > 1024) return RC_TOO_LARGE;
-  const int per = a.tpr >= 256 ? 1 : 256 / a.tpr, threads = per * a.tpr;
-  const unsigned grid = (unsigned)((a.rows + per - 1) / per);
+  const int chunks = a.K / 8;
+  int nv = a.rows <= 2L * sm_count() ? 1 : 4;
+  while (nv < 4 && chunks > 1024 * nv) nv *= 2;
+  while (nv > 1 && chunks <= 32 * (nv / 2)) nv /= 2;
+  const int tpr = (chunks + 32 * nv - 1) / (32 * nv) * 32;
+  if (tpr > 1024) return RC_TOO_LARGE;
+  const dim3 block(tpr, tpr >= 256 ? 1 : 256 / tpr);
+  const unsigned grid = (unsigned)((a.rows + block.y - 1) / block.y);
+  a.inv_k = 1.0f / (float)a.K;
+  if (nv == 4 && tpr > 512) return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 4, 1024>, grid, block, 0, s, a);
   switch (nv) {
-    case 1: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 1>, grid, threads, 0, s, a);
-    case 2: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 2>, grid, threads, 0, s, a);
-    default: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 4>, grid, threads, 0, s, a);
+    case 1: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 1, 1024>, grid, block, 0, s, a);
+    case 2: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 2, 1024>, grid, block, 0, s, a);
+    default: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 4, 512>, grid, block, 0, s, a);
   }
 }
 
