@@ -256,21 +256,21 @@ struct RowTile {
   int expert, rows, scale_tile;
   long row0;
 };
+// Loads only, so that a role can ask for its next tile before it works on this one; expert < 0: no more tiles (used ones come first).
 template <int XR>
-__device__ __forceinline__ bool row_tile(const Fp4Args& a, int t, RowTile& r) {
+__device__ __forceinline__ RowTile row_tile(const Fp4Args& a, int t) {
+  RowTile r;
+  r.scale_tile = t * (XR > 128 ? 2 : 1);      // XR = 16, 64: one tile only, or an expert's
   if (a.tile_expert) {
     r.expert = a.tile_expert[t];
-    if (r.expert < 0) return false;           // used tiles come first
     r.row0 = a.tile_row0[t];
     r.rows = a.tile_rows[t];
-    r.scale_tile = t * (XR > 128 ? 2 : 1);
-    return true;
+  } else {
+    r.expert = 0;
+    r.row0 = (long)t * XR;
+    r.rows = min(XR, a.M - t * XR);
   }
-  r.expert = 0;
-  r.row0 = (long)t * XR;
-  r.rows = min(XR, a.M - t * XR);
-  r.scale_tile = t * (XR > 128 ? 2 : 1);      // XR = 64 has one tile only, or an expert's
-  return true;
+  return r;
 }
 
 template <int FMT, int XR, int EPI, bool PAIR>
@@ -334,6 +334,8 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
   auto tile_of = [&](int it) { return experts ? it / num_n : it % a.max_tiles; };
   auto block_of = [&](int it) { return (experts ? it % num_n : it / a.max_tiles) * (PAIR ? 2 : 1) + rank; };
 
+  auto tile_at = [&](int it) { return row_tile<XR>(a, tile_of(min(it, num_items - 1))); };
+
   // the first item's weights into L2 while the kernel before (the rows' quantiser) runs out
   if (!experts && warp == 0 && first < num_items && elect_one())
     for (int kb = kb0; kb < kb1 && kb < kb0 + PREFETCH; ++kb) {
@@ -347,9 +349,11 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
     if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
+      RowTile next = tile_at(first);
       for (int it = first; it < num_items; it += step) {
-        RowTile t;
-        if (!row_tile<XR>(a, tile_of(it), t)) break;
+        const RowTile t = next;
+        if (t.expert < 0) break;
+        next = tile_at(it + step);
         const int nb = block_of(it), mine = PAIR ? (t.rows + 31) / 32 * 16 : t.rows, boxes = (mine + Cfg::BOX - 1) / Cfg::BOX;
         const int x0 = (int)t.row0 + rank * mine;
         const uint32_t bytes = Cfg::W_BYTES + boxes * Cfg::BOX * 128 + Cfg::WS_BYTES + Cfg::XS_BYTES;
@@ -379,9 +383,11 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
     if (rank == 0 && elect_one()) {
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
+      RowTile next = tile_at(first);
       for (int it = first; it < num_items; it += step) {
-        RowTile t;
-        if (!row_tile<XR>(a, tile_of(it), t)) break;
+        const RowTile t = next;
+        if (t.expert < 0) break;
+        next = tile_at(it + step);
         const uint32_t n = (t.rows + STEP - 1) / STEP * STEP;
         const uint32_t idesc = fp4_idesc<FMT>(PAIR ? 256 : 128, n, 0);
         mbar_wait(smem_u32(&tempty_bar[acc]), acc_phase ^ 1, &s_abort, status, ERR_WAIT_TMEM_EMPTY);
@@ -432,9 +438,11 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
     const uint32_t turned = smem_base + STAGES * Cfg::STAGE_PITCH + (warp - 2) * 1024;
     int acc = 0;
     uint32_t acc_phase = 0;
+    RowTile next = tile_at(first);
     for (int it = first; it < num_items; it += step) {
-      RowTile t;
-      if (!row_tile<XR>(a, tile_of(it), t)) break;
+      const RowTile t = next;
+      if (t.expert < 0) break;
+      next = tile_at(it + step);
       const int n0 = block_of(it) * 128 + q * 32, c0 = part * 16 * Cfg::CHUNKS;
       Fp4Lane<EPI> keep;
       keep.load(a, (long)t.expert * a.N, n0, lane);
@@ -514,8 +522,8 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
     // [owner][row of X][width]; the owner reads its block of every CTA where it lies and adds them in the order of the shares.
     __syncwarp();
     cluster_sync_all();
-    RowTile t;
-    if (first < num_items && row_tile<XR>(a, tile_of(first), t)) {
+    if (first < num_items) {
+      const RowTile t = tile_at(first);
       const int width = 128 / a.split, n0 = block_of(first) * 128 + share * width, outs = GATED ? width / 2 : width, quads = outs / 4, total = t.rows * quads;
       const uint32_t block = smem_base + share * t.rows * width * 4;
       auto column = [&](int o) { return GATED ? o / 8 * 16 + o % 8 : o; };       // of the block, where output o (or its gate) stands

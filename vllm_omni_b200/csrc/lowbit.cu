@@ -86,7 +86,8 @@ extern "C" int omni_lowbit_linear(const LowbitLinear* c) {
 }
 
 // Rows of x (pair p reads row p / per, pairs a multiple of per) through `up` (gated, N = 2 F) to h [pairs, F] and through `down` to y [pairs, D], both in the
-// plan's order of rows; tile: the most rows a tile has, 64 / 128 / 256; n_rows: how many rows the plan has; place_of_row [pairs]: scratch.
+// plan's order of rows; tile: the most rows a tile has, 64 / 128 / 256; place_of_pair: for tiles from every 128 rows on (tile 256: 256); n_rows: how many rows the
+// plan has; place_of_row [pairs]: scratch.
 struct ExpertOperand {           // one product's rows in a workspace, and its weights
   void *codes, *scales, *row_scale;
   const void *w, *ws, *wf;
@@ -96,7 +97,7 @@ struct LowbitExperts {
   const void* x;
   long ldx, per, pairs, experts, fmt;
   void *h, *y;
-  const int *row_of_pair, *tile_expert, *tile_row0, *tile_rows;
+  const int *row_of_pair, *place_of_pair, *tile_expert, *tile_row0, *tile_rows;
   long max_tiles, tile;
   const int* n_rows;
   int* place_of_row;
@@ -106,7 +107,7 @@ struct LowbitExperts {
 extern "C" int omni_lowbit_experts(const LowbitExperts* c) {
   const ExpertOperand &up = c->up, &down = c->down;
   if (c->pairs <= 0 || c->max_tiles <= 0) return RC_OK;
-  if (c->pairs > 0x7fffff00L || c->per < 1 || c->pairs % c->per || c->experts < 1 || !c->row_of_pair || !c->n_rows || !c->place_of_row || !c->tile_expert ||
+  if (c->pairs > 0x7fffff00L || c->per < 1 || c->pairs % c->per || c->experts < 1 || !c->row_of_pair || !c->place_of_pair || !c->n_rows || !c->place_of_row || !c->tile_expert ||
       !c->tile_row0 || !c->tile_rows || up.N % 16 || up.N != 2 * down.K || up.K != down.N || up.K % 32 || down.K % 32 || c->fmt == FMT_FP8)
     return RC_BAD_ARG;
   cudaStream_t s = (cudaStream_t)c->stream;
@@ -116,7 +117,7 @@ extern "C" int omni_lowbit_experts(const LowbitExperts* c) {
     RowsArgs r = {};
     r.x = (const bf16*)(half ? c->h : c->x); r.ldx = half ? o.K : c->ldx; r.rows = half ? c->pairs : c->pairs / c->per; r.K = (int)o.K;
     r.codes = (uint8_t*)o.codes; r.scales = o.scales; r.row_scale = (float*)o.row_scale;
-    r.place = {1, half ? nullptr : c->row_of_pair, c->tile_expert, c->tile_row0, c->tile_rows, c->n_rows, c->place_of_row, (int)c->per, (int)c->max_tiles, pitch};
+    r.place = {1, half ? nullptr : c->row_of_pair, c->place_of_pair, c->n_rows, c->place_of_row, (int)c->per};
     if (int e = rows_any(r, (int)c->fmt, s)) return e;
     Fp4Args a = {};
     a.y = (bf16*)(half ? c->y : c->h); a.ldy = half ? o.N : o.N / 2; a.wf = (const float*)o.wf; a.xf = (const float*)o.row_scale;

@@ -14,14 +14,14 @@
 namespace omni {
 
 // Where a launch's rows go.  ROWS: row r of x to row r, scales by groups of `group` rows (the experts of a weight), each from a new tile of 128 on.
-// GATHER: item t is a token, its row goes to the rows row_of_pair[t * per ..] of its choices, and scales to the place of the tile those lie in: row i of
-// tile t at t * pitch + i; place_of_row keeps that.  PLACED: row r to row r, scales to place_of_row[r] (rows that no choice has are left out).
+// GATHER: item t is a token, its row goes to the rows row_of_pair[t * per ..] of its choices (< 0: nowhere), their scales to place_of_pair[t * per ..], which
+// place_of_row keeps.  PLACED: row r to row r, scales to place_of_row[r]; rows from *n_rows on are left out.
 enum RowMode : int { ROWS = 0, GATHER = 1, PLACED = 2 };
 struct RowPlace {
   long group;
-  const int *row_of_pair, *tile_expert, *tile_row0, *tile_rows, *n_rows;
+  const int *row_of_pair, *place_of_pair, *n_rows;
   int* place_of_row;
-  int per, max_tiles, pitch;
+  int per;
 };
 
 struct RowsArgs {
@@ -172,8 +172,6 @@ template <int FMT> struct ChunkPlace {
   }
 };
 
-constexpr int GATHER_MOST = 8;   // choices placed at a time
-
 // NV chunks per thread, blockDim.x threads (a multiple of 32) per row, blockDim.y rows per block.
 template <int FMT, bool NORM, int MODE, int NV, int MOST>
 __global__ void __launch_bounds__(MOST)
@@ -277,32 +275,25 @@ lowbit_rows_kernel(const RowsArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) to.store(c[i], i, tpr);
   } else {
-    // quantised once, written once per choice; the tiles of up to eight choices are looked for together, a tile per thread
-    __shared__ int found[32][GATHER_MOST];
-    for (int j0 = 0; j0 < pl.per; j0 += GATHER_MOST) {
-      int row[GATHER_MOST];
-#pragma unroll
-      for (int j = 0; j < GATHER_MOST; ++j) row[j] = live && j0 + j < pl.per ? pl.row_of_pair[item * pl.per + j0 + j] : -1;
-      __syncthreads();
-      if (tid < GATHER_MOST) found[sub][tid] = -1;
-      __syncthreads();
-      for (int t = tid; t < pl.max_tiles; t += tpr) {
-        const int first = pl.tile_row0[t], n = pl.tile_expert[t] >= 0 ? pl.tile_rows[t] : 0;
-#pragma unroll
-        for (int j = 0; j < GATHER_MOST; ++j)
-          if (row[j] >= first && row[j] < first + n) found[sub][j] = t * pl.pitch + (row[j] - first);
-      }
-      __syncthreads();
+    // quantised once, written once per choice
+    if (!live) return;
 #pragma unroll 1
-      for (int j = 0; j < GATHER_MOST; ++j) {
-        const int r = __shfl_sync(0xffffffffu, live && j0 + j < pl.per ? pl.row_of_pair[item * pl.per + j0 + j] : -1, 0);
-        const int at = found[sub][j];
-        if (r < 0 || at < 0) continue;
+    for (int j0 = 0; j0 < pl.per; j0 += 4) {
+      int row[4], place[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = j0 + j < pl.per;
+        row[j] = in ? pl.row_of_pair[item * pl.per + j0 + j] : -1;
+        place[j] = in ? pl.place_of_pair[item * pl.per + j0 + j] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (row[j] < 0) continue;
         if (tid == 0) {
-          pl.place_of_row[r] = at;
-          if (FMT == FMT_NVFP4) a.row_scale[r] = factor;
+          pl.place_of_row[row[j]] = place[j];
+          if (FMT == FMT_NVFP4) a.row_scale[row[j]] = factor;
         }
-        const ChunkPlace<FMT> to(a, r, at, tid, tpr);
+        const ChunkPlace<FMT> to(a, row[j], place[j], tid, tpr);
 #pragma unroll
         for (int i = 0; i < NV; ++i) to.store(c[i], i, tpr);
       }

@@ -391,7 +391,7 @@ __device__ __forceinline__ void block_scan2(int& a, int& b, int& total_a, int& t
 // expert -1.  The place of a pair among its expert's rows is what its atomic add to the expert's count returns (the order
 // inside an expert does not affect results).  One cluster of CL blocks: each counts its share of the pairs, reads the others' counts where they lie and
 // numbers its own; bound by the chain of loads and
-// atomic adds of a thread.
+// atomic adds of a thread.  place_of_pair (may be null): where a pair's row stands if every tile began at a multiple of `pitch` rows.
 constexpr int PLAN_CLUSTER = 8;
 __device__ __forceinline__ int ld_cluster_i32(uint32_t addr) {
   int v;
@@ -402,9 +402,10 @@ template <int CL>
 __global__ void __launch_bounds__(1024)
 moe_plan_tiles_kernel(const int* ids, int n_pairs, int E, int e_lo, int e_hi, int tile_cap, int max_tiles,
                         int* __restrict__ row_of_pair, int* __restrict__ tile_expert, int* __restrict__ tile_row0,
-                        int* __restrict__ tile_rows, int* __restrict__ n_rows_out, MoeBounds bd) {
+                        int* __restrict__ tile_rows, int* __restrict__ n_rows_out, int* __restrict__ place_of_pair, int pitch, MoeBounds bd) {
   __shared__ int cnt[1024];
   __shared__ int off[1024];
+  __shared__ int row0[1024], tile0[1024], tile_size[1024];         // of an expert: its first row, its first tile, rows of a tile
   const int rank = CL > 1 ? (int)cluster_ctarank() : 0, first = rank * 1024 + threadIdx.x;
   cnt[threadIdx.x] = 0;
   __syncthreads();
@@ -432,6 +433,7 @@ moe_plan_tiles_kernel(const int* ids, int n_pairs, int E, int e_lo, int e_hi, in
   int row = mine, tile = own, rows, tiles;
   block_scan2(row, tile, rows, tiles);
   off[e] = row + before;
+  row0[e] = row; tile0[e] = tile; tile_size[e] = size;
   if (rank == 0) {
     if (e == 0) *n_rows_out = rows;
     for (int i = 0; i < own; ++i) {                     // never empty: (own - 1) * size < mine, as tile_cap is a multiple of 64
@@ -449,7 +451,14 @@ moe_plan_tiles_kernel(const int* ids, int n_pairs, int E, int e_lo, int e_hi, in
 #pragma unroll 4
   for (int i = first; i < n_pairs; i += CL * 1024) {
     const int r = row_of_pair[i];
-    if (r >= 0) row_of_pair[i] = off[ids[i]] + r;
+    if (r >= 0) {
+      const int x = ids[i], at = off[x] + r;
+      row_of_pair[i] = at;
+      if (place_of_pair) {
+        const int j = at - row0[x], n = tile_size[x];
+        place_of_pair[i] = (tile0[x] + j / n) * pitch + j % n;
+      }
+    }
   }
   if (CL > 1) cluster_sync_all();                       // counts stay until everyone has read them
 }
@@ -809,17 +818,27 @@ extern "C" int omni_moe_plan(const int* ids, int n_pairs, int E, int e_lo, int e
 }
 
 // Even tiles of at most tile_cap (64, 128 or 256) rows for omni_gemm_bf16_experts; max_tiles: at least min(E, n_pairs) + n_pairs / tile_cap.
-extern "C" int omni_moe_plan_tiles(const int* ids, int n_pairs, int E, int e_lo, int e_hi, int tile_cap, int max_tiles, int* row_of_pair,
-                                   int* tile_expert, int* tile_row0, int* tile_rows, int* n_rows_out, void* stream) {
+static int plan_tiles(const int* ids, int n_pairs, int E, int e_lo, int e_hi, int tile_cap, int max_tiles, int* row_of_pair, int* tile_expert, int* tile_row0,
+                      int* tile_rows, int* n_rows_out, int* place_of_pair, int pitch, void* stream) {
   if (E > 1024 || (tile_cap != 64 && tile_cap != 128 && tile_cap != 256)) return RC_BAD_ARG;
   // 128 experts, one block against eight: 512 pairs 2.6 and 4.4 us (the cluster's barriers), 8000 4.8 and 4.9, 19704 9.3 and 6.1, 64000 29 and 7.9
   if (n_pairs > 8192)
     launch_with(true, PLAN_CLUSTER, moe_plan_tiles_kernel<PLAN_CLUSTER>, PLAN_CLUSTER, 1024, 0, (cudaStream_t)stream, ids, n_pairs, E, e_lo, e_hi, tile_cap, max_tiles,
-                row_of_pair, tile_expert, tile_row0, tile_rows, n_rows_out, g_moe_bounds);
+                row_of_pair, tile_expert, tile_row0, tile_rows, n_rows_out, place_of_pair, pitch, g_moe_bounds);
   else
     launch_overlapped(moe_plan_tiles_kernel<1>, 1, 1024, 0, (cudaStream_t)stream, ids, n_pairs, E, e_lo, e_hi, tile_cap, max_tiles, row_of_pair,
-                      tile_expert, tile_row0, tile_rows, n_rows_out, g_moe_bounds);
+                      tile_expert, tile_row0, tile_rows, n_rows_out, place_of_pair, pitch, g_moe_bounds);
   return (int)cudaGetLastError();
+}
+extern "C" int omni_moe_plan_tiles(const int* ids, int n_pairs, int E, int e_lo, int e_hi, int tile_cap, int max_tiles, int* row_of_pair,
+                                   int* tile_expert, int* tile_row0, int* tile_rows, int* n_rows_out, void* stream) {
+  return plan_tiles(ids, n_pairs, E, e_lo, e_hi, tile_cap, max_tiles, row_of_pair, tile_expert, tile_row0, tile_rows, n_rows_out, nullptr, 1, stream);
+}
+// The same, and for every pair of a local expert where its row stands if tile t began at row t * pitch (pitch >= tile_cap): row i of the tile at t * pitch + i.
+extern "C" int omni_moe_plan_places(const int* ids, int n_pairs, int E, int e_lo, int e_hi, int tile_cap, int max_tiles, int* row_of_pair, int* tile_expert,
+                                    int* tile_row0, int* tile_rows, int* n_rows_out, int* place_of_pair, int pitch, void* stream) {
+  if (!place_of_pair || pitch < tile_cap) return RC_BAD_ARG;
+  return plan_tiles(ids, n_pairs, E, e_lo, e_hi, tile_cap, max_tiles, row_of_pair, tile_expert, tile_row0, tile_rows, n_rows_out, place_of_pair, pitch, stream);
 }
 
 // Plan of at most FEW_PAIRS pairs.  `logits` bf16 [T, E] (E <= 256, k <= 16): the choice is made here, ids and weights are outputs; null:

@@ -167,7 +167,7 @@ _current, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 # operands of an entry point as one block of 8-byte fields (csrc/lowbit.cu)
-_BLOCKS = {"omni_lowbit_rows": "9qd8q", "omni_lowbit_dequantize": "10q", "omni_lowbit_linear": "26q", "omni_lowbit_experts": "34q"}
+_BLOCKS = {"omni_lowbit_rows": "9qd8q", "omni_lowbit_dequantize": "10q", "omni_lowbit_linear": "26q", "omni_lowbit_experts": "35q"}
 
 
 @functools.lru_cache(maxsize=None)
@@ -480,10 +480,10 @@ def _check_operand(name: str, t: torch.Tensor, shape: tuple, index: int) -> None
 
 @functools.lru_cache(maxsize=1024)
 def _expert_layout(fmt: str, pairs: int, max_tiles: int, scale_rows: int, D: int, Fd: int) -> tuple[int, list[int]]:
-    """Bytes of the workspace of ``experts`` and where its parts begin: pairs' rows, three tables of tiles, the number of rows, the rows' places, what lies between the
+    """Bytes of the workspace of ``experts`` and where its parts begin: pairs' rows, three tables of tiles, the number of rows, places of pairs and rows, what lies between the
     products, the results; codes, scales and factors of the rows of either product."""
     at, end = [], 0
-    for size in (4 * pairs, 4 * max_tiles, 4 * max_tiles, 4 * max_tiles, 4, 4 * pairs, 2 * pairs * Fd, 2 * pairs * D,
+    for size in (4 * pairs, 4 * max_tiles, 4 * max_tiles, 4 * max_tiles, 4, 4 * pairs, 4 * pairs, 2 * pairs * Fd, 2 * pairs * D,
                  *(v for cols in (D, Fd) for v in (pairs * cols // 2, scale_rows * 4 * scale_words(fmt, cols), 4 * pairs))):
         at.append(end)
         end += -(-size // 256) * 256
@@ -542,20 +542,20 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
     o2 = out if out.stride(1) == 1 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0 else torch.empty_like(out, memory_format=torch.contiguous_format)
     pairs, dev = T * k, x.device
     tile = _tile_rows(pairs, E)
-    max_tiles = min(E, pairs) + pairs // tile
-    scale_rows = max_tiles * (256 if tile > 128 else 128)
+    max_tiles, pitch = min(E, pairs) + pairs // tile, 256 if tile > 128 else 128
+    scale_rows = max_tiles * pitch
     # one workspace: the plan, both products' rows, what is between them, the experts' results
     size, at = _expert_layout(fmt, pairs, max_tiles, scale_rows, D, Fd)
     work = torch.empty(size, dtype=torch.uint8, device=dev)
     base = work.data_ptr()
-    row_of_pair, te, tr, tn, n_rows, place, h, y, *ops = [base + v for v in at]
+    row_of_pair, te, tr, tn, n_rows, of_pair, of_row, h, y, *ops = [base + v for v in at]
     if fmt != "nvfp4":
         ops[2] = ops[5] = 0
     status, stream = _status(up.index), _stream(up.index)
     if nv.bounds_check_enabled():
         nv.lib("moe").omni_moe_set_bounds(c_long(pairs), ctypes.c_void_p(status))
-    rc = _moe_entry("omni_moe_plan_tiles", "piiiiiipppppp")(ids.data_ptr(), pairs, E, 0, E, tile, max_tiles, row_of_pair, te, tr, tn, n_rows, stream)
-    rc = rc or _entry("omni_lowbit_experts")(x2.data_ptr(), x2.stride(0), k, pairs, E, FORMATS[fmt], h, y, row_of_pair, te, tr, tn, max_tiles, tile, n_rows, place, status,
+    rc = _moe_entry("omni_moe_plan_places", "piiiiiippppppip")(ids.data_ptr(), pairs, E, 0, E, tile, max_tiles, row_of_pair, te, tr, tn, n_rows, of_pair, pitch, stream)
+    rc = rc or _entry("omni_lowbit_experts")(x2.data_ptr(), x2.stride(0), k, pairs, E, FORMATS[fmt], h, y, row_of_pair, of_pair, te, tr, tn, max_tiles, tile, n_rows, of_row, status,
                                              stream, *ops[:3], *up._at, up.rows, D, *ops[3:], *down._at, down.rows, Fd)
     rc = rc or _moe_entry("omni_moe_combine", "pppiiiplplp")(y, row_of_pair, weights.data_ptr(), T, k, D, 0 if res is None else res.data_ptr(),
                                                              0 if res is None else res.stride(0), o2.data_ptr(), o2.stride(0), stream)
