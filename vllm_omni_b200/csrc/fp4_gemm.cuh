@@ -70,12 +70,12 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// x / (1 + e^-x), by a reciprocal good to a step of fp32
-__device__ __forceinline__ float silu_of(float x) { return x * rcp_approx(1.0f + __expf(-x)); }
-// 0.5 x (1 + tanh u) = x / (1 + e^-2u)
+// x / (1 + e^-x), by a reciprocal and a power of two each good to two steps of fp32
+__device__ __forceinline__ float silu_of(float x) { return x * rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * x)); }
+// 0.5 x (1 + tanh u) = x / (1 + e^-2u), u = sqrt(2 / pi) (x + 0.044715 x^3)
 __device__ __forceinline__ float gelu_of(float x) {
-  const float u = 0.7978845608028654f * x * fmaf(0.044715f * x, x, 1.0f);
-  return x * rcp_approx(1.0f + __expf(-2.0f * u));
+  constexpr float C = -2.0f * 0.7978845608028654f * 1.4426950408889634f;
+  return x * rcp_approx(1.0f + ex2_approx(x * fmaf(C * 0.044715f, x * x, C)));
 }
 
 // One result of row m of X: weight row n of the matrix (already times both factors).
