@@ -33,6 +33,7 @@ def scale_words(fmt: str, cols: int) -> int:
     return -(-cols // (4 * BLOCK[fmt]))
 
 
+@functools.lru_cache(maxsize=4096)
 def scale_shape(fmt: str, rows: int, cols: int) -> tuple[int, ...]:
     """Shape of the scales of a matrix [rows, cols]: 4-bit formats uint8 [rows / 128, words, 32, 4, 4], where the scale of row r and block b stands at
     [r // 128, b // 4, r % 32, r // 32 % 4, b % 4]; fp8 fp32 [rows, cols / 128]."""
@@ -50,30 +51,30 @@ class QuantRows:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, row_scale: torch.Tensor | None = None, gated: bool = False):
         if fmt not in FORMATS:
             raise ValueError(f"format {fmt!r}: one of {', '.join(FORMATS)}")
-        if codes.dtype != torch.uint8 or codes.dim() not in (2, 3) or not codes.is_contiguous() or not scales.is_contiguous():
+        shape = codes.shape
+        if codes.dtype is not torch.uint8 or len(shape) not in (2, 3) or not codes.is_contiguous() or not scales.is_contiguous():
             raise ValueError("codes: contiguous uint8 [rows, cols] or [experts, rows, cols], scales contiguous")
-        shape = tuple(codes.shape)
-        lead, rows, cols = shape[:-2], shape[-2], shape[-1] * (1 if fmt == "fp8" else 2)
-        step = 128 if fmt == "fp8" else 32
+        lead, rows, cols = tuple(shape[:-2]), shape[-2], shape[-1] * (1 if fmt == "fp8" else 2)
+        step, index = 128 if fmt == "fp8" else 32, codes.get_device()
         if cols % step or cols == 0:
             raise ValueError(f"{fmt}: columns ({cols}) must be a multiple of {step}")
         if fmt == "fp8" and lead:
             raise ValueError("fp8: rows of one matrix only")
-        want, index = lead + scale_shape(fmt, rows, cols), codes.get_device()
-        if tuple(scales.shape) != want or scales.dtype != (torch.float32 if fmt == "fp8" else torch.uint8) or scales.get_device() != index:
-            raise ValueError(f"{fmt} scales of {shape} codes: {want} expected on {codes.device}, got {scales.dtype} {tuple(scales.shape)} on {scales.device}")
+        want = lead + scale_shape(fmt, rows, cols)
+        if scales.shape != want or scales.dtype is not (torch.float32 if fmt == "fp8" else torch.uint8) or scales.get_device() != index:
+            raise ValueError(f"{fmt} scales of {tuple(shape)} codes: {want} expected on {codes.device}, got {scales.dtype} {tuple(scales.shape)} on {scales.device}")
         if fmt == "nvfp4":
-            if row_scale is None or row_scale.dtype != torch.float32 or tuple(row_scale.shape) != lead + (rows,) or not row_scale.is_contiguous() \
+            if row_scale is None or row_scale.dtype is not torch.float32 or row_scale.shape != lead + (rows,) or not row_scale.is_contiguous() \
                     or row_scale.get_device() != index:
                 raise ValueError(f"nvfp4 needs fp32 row scales {lead + (rows,)} on {codes.device}")
         elif row_scale is not None:
             raise ValueError(f"{fmt} has no row scales")
         if gated and rows % 16:
             raise ValueError(f"gated weight: rows ({rows}) must be a multiple of 16")
-        if index >= 0 and (codes.data_ptr() % 16 or scales.data_ptr() % 16):
+        self._at = at = (codes.data_ptr(), scales.data_ptr(), 0 if row_scale is None else row_scale.data_ptr())
+        if index >= 0 and (at[0] | at[1]) & 15:
             raise ValueError("codes and scales must begin on 16 bytes")
         self._codes, self._scales, self._row, self._buf = codes, scales, row_scale, None
-        self._at = (codes.data_ptr(), scales.data_ptr(), 0 if row_scale is None else row_scale.data_ptr())
         self.fmt, self.gated, self.rows, self.cols, self.experts, self.index = fmt, gated, rows, cols, lead[0] if lead else None, index
 
     @classmethod
@@ -352,16 +353,14 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, fmt: str, eps: floa
 
     ``total`` (may be ``residual`` or ``x``) receives s, ``normed`` the norm itself, both bf16 of ``x``'s shape; s and the norm are rounded to
     bf16 where a store of them would."""
-    cols = x.shape[-1]
+    shape, index = x.shape, x.get_device()
+    cols = shape[-1]
     _check_cols(fmt, cols)
-    if weight.shape != (cols,) or weight.dtype != torch.bfloat16:
-        raise ValueError(f"weight: bf16 [{cols}] expected, got {weight.dtype} {tuple(weight.shape)}")
+    _check_operand("weight", weight, (cols,), index)
     for name, t in (("residual", residual), ("total", total), ("normed", normed)):
-        if t is not None and (t.shape != x.shape or t.dtype != torch.bfloat16 or t.device != x.device):
-            raise ValueError(f"{name}: bf16 {tuple(x.shape)} on {x.device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if weight.device != x.device:
-        raise ValueError(f"weight is on {weight.device}, x on {x.device}")
-    if not x.is_cuda:
+        if t is not None:
+            _check_operand(name, t, shape, index)
+    if index < 0:
         s = _rows16(x, "x")
         if residual is not None:
             s = (s.float() + residual.reshape(s.shape).float()).to(x.dtype)
@@ -374,7 +373,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, fmt: str, eps: floa
         return _quantize_torch(y, fmt)
 
     def out_rows(t, name):
-        t2 = t.view(-1, cols)
+        t2 = t if t.dim() == 2 else t.view(-1, cols)
         if t2.stride(1) != 1 or t2.stride(0) % 8 or t2.data_ptr() % 16:
             raise ValueError(f"{name}: rows must begin on 16 bytes")
         return t2
@@ -504,23 +503,23 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
     for name, w in (("up", up), ("down", down)):
         if not isinstance(w, QuantRows) or w.experts is None:
             raise ValueError(f"{name}: the packed weights of experts expected, got {w!r}")
-    if not up.gated or down.gated or up.fmt != down.fmt or up.experts != down.experts or up.rows != 2 * down.cols or up.cols != down.rows \
-            or up.device != down.device:
+    D, Fd, E, fmt, index = up.cols, down.cols, up.experts, up.fmt, up.index
+    if not up.gated or down.gated or fmt != down.fmt or E != down.experts or up.rows != 2 * Fd or D != down.rows or index != down.index:
         raise ValueError(f"up {up!r} and down {down!r} do not fit")
-    T, k = ids.shape if ids.dim() == 2 else (-1, 0)
-    D, Fd, E, fmt = up.cols, down.cols, up.experts, up.fmt
-    if tuple(x.shape) != (T, D) or x.dtype != torch.bfloat16 or x.device != up.device:
-        raise ValueError(f"x: bf16 [{T}, {D}] on {up.device} expected, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    if ids.dtype != torch.int32 or k < 1 or ids.device != x.device:
-        raise ValueError(f"ids: int32 [T, k] on {x.device} expected, got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
-    if weights.dtype != torch.float32 or weights.shape != ids.shape or weights.device != x.device:
-        raise ValueError(f"weights: fp32 {tuple(ids.shape)} on {x.device} expected, got {weights.dtype} {tuple(weights.shape)} on {weights.device}")
-    for name, t in (("residual", residual), ("out", out)):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
-            raise ValueError(f"{name}: bf16 {tuple(x.shape)} on {x.device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    chosen = ids.shape
+    T, k = chosen if len(chosen) == 2 else (-1, 0)
+    if k < 1 or ids.dtype is not torch.int32 or ids.get_device() != index:
+        raise ValueError(f"ids: int32 [T, k] on {up.device} expected, got {ids.dtype} {tuple(chosen)} on {ids.device}")
+    if weights.dtype is not torch.float32 or weights.shape != chosen or weights.get_device() != index:
+        raise ValueError(f"weights: fp32 {tuple(chosen)} on {up.device} expected, got {weights.dtype} {tuple(weights.shape)} on {weights.device}")
+    _check_operand("x", x, (T, D), index)
+    if residual is not None:
+        _check_operand("residual", residual, (T, D), index)
+    if out is not None:
+        _check_operand("out", out, (T, D), index)
     if E > 1024:
         raise ValueError(f"at most 1024 experts, got {E}")
-    if not x.is_cuda:
+    if index < 0:
         xv, y = _values_torch(_quantize_torch(x, fmt)), torch.zeros(T, D)
         for e in range(E):
             t, j = (ids == e).nonzero(as_tuple=True)
@@ -531,27 +530,30 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
         y = (y if residual is None else y + residual.float()).to(x.dtype)
         return y if out is None else out.copy_(y)
     if out is None:
-        out = torch.empty(T, D, dtype=x.dtype, device=x.device)
+        out = o2 = torch.empty(T, D, dtype=torch.bfloat16, device=_device(index))
+    else:
+        o2 = out if out.stride(1) == 1 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0 else torch.empty_like(out, memory_format=torch.contiguous_format)
     if T == 0:
         return out
-    if _current() != up.index:
-        with torch.cuda.device(up.index):
+    if _current() != index:
+        with torch.cuda.device(index):
             return experts(x, ids, weights, up, down, residual, out)
-    x2, ids, weights = _rows16(x, "x"), ids.contiguous(), weights.contiguous()
+    x2 = _rows16(x, "x")
+    ids = ids if ids.is_contiguous() else ids.contiguous()
+    weights = weights if weights.is_contiguous() else weights.contiguous()
     res = None if residual is None else _rows16(residual, "residual")
-    o2 = out if out.stride(1) == 1 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0 else torch.empty_like(out, memory_format=torch.contiguous_format)
-    pairs, dev = T * k, x.device
+    pairs = T * k
     tile = _tile_rows(pairs, E)
     max_tiles, pitch = min(E, pairs) + pairs // tile, 256 if tile > 128 else 128
     scale_rows = max_tiles * pitch
     # one workspace: the plan, both products' rows, what is between them, the experts' results
     size, at = _expert_layout(fmt, pairs, max_tiles, scale_rows, D, Fd)
-    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    work = torch.empty(size, dtype=torch.uint8, device=_device(index))
     base = work.data_ptr()
     row_of_pair, te, tr, tn, n_rows, of_pair, of_row, h, y, *ops = [base + v for v in at]
     if fmt != "nvfp4":
         ops[2] = ops[5] = 0
-    status, stream = _status(up.index), _stream(up.index)
+    status, stream = _status(index), _stream(index)
     if nv.bounds_check_enabled():
         nv.lib("moe").omni_moe_set_bounds(c_long(pairs), ctypes.c_void_p(status))
     rc = _moe_entry("omni_moe_plan_places", "piiiiiippppppip")(ids.data_ptr(), pairs, E, 0, E, tile, max_tiles, row_of_pair, te, tr, tn, n_rows, of_pair, pitch, stream)
