@@ -196,6 +196,18 @@ def test_norm(fmt, rows, cols, residual):
 
 @gpu
 @pytest.mark.parametrize("fmt", tuple(L.FORMATS))
+@pytest.mark.parametrize("rows", [3, 400])
+def test_norm_at_the_ends_of_bf16(fmt, rows):
+    """Norms near the largest bf16 and near the smallest, by the gain; a zero gain; one channel that is nearly the whole row."""
+    x = rows_of(rows, 256, device="cuda").clamp(-3, 3)
+    x[1] = 0
+    x[1, 17] = 1e10
+    for g in (1e37, 1e-37, 0.0):
+        check_norm(x, torch.full((256,), g, dtype=BF, device="cuda"), fmt, None)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", tuple(L.FORMATS))
 def test_norm_in_place_and_strided(fmt):
     gain = (weight_of(256) * 16).cuda()
     x, r = rows_of(40, 512, device="cuda"), rows_of(40, 512, 3, "cuda")
@@ -340,6 +352,18 @@ def test_linear_nan_rows_stay_alone(fmt, tile, split, M):
 
 
 @gpu
+@pytest.mark.parametrize("fmt", FMT4)
+def test_linear_beyond_32_bits(fmt):
+    """More than 2^31 results: the last rows as they are by themselves."""
+    x, w = rows_of(66000, 64, device="cuda"), L.pack_weight(weight_of(33000, 64, device="cuda"), fmt)
+    r = torch.zeros(66000, 33000, dtype=BF, device="cuda")
+    r[-2:] = 3.0
+    y = L.linear(x, w, residual=r, out=r)
+    close(y[-2:], want_linear(L.quantize(x[-2:], fmt), w, residual=torch.full((2, 33000), 3.0, dtype=BF)))
+    close(y[:2], want_linear(L.quantize(x[:2], fmt), w))
+
+
+@gpu
 def test_linear_no_rows():
     w = L.pack_weight(weight_of(64, 64, device="cuda"), "nvfp4")
     assert L.linear(torch.empty(0, 64, dtype=BF, device="cuda"), w).shape == (0, 64)
@@ -451,6 +475,24 @@ def test_experts_uneven(fmt):
     L.experts(x, mixed, w, up, down, out=wide[:, 3:3 + D])
     close(wide[:, 3:3 + D], want_experts(x, mixed, w, up, down))
     assert (wide[:, :3] == 7).all() and (wide[:, 3 + D:] == 7).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_route(device, renorm):
+    from vllm_omni_b200.ops.moe import route
+    z = (torch.randperm(40 * 60, generator=torch.Generator().manual_seed(1)).view(40, 60).float() / 256).to(BF).unique(dim=1)[:, :24]
+    z = z.sort(-1).values[:, torch.randperm(24)].contiguous()
+    ids, w = route(z.to(device), 5, renorm)
+    p = torch.softmax(z.double(), -1)
+    got = p.gather(1, ids.long().cpu())
+    rest = p.scatter(1, ids.long().cpu(), 0).amax(-1, keepdim=True)
+    assert ids.dtype == torch.int32 and (got >= rest).all() and (ids.sort(-1).values.diff(dim=-1) > 0).all()
+    want = got / got.sum(-1, keepdim=True) if renorm else got
+    np.testing.assert_allclose(w.double().cpu(), want, rtol=2.0 ** -16)           # 24 powers by __expf, their sum, a quotient
+    for k in (0, 17, 25):
+        with pytest.raises(ValueError, match="route"):
+            route(z.to(device), k)
 
 
 # ------------------------------------------------------------------ as they are used

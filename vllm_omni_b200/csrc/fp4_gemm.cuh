@@ -490,7 +490,8 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
           if (j == STEPS - 1) {
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[acc]), even));
+            // relaxed: a release waits for the stores of the tile before, 8192 x 24576 x 4096 375 -> 322 us without, 2463 tokens of experts 182 -> 161
+            if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&tempty_bar[acc]), even));
           }
 #pragma unroll
           for (int i = 0; i < PER; ++i) {

@@ -36,20 +36,23 @@ struct RowsArgs {
   RowPlace place;
 };
 
-// The larger magnitudes of pairs of bf16, NaN above all: one instruction per pair of registers.
-__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+// larger ones of two pairs of bf16 that are not negative, NaN above all
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
   uint32_t d;
-  asm("{\n\t.reg .b32 x, y;\n\tabs.bf16x2 x, %1;\n\tabs.bf16x2 y, %2;\n\tmax.NaN.bf16x2 %0, x, y;\n\t}" : "=r"(d) : "r"(a), "r"(b));
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 // of eight bf16, two magnitudes side by side that hold the largest
-__device__ __forceinline__ uint32_t max_pair(const uint4& u) { return max_abs2(max_abs2(u.x, u.y), max_abs2(u.z, u.w)); }
+__device__ __forceinline__ uint32_t max_pair(const uint4& u) {
+  constexpr uint32_t M = 0x7fff7fffu;
+  return max2(max2(u.x & M, u.y & M), max2(u.z & M, u.w & M));
+}
 // Largest magnitude of LANES neighbouring lanes as a 15-bit pattern: ordered like the magnitudes, infinity and NaN from 0x7f80 on.
 template <int LANES>
 __device__ __forceinline__ uint32_t group_top(uint32_t pair) {
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) pair = max_abs2(pair, __shfl_xor_sync(0xffffffffu, pair, o));
-  return max_abs2(pair, pair >> 16) & 0xffffu;
+  for (int o = LANES / 2; o > 0; o >>= 1) pair = max2(pair, __shfl_xor_sync(0xffffffffu, pair, o));
+  return max2(pair, pair >> 16) & 0xffffu;
 }
 
 // eight values to e2m1, the first in the lowest half byte (the converted bytes merge into one register)
@@ -72,7 +75,7 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
 
 __device__ __forceinline__ float rcp_fast(float x) {
   float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -254,8 +257,8 @@ lowbit_rows_kernel(const RowsArgs a) {
     // the row's factor: the power of two that puts the row's largest magnitude into [2^10, 2^11), its block's scale into [170, 342)
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) top = max_abs2(top, max_pair(u[i]));
-    top = __reduce_max_sync(0xffffffffu, max_abs2(top, top >> 16) & 0xffffu);
+    for (int i = 0; i < NV; ++i) top = max2(top, max_pair(u[i]));
+    top = __reduce_max_sync(0xffffffffu, max2(top, top >> 16) & 0xffffu);
     if (warps > 1) {
       if (lane == 0) red[warp] = top;
       __syncthreads();

@@ -272,6 +272,11 @@ __device__ __forceinline__ void cluster_sync_all() {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
+// The same without ordering this thread's memory accesses, for arrivals that hand back tensor memory whose loads are complete (tcgen05.wait::ld): a releasing
+// one waits until the thread's earlier stores to global memory have arrived.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
 // TMA tile load into this CTA's shared memory whose byte count is credited to an mbarrier that
 // may live in the pair's other CTA (no multicast: every CTA fetches its own tiles)
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* tmap, uint32_t cluster_bar,
