@@ -477,6 +477,18 @@ def test_experts_uneven(fmt):
     assert (wide[:, :3] == 7).all() and (wide[:, 3 + D:] == 7).all()
 
 
+@gpu
+@pytest.mark.parametrize("fmt", FMT4)
+def test_experts_few_rows_uneven(fmt):
+    """Few rows per expert on the whole, but one expert with all of them; and as many as the smallest tile takes, one more, and one expert less."""
+    E, D, F = 70, 160, 96
+    up, down = L.pack_weight(weight_of(E, 2 * F, D, device="cuda"), fmt, gated=True), L.pack_weight(weight_of(E, D, F, seed=2, device="cuda"), fmt)
+    for T, ids in ((100, torch.full((100, 2), 69)), (33, torch.arange(33)[:, None] // 16 * 3), (70 * 16 + 1, torch.arange(70 * 16 + 1)[:, None] % 70),
+                   (70 * 16, torch.arange(70 * 16)[:, None] % 69)):
+        x, w, ids = rows_of(T, D, device="cuda") / 4, torch.rand(T, ids.shape[1], device="cuda"), ids.int().cuda()
+        close(L.experts(x, ids, w, up, down), want_experts(x, ids, w, up, down))
+
+
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
 @pytest.mark.parametrize("renorm", [False, True])
 def test_route(device, renorm):

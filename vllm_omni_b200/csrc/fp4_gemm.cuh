@@ -15,7 +15,10 @@
 //     XR = 256, pairs   (cta_group::2) 256 x 256 tiles: each CTA brings 128 rows of W and half of the rows of X, and an MMA reads both: half the
 //                       L2 traffic per product, which is what bounds 4-bit tiles (128 x 128: 32 KB per 8.4 Mflop).
 //                       One accumulator: the scales take the rest of tensor memory; sixteen warps drain it into registers at once
-//                       and hand it back before they work on it.
+//                       and hand it back before they work on it.  8192 x 24576 x 4096, nvfp4, SwiGLU: 322 us, 5.1 PFLOP/s, tensor pipe 69 % busy; loads
+//                       alone 78 % of the time (8192 x 8192 x 4096: 88 of 113 us, 14.3 TB/s).  In 128-row tiles on single CTAs 478 us.
+//     One row of 24576 x 4096, nvfp4: 12.6 us alone (57 MB at 4.5 TB/s), 13.8 with its quantisation before it, during which
+//     the first weights come; 33 x 4096 x 12288 in four shares 10.0 us.
 //     few tiles         2 or 4 CTAs (2 pairs) of a cluster share a tile along K; each finishes its part of the outputs from the sums of all
 //
 // All waits are bounded (ptx_sm100.cuh).  No load is a multicast.
@@ -36,7 +39,7 @@ struct Fp4Args {
   int M, N, K;                                // rows of X, rows of W (of an expert), contraction
   const int *tile_expert, *tile_row0, *tile_rows;        // null: one matrix, tiles of XR rows
   int max_tiles, split;                       // tiles of rows, CTAs that share a tile along K
-  int by16;                                   // y (and residual, gate, bias) in pieces of 16 bytes
+  int by16;                                   // y and residual in pieces of 16 bytes (gates and biases are read one by one)
 };
 
 template <int FMT, int XR, bool PAIR>
@@ -119,7 +122,7 @@ template <int EPI> struct Fp4Lane {
 // for rows 2 (lane % 4) and the next of either eight the weight rows lane / 4 + 0, 8, 16, 24: the gate and the lift of an output are its own, factors and biases of
 // weight rows stay for the tile, and the transposing matrix stores turn rounded results in 1 KB of the warp's own, from where they leave in pieces of 16
 // bytes.  Residuals come in the same way.  m0: the first row, rows: how many there are; n0: the warp's first weight row; xf: the factor of row lane % 16.
-// (A lane per weight row and a turn of fp32 took 500 instructions per 16 x 32: 2390 x 8192 x 2048 with GELU 59 us, FIXME.)
+// (A lane per weight row and a turn of fp32 took three times the instructions: 2463 tokens' rows of experts, 768 -> 2048, 121 us, 67 so.)
 template <int EPI>
 __device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v0, const uint32_t* v1, uint32_t turned, long m0, int rows, int n0,
                                           const Fp4Lane<EPI>& keep, float xf, int lane) {
@@ -248,7 +251,7 @@ __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* tmap, int c0,
 
 constexpr int SPLIT_MOST = 4;    // CTAs or pairs that share a tile
 // Stages of weights that a CTA asks for ahead of its first item.  One row of 24576 x 4096 with its quantisation: 14.2 us without, 13.8 with 4, 14.4 with 8,
-// 15.8 with 16 (asked for ahead of what other CTAs need first).
+// 15.8 with 16 (asked for ahead of what other CTAs need first).  64 tokens x 8 of 128 experts, 2048 -> 768 -> 2048: 51 us without, 47.5 with 4.
 constexpr int PREFETCH = 4;
 
 // a tile of rows: which expert, its first row in X and y, how many rows, and where its scales begin
@@ -260,7 +263,7 @@ struct RowTile {
 template <int XR>
 __device__ __forceinline__ RowTile row_tile(const Fp4Args& a, int t) {
   RowTile r;
-  r.scale_tile = t * (XR > 128 ? 2 : 1);      // XR = 16, 64: one tile only, or an expert's
+  r.scale_tile = t * (XR > 128 ? 2 : 1);      // XR = 16, 64: one tile only, or tiles of experts, whose scales begin anew
   if (a.tile_expert) {
     r.expert = a.tile_expert[t];
     r.row0 = a.tile_row0[t];
@@ -336,12 +339,15 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
 
   auto tile_at = [&](int it) { return row_tile<XR>(a, tile_of(min(it, num_items - 1))); };
 
-  // the first item's weights into L2 while the kernel before (the rows' quantiser) runs out
-  if (!experts && warp == 0 && first < num_items && elect_one())
-    for (int kb = kb0; kb < kb1 && kb < kb0 + PREFETCH; ++kb) {
-      tma_prefetch_3d(&a.tmW, kb * 128, block_of(first) * 128, 0);
-      tma_prefetch_4d(&a.tmWS, 0, kb * Cfg::WORDS, block_of(first), 0);
+  // The first item's weights into L2 while the kernel before (the rows' quantiser) runs out.  Experts: the plan ran before that kernel, which let this one start
+  // only when it had waited for the plan itself; what is asked for is in bounds or not fetched, whatever the table holds.
+  if (warp == 0 && first < num_items && elect_one()) {
+    const int expert = experts ? __ldcg(a.tile_expert + tile_of(first)) : 0;
+    for (int kb = kb0; expert >= 0 && kb < kb1 && kb < kb0 + PREFETCH; ++kb) {
+      tma_prefetch_3d(&a.tmW, kb * 128, block_of(first) * 128, expert);
+      tma_prefetch_4d(&a.tmWS, 0, kb * Cfg::WORDS, block_of(first), expert);
     }
+  }
   __syncwarp();
   pdl_begin();
 
@@ -689,11 +695,13 @@ static int launch_any(Fp4Args& a, const Fp4Operands& o, int fmt, bool gated, int
 }
 
 // Tile and split of a linear layer: the tile's rows, or a negative code.
+// Up to 16 rows: two CTAs per SM with tiles of 16 (16 rows of 24576 x 4096 12.4 us, in a tile of 64 14.2); up to 64: one (64 rows 14.5, in a tile of 128 15.3).
 // More than 128 rows: 128-row tiles on single CTAs or 256-row tiles on pairs, by the rounds that each take.  In a full round a block of 256 of K costs 0.4 us
-// on single CTAs and 0.5 on pairs (what L2 delivers), in a last round that is not full 0.3 and 0.4.  N x K = 4096 x 4096, 512 rows 8.3 us on single
-// CTAs, 11 on pairs; 1000 rows 13.1 and 12.2; 24576 x 4096, 200 rows 19.2 and 18.4, 8192 rows 494 and 375.
-// Few tiles: a split saves blocks of K (0.28 us each) and costs an exchange of 1.4 us and 14 ns per row, 0.6 more in fours.  4096 x 12288, 33 rows: 15.2 us
-// whole, 12.9 in two, 10.1 in four; 4096 x 1024: 3.6, 4.8, 5.5.  (Clusters of 8 of these CTAs, one per SM, do not all find room: 22 us.)
+// on single CTAs and 0.5 on pairs (what L2 delivers), in a last round that is not full 0.3 and 0.4.  N x K = 4096 x 4096, 512 rows 8.7 us on single
+// CTAs, 10.6 on pairs; 1000 rows 13.6 and 12.0; gated 24576 x 4096, 200 rows 19.0 and 18.0, 8192 rows 478 and 322.
+// Few tiles: a split saves blocks of K (0.28 us each) and costs an exchange of 1.4 us and 14 ns per row, 0.6 more in fours.  4096 x 12288, 33 rows: 15.9 us
+// whole, 12.3 in two, 10.0 in four; 200 rows 16.8 whole, 14.3 in two; 4096 x 1024, 33 rows: 3.9, 5.1, 5.7.  (Clusters of 8 of these CTAs, one per SM, do
+// not all find room: 22 us.)
 static int pick_tiles(Fp4Args& a, int force_tile, int force_split) {
   const int sms = sm_count(), kb = (a.K + 255) / 256;
   int tile = force_tile ? force_tile : a.M <= 16 ? 16 : a.M <= 64 ? 64 : 128;

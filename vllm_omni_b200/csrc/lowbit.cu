@@ -86,7 +86,7 @@ extern "C" int omni_lowbit_linear(const LowbitLinear* c) {
 }
 
 // Rows of x (pair p reads row p / per, pairs a multiple of per) through `up` (gated, N = 2 F) to h [pairs, F] and through `down` to y [pairs, D], both in the
-// plan's order of rows; tile: the most rows a tile has, 64 / 128 / 256; place_of_pair: for tiles from every 128 rows on (tile 256: 256); n_rows: how many rows the
+// plan's order of rows; tile: the most rows a tile has, 16 / 128 / 256; place_of_pair: for tiles from every 128 rows on (tile 256: 256); n_rows: how many rows the
 // plan has; place_of_row [pairs]: scratch.
 struct ExpertOperand {           // one product's rows in a workspace, and its weights
   void *codes, *scales, *row_scale;

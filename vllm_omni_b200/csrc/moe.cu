@@ -436,7 +436,7 @@ moe_plan_tiles_kernel(const int* ids, int n_pairs, int E, int e_lo, int e_hi, in
   row0[e] = row; tile0[e] = tile; tile_size[e] = size;
   if (rank == 0) {
     if (e == 0) *n_rows_out = rows;
-    for (int i = 0; i < own; ++i) {                     // never empty: (own - 1) * size < mine, as tile_cap is a multiple of 64
+    for (int i = 0; i < own; ++i) {                     // never empty: (own - 1) * size < mine, as tile_cap is 16 (size then too) or a multiple of 64
       tile_expert[tile + i] = e - e_lo;
       tile_row0[tile + i] = row + i * size;
       tile_rows[tile + i] = min(size, mine - i * size);
@@ -817,10 +817,10 @@ extern "C" int omni_moe_plan(const int* ids, int n_pairs, int E, int e_lo, int e
   return (int)cudaGetLastError();
 }
 
-// Even tiles of at most tile_cap (64, 128 or 256) rows for omni_gemm_bf16_experts; max_tiles: at least min(E, n_pairs) + n_pairs / tile_cap.
+// Even tiles of at most tile_cap rows (64, 128 or 256; 16 for 4-bit experts); max_tiles: at least min(E, n_pairs) + n_pairs / tile_cap.
 static int plan_tiles(const int* ids, int n_pairs, int E, int e_lo, int e_hi, int tile_cap, int max_tiles, int* row_of_pair, int* tile_expert, int* tile_row0,
                       int* tile_rows, int* n_rows_out, int* place_of_pair, int pitch, void* stream) {
-  if (E > 1024 || (tile_cap != 64 && tile_cap != 128 && tile_cap != 256)) return RC_BAD_ARG;
+  if (E > 1024 || (!(tile_cap == 16 && place_of_pair) && tile_cap != 64 && tile_cap != 128 && tile_cap != 256)) return RC_BAD_ARG;
   // 128 experts, one block against eight: 512 pairs 2.6 and 4.4 us (the cluster's barriers), 8000 4.8 and 4.9, 19704 9.3 and 6.1, 64000 29 and 7.9
   if (n_pairs > 8192)
     launch_with(true, PLAN_CLUSTER, moe_plan_tiles_kernel<PLAN_CLUSTER>, PLAN_CLUSTER, 1024, 0, (cudaStream_t)stream, ids, n_pairs, E, e_lo, e_hi, tile_cap, max_tiles,

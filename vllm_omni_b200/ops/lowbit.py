@@ -490,7 +490,9 @@ def _expert_layout(fmt: str, pairs: int, max_tiles: int, scale_rows: int, D: int
 
 
 def _tile_rows(pairs: int, experts: int) -> int:
-    return 64 if pairs <= 32 * experts else 128 if pairs <= 64 * experts else 256
+    """The most rows of a tile.  128 experts, 2048 -> 768 -> 2048, nvfp4, us with 16, 128, 256: 8 pairs 19.1, 20.3, 22.6; 4 per expert 71, 74, 86; 16: 78, 84, 93; 32: 98, 92, 98;
+    64: 148, 106, 114; 128: -, 140, 140; 154: -, 172, 147.  (64 takes as long as 128.)"""
+    return 16 if pairs <= 16 * experts else 128 if pairs <= 128 * experts else 256
 
 
 def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: QuantRows, down: QuantRows, residual: torch.Tensor | None = None,
