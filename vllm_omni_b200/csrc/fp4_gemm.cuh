@@ -66,7 +66,8 @@ struct Fp4Cfg {
 };
 
 enum Fp4Act : int { FP4_NONE = 0, FP4_GELU_TANH = 1, FP4_SILU = 2 };
-enum Fp4Epilogue : int { EPI_PLAIN = 0, EPI_GATED = 1, EPI_ANY = 2 };         // the sums; silu(gate) * lift; bias, activation, gate and residual where given
+// the sums; silu(gate) * lift; bias and activation where given; these and a gate and a residual
+enum Fp4Epilogue : int { EPI_PLAIN = 0, EPI_GATED = 1, EPI_ACT = 2, EPI_ANY = 3 };
 
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
@@ -107,13 +108,13 @@ __device__ __forceinline__ uint4 load_some(const bf16* p, int n) {
 
 // What a draining lane keeps of a tile, loaded while the tile is waited for: factors and biases of weight rows n0 + 8 i + lane / 4 of its warp's 32.
 template <int EPI> struct Fp4Lane {
-  float wf[4], bias[EPI == EPI_ANY ? 4 : 1];
+  float wf[4], bias[EPI >= EPI_ACT ? 4 : 1];
   __device__ __forceinline__ void load(const Fp4Args& a, long wf0, int n0, int lane) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = n0 + 8 * i + (lane >> 2);
       wf[i] = a.wf && n < a.N ? a.wf[wf0 + n] : 1.0f;
-      if (EPI == EPI_ANY) bias[i] = a.bias && n < a.N ? __bfloat162float(a.bias[n]) : 0.0f;
+      if (EPI >= EPI_ACT) bias[i] = a.bias && n < a.N ? __bfloat162float(a.bias[n]) : 0.0f;
     }
   }
 };
@@ -179,9 +180,9 @@ __device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v0, 
       for (int i = 0; i < 8; ++i) {
         const int s = i >> 2, g = (i >> 1) & 1, c = i & 1;
         r[h][i] = __uint_as_float((h ? v1 : v0)[4 * g + 2 * s + c]) * keep.wf[2 * h + s] * f[2 * g + c];
-        if (EPI == EPI_ANY) r[h][i] += keep.bias[2 * h + s];
+        if (EPI >= EPI_ACT) r[h][i] += keep.bias[2 * h + s];
       }
-    if (EPI == EPI_ANY) {
+    if (EPI >= EPI_ACT) {
       // a step for all sixteen values at a time: they do not depend on one another, and the branches are the same for all
       if (a.act == FP4_SILU) {
 #pragma unroll
@@ -190,7 +191,7 @@ __device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v0, 
 #pragma unroll
         for (int i = 0; i < 16; ++i) r[i >> 3][i & 7] = gelu_of(r[i >> 3][i & 7]);
       }
-      if (a.gate) {
+      if (EPI == EPI_ANY && a.gate) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int h = i >> 3, s = (i >> 2) & 1, g = (i >> 1) & 1, c = i & 1;
@@ -198,7 +199,7 @@ __device__ __forceinline__ void fp4_store(const Fp4Args& a, const uint32_t* v0, 
           r[h][i & 7] *= __bfloat162float(a.gate[(m0 + row) / a.rows_per_gate * a.gate_stride + col]);
         }
       }
-      if (a.residual) {
+      if (EPI == EPI_ANY && a.residual) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t res[4];
@@ -483,7 +484,8 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
         break;
       }
       if constexpr (PAIR) {
-        // 64 of the 256 rows per warp, into registers (with operands in the epilogue in two steps, for want of registers); then the accumulator is free
+        // 64 of the 256 rows per warp, into registers; then the accumulator is free.  With a gate or a residual in two steps, for want of registers (18 warps leave
+        // 96 a thread): 2390 x 8192 x 2048 with a residual 40 us, in one step 52; with a bias and GELU, which have a form of their own, 34 and 29.
         constexpr int STEPS = EPI == EPI_ANY ? 2 : 1, PER = Cfg::CHUNKS / STEPS;
 #pragma unroll
         for (int j = 0; j < STEPS; ++j) {
@@ -570,7 +572,7 @@ fp4_kernel(const __grid_constant__ Fp4Args a, int* status) {
           for (int e = 0; e < 4; ++e) {
             s[e] *= f;
             if (GATED) s[e] = silu_of(s[e]) * (sums[u][COLS - 1][e] * f);
-            else if (EPI == EPI_ANY && e < left) s[e] = fp4_finish(a, s[e], m, n0 + o + e, !a.by16);
+            else if (EPI >= EPI_ACT && e < left) s[e] = fp4_finish(a, s[e], m, n0 + o + e, !a.by16);
           }
           if (EPI == EPI_ANY && a.residual && a.by16) {
             const float2 lo = unpack_bf16(res[u].x), hi = unpack_bf16(res[u].y);
@@ -685,8 +687,8 @@ static int launch_rows_of(Fp4Args& a, const Fp4Operands& o, int tile, int* statu
 template <int FMT>
 static int launch_epi(Fp4Args& a, const Fp4Operands& o, bool gated, int tile, int* status, cudaStream_t s) {
   if (gated) return launch_rows_of<FMT, EPI_GATED>(a, o, tile, status, s);
-  const bool any = a.bias || a.act || a.gate || a.residual;
-  return any ? launch_rows_of<FMT, EPI_ANY>(a, o, tile, status, s) : launch_rows_of<FMT, EPI_PLAIN>(a, o, tile, status, s);
+  if (a.gate || a.residual) return launch_rows_of<FMT, EPI_ANY>(a, o, tile, status, s);
+  return a.bias || a.act ? launch_rows_of<FMT, EPI_ACT>(a, o, tile, status, s) : launch_rows_of<FMT, EPI_PLAIN>(a, o, tile, status, s);
 }
 static int launch_any(Fp4Args& a, const Fp4Operands& o, int fmt, bool gated, int tile, int* status, cudaStream_t s) {
   if (fmt == FMT_MXFP4) return launch_epi<FMT_MXFP4>(a, o, gated, tile, status, s);
