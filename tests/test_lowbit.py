@@ -325,6 +325,22 @@ def test_linear_epilogue(fmt, M, N, K, tile, split, act):
 
 @gpu
 @pytest.mark.parametrize("fmt", FMT4)
+@pytest.mark.parametrize("M,N,K,tile,split", [(1, 136, 512, 16, 1), (16, 77, 1056, 16, 4), (40, 333, 512, 64, 2), (130, 264, 512, 128, 1), (200, 77, 544, 128, 2), (260, 1000, 288, 256, 0),
+                                              (700, 333, 96, 256, 1), (200, 520, 1056, 256, 2)])
+@pytest.mark.parametrize("act", [None, "silu", "gelu_tanh"])
+def test_linear_bias_and_activation(fmt, M, N, K, tile, split, act):
+    q, p = L.quantize(rows_of(M, K, device="cuda"), fmt), L.pack_weight(weight_of(N, K, device="cuda"), fmt)
+    b, kw = rows_of(1, N, 5, "cuda")[0], dict(force_tile=tile, force_split=split)
+    close(L.linear(q, p, b, act, **kw), want_linear(q, p, b, act))
+    close(L.linear(q, p, None, act, **kw), want_linear(q, p, None, act))
+    wide = torch.full((M, N + 5), 7.0, dtype=BF, device="cuda")
+    L.linear(q, p, b, act, out=wide[:, 3:3 + N], **kw)
+    close(wide[:, 3:3 + N], want_linear(q, p, b, act))
+    assert (wide[:, :3] == 7).all() and (wide[:, 3 + N:] == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FMT4)
 @pytest.mark.parametrize("M,N,K,tile,split", [(1, 32, 64, 0, 0), (5, 272, 512, 16, 1), (5, 272, 512, 64, 1), (5, 272, 2080, 64, 4), (5, 272, 2080, 16, 2), (40, 4096, 512, 0, 0), (130, 528, 544, 128, 1), (100, 528, 1024, 128, 4),
                                               (300, 1040, 288, 256, 1), (300, 1040, 1056, 256, 2), (513, 512, 512, 256, 0)])
 def test_linear_gated(fmt, M, N, K, tile, split):
