@@ -1,4 +1,4 @@
-"""Linear layers on 4-bit operands (csrc/gemm_fp4_sm100.cu) and the kernels that make them (csrc/lowbit.cu).
+"""Linear layers on 4-bit operands and the kernels that make them (csrc/lowbit.cu, fp4_gemm.cuh, lowbit_rows.cuh).
 
 Formats: ``mxfp4`` — e2m1 values with a power of two per block of 32; ``nvfp4`` — e2m1 values with an e4m3 scale per block of 16 and an
 fp32 factor per row; ``fp8`` (norm outputs only) — e4m3 values with an fp32 scale per block of 128, what the fp8 layers read.
