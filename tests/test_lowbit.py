@@ -195,6 +195,18 @@ def test_norm(fmt, rows, cols, residual):
 
 
 @gpu
+@pytest.mark.parametrize("rows,cols", [(1500, 512), (1500, 768), (1300, 1024), (75777, 32), (2400, 256)])
+def test_chunks_per_lane(rows, cols):
+    """Many rows of one to four chunks per lane."""
+    x = rows_of(rows, cols, device="cuda")
+    for fmt in FMT4:
+        same_as_oracle(L.quantize(x, fmt), x)
+    for fmt in L.FORMATS:
+        if cols % L.BLOCK[fmt] == 0:
+            check_norm(x, (weight_of(cols) * 16).cuda(), fmt, rows_of(rows, cols, 3, "cuda"))
+
+
+@gpu
 @pytest.mark.parametrize("fmt", tuple(L.FORMATS))
 @pytest.mark.parametrize("rows", [3, 400])
 def test_norm_at_the_ends_of_bf16(fmt, rows):

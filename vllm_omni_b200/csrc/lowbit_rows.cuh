@@ -386,13 +386,14 @@ dequantize_kernel(const DequantArgs a) {
 
 // Threads per row and chunks per thread.  Up to 512 chunks per SM, none of a row longer than that: a lane per chunk (nvfp4, us with one and with up to four
 // chunks: 8 x 4096 1.75, 2.06, with the norm 2.41, 2.91; 148 x 4096 1.89, 2.23; 296 x 2048 1.88, 2.06).  Beyond: up to four, which share what a thread does
-// once per row, with fewer warps to wait for (1 x 8192 2.57, 2.23, with the norm 3.94, 3.08; 296 x 4096 with the norm 3.59, 3.10; 8192 x 4096 35.0, 20.3).
+// once per row, with fewer warps to wait for (1 x 8192 2.57, 2.23, with the norm 3.94, 3.08; 296 x 4096 with the norm 3.59, 3.10; 8192 x 4096 35.0, 20.3), and no more of them than
+// the row's threads need: 19704 x 768 in three 9.2 us, in four 11.1, 8192 x 1536 8.4, 9.9.
 template <int FMT, bool NORM, int MODE>
 static int launch_rows(RowsArgs& a, cudaStream_t s) {
   const int chunks = a.K / 8;
   int nv = chunks <= 512 && a.rows * chunks <= 512L * sm_count() ? 1 : 4;
-  while (nv > 1 && chunks <= 32 * (nv / 2)) nv /= 2;
   const int tpr = (chunks + 32 * nv - 1) / (32 * nv) * 32;
+  nv = (chunks + tpr - 1) / tpr;
   if (tpr > 1024) return RC_TOO_LARGE;
   const dim3 block(tpr, tpr >= 256 ? 1 : 256 / tpr);
   const unsigned grid = (unsigned)((a.rows + block.y - 1) / block.y);
@@ -401,6 +402,7 @@ static int launch_rows(RowsArgs& a, cudaStream_t s) {
   switch (nv) {
     case 1: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 1, 512>, grid, block, 0, s, a);
     case 2: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 2, 512>, grid, block, 0, s, a);
+    case 3: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 3, 512>, grid, block, 0, s, a);
     default: return launch_overlapped(lowbit_rows_kernel<FMT, NORM, MODE, 4, 512>, grid, block, 0, s, a);
   }
 }
