@@ -835,10 +835,17 @@ extern "C" int omni_moe_plan_tiles(const int* ids, int n_pairs, int E, int e_lo,
   return plan_tiles(ids, n_pairs, E, e_lo, e_hi, tile_cap, max_tiles, row_of_pair, tile_expert, tile_row0, tile_rows, n_rows_out, nullptr, 1, stream);
 }
 // The same, and for every pair of a local expert where its row stands if tile t began at row t * pitch (pitch >= tile_cap): row i of the tile at t * pitch + i.
-extern "C" int omni_moe_plan_places(const int* ids, int n_pairs, int E, int e_lo, int e_hi, int tile_cap, int max_tiles, int* row_of_pair, int* tile_expert,
-                                    int* tile_row0, int* tile_rows, int* n_rows_out, int* place_of_pair, int pitch, void* stream) {
-  if (!place_of_pair || pitch < tile_cap) return RC_BAD_ARG;
-  return plan_tiles(ids, n_pairs, E, e_lo, e_hi, tile_cap, max_tiles, row_of_pair, tile_expert, tile_row0, tile_rows, n_rows_out, place_of_pair, pitch, stream);
+struct PlanPlaces {          // operands as one block of 8-byte fields
+  const int* ids;
+  long n_pairs, E, e_lo, e_hi, tile_cap, max_tiles;
+  int *row_of_pair, *tile_expert, *tile_row0, *tile_rows, *n_rows_out, *place_of_pair;
+  long pitch;
+  void* stream;
+};
+extern "C" int omni_moe_plan_places(const PlanPlaces* c) {
+  if (!c->place_of_pair || c->pitch < c->tile_cap || c->n_pairs > 0x7fffff00L || c->max_tiles * c->pitch > 0x7fffff00L) return RC_BAD_ARG;
+  return plan_tiles(c->ids, (int)c->n_pairs, (int)c->E, (int)c->e_lo, (int)c->e_hi, (int)c->tile_cap, (int)c->max_tiles, c->row_of_pair, c->tile_expert, c->tile_row0,
+                    c->tile_rows, c->n_rows_out, c->place_of_pair, (int)c->pitch, c->stream);
 }
 
 // Plan of at most FEW_PAIRS pairs.  `logits` bf16 [T, E] (E <= 256, k <= 16): the choice is made here, ids and weights are outputs; null:

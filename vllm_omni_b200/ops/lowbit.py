@@ -40,6 +40,25 @@ def scale_shape(fmt: str, rows: int, cols: int) -> tuple[int, ...]:
     return (rows, cols // 128) if fmt == "fp8" else (-(-rows // 128), scale_words(fmt, cols), 32, 4, 4)
 
 
+@functools.lru_cache(maxsize=4096)
+def _parts(fmt: str, shape: tuple, gated: bool):
+    """What codes of a shape stand for: experts, rows, columns, the scales' shape and type, the shape of the rows' factors."""
+    if fmt not in FORMATS:
+        raise ValueError(f"format {fmt!r}: one of {', '.join(FORMATS)}")
+    if len(shape) not in (2, 3):
+        raise ValueError("codes: contiguous uint8 [rows, cols] or [experts, rows, cols], scales contiguous")
+    lead, rows, cols = tuple(shape[:-2]), shape[-2], shape[-1] * (1 if fmt == "fp8" else 2)
+    step = 128 if fmt == "fp8" else 32
+    if cols % step or cols == 0:
+        raise ValueError(f"{fmt}: columns ({cols}) must be a multiple of {step}")
+    if fmt == "fp8" and lead:
+        raise ValueError("fp8: rows of one matrix only")
+    if gated and rows % 16:
+        raise ValueError(f"gated weight: rows ({rows}) must be a multiple of 16")
+    return (lead[0] if lead else None, rows, cols, lead + scale_shape(fmt, rows, cols), torch.float32 if fmt == "fp8" else torch.uint8,
+            lead + (rows,) if fmt == "nvfp4" else None)
+
+
 class QuantRows:
     """Rows in a low-bit format, as the tensor cores read them: a batch's activations [R, K], a weight [N, K], or the weights of experts [E, N, K].
 
@@ -49,33 +68,24 @@ class QuantRows:
     __slots__ = ("fmt", "gated", "rows", "cols", "experts", "index", "_codes", "_scales", "_row", "_buf", "_at")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, row_scale: torch.Tensor | None = None, gated: bool = False):
-        if fmt not in FORMATS:
-            raise ValueError(f"format {fmt!r}: one of {', '.join(FORMATS)}")
-        shape = codes.shape
-        if codes.dtype is not torch.uint8 or len(shape) not in (2, 3) or not codes.is_contiguous() or not scales.is_contiguous():
+        index = codes.get_device()
+        if codes.dtype is not torch.uint8 or not codes.is_contiguous() or not scales.is_contiguous():
             raise ValueError("codes: contiguous uint8 [rows, cols] or [experts, rows, cols], scales contiguous")
-        lead, rows, cols = tuple(shape[:-2]), shape[-2], shape[-1] * (1 if fmt == "fp8" else 2)
-        step, index = 128 if fmt == "fp8" else 32, codes.get_device()
-        if cols % step or cols == 0:
-            raise ValueError(f"{fmt}: columns ({cols}) must be a multiple of {step}")
-        if fmt == "fp8" and lead:
-            raise ValueError("fp8: rows of one matrix only")
-        want = lead + scale_shape(fmt, rows, cols)
-        if scales.shape != want or scales.dtype is not (torch.float32 if fmt == "fp8" else torch.uint8) or scales.get_device() != index:
-            raise ValueError(f"{fmt} scales of {tuple(shape)} codes: {want} expected on {codes.device}, got {scales.dtype} {tuple(scales.shape)} on {scales.device}")
-        if fmt == "nvfp4":
-            if row_scale is None or row_scale.dtype is not torch.float32 or row_scale.shape != lead + (rows,) or not row_scale.is_contiguous() \
+        experts, rows, cols, want, dtype, want_row = _parts(fmt, codes.shape, gated)
+        if scales.shape != want or scales.dtype is not dtype or scales.get_device() != index:
+            raise ValueError(f"{fmt} scales of {tuple(codes.shape)} codes: {want} expected on {codes.device}, got {scales.dtype} {tuple(scales.shape)} on {scales.device}")
+        at, sat, rat = codes.data_ptr(), scales.data_ptr(), 0
+        if want_row is not None:
+            if row_scale is None or row_scale.dtype is not torch.float32 or row_scale.shape != want_row or not row_scale.is_contiguous() \
                     or row_scale.get_device() != index:
-                raise ValueError(f"nvfp4 needs fp32 row scales {lead + (rows,)} on {codes.device}")
+                raise ValueError(f"nvfp4 needs fp32 row scales {want_row} on {codes.device}")
+            rat = row_scale.data_ptr()
         elif row_scale is not None:
             raise ValueError(f"{fmt} has no row scales")
-        if gated and rows % 16:
-            raise ValueError(f"gated weight: rows ({rows}) must be a multiple of 16")
-        self._at = at = (codes.data_ptr(), scales.data_ptr(), 0 if row_scale is None else row_scale.data_ptr())
-        if index >= 0 and (at[0] | at[1]) & 15:
+        if index >= 0 and (at | sat) & 15:
             raise ValueError("codes and scales must begin on 16 bytes")
-        self._codes, self._scales, self._row, self._buf = codes, scales, row_scale, None
-        self.fmt, self.gated, self.rows, self.cols, self.experts, self.index = fmt, gated, rows, cols, lead[0] if lead else None, index
+        self._at, self._codes, self._scales, self._row, self._buf = (at, sat, rat), codes, scales, row_scale, None
+        self.fmt, self.gated, self.rows, self.cols, self.experts, self.index = fmt, gated, rows, cols, experts, index
 
     @classmethod
     def _empty(cls, fmt: str, rows: int, cols: int, index: int, experts: int | None = None, gated: bool = False) -> "QuantRows":
@@ -167,25 +177,28 @@ def _status(index: int) -> int:
 _current, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-# operands of an entry point as one block of 8-byte fields (csrc/lowbit.cu)
-_BLOCKS = {"omni_lowbit_rows": "9qd8q", "omni_lowbit_dequantize": "10q", "omni_lowbit_linear": "26q", "omni_lowbit_experts": "35q"}
+# operands of an entry point as one block of 8-byte fields (csrc/lowbit.cu, csrc/moe.cu)
+_BLOCKS = {"omni_lowbit_rows": "9qd8q", "omni_lowbit_dequantize": "10q", "omni_lowbit_linear": "26q", "omni_lowbit_experts": "35q", "omni_moe_plan_places": "15q"}
 
 
 @functools.lru_cache(maxsize=None)
 def _entry(name: str):
     """``call(*numbers)`` of an entry point; pointers that are absent are 0."""
-    lib, pack = nv.lib("lowbit"), struct.Struct(_BLOCKS[name]).pack
+    lib, pack = nv.lib("moe" if name == "omni_moe_plan_places" else "lowbit"), struct.Struct(_BLOCKS[name]).pack
     getattr(lib._cdll, name).argtypes = [ctypes.c_char_p]
     fn = getattr(lib, name)
     return lambda *fields: fn(pack(*fields))
 
 
+_bounds = functools.lru_cache(maxsize=None)(nv.bounds_check_enabled)       # as it is when a library is loaded
+
+
 @functools.lru_cache(maxsize=None)
-def _moe_entry(name: str, kinds: str):
-    """An entry point of the ``moe`` library that takes plain Python numbers."""
+def _combine():
+    """``omni_moe_combine`` with plain Python numbers."""
     lib = nv.lib("moe")
-    getattr(lib._cdll, name).argtypes = [{"p": ctypes.c_void_p, "l": c_long, "i": c_int}[k] for k in kinds]
-    return getattr(lib, name)
+    lib._cdll.omni_moe_combine.argtypes = [{"p": ctypes.c_void_p, "l": c_long, "i": c_int}[k] for k in "pppiiiplplp"]
+    return lib.omni_moe_combine
 
 
 def _rows16(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -502,9 +515,8 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
 
     x bf16 [T, D]; ids int32 and weights fp32 [T, k]; up (gated) [E, 2 F, D] and down [E, D, F] of one 4-bit format.  Rows are quantised as they
     are gathered, what leaves ``up`` once more; an expert's result is a bf16 row, their sum is fp32."""
-    for name, w in (("up", up), ("down", down)):
-        if not isinstance(w, QuantRows) or w.experts is None:
-            raise ValueError(f"{name}: the packed weights of experts expected, got {w!r}")
+    if not isinstance(up, QuantRows) or up.experts is None or not isinstance(down, QuantRows) or down.experts is None:
+        raise ValueError(f"up and down: the packed weights of experts expected, got {up!r} and {down!r}")
     D, Fd, E, fmt, index = up.cols, down.cols, up.experts, up.fmt, up.index
     if not up.gated or down.gated or fmt != down.fmt or E != down.experts or up.rows != 2 * Fd or D != down.rows or index != down.index:
         raise ValueError(f"up {up!r} and down {down!r} do not fit")
@@ -556,13 +568,13 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
     if fmt != "nvfp4":
         ops[2] = ops[5] = 0
     status, stream = _status(index), _stream(index)
-    if nv.bounds_check_enabled():
+    if _bounds():
         nv.lib("moe").omni_moe_set_bounds(c_long(pairs), ctypes.c_void_p(status))
-    rc = _moe_entry("omni_moe_plan_places", "piiiiiippppppip")(ids.data_ptr(), pairs, E, 0, E, tile, max_tiles, row_of_pair, te, tr, tn, n_rows, of_pair, pitch, stream)
+    rc = _entry("omni_moe_plan_places")(ids.data_ptr(), pairs, E, 0, E, tile, max_tiles, row_of_pair, te, tr, tn, n_rows, of_pair, pitch, stream)
     rc = rc or _entry("omni_lowbit_experts")(x2.data_ptr(), x2.stride(0), k, pairs, E, FORMATS[fmt], h, y, row_of_pair, of_pair, te, tr, tn, max_tiles, tile, n_rows, of_row, status,
                                              stream, *ops[:3], *up._at, up.rows, D, *ops[3:], *down._at, down.rows, Fd)
-    rc = rc or _moe_entry("omni_moe_combine", "pppiiiplplp")(y, row_of_pair, weights.data_ptr(), T, k, D, 0 if res is None else res.data_ptr(),
-                                                             0 if res is None else res.stride(0), o2.data_ptr(), o2.stride(0), stream)
+    rc = rc or _combine()(y, row_of_pair, weights.data_ptr(), T, k, D, 0 if res is None else res.data_ptr(), 0 if res is None else res.stride(0), o2.data_ptr(),
+                          o2.stride(0), stream)
     if rc:
         nv.check_rc(rc, "experts")
     return out if o2 is out else out.copy_(o2)
