@@ -284,22 +284,15 @@ def _swiglu_torch(y):
 
 
 # ------------------------------------------------------------------ quantisation
-def _rows(x, fmt, *, residual=None, gain=None, eps=0.0, total=None, normed=None, experts=None, gated=False) -> QuantRows:
+def _rows(x, fmt, experts=None, gated=False) -> QuantRows:
     index = x.get_device()
     if _current() != index:                       # kernels go to the current device's stream
         with torch.cuda.device(index):
-            return _rows(x, fmt, residual=residual, gain=gain, eps=eps, total=total, normed=normed, experts=experts, gated=gated)
+            return _rows(x, fmt, experts, gated)
     rows, cols = x.shape
     per = rows // experts if experts else rows
     q = QuantRows._empty(fmt, per, cols, index, experts, gated)
-    codes, scales, row = q._at
-    if gain is None:
-        rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], 0, 0, 0, 0.0, 0, 0, 0, 0, codes, scales, row,
-                                        _stream(index))
-    else:
-        at = lambda t: (0, 0) if t is None else (t.data_ptr(), t.stride(0))
-        rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], *at(residual), gain.data_ptr(), eps, *at(total), *at(normed),
-                                        codes, scales, row, _stream(index))
+    rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], 0, 0, 0, 0.0, 0, 0, 0, 0, *q._at, _stream(index))
     if rc:
         nv.check_rc(rc, "omni_lowbit_rows")
     return q
@@ -338,7 +331,7 @@ def pack_weight(w: torch.Tensor, fmt: str, gated: bool = False) -> QuantRows:
         if w.dtype != torch.bfloat16:
             raise ValueError(f"w: bf16 expected, got {w.dtype}")
         return _quantize_torch(w, fmt, gated)
-    return _rows(_rows16(w, "w"), fmt, experts=w.shape[0] if w.dim() == 3 else None, gated=gated)
+    return _rows(_rows16(w, "w"), fmt, w.shape[0] if w.dim() == 3 else None, gated)
 
 
 def dequantize(q: QuantRows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -370,9 +363,12 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, fmt: str, eps: floa
     cols = shape[-1]
     _check_cols(fmt, cols)
     _check_operand("weight", weight, (cols,), index)
-    for name, t in (("residual", residual), ("total", total), ("normed", normed)):
-        if t is not None:
-            _check_operand(name, t, shape, index)
+    if residual is not None:
+        _check_operand("residual", residual, shape, index)
+    if total is not None:
+        _check_operand("total", total, shape, index)
+    if normed is not None:
+        _check_operand("normed", normed, shape, index)
     if index < 0:
         s = _rows16(x, "x")
         if residual is not None:
@@ -385,15 +381,34 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, fmt: str, eps: floa
             normed.copy_(y.view(x.shape))
         return _quantize_torch(y, fmt)
 
-    def out_rows(t, name):
-        t2 = t if t.dim() == 2 else t.view(-1, cols)
-        if t2.stride(1) != 1 or t2.stride(0) % 8 or t2.data_ptr() % 16:
-            raise ValueError(f"{name}: rows must begin on 16 bytes")
-        return t2
+    if _current() != index:
+        with torch.cuda.device(index):
+            return rms_norm_quantize(x, weight, fmt, eps, residual, total, normed)
+    x, weight = _rows16(x, "x"), _aligned(weight)
+    rp = lr = tp = lt = np_ = ln = 0
+    if residual is not None:
+        residual = _rows16(residual, "residual")
+        rp, lr = residual.data_ptr(), residual.stride(0)
+    if total is not None:
+        tp, lt = _out_rows(total, "total", cols)
+    if normed is not None:
+        np_, ln = _out_rows(normed, "normed", cols)
+    rows = x.shape[0]
+    q = QuantRows._empty(fmt, rows, cols, index)
+    rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, rows, FORMATS[fmt], rp, lr, weight.data_ptr(), eps, tp, lt, np_, ln, *q._at, _stream(index))
+    if rc:
+        nv.check_rc(rc, "omni_lowbit_rows")
+    return q
 
-    x2 = _rows16(x, "x")
-    return _rows(x2, fmt, residual=None if residual is None else _rows16(residual, "residual"), gain=_aligned(weight), eps=eps,
-                 total=None if total is None else out_rows(total, "total"), normed=None if normed is None else out_rows(normed, "normed"))
+
+def _out_rows(t: torch.Tensor, name: str, cols: int) -> tuple[int, int]:
+    """Where the rows of a result begin, and their pitch."""
+    if t.dim() != 2:
+        t = t.view(-1, cols)
+    (ld, one), at = t.stride(), t.data_ptr()
+    if one != 1 or ld % 8 or at % 16:
+        raise ValueError(f"{name}: rows must begin on 16 bytes")
+    return at, ld
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
