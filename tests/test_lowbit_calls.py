@@ -1,0 +1,69 @@
+"""Calls of the low-bit layers (ops/lowbit.py) that their documentation allows beside the ordinary ones, and results that have to be exact."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from vllm_omni_b200.ops import lowbit as L
+
+BF = torch.bfloat16
+FMT4 = ("mxfp4", "nvfp4")
+gpu = pytest.mark.gpu
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+
+
+def rows_of(rows, cols, seed=0, device="cpu"):
+    return torch.randn(rows, cols, generator=torch.Generator().manual_seed(seed)).to(BF).to(device)
+
+
+# ------------------------------------------------------------------ fp8 rows of a norm
+def by_definition(normed):
+    """(codes' values, scales) of bf16 rows on the CPU: s = fp32(max / 448), e4m3(fp32(x / s)), ties to even.  ``to`` rounds to nearest."""
+    y = normed.float().cpu().unflatten(-1, (-1, 128))
+    top = y.abs().amax(-1, keepdim=True).clamp(min=1e-8)
+    scale = top / torch.full_like(top, 448.0)
+    return (y / scale).to(torch.float8_e4m3fn).float(), scale
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows", [8, 2500])
+def test_fp8_rows_are_the_definition_s(rows, device):
+    x = rows_of(rows, 512, device=device) * torch.exp(2 * rows_of(rows, 1, 1, device).float()).to(BF)
+    normed = torch.empty_like(x)
+    q = L.rms_norm_quantize(x, 1 + rows_of(1, 512, 2, device)[0] / 4, "fp8", normed=normed)
+    code, scale = by_definition(normed)
+    assert torch.equal(q.scales.cpu(), scale[..., 0])
+    assert torch.equal(q.codes.cpu().view(torch.float8_e4m3fn).float().unflatten(-1, (-1, 128)), code)
+    for dtype in (torch.float32, BF):
+        assert torch.equal(L.dequantize(q, dtype).cpu().unflatten(-1, (-1, 128)), (code * scale).to(dtype))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("top", [2.0, 2.0 ** -40, 2.0 ** 100, 2.0 ** 126])
+def test_fp8_codes_of_every_pair_of_mantissas(top, device):
+    """Every maximum of a binade beside every bf16 of it and of the fifteen below (then what an e4m3 code rounds to zero).  The norm of equal values is one,
+    times the gain: a row of ones quantises the gain."""
+    m = (1 + torch.arange(128) / 128) * top                               # 128 maxima
+    y = ((1 + torch.arange(128) / 128) * 2.0 ** -torch.arange(16)[:, None]).flatten() * top          # 2048 values, 127 a block
+    y = torch.cat([y, torch.zeros(-y.numel() % 127)]).view(1, -1, 127).expand(128, -1, -1)
+    y = torch.where(y <= m[:, None, None], y, 0.0)
+    gain = torch.cat([m[:, None, None].expand(*y.shape[:2], 1), y], -1).to(BF).flatten(1)             # [128, 17 blocks]
+    x = torch.ones(1, gain.shape[1], dtype=BF, device=device)
+    for g in gain:
+        q = L.rms_norm_quantize(x, g.to(device), "fp8", eps=0.0)
+        code, scale = by_definition(g[None])
+        assert torch.equal(q.scales.cpu(), scale[..., 0])
+        assert torch.equal(q.codes.cpu().view(torch.float8_e4m3fn).float().unflatten(-1, (-1, 128)), code)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_fp8_scales_of_every_maximum(device):
+    """A block for every finite bf16 as its maximum."""
+    top = torch.arange(0, 0x7F80, dtype=torch.int32).to(torch.int16).view(BF)
+    gain = torch.zeros(-(-top.numel() // 64) * 64, 128, dtype=BF)         # 64 blocks a row of 8192
+    gain[:top.numel(), 3] = top
+    x = torch.ones(1, 8192, dtype=BF, device=device)
+    for g in gain.view(-1, 8192):
+        normed = torch.empty_like(x)
+        q = L.rms_norm_quantize(x, g.to(device), "fp8", eps=0.0, normed=normed)
+        assert torch.equal(normed.cpu().view(-1), g) and torch.equal(q.scales.cpu(), by_definition(normed)[1][..., 0])

@@ -237,8 +237,9 @@ def _quantize_torch(x: torch.Tensor, fmt: str, gated: bool = False) -> QuantRows
     size = b.abs().amax(-1)
     if fmt == "fp8":
         size = size.clamp_min(1e-8)
-        scale = torch.where(torch.isfinite(size), size * torch.tensor(1.0 / 448.0, dtype=torch.float32), float("nan"))
-        q = (b * 448.0 / size[..., None]).clamp(-448.0, 448.0)
+        scale = size / torch.full_like(size, 448.0)            # a quotient of two tensors: one by a number is a product on a GPU
+        q = (b / scale[..., None]).clamp(-448.0, 448.0)
+        scale = torch.where(torch.isfinite(size), scale, float("nan"))
         return QuantRows(q.flatten(-2).to(torch.float8_e4m3fn).view(torch.uint8), scale.contiguous(), fmt)
     fine = torch.isfinite(size)
     size = torch.where(fine, size, 0.0)
