@@ -67,3 +67,46 @@ def test_fp8_scales_of_every_maximum(device):
         normed = torch.empty_like(x)
         q = L.rms_norm_quantize(x, g.to(device), "fp8", eps=0.0, normed=normed)
         assert torch.equal(normed.cpu().view(-1), g) and torch.equal(q.scales.cpu(), by_definition(normed)[1][..., 0])
+
+
+def same(a, b):
+    assert torch.equal(a.codes, b.codes) and torch.equal(L.dequantize(a), L.dequantize(b))
+
+
+# ------------------------------------------------------------------ a single row, whose stride says nothing
+def odd_row(cols, seed=0, device="cpu", at=0):
+    """[1, cols] of a buffer whose pitch is no multiple of 8 elements."""
+    return rows_of(4, cols + 4 + at, seed, device)[:1, at:at + cols]
+
+
+@pytest.mark.parametrize("at", [0, 1, 3])
+def test_single_row_has_its_own_pitch(at):
+    x = odd_row(64, at=at)
+    assert x.stride(0) % 8
+    y = L._rows16(x, "x")
+    assert y.stride() == (64, 1) and y.data_ptr() % 16 == 0 and torch.equal(x, y)
+    if not at:
+        assert y.data_ptr() == x.data_ptr()                              # in place where it begins on 16 bytes
+        assert L._out_rows(x, "total", 64) == (x.data_ptr(), 64)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("at", [0, 1])
+@pytest.mark.parametrize("fmt", FMT4)
+def test_single_rows_of_an_odd_pitch(fmt, at, device):
+    x, r, gain = odd_row(128, 1, device, at), odd_row(128, 2, device, at), rows_of(1, 128, 3, device)[0]
+    xc, rc = x.clone(memory_format=torch.contiguous_format), r.clone(memory_format=torch.contiguous_format)
+    same(L.quantize(x, fmt), L.quantize(xc, fmt))
+    w = L.pack_weight(rows_of(48, 128, 4, device), fmt)
+    assert torch.equal(L.linear(x, w), L.linear(xc, w))
+    for f in L.FORMATS:
+        total, normed = torch.empty_like(xc), torch.empty_like(xc)
+        want = L.rms_norm_quantize(xc, gain, f, residual=rc, total=total, normed=normed)
+        wide = torch.full((4, 132), 7.0, dtype=BF, device=device)
+        n2 = torch.empty(2, 133, dtype=BF, device=device)[:1, :128]
+        got = L.rms_norm_quantize(x, gain, f, residual=r, total=wide[:1, :128], normed=n2)
+        same(got, want)
+        assert torch.equal(wide[:1, :128], total) and torch.equal(n2, normed) and (wide[:, 128:] == 7).all() and (wide[1:] == 7).all()
+    up, down = L.pack_weight(rows_of(3 * 64, 128, 5, device).view(3, 64, 128), fmt, gated=True), L.pack_weight(rows_of(3 * 128, 32, 6, device).view(3, 128, 32), fmt)
+    ids, p = torch.tensor([[2, 0]], dtype=torch.int32, device=device), torch.tensor([[0.5, 0.25]], device=device)
+    assert torch.equal(L.experts(x, ids, p, up, down, residual=r), L.experts(xc, ids, p, up, down, residual=rc))

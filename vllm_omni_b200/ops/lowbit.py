@@ -202,16 +202,16 @@ def _combine():
 
 
 def _rows16(t: torch.Tensor, name: str) -> torch.Tensor:
-    """[rows, cols] bf16 whose rows begin on 16 bytes (a copy where they do not)."""
+    """[rows, cols] bf16 whose rows begin on 16 bytes (a copy where they do not); a single row has the pitch ``cols``, whatever its stride says."""
     if t.dtype is not torch.bfloat16:
         raise ValueError(f"{name}: bf16 expected, got {t.dtype}")
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     (rows, cols), (ld, one) = t.shape, t.stride()
     if one != 1 or ld % 8 or t.data_ptr() % 16 or (rows > 1 and ld < cols):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
+        if rows == 1 and one == 1 and not t.data_ptr() % 16:
+            return t.as_strided((1, cols), (cols, 1))
+        t = t.clone(memory_format=torch.contiguous_format)       # (contiguous() keeps a single row where it is, pitch and all)
     return t
 
 
@@ -407,6 +407,8 @@ def _out_rows(t: torch.Tensor, name: str, cols: int) -> tuple[int, int]:
     if t.dim() != 2:
         t = t.view(-1, cols)
     (ld, one), at = t.stride(), t.data_ptr()
+    if t.shape[0] == 1:
+        ld = cols
     if one != 1 or ld % 8 or at % 16:
         raise ValueError(f"{name}: rows must begin on 16 bytes")
     return at, ld
