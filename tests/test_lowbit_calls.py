@@ -1,6 +1,9 @@
 """Calls of the low-bit layers (ops/lowbit.py) that their documentation allows beside the ordinary ones, and results that have to be exact."""
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -84,10 +87,10 @@ def test_single_row_has_its_own_pitch(at):
     x = odd_row(64, at=at)
     assert x.stride(0) % 8
     y = L._rows16(x, "x")
-    assert y.stride() == (64, 1) and y.data_ptr() % 16 == 0 and torch.equal(x, y)
+    assert y.stride() == (64, 1) and y.data_at() % 16 == 0 and torch.equal(x, y)
     if not at:
-        assert y.data_ptr() == x.data_ptr()                              # in place where it begins on 16 bytes
-        assert L._out_rows(x, "total", 64) == (x.data_ptr(), 64)
+        assert y.data_at() == x.data_at()                              # in place where it begins on 16 bytes
+        assert L._out_rows(x, "total", 64) == (x.data_at(), 64)
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -110,3 +113,21 @@ def test_single_rows_of_an_odd_pitch(fmt, at, device):
     up, down = L.pack_weight(rows_of(3 * 64, 128, 5, device).view(3, 64, 128), fmt, gated=True), L.pack_weight(rows_of(3 * 128, 32, 6, device).view(3, 128, 32), fmt)
     ids, p = torch.tensor([[2, 0]], dtype=torch.int32, device=device), torch.tensor([[0.5, 0.25]], device=device)
     assert torch.equal(L.experts(x, ids, p, up, down, residual=r), L.experts(xc, ids, p, up, down, residual=rc))
+
+
+# ------------------------------------------------------------------ copies
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fmt", tuple(L.FORMATS))
+def test_copies_have_addresses_of_their_own(fmt, device):
+    """A copy outlives what it was made of: its kernels must not be given the original's addresses."""
+    gain = rows_of(1, 256, 3, device)[0]
+    q = L.rms_norm_quantize(rows_of(5, 256, device=device), gain, fmt)
+    for other in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), copy.copy(q)):
+        assert other._ptr == tuple(0 if t is None else t.data_at() for t in (other.codes, other.scales, other.row_scale))
+        assert (other.fmt, other.shape, other.gated, other.index) == (q.fmt, q.shape, q.gated, q.index)
+        same(other, q)
+    assert copy.deepcopy(q)._ptr[0] != q._ptr[0]
+    w = L.pack_weight(rows_of(3 * 32, 64, 4, device).view(3, 32, 64), "nvfp4", gated=True)
+    other = copy.deepcopy(w)
+    assert other.gated and other.shape == (3, 32, 64) and other._ptr[0] != w._ptr[0]
+    same(other, w)

@@ -65,7 +65,7 @@ class QuantRows:
     ``codes`` uint8 [.., R, K / 2] (fp8: [R, K]), element 2 i in the low half of byte i; ``scales`` as ``scale_shape`` says; ``row_scale`` fp32
     [.., R] for nvfp4.  ``gated``: the rows of a SwiGLU weight, 8 gate rows, their 8 lift rows, the next 8 gate rows and so on."""
 
-    __slots__ = ("fmt", "gated", "rows", "cols", "experts", "index", "_codes", "_scales", "_row", "_buf", "_at")
+    __slots__ = ("fmt", "gated", "rows", "cols", "experts", "index", "_codes", "_scales", "_row", "_buf", "_ptr")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, row_scale: torch.Tensor | None = None, gated: bool = False):
         index = codes.get_device()
@@ -84,7 +84,7 @@ class QuantRows:
             raise ValueError(f"{fmt} has no row scales")
         if index >= 0 and (at | sat) & 15:
             raise ValueError("codes and scales must begin on 16 bytes")
-        self._at, self._codes, self._scales, self._row, self._buf = (at, sat, rat), codes, scales, row_scale, None
+        self._ptr, self._codes, self._scales, self._row, self._buf = (at, sat, rat), codes, scales, row_scale, None
         self.fmt, self.gated, self.rows, self.cols, self.experts, self.index = fmt, gated, rows, cols, experts, index
 
     @classmethod
@@ -96,8 +96,11 @@ class QuantRows:
         q._buf = buf = torch.empty(size, dtype=torch.uint8, device=_device(index))
         q.fmt, q.gated, q.rows, q.cols, q.experts, q.index = fmt, gated, rows, cols, experts, index
         p = buf.data_ptr()
-        q._at = (p, p + scales, p + row if fmt == "nvfp4" else 0)
+        q._ptr = (p, p + scales, p + row if fmt == "nvfp4" else 0)
         return q
+
+    def __reduce__(self):              # copies have addresses of their own
+        return QuantRows, (self.codes, self.scales, self.fmt, self.row_scale, self.gated)
 
     def _part(self, which: int) -> torch.Tensor:
         _, scales, row = _layout(self.fmt, self.rows, self.cols, self.experts or 1)
@@ -293,7 +296,7 @@ def _rows(x, fmt, experts=None, gated=False) -> QuantRows:
     rows, cols = x.shape
     per = rows // experts if experts else rows
     q = QuantRows._empty(fmt, per, cols, index, experts, gated)
-    rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], 0, 0, 0, 0.0, 0, 0, 0, 0, *q._at, _stream(index))
+    rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], 0, 0, 0, 0.0, 0, 0, 0, 0, *q._ptr, _stream(index))
     if rc:
         nv.check_rc(rc, "omni_lowbit_rows")
     return q
@@ -345,7 +348,7 @@ def dequantize(q: QuantRows, dtype: torch.dtype = torch.bfloat16) -> torch.Tenso
         with torch.cuda.device(q.index):
             return dequantize(q, dtype)
     out = torch.empty(q.shape, dtype=dtype, device=_device(q.index))
-    codes, scales, row = q._at
+    codes, scales, row = q._ptr
     rc = _entry("omni_lowbit_dequantize")(codes, scales, row, q.rows * (q.experts or 1), q.cols, q.rows, FORMATS[q.fmt], int(dtype is torch.float32),
                                           out.data_ptr(), _stream(q.index))
     if rc:
@@ -396,7 +399,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, fmt: str, eps: floa
         np_, ln = _out_rows(normed, "normed", cols)
     rows = x.shape[0]
     q = QuantRows._empty(fmt, rows, cols, index)
-    rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, rows, FORMATS[fmt], rp, lr, weight.data_ptr(), eps, tp, lt, np_, ln, *q._at, _stream(index))
+    rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, rows, FORMATS[fmt], rp, lr, weight.data_ptr(), eps, tp, lt, np_, ln, *q._ptr, _stream(index))
     if rc:
         nv.check_rc(rc, "omni_lowbit_rows")
     return q
@@ -496,7 +499,7 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
     if gate is not None:
         gp, B = gate.data_ptr(), gate.shape[0]
         lds, per = gate.stride(0) if B > 1 else 0, max(1, M // B)
-    rc = _entry("omni_lowbit_linear")(raw, ldx, *q._at, *w._at, yp, ldo[0], M, w.rows, cols, FORMATS[fmt], int(gated), bp, ACT[act], gp, lds, per, rp, ldr[0],
+    rc = _entry("omni_lowbit_linear")(raw, ldx, *q._ptr, *w._ptr, yp, ldo[0], M, w.rows, cols, FORMATS[fmt], int(gated), bp, ACT[act], gp, lds, per, rp, ldr[0],
                                       force_tile, force_split, _status(index), _stream(index))
     if rc:
         nv.check_rc(rc, "omni_lowbit_linear")
@@ -590,7 +593,7 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
         nv.lib("moe").omni_moe_set_bounds(c_long(pairs), ctypes.c_void_p(status))
     rc = _entry("omni_moe_plan_places")(ids.data_ptr(), pairs, E, 0, E, tile, max_tiles, row_of_pair, te, tr, tn, n_rows, of_pair, pitch, stream)
     rc = rc or _entry("omni_lowbit_experts")(x2.data_ptr(), x2.stride(0), k, pairs, E, FORMATS[fmt], h, y, row_of_pair, of_pair, te, tr, tn, max_tiles, tile, n_rows, of_row, status,
-                                             stream, *ops[:3], *up._at, up.rows, D, *ops[3:], *down._at, down.rows, Fd)
+                                             stream, *ops[:3], *up._ptr, up.rows, D, *ops[3:], *down._ptr, down.rows, Fd)
     rc = rc or _combine()(y, row_of_pair, weights.data_ptr(), T, k, D, 0 if res is None else res.data_ptr(), 0 if res is None else res.stride(0), o2.data_ptr(),
                           o2.stride(0), stream)
     if rc:
