@@ -87,10 +87,10 @@ def test_single_row_has_its_own_pitch(at):
     x = odd_row(64, at=at)
     assert x.stride(0) % 8
     y = L._rows16(x, "x")
-    assert y.stride() == (64, 1) and y.data_at() % 16 == 0 and torch.equal(x, y)
+    assert y.stride() == (64, 1) and y.data_ptr() % 16 == 0 and torch.equal(x, y)
     if not at:
-        assert y.data_at() == x.data_at()                              # in place where it begins on 16 bytes
-        assert L._out_rows(x, "total", 64) == (x.data_at(), 64)
+        assert y.data_ptr() == x.data_ptr()                              # in place where it begins on 16 bytes
+        assert L._out_rows(x, "total", 64) == (x.data_ptr(), 64)
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -123,7 +123,7 @@ def test_copies_have_addresses_of_their_own(fmt, device):
     gain = rows_of(1, 256, 3, device)[0]
     q = L.rms_norm_quantize(rows_of(5, 256, device=device), gain, fmt)
     for other in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), copy.copy(q)):
-        assert other._ptr == tuple(0 if t is None else t.data_at() for t in (other.codes, other.scales, other.row_scale))
+        assert other._ptr == tuple(0 if t is None else t.data_ptr() for t in (other.codes, other.scales, other.row_scale))
         assert (other.fmt, other.shape, other.gated, other.index) == (q.fmt, q.shape, q.gated, q.index)
         same(other, q)
     assert copy.deepcopy(q)._ptr[0] != q._ptr[0]
