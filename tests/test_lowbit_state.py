@@ -1,0 +1,97 @@
+"""Quantised weights as the state of their modules: copies, moves, casts, saved states, sleep and offloading."""
+from __future__ import annotations
+
+import copy
+
+import pytest
+import torch
+
+from vllm_omni_b200.diffusion.layers.linear import FusedLinear, weight_tensors
+from vllm_omni_b200.diffusion.quantization.fp8 import quantize_layer
+from test_lowbit_layers import decoder, prompt
+
+BF = torch.bfloat16
+FORMATS = ("fp8", "mxfp4", "nvfp4")
+gpu = pytest.mark.gpu
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+
+
+def layer(fmt, device="cpu", seed=0, n_in=256, n_out=128):
+    g = torch.Generator().manual_seed(seed)
+    m = FusedLinear(n_in, n_out, bias=True, device=device)
+    m.weight.data.copy_(torch.randn(n_out, n_in, generator=g) / n_in ** 0.5)
+    m.bias.data.copy_(torch.randn(n_out, generator=g))
+    if fmt != "bf16":
+        quantize_layer(m, fmt)
+    return m
+
+
+def rows(n=5, cols=256, device="cpu"):
+    return torch.randn(n, cols, generator=torch.Generator().manual_seed(9)).to(BF).to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_weights_are_the_module_s_state(fmt, device):
+    m, x = layer(fmt, device), rows(device=device)
+    y = m(x)
+    size = sum(t.numel() * t.element_size() for _, t in weight_tensors(m))
+    bits = {"fp8": 8, "mxfp4": 4.25, "nvfp4": 4.5}[fmt]
+    assert size >= 128 * 256 * bits / 8 + 2 * 128                         # codes, scales and the bias
+    other = copy.deepcopy(m)
+    assert torch.equal(other(x), y)
+    for _, t in weight_tensors(other):                                    # the copy's own memory
+        if not t.is_floating_point() or t.dtype == torch.float8_e4m3fn:
+            t.view(torch.uint8).zero_()
+    assert torch.equal(m(x), y) and not torch.equal(other(x), y)
+    fresh = layer(fmt, device, seed=5)
+    fresh.load_state_dict(m.state_dict())
+    assert torch.equal(fresh(x), y)
+    cast = copy.deepcopy(m).to(torch.float64).to(BF)                      # (the bias survives the way there and back)
+    assert torch.equal(cast(x), y)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_layers_move_between_devices(fmt):
+    m, x = layer(fmt, "cuda", n_in=4096, n_out=4096), rows(cols=4096, device="cuda")
+    y = m(x)
+    before = torch.cuda.memory_allocated()
+    m.to("cpu")
+    assert before - torch.cuda.memory_allocated() >= 4096 * 4096 // 2
+    on_cpu = m(x.cpu())
+    assert ((on_cpu.float() - y.cpu().float()).abs() <= 0.05 * y.cpu().float().abs() + 0.05).all()        # the same weights, by the restatement
+    m.to("cuda")
+    assert torch.equal(m(x), y)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_data_of_buffers_may_be_exchanged(fmt):
+    """As sleep and offloading do it: a layer without its bytes refuses, and gives the same again with them back at another address."""
+    m, x = layer(fmt, "cuda"), rows(device="cuda")
+    y, kept = m(x), {n: t.data for n, t in weight_tensors(m)}
+    for _, t in weight_tensors(m):
+        t.data = torch.empty(0, dtype=t.dtype, device="cuda")
+    with pytest.raises((RuntimeError, IndexError, ValueError)):
+        m(x)
+    for n, t in weight_tensors(m):
+        t.data = kept[n].clone()
+        kept[n].view(torch.uint8).fill_(1)
+    assert torch.equal(m(x), y)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("experts", [False, True])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_copied_decoder(fmt, experts, device):
+    m = decoder(experts, device)
+    m.quantize(fmt)
+    names = [n for n, _ in weight_tensors(m)]
+    assert not experts or fmt == "fp8" or {"layers.0.w13_fp4_bytes", "layers.1.w2_fp4_bytes"} <= set(names)
+    batch = prompt(9, device)
+    want = m(batch)[0].clone()
+    other = copy.deepcopy(m)
+    for _, t in weight_tensors(m):
+        t.view(torch.uint8).zero_()
+    assert torch.equal(other(batch)[0], want)

@@ -14,7 +14,56 @@ from torch.nn.modules.module import _has_any_global_hook
 from ...ops import gemm
 
 
-class FusedLinear(nn.Module):
+class QuantizedState:
+    """Mix-in of modules with quantised weights: their bytes are buffers of the module, so that they move, copy and save with it (and keep their type in a
+    cast of the module).  ``quantized_buffers`` names them; the attributes that layers use (``QuantRows``; codes and scales of fp8) share their memory."""
+
+    def set_packed(self, name: str, q) -> None:
+        """``self.<name>``: 4-bit weights (ops/lowbit.py ``QuantRows``)."""
+        self.register_buffer(name + "_bytes", q.storage())
+        setattr(self, name, q.over(getattr(self, name + "_bytes"), *q._like))
+
+    def set_fp8(self, codes: torch.Tensor, scale: torch.Tensor) -> None:
+        """``self.fp8``: block-scaled e4m3 codes (uint8 on a GPU) and their fp32 scales."""
+        self.register_buffer("fp8_codes", codes)
+        self.register_buffer("fp8_scale", scale)
+        self.fp8 = (self.fp8_codes, self.fp8_scale)
+
+    def quantized_buffers(self) -> list[str]:
+        return [n for n in self._buffers if n in ("fp8_codes", "fp8_scale") or n.endswith("_bytes")]
+
+    def _apply(self, fn, recurse=True):
+        names = self.quantized_buffers()
+        for n in names:                                # whole numbers, which a cast to another floating-point type leaves alone
+            if self._buffers[n].is_floating_point():
+                self._buffers[n] = self._buffers[n].view(torch.int32 if n == "fp8_scale" else torch.uint8)
+        try:
+            super()._apply(fn, recurse)
+        finally:
+            for n in names:
+                t = self._buffers[n]
+                if n == "fp8_scale":
+                    self._buffers[n] = t.view(torch.float32)
+                elif n == "fp8_codes":
+                    self._buffers[n] = t if t.is_cuda else t.view(torch.float8_e4m3fn)
+                else:
+                    q = getattr(self, n.removesuffix("_bytes"))
+                    setattr(self, n.removesuffix("_bytes"), q.over(t, *q._like))
+            if "fp8_codes" in names:
+                self.fp8 = (self.fp8_codes, self.fp8_scale)
+        return self
+
+
+def weight_tensors(module: nn.Module):
+    """(name, tensor) of a module's weights: its parameters and the bytes of its quantised ones."""
+    yield from module.named_parameters()
+    for prefix, m in module.named_modules():
+        if isinstance(m, QuantizedState):
+            for n in m.quantized_buffers():
+                yield (prefix + "." if prefix else "") + n, m._buffers[n]
+
+
+class FusedLinear(QuantizedState, nn.Module):
     def __init__(self, in_features: int, out_features: int, bias: bool = True, dtype=torch.bfloat16,
                  device=None, init_std: float = 0.02):
         super().__init__()
@@ -46,7 +95,7 @@ class FusedLinear(nn.Module):
     def to_fp4(self, fmt: str, gated: bool = False) -> None:
         """Replaces the weight by its ``mxfp4`` or ``nvfp4`` form.  ``gated``: its rows are [gate | lift], for layers that are used through ``swiglu``."""
         from ...ops import lowbit
-        self.fp4 = lowbit.pack_weight(self.weight.data.to(torch.bfloat16), fmt, gated=gated)
+        self.set_packed("fp4", lowbit.pack_weight(self.weight.data.to(torch.bfloat16), fmt, gated=gated))
         self.weight.data = torch.empty(0, dtype=self.weight.dtype, device=self.weight.device)
 
     def _forward_fp4(self, x, act, residual, gate, out, kw):
@@ -63,7 +112,7 @@ class FusedLinear(nn.Module):
         if act in lowbit.ACT and bf16 and not self.lora and not self.fp4.gated:
             return lowbit.linear(x, self.fp4, self.bias, act, residual=residual, gate=gate, out=out)
         w = self.fp4
-        y = lowbit.linear(rows, lowbit.QuantRows(w.codes, w.scales, w.fmt, row_scale=w.row_scale) if w.gated else w)
+        y = lowbit.linear(rows, w.as_rows() if w.gated else w)
         if w.gated:                                    # asked for as [gate | lift] rows
             y = y.unflatten(-1, (-1, 2, 8)).transpose(-3, -2).flatten(-3)
         y = y.reshape(*lead, N)

@@ -100,6 +100,8 @@ def _epi(y, bias, act, residual, gate):
 def fp8_linear(x, fp8_state, bias=None, act=None, residual=None, gate=None, out=None, **_):
     """``x``: rows of bf16, quantised here, or fp8 ``QuantRows`` that a norm left (ops/lowbit.py)."""
     w8, sw = fp8_state
+    if w8.dim() != 2:
+        raise RuntimeError("fp8 layer: its weights are not in memory (asleep or offloaded)")
     K, N = x.shape[-1], w8.shape[0]
     ready = isinstance(x, QuantRows)
     if ready and (x.fmt != "fp8" or K != w8.shape[1]):
@@ -148,7 +150,7 @@ def quantize_layer(m, fmt: str, gated: bool = False) -> None:
         m.to_fp4(fmt, gated=gated)
         return
     w8, sw = quantize_weight_blockwise(m.weight.data)
-    m.fp8 = (w8.view(torch.uint8) if w8.is_cuda else w8, sw)
+    m.set_fp8(w8.view(torch.uint8) if w8.is_cuda else w8, sw)
     m.weight.data = torch.empty(0, dtype=m.weight.dtype, device=m.weight.device)
 
 

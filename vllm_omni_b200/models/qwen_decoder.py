@@ -19,7 +19,7 @@ from dataclasses import dataclass, field
 import torch
 from torch import nn
 
-from ..diffusion.layers.linear import FusedLinear
+from ..diffusion.layers.linear import FusedLinear, QuantizedState
 from ..ops import fused, kv_cache as KC, lowbit
 from ..ops.attention import attention
 from ..ops.moe import MoEScratch, MoEWorkspace, moe_forward, route
@@ -144,7 +144,7 @@ class RotaryTable:
         return ang.cos().contiguous(), ang.sin().contiguous()
 
 
-class DecoderLayer(nn.Module):
+class DecoderLayer(QuantizedState, nn.Module):
     def __init__(self, cfg: DecoderConfig, dtype, device, moe_scratch: MoEScratch):
         super().__init__()
         D, H, Hkv, Dh = cfg.hidden_size, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
@@ -229,8 +229,8 @@ class QwenDecoderModel(nn.Module):
                 quantize_layer(getattr(layer, name), fmt, gated=name == "gate_up")
                 n += 1
             if experts:
-                layer.w13_fp4 = lowbit.pack_weight(layer.w13.data.to(torch.bfloat16), fmt, gated=True)
-                layer.w2_fp4 = lowbit.pack_weight(layer.w2.data.to(torch.bfloat16), fmt)
+                layer.set_packed("w13_fp4", lowbit.pack_weight(layer.w13.data.to(torch.bfloat16), fmt, gated=True))
+                layer.set_packed("w2_fp4", lowbit.pack_weight(layer.w2.data.to(torch.bfloat16), fmt))
                 for p in (layer.w13, layer.w2):
                     p.data = torch.empty(0, dtype=p.dtype, device=p.device)
                 n += 2

@@ -65,7 +65,7 @@ class QuantRows:
     ``codes`` uint8 [.., R, K / 2] (fp8: [R, K]), element 2 i in the low half of byte i; ``scales`` as ``scale_shape`` says; ``row_scale`` fp32
     [.., R] for nvfp4.  ``gated``: the rows of a SwiGLU weight, 8 gate rows, their 8 lift rows, the next 8 gate rows and so on."""
 
-    __slots__ = ("fmt", "gated", "rows", "cols", "experts", "index", "_codes", "_scales", "_row", "_buf", "_ptr")
+    __slots__ = ("fmt", "gated", "rows", "cols", "experts", "index", "_codes", "_scales", "_row", "_buf", "_ptr", "_seen")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, row_scale: torch.Tensor | None = None, gated: bool = False):
         index = codes.get_device()
@@ -99,7 +99,48 @@ class QuantRows:
         q._ptr = (p, p + scales, p + row if fmt == "nvfp4" else 0)
         return q
 
+    @classmethod
+    def over(cls, buf: torch.Tensor, fmt: str, rows: int, cols: int, experts: int | None = None, gated: bool = False) -> "QuantRows":
+        """Rows that lie in ``buf`` (what ``storage`` of such rows is), wherever that is at the time of a call: a module keeps a weight's bytes as a buffer, whose
+        data may be moved off the GPU and back."""
+        q = cls.__new__(cls)
+        q._codes = q._scales = q._row = q._ptr = None
+        q._seen = (0, 0, 0)
+        q._buf, q.fmt, q.gated, q.rows, q.cols, q.experts, q.index = buf, fmt, gated, rows, cols, experts, buf.get_device()
+        return q
+
+    @property
+    def _like(self) -> tuple:
+        return self.fmt, self.rows, self.cols, self.experts, self.gated
+
+    def storage(self) -> torch.Tensor:
+        """Codes, scales and row factors as one uint8 tensor, each on 256 bytes."""
+        if self._buf is None:
+            size, *at = _layout(self.fmt, self.rows, self.cols, self.experts or 1)
+            buf = torch.zeros(size, dtype=torch.uint8, device=self.device)
+            for t, o in zip((self.codes, self.scales, self.row_scale), (0, *at)):
+                if t is not None:
+                    b = t.reshape(-1).view(torch.uint8)
+                    buf[o:o + b.numel()] = b
+            return buf
+        return self._buf
+
+    @property
+    def _at(self) -> tuple[int, int, int]:
+        """Where codes, scales and row factors lie."""
+        if self._ptr is not None:
+            return self._ptr
+        p = self._buf.data_ptr()
+        if p != self._seen[0] or not p:
+            size, scales, row = _layout(self.fmt, self.rows, self.cols, self.experts or 1)
+            if self._buf.numel() != size or p & 15:
+                raise RuntimeError(f"{self!r}: its weights are not in memory (asleep or offloaded), or not on 16 bytes")
+            self._seen = (p, p + scales, p + row if self.fmt == "nvfp4" else 0)
+        return self._seen
+
     def __reduce__(self):              # copies have addresses of their own
+        if self._ptr is None:
+            return QuantRows.over, (self._buf, *self._like)
         return QuantRows, (self.codes, self.scales, self.fmt, self.row_scale, self.gated)
 
     def _part(self, which: int) -> torch.Tensor:
@@ -117,21 +158,15 @@ class QuantRows:
 
     @property
     def codes(self) -> torch.Tensor:
-        if self._codes is None:
-            self._codes = self._part(0)
-        return self._codes
+        return self._part(0) if self._codes is None else self._codes
 
     @property
     def scales(self) -> torch.Tensor:
-        if self._scales is None:
-            self._scales = self._part(1)
-        return self._scales
+        return self._part(1) if self._scales is None else self._scales
 
     @property
     def row_scale(self) -> torch.Tensor | None:
-        if self._row is None and self.fmt == "nvfp4":
-            self._row = self._part(2)
-        return self._row
+        return self._part(2) if self._row is None and self.fmt == "nvfp4" else self._row
 
     @property
     def shape(self) -> tuple[int, ...]:
@@ -144,6 +179,10 @@ class QuantRows:
     @property
     def is_cuda(self) -> bool:
         return self.index >= 0
+
+    def as_rows(self) -> "QuantRows":
+        """A gated weight's rows as those of an ordinary one."""
+        return QuantRows.over(self.storage(), self.fmt, self.rows, self.cols, self.experts)
 
     @property
     def out_features(self) -> int:
@@ -296,7 +335,7 @@ def _rows(x, fmt, experts=None, gated=False) -> QuantRows:
     rows, cols = x.shape
     per = rows // experts if experts else rows
     q = QuantRows._empty(fmt, per, cols, index, experts, gated)
-    rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], 0, 0, 0, 0.0, 0, 0, 0, 0, *q._ptr, _stream(index))
+    rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, per, FORMATS[fmt], 0, 0, 0, 0.0, 0, 0, 0, 0, *q._at, _stream(index))
     if rc:
         nv.check_rc(rc, "omni_lowbit_rows")
     return q
@@ -348,7 +387,7 @@ def dequantize(q: QuantRows, dtype: torch.dtype = torch.bfloat16) -> torch.Tenso
         with torch.cuda.device(q.index):
             return dequantize(q, dtype)
     out = torch.empty(q.shape, dtype=dtype, device=_device(q.index))
-    codes, scales, row = q._ptr
+    codes, scales, row = q._at
     rc = _entry("omni_lowbit_dequantize")(codes, scales, row, q.rows * (q.experts or 1), q.cols, q.rows, FORMATS[q.fmt], int(dtype is torch.float32),
                                           out.data_ptr(), _stream(q.index))
     if rc:
@@ -399,7 +438,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, fmt: str, eps: floa
         np_, ln = _out_rows(normed, "normed", cols)
     rows = x.shape[0]
     q = QuantRows._empty(fmt, rows, cols, index)
-    rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, rows, FORMATS[fmt], rp, lr, weight.data_ptr(), eps, tp, lt, np_, ln, *q._ptr, _stream(index))
+    rc = _entry("omni_lowbit_rows")(x.data_ptr(), x.stride(0), rows, cols, rows, FORMATS[fmt], rp, lr, weight.data_ptr(), eps, tp, lt, np_, ln, *q._at, _stream(index))
     if rc:
         nv.check_rc(rc, "omni_lowbit_rows")
     return q
@@ -499,7 +538,7 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
     if gate is not None:
         gp, B = gate.data_ptr(), gate.shape[0]
         lds, per = gate.stride(0) if B > 1 else 0, max(1, M // B)
-    rc = _entry("omni_lowbit_linear")(raw, ldx, *q._ptr, *w._ptr, yp, ldo[0], M, w.rows, cols, FORMATS[fmt], int(gated), bp, ACT[act], gp, lds, per, rp, ldr[0],
+    rc = _entry("omni_lowbit_linear")(raw, ldx, *q._at, *w._at, yp, ldo[0], M, w.rows, cols, FORMATS[fmt], int(gated), bp, ACT[act], gp, lds, per, rp, ldr[0],
                                       force_tile, force_split, _status(index), _stream(index))
     if rc:
         nv.check_rc(rc, "omni_lowbit_linear")
@@ -593,7 +632,7 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
         nv.lib("moe").omni_moe_set_bounds(c_long(pairs), ctypes.c_void_p(status))
     rc = _entry("omni_moe_plan_places")(ids.data_ptr(), pairs, E, 0, E, tile, max_tiles, row_of_pair, te, tr, tn, n_rows, of_pair, pitch, stream)
     rc = rc or _entry("omni_lowbit_experts")(x2.data_ptr(), x2.stride(0), k, pairs, E, FORMATS[fmt], h, y, row_of_pair, of_pair, te, tr, tn, max_tiles, tile, n_rows, of_row, status,
-                                             stream, *ops[:3], *up._ptr, up.rows, D, *ops[3:], *down._ptr, down.rows, Fd)
+                                             stream, *ops[:3], *up._at, up.rows, D, *ops[3:], *down._at, down.rows, Fd)
     rc = rc or _combine()(y, row_of_pair, weights.data_ptr(), T, k, D, 0 if res is None else res.data_ptr(), 0 if res is None else res.stride(0), o2.data_ptr(),
                           o2.stride(0), stream)
     if rc:
