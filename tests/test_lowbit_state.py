@@ -2,9 +2,11 @@
 from __future__ import annotations
 
 import copy
+import types
 
 import pytest
 import torch
+from torch import nn
 
 from vllm_omni_b200.diffusion.layers.linear import FusedLinear, weight_tensors
 from vllm_omni_b200.diffusion.quantization.fp8 import quantize_layer
@@ -95,3 +97,61 @@ def test_copied_decoder(fmt, experts, device):
     for _, t in weight_tensors(m):
         t.view(torch.uint8).zero_()
     assert torch.equal(other(batch)[0], want)
+
+
+# ------------------------------------------------------------------ sleep
+class Denoiser(nn.Module):
+    graph_safe_forward = True
+
+    def __init__(self, fmt, device):
+        super().__init__()
+        self.blocks = nn.ModuleList(layer(fmt, device, seed, 1024, 1024) for seed in range(3))
+
+    def forward(self, x):
+        for b in self.blocks:
+            x = b(x, act="silu")
+        return x
+
+
+class Pipe(nn.Module):
+    def __init__(self, fmt, device="cpu"):
+        super().__init__()
+        self.transformer = Denoiser(fmt, device)
+
+
+def worker_of(pipe, device):
+    from vllm_omni_b200.diffusion.data import OmniDiffusionConfig
+    from vllm_omni_b200.diffusion.worker import DiffusionWorker
+    w = DiffusionWorker(0, 0, OmniDiffusionConfig(model="none", diffusion_load_format="dummy"))
+    w.device, w.model_runner = torch.device(device), types.SimpleNamespace(pipeline=pipe)
+    return w
+
+
+def test_graphs_of_moving_weights_are_released():
+    """On the CPU, with captures that are only names: a pipeline's graphed forwards and its captured loops."""
+    from vllm_omni_b200.diffusion.graphed import GraphedForward, _Entry, release_graphs
+    pipe = Pipe("bf16")
+    f = pipe.transformer.forward = GraphedForward(pipe.transformer.forward)
+    f.entries["a"], f.entries["b"] = _Entry(), _Entry()
+    f.entries["a"].graph = "captured"
+    pipe._loop_cache = {1: types.SimpleNamespace(graph="captured"), 2: types.SimpleNamespace(graph=None)}
+    assert release_graphs(pipe) == 2 and not f.entries and not pipe._loop_cache
+    assert release_graphs(pipe) == 0
+
+
+@gpu
+def test_sleep_after_a_capture():
+    from vllm_omni_b200.diffusion.graphed import maybe_graph_transformer
+    pipe, x = Pipe("bf16", "cuda"), rows(5, 1024, "cuda")
+    want = pipe.transformer(x).clone()
+    assert maybe_graph_transformer(pipe, types.SimpleNamespace(enforce_eager=False))
+    w = worker_of(pipe, "cuda")
+    for _ in range(2):
+        for _ in range(4):
+            assert torch.equal(pipe.transformer(x), want)
+        assert pipe.transformer.forward.replays
+        w.sleep(1)
+        assert not pipe.transformer.forward.entries
+        held = torch.full((3 * 1024 * 1024,), 7.0, dtype=BF, device="cuda")          # where the weights were
+        w.wake_up()
+        del held

@@ -180,3 +180,19 @@ def maybe_graph_transformer(pipe, od_config) -> bool:
                 and getattr(tr, "block_hook", None) is None and not getattr(tr, "_lora_active", False))
     tr.forward = GraphedForward(tr.forward, enabled=enabled)
     return True
+
+
+def release_graphs(pipe) -> int:
+    """Drops what was captured of a pipeline whose weights are about to move: a graph replays the addresses it was captured with.  Forwards warm up and
+    are captured again afterwards.  Returns the number of captures dropped."""
+    n = 0
+    for m in pipe.modules():
+        f = m.__dict__.get("forward")
+        if isinstance(f, GraphedForward):
+            n += sum(e.graph is not None for e in f.entries.values())
+            f.entries.clear()
+    loops = getattr(pipe, "_loop_cache", None)
+    if loops:
+        n += sum(st.graph is not None for st in loops.values())
+        loops.clear()
+    return n

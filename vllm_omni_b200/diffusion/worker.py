@@ -108,6 +108,9 @@ class DiffusionWorker:
         if self._sleeping_level or self.device.type != "cuda":
             self._sleeping_level = level
             return 0
+        from .graphed import release_graphs
+        torch.cuda.synchronize()
+        release_graphs(self.model_runner.pipeline)
         freed = 0
         for name, p in self.model_runner.pipeline.named_parameters():
             freed += p.numel() * p.element_size()
