@@ -155,3 +155,24 @@ def test_sleep_after_a_capture():
         held = torch.full((3 * 1024 * 1024,), 7.0, dtype=BF, device="cuda")          # where the weights were
         w.wake_up()
         del held
+
+
+@gpu
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_sleep_moves_quantised_weights(fmt, captured):
+    from vllm_omni_b200.diffusion.graphed import maybe_graph_transformer
+    pipe, x = Pipe(fmt, "cuda"), rows(5, 1024, "cuda")
+    want = pipe.transformer(x).clone()
+    if captured:
+        maybe_graph_transformer(pipe, types.SimpleNamespace(enforce_eager=False))
+    w = worker_of(pipe, "cuda")
+    for _ in range(2):
+        for _ in range(3):
+            assert torch.equal(pipe.transformer(x), want)
+        before = torch.cuda.memory_allocated()
+        freed = w.sleep(1)
+        assert freed >= 3 * 1024 * 1024 // 2 and before - torch.cuda.memory_allocated() >= freed
+        held = torch.full((8 * 1024 * 1024,), 0x55, dtype=torch.uint8, device="cuda")
+        w.wake_up()
+        del held

@@ -103,16 +103,17 @@ class DiffusionWorker:
 
     # ------------------------------------------------------------------ sleep mode
     def sleep(self, level: int = 1) -> int:
-        """Level 1 moves the weights to pinned host memory, level 2 discards them; both
+        """Level 1 moves the weights (quantised ones too) to pinned host memory, level 2 discards them; both
         release the GPU memory.  Returns the number of bytes freed."""
         if self._sleeping_level or self.device.type != "cuda":
             self._sleeping_level = level
             return 0
         from .graphed import release_graphs
+        from .layers.linear import weight_tensors
         torch.cuda.synchronize()
         release_graphs(self.model_runner.pipeline)
         freed = 0
-        for name, p in self.model_runner.pipeline.named_parameters():
+        for name, p in weight_tensors(self.model_runner.pipeline):
             freed += p.numel() * p.element_size()
             if level == 1:
                 host = torch.empty(p.shape, dtype=p.dtype, pin_memory=self.od_config.pin_cpu_memory)
@@ -130,7 +131,8 @@ class DiffusionWorker:
         if self._sleeping_level == 2 and not self._offloaded and self.device.type == "cuda":
             self.model_runner.load_model()        # weights were discarded: reload
         else:
-            params = dict(self.model_runner.pipeline.named_parameters())
+            from .layers.linear import weight_tensors
+            params = dict(weight_tensors(self.model_runner.pipeline))
             for name, host in self._offloaded.items():
                 params[name].data = host.to(self.device, non_blocking=True)
             if self.device.type == "cuda":
