@@ -176,3 +176,58 @@ def test_sleep_moves_quantised_weights(fmt, captured):
         held = torch.full((8 * 1024 * 1024,), 0x55, dtype=torch.uint8, device="cuda")
         w.wake_up()
         del held
+
+
+# ------------------------------------------------------------------ offloading
+def image_transformer():
+    from vllm_omni_b200.diffusion.models.qwen_image.transformer import QwenImageTransformer2DModel, QwenImageTransformerConfig
+    cfg = QwenImageTransformerConfig(num_layers=3, attention_head_dim=128, num_attention_heads=2, joint_attention_dim=64, in_channels=16, out_channels=4,
+                                     axes_dims_rope=(16, 56, 56))
+    torch.manual_seed(0)
+    m = QwenImageTransformer2DModel(cfg, dtype=BF, device="cuda")
+    for p in m.parameters():
+        if p.dim() > 1:
+            p.data.normal_(0, 0.05)
+    return m
+
+
+def quantised(m, fmt):
+    from vllm_omni_b200.diffusion.quantization.fp8 import quantize_pipeline
+    if fmt != "bf16":
+        assert quantize_pipeline(types.SimpleNamespace(transformer=m), types.SimpleNamespace(quantization=fmt, quantization_config={"min_features": 128})) >= 24
+    return m
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ("bf16", *FORMATS))
+def test_layerwise_offload(fmt):
+    from vllm_omni_b200.diffusion.offloader import LayerWiseOffloadBackend
+    args = (torch.randn(1, 64, 16, device="cuda").to(BF), torch.randn(1, 6, 64, device="cuda").to(BF), torch.tensor([0.5], device="cuda"), (1, 8, 8))
+    m = quantised(image_transformer(), fmt)
+    want = m(*args).clone()
+    before = torch.cuda.memory_allocated()
+    b = LayerWiseOffloadBackend(torch.device("cuda", 0))
+    b.enable(types.SimpleNamespace(transformer=m))
+    bits = {"bf16": 16, "fp8": 8, "mxfp4": 4.25, "nvfp4": 4.5}[fmt]
+    block = 2 * (4 + 8) * 256 * 256 * bits / 8                               # both streams: qkv and out, MLP up and down
+    assert before - torch.cuda.memory_allocated() >= 3 * block and all(h.numel() >= block for h in b.host)
+    for _ in range(2):
+        assert torch.equal(m(*args), want)
+        assert not b.resident
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ("bf16", *FORMATS))
+def test_model_level_offload(fmt):
+    from vllm_omni_b200.diffusion.offloader import ModelLevelOffloadBackend
+    args = (torch.randn(1, 64, 16, device="cuda").to(BF), torch.randn(1, 6, 64, device="cuda").to(BF), torch.tensor([0.5], device="cuda"), (1, 8, 8))
+    m = quantised(image_transformer(), fmt)
+    want = m(*args).clone()
+    b = ModelLevelOffloadBackend(torch.device("cuda", 0))
+    b.enable(types.SimpleNamespace(transformer=m, text_encoder=nn.Linear(4, 4, device="cuda")))
+    assert all(t.device.type == "cpu" for _, t in weight_tensors(m))
+    for _ in range(2):
+        b.use("transformer")
+        assert torch.equal(m(*args), want)
+        b.use("text_encoder")
+        assert all(t.device.type == "cpu" for _, t in weight_tensors(m))

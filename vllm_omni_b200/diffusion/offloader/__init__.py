@@ -11,6 +11,10 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from ..layers.linear import weight_tensors
+
+ALIGN = 256                                     # bytes: every tensor of a block begins as an allocation of its own would (the tensor cores' operands: on 16)
+
 
 def get_offload_backend(od_config, device):
     if device.type != "cuda":
@@ -46,8 +50,8 @@ class LayerWiseOffloadBackend:
         self.blocks = self._blocks(tr)
         self.copy_stream = torch.cuda.Stream(self.device)
         for blk in self.blocks:
-            params = [p for p in blk.parameters()]
-            total = sum(p.numel() * p.element_size() for p in params)
+            params = [p for _, p in weight_tensors(blk)]
+            total = sum(-(-p.numel() * p.element_size() // ALIGN) * ALIGN for p in params)
             flat = torch.empty(total, dtype=torch.uint8, pin_memory=self.pin)
             lay, off = [], 0
             for p in params:
@@ -55,7 +59,7 @@ class LayerWiseOffloadBackend:
                 flat[off:off + n].copy_(p.data.detach().contiguous().view(torch.uint8).reshape(-1).cpu())
                 lay.append((p, off, n, p.shape, p.dtype))
                 p.data = torch.empty(0, dtype=p.dtype, device=self.device)
-                off += n
+                off += -(-n // ALIGN) * ALIGN
             self.host.append(flat)
             self.layout.append(lay)
         torch.cuda.empty_cache()
