@@ -178,6 +178,21 @@ def test_sleep_moves_quantised_weights(fmt, captured):
         del held
 
 
+def test_weights_of_quantised_layers_are_not_loaded_again():
+    for fmt in ("bf16", *FORMATS):
+        pipe = Pipe(fmt)
+        seen = []
+        pipe.load_weights = lambda w: seen.append(dict(w))
+        w = worker_of(pipe, "cpu")
+        if fmt == "bf16":
+            w.load_weights([("a", 1)])
+            assert seen == [{"a": 1}]
+        else:
+            with pytest.raises(NotImplementedError, match="quantised"):
+                w.load_weights([("a", 1)])
+            assert not seen
+
+
 # ------------------------------------------------------------------ offloading
 def image_transformer():
     from vllm_omni_b200.diffusion.models.qwen_image.transformer import QwenImageTransformer2DModel, QwenImageTransformerConfig

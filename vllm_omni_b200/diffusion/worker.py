@@ -142,6 +142,9 @@ class DiffusionWorker:
         return True
 
     def load_weights(self, weights) -> set:
+        from .layers.linear import FusedLinear
+        if any(isinstance(m, FusedLinear) and m.quantized for m in self.model_runner.pipeline.modules()):
+            raise NotImplementedError("load_weights: this pipeline's weights are quantised; load the model anew instead")
         return self.model_runner.pipeline.load_weights(weights)
 
     # ------------------------------------------------------------------ profiling
