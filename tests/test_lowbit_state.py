@@ -10,6 +10,7 @@ from torch import nn
 
 from vllm_omni_b200.diffusion.layers.linear import FusedLinear, weight_tensors
 from vllm_omni_b200.diffusion.quantization.fp8 import quantize_layer
+from vllm_omni_b200.ops import lowbit as L
 from test_lowbit_layers import decoder, prompt
 
 BF = torch.bfloat16
@@ -97,6 +98,33 @@ def test_copied_decoder(fmt, experts, device):
     for _, t in weight_tensors(m):
         t.view(torch.uint8).zero_()
     assert torch.equal(other(batch)[0], want)
+
+
+# ------------------------------------------------------------------ adapters
+def adapters(device, n_in=256, n_out=128):
+    g = torch.Generator().manual_seed(3)
+    return [((torch.randn(8, n_in, generator=g) / 16).to(BF).to(device), torch.randn(n_out, 8, generator=g).to(BF).to(device), s) for s in (0.5, -0.25)]
+
+
+def with_deltas(base, x, lora):
+    """(base + the adapters' products, bound) in 64 bits: per adapter bf16 roundings of two products, of its scaling and of the sum."""
+    y, size = base.double(), base.double().abs()
+    for A, B, s in lora:
+        y = y + s * (x.double() @ A.double().t()) @ B.double().t()
+        size = size + abs(s) * (x.double().abs() @ A.double().abs().t()) @ B.double().abs().t()
+    return y, 4 * len(lora) * 2.0 ** -8 * size + 1e-30
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fmt", ("mxfp4", "nvfp4"))
+def test_adapters_of_a_layer_that_gets_quantised_rows(fmt, device):
+    m, x = layer(fmt, device), rows(device=device)
+    q = L.rms_norm_quantize(x, torch.ones(256, dtype=BF, device=device), fmt)
+    base = m(q)
+    m.lora = adapters(device)
+    want, tol = with_deltas(base, L.dequantize(q), m.lora)
+    assert ((m(q).double() - want).abs() <= tol).all()
+    assert m.swiglu(q).shape == (5, 64)
 
 
 # ------------------------------------------------------------------ sleep

@@ -120,9 +120,16 @@ class FusedLinear(QuantizedState, nn.Module):
             y = y.to(x.dtype)
         if self.bias is not None:
             y = y + self.bias
+        return _epilogue(self._adapted(y, x), act, residual, gate, out, kw.get("coef", (0.0, 0.0)))
+
+    def _adapted(self, y, x):
+        """y + the adapters' products of x (of the values of rows that a norm has quantised)."""
+        if self.lora and not isinstance(x, torch.Tensor):
+            from ...ops import lowbit
+            x = lowbit.dequantize(x)
         for (A, B, scale) in self.lora or ():
             y = y + scale * gemm.linear(gemm.linear(x, A), B)
-        return _epilogue(y, act, residual, gate, out, kw.get("coef", (0.0, 0.0)))
+        return y
 
     def forward(self, x, act=None, residual=None, gate=None, out=None, **kw):
         if self.fp4 is not None:
