@@ -127,6 +127,19 @@ def test_adapters_of_a_layer_that_gets_quantised_rows(fmt, device):
     assert m.swiglu(q).shape == (5, 64)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_adapters_of_an_fp8_layer(device):
+    """They take part, before the activation, for rows of bf16 and for rows that a norm has quantised."""
+    m, x = layer("fp8", device), rows(device=device)
+    q = L.rms_norm_quantize(x, torch.ones(256, dtype=BF, device=device), "fp8")
+    plain, normed = m(x), m(q)
+    m.lora = adapters(device)
+    for got, base, v in ((m(x), plain, x), (m(q), normed, L.dequantize(q))):
+        want, tol = with_deltas(base, v, m.lora)
+        assert ((got.double() - want).abs() <= tol).all()
+    assert torch.equal(m(x, act="silu"), torch.nn.functional.silu(m(x)))
+
+
 # ------------------------------------------------------------------ sleep
 class Denoiser(nn.Module):
     graph_safe_forward = True

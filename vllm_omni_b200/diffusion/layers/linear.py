@@ -136,12 +136,12 @@ class FusedLinear(QuantizedState, nn.Module):
             return self._forward_fp4(x, act, residual, gate, out, kw)
         if self.fp8 is not None:
             from ..quantization.fp8 import fp8_linear
-            y = fp8_linear(x, self.fp8, self.bias, act=act, residual=residual, gate=gate, out=out, **kw)
+            if not self.lora:
+                return fp8_linear(x, self.fp8, self.bias, act=act, residual=residual, gate=gate, out=out, **kw)
+            y = _epilogue(self._adapted(fp8_linear(x, self.fp8, self.bias), x), act, residual, gate, out, kw.get("coef", (0.0, 0.0)))
         elif self.lora:
             # the LoRA delta enters before the activation / gate, so apply the epilogue last
-            y = gemm.linear(x, self.weight, self.bias)
-            for (A, B, scale) in self.lora:
-                y = y + scale * gemm.linear(gemm.linear(x, A), B)
+            y = self._adapted(gemm.linear(x, self.weight, self.bias), x)
             y = _epilogue(y, act, residual, gate, out, kw.get("coef", (0.0, 0.0)))
         else:
             y = gemm.linear(x, self.weight, self.bias, act=act, residual=residual, gate=gate, out=out, **kw)
