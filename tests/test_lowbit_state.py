@@ -287,3 +287,19 @@ def test_model_level_offload(fmt):
         assert torch.equal(m(*args), want)
         b.use("text_encoder")
         assert all(t.device.type == "cpu" for _, t in weight_tensors(m))
+
+
+# ------------------------------------------------------------------ what a request for quantised weights reaches
+def test_quantization_beside_a_stage_configuration(tmp_path, monkeypatch):
+    """The stages of a configuration take it from there; asked for beside one it is refused (fp8: said not to have any effect), before a stage is started."""
+    from vllm_omni_b200.entrypoints import stage_runtime
+    path, said = tmp_path / "stages.yaml", []
+    path.write_text("stage_args: []\n")
+    monkeypatch.setattr(stage_runtime.logger, "warning", lambda text, *args: said.append(text % args))
+    for fmt in ("mxfp4", "nvfp4"):
+        with pytest.raises(ValueError, match="engine_args.quantization"):
+            stage_runtime.build_stages(None, str(path), {"quantization": fmt})
+    stage_runtime.build_stages(None, str(path), {"quantization": None})
+    assert not said
+    assert stage_runtime.build_stages(None, str(path), {"quantization": "fp8"})[0] == []
+    assert len(said) == 1 and "engine_args.quantization" in said[0]

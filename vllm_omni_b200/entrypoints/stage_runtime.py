@@ -524,6 +524,12 @@ def build_stages(model, stage_configs_path, kwargs: dict, stage_init_timeout=300
         ray_utils.initialize_ray_cluster()
     path = stage_configs_path or resolve_model_config_path(model)
     if path is not None:
+        if kwargs.get("quantization"):
+            # which stages it is for only the configuration can say.  fp8 has been passed over here before low-bit stages existed: such calls go on
+            text = f"quantization={kwargs['quantization']!r} does not reach the stages of {path}: set engine_args.quantization of those it is for"
+            if kwargs["quantization"] != "fp8":
+                raise ValueError(text)
+            logger.warning("%s; they run unquantised", text)
         base = {k: v for k, v in kwargs.items() if k in ("dtype", "seed", "device", "load_format")}
         pcfg = load_stage_configs_from_yaml(path, base)
     else:
