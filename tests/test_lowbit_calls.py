@@ -3,6 +3,8 @@ from __future__ import annotations
 
 import copy
 import pickle
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -131,3 +133,13 @@ def test_copies_have_addresses_of_their_own(fmt, device):
     other = copy.deepcopy(w)
     assert other.gated and other.shape == (3, 32, 64) and other._ptr[0] != w._ptr[0]
     same(other, w)
+
+
+# ------------------------------------------------------------------ launches
+CSRC = Path(__file__).resolve().parent.parent / "vllm_omni_b200" / "csrc"
+
+
+def test_resident_pairs_are_kept_per_kernel_and_device(tmp_path):
+    exe = tmp_path / "per_device"
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-o", str(exe), str(CSRC / "host_tests" / "per_device.cpp")], check=True)
+    assert subprocess.run([str(exe)]).returncode == 0

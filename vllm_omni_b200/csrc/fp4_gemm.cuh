@@ -25,6 +25,7 @@
 #pragma once
 #include "host_util.h"
 #include "lowbit.cuh"
+#include "per_device.h"
 
 namespace omni {
 
@@ -627,23 +628,27 @@ struct Fp4Operands {
   long x_rows, xs_tiles;         // rows of X, its scale tiles of 128 rows
 };
 
-// How many pairs run at once: a persistent kernel of more would leave its last ones to a round of their own.
-static int resident_pairs(const void* kernel, int threads, int smem) {
-  static int cached = 0;
-  if (cached) return cached;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(sm_count() & ~1);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
-  (void)cudaGetLastError();
-  return cached = n <= 0 || n > sm_count() / 2 ? sm_count() / 2 : n;
+// How many pairs of a kernel run at once on the current device: a persistent kernel of more would leave its last ones to a round of their own.
+static int resident_pairs(PerDevice& known, const void* kernel, int threads, int smem) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int half = sm_count() / 2;
+  const int n = known.get(dev, half, [&] {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * half);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0;
+    (void)cudaGetLastError();
+    return clusters;
+  });
+  return n < half ? n : half;
 }
 
 template <int FMT, int XR, int EPI, bool PAIR>
@@ -664,10 +669,11 @@ static int launch_fp4(Fp4Args& a, const Fp4Operands& o, int* status, cudaStream_
   if (int rc = make_map(&a.tmXS, o.xs, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, xsd, xsp, xsb, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
 
   static unsigned long long prepared = 0;
+  static PerDevice pairs;
   auto* kernel = fp4_kernel<FMT, XR, EPI, PAIR>;
   if (int e = ensure_dynamic_smem((const void*)kernel, Cfg::SMEM_BYTES, prepared)) return e;
   const long items = (long)a.max_tiles * ((a.N + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128));
-  const int group = (PAIR ? 2 : 1) * a.split, most = PAIR ? resident_pairs((const void*)kernel, Cfg::THREADS, Cfg::SMEM_BYTES) : Cfg::CTAS * sm_count();
+  const int group = (PAIR ? 2 : 1) * a.split, most = PAIR ? resident_pairs(pairs, (const void*)kernel, Cfg::THREADS, Cfg::SMEM_BYTES) : Cfg::CTAS * sm_count();
   const long run = a.split > 1 ? items : items < most ? items : most;
   if (run <= 0 || run * group > 0x7fffffffL) return RC_BAD_ARG;
   return launch_with(true, group, kernel, (unsigned)(run * group), Cfg::THREADS, Cfg::SMEM_BYTES, stream, a, status);
