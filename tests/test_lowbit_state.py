@@ -12,6 +12,7 @@ from vllm_omni_b200.diffusion.layers.linear import FusedLinear, weight_tensors
 from vllm_omni_b200.diffusion.quantization.fp8 import quantize_layer
 from vllm_omni_b200.ops import lowbit as L
 from test_lowbit_layers import decoder, prompt
+from test_model_zoo import GPU_CASES
 
 BF = torch.bfloat16
 FORMATS = ("fp8", "mxfp4", "nvfp4")
@@ -98,6 +99,53 @@ def test_copied_decoder(fmt, experts, device):
     for _, t in weight_tensors(m):
         t.view(torch.uint8).zero_()
     assert torch.equal(other(batch)[0], want)
+
+
+# ------------------------------------------------------------------ operands
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fmt", ("mxfp4", "nvfp4"))
+def test_residual_and_out_of_another_shape(fmt, device):
+    """Rows are what counts, as in the bf16 layer: [B, S, N] or [B S, N]."""
+    m, x = layer(fmt, device), rows(6, 256, device).view(2, 3, 256)
+    r = rows(6, 128, device)
+    q = L.quantize(x, fmt)
+    for act in (None, "relu2"):                                             # in the product's epilogue, and after it
+        want = m(x, act=act, residual=r.view(2, 3, 128))
+        assert want.shape == (2, 3, 128)
+        for res in (r, r.view(1, 6, 128), r.view(3, 2, 128)):
+            assert torch.equal(m(x, act=act, residual=res), want)
+            assert torch.equal(m(q, act=act, residual=res), want.view(6, 128))
+        for out in (torch.zeros_like(r), torch.zeros_like(r).view(1, 6, 128), torch.zeros(6, 136, dtype=BF, device=device)[:, :128],
+                    torch.zeros(6, 1, 256, dtype=BF, device=device)[..., :128], torch.zeros(3, 4, 128, dtype=BF, device=device)[:, 1:3]):
+            assert m(x, act=act, residual=r, out=out) is out and torch.equal(out.reshape(6, 128), want.view(6, 128))
+            own = r.clone().view(out.shape)
+            assert m(x, act=act, residual=own, out=own) is own and torch.equal(own.reshape(6, 128), want.view(6, 128))
+    for bad in (dict(residual=r[:5]), dict(out=torch.zeros(5, 128, dtype=BF, device=device))):
+        with pytest.raises((ValueError, RuntimeError)):
+            m(x, **bad)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ("mxfp4", "nvfp4"))
+@pytest.mark.parametrize("name", sorted(GPU_CASES))
+def test_every_pipeline_on_a_gpu(name, fmt, monkeypatch):
+    """All layers of all transformers that 4 bits can hold, in bf16 on the GPU, through two steps: no operand of theirs is refused."""
+    from vllm_omni_b200.diffusion.quantization import fp8
+    from vllm_omni_b200.entrypoints.omni_diffusion import OmniDiffusion
+    from vllm_omni_b200.inputs import OmniDiffusionSamplingParams
+    counted, convert = [], fp8.quantize_pipeline
+    monkeypatch.setattr(fp8, "quantize_pipeline", lambda *a: counted.append(convert(*a)))
+    tf, vae = GPU_CASES[name]
+    o = OmniDiffusion(name, dtype="bfloat16", device="cuda", tf_model_config=tf, quantization=fmt, quantization_config={"min_features": 32},
+                      vae_config=vae if vae is not None else dict(block_out_channels=(32, 32, 32, 32), layers_per_block=1, norm_num_groups=8))
+    try:
+        out = o.generate([{"prompt": "a small test", "negative_prompt": " "}],
+                         OmniDiffusionSamplingParams(height=128, width=128, num_inference_steps=2, seed=0, num_frames=5, guidance_scale=3.0,
+                                                     extra_args={"audio_seconds": 0.05}))[0]
+        assert out.images or out.multimodal_output
+        assert len(counted) == 1 and counted[0] > 0
+    finally:
+        o.close()
 
 
 # ------------------------------------------------------------------ adapters

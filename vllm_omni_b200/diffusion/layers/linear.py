@@ -7,6 +7,8 @@ weights attach to the same object.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 from torch import nn
 from torch.nn.modules.module import _has_any_global_hook
@@ -109,6 +111,15 @@ class FusedLinear(QuantizedState, nn.Module):
         if not bf16:
             rows = rows.to(torch.bfloat16)             # the CPU's fp32 models: products of 4-bit operands are bf16
         N = self.out_features
+        if residual is not None and residual.shape != (*lead, N):
+            residual = residual.reshape(*lead, N)      # rows are what counts, as in the bf16 layer
+        if out is not None and out.shape != (*lead, N) and out.numel() == math.prod(lead) * N:
+            try:
+                there = out.view(*lead, N)
+            except RuntimeError:                       # no view of these strides: by a result of its own
+                return out.copy_(self._forward_fp4(x, act, residual, gate, None, kw).reshape(out.shape))
+            self._forward_fp4(x, act, residual, gate, there, kw)
+            return out
         if act in lowbit.ACT and bf16 and not self.lora and not self.fp4.gated:
             return lowbit.linear(x, self.fp4, self.bias, act, residual=residual, gate=gate, out=out)
         w = self.fp4
