@@ -117,6 +117,28 @@ def test_single_rows_of_an_odd_pitch(fmt, at, device):
     assert torch.equal(L.experts(x, ids, p, up, down, residual=r), L.experts(xc, ids, p, up, down, residual=rc))
 
 
+# ------------------------------------------------------------------ results whose rows lie on one another
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_of_a_result_must_not_overlap(device):
+    x, gain = rows_of(6, 64, device=device), rows_of(1, 64, 3, device)[0]
+    w = L.pack_weight(rows_of(64, 64, 4, device), "nvfp4")
+    up, down = L.pack_weight(rows_of(3 * 64, 64, 5, device).view(3, 64, 64), "nvfp4", gated=True), L.pack_weight(rows_of(3 * 64, 32, 6, device).view(3, 64, 32), "nvfp4")
+    ids, p = torch.zeros(6, 1, dtype=torch.int32, device=device), torch.ones(6, 1, device=device)
+    buf = torch.zeros(6 * 64, dtype=BF, device=device)
+    for bad in (buf[:64].expand(6, 64), buf.as_strided((6, 64), (48, 1))):
+        for call in (lambda: L.rms_norm_quantize(x, gain, "nvfp4", total=bad), lambda: L.rms_norm_quantize(x, gain, "nvfp4", normed=bad),
+                     lambda: L.linear(x, w, out=bad), lambda: L.experts(x, ids, p, up, down, out=bad)):
+            with pytest.raises(ValueError, match="overlap"):
+                call()
+    with pytest.raises((ValueError, RuntimeError)):
+        L.linear(x.view(2, 3, 64), w, out=buf[:64].expand(2, 3, 64))
+    turned = torch.zeros(64, 6, dtype=BF, device=device).t()               # columns side by side: copied into
+    assert torch.equal(L.experts(x, ids, p, up, down, out=turned), L.experts(x, ids, p, up, down))
+    one = buf.as_strided((1, 64), (0, 1))                                 # a single row: its stride does not count
+    assert torch.equal(L.linear(x[:1], w, out=one), L.linear(x[:1], w))
+    same(L.rms_norm_quantize(x, gain, "nvfp4", residual=gain.expand(6, 64)), L.rms_norm_quantize(x, gain, "nvfp4", residual=gain.repeat(6, 1)))      # read only: may
+
+
 # ------------------------------------------------------------------ copies
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("fmt", tuple(L.FORMATS))

@@ -413,6 +413,9 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, fmt: str, eps: floa
     if normed is not None:
         _check_operand("normed", normed, shape, index)
     if index < 0:
+        for name, t in (("total", total), ("normed", normed)):
+            if t is not None and t.dim() == 2:
+                _check_apart(name, t)
         s = _rows16(x, "x")
         if residual is not None:
             s = (s.float() + residual.reshape(s.shape).float()).to(x.dtype)
@@ -453,7 +456,14 @@ def _out_rows(t: torch.Tensor, name: str, cols: int) -> tuple[int, int]:
         ld = cols
     if one != 1 or ld % 8 or at % 16:
         raise ValueError(f"{name}: rows must begin on 16 bytes")
+    _check_apart(name, t)
     return at, ld
+
+
+def _check_apart(name: str, t: torch.Tensor) -> None:
+    """Rows that a kernel writes must not share memory (an expanded tensor's do).  Other layouts are copied into, which checks them."""
+    if t.shape[0] > 1 and t.stride(1) == 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}: rows overlap (pitch {t.stride(0)}, {t.shape[1]} columns)")
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -494,6 +504,8 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
                              or gate.dtype is not torch.bfloat16 or gate.get_device() != index):
         raise ValueError(f"gate: bf16 [B, {N}] with B dividing {M} rows expected, got {gate.dtype} {tuple(gate.shape)}")
     if index < 0:
+        if out is not None and out.dim() == 2:
+            _check_apart("out", out)
         y = _values_torch(q if q is not None else quantize(x, w.fmt)) @ _values_torch(w).t()
         if w.gated:
             y = _swiglu_torch(y)
@@ -524,6 +536,7 @@ def linear(x, w: QuantRows, bias: torch.Tensor | None = None, act: str | None = 
             o2 = out if out.dim() == 2 else out.view(M, N)
         except RuntimeError:                      # rows of several batches that no single pitch reaches
             return out.copy_(linear(x.view(*lead, cols) if raw else x, w, bias, act, residual, gate, None, force_tile, force_split))
+        _check_apart("out", o2)
     ldo, yp = o2.stride(), o2.data_ptr()
     rp = bp = gp = lds = per = 0
     ldr = (0, 1)
@@ -591,6 +604,7 @@ def experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, up: Quant
         _check_operand("residual", residual, (T, D), index)
     if out is not None:
         _check_operand("out", out, (T, D), index)
+        _check_apart("out", out)
     if E > 1024:
         raise ValueError(f"at most 1024 experts, got {E}")
     if index < 0:
