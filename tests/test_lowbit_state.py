@@ -148,6 +148,22 @@ def test_every_pipeline_on_a_gpu(name, fmt, monkeypatch):
         o.close()
 
 
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_rows_and_weights_on_different_devices(fmt):
+    """Refused before a kernel is given an address of the other side."""
+    ones = torch.ones(256, dtype=BF)
+    here, there = layer(fmt, "cuda"), layer(fmt, "cpu")
+    x = rows()
+    for m, v in ((there, x.cuda()), (there, L.rms_norm_quantize(x.cuda(), ones.cuda(), fmt)), (here, x), (here, L.rms_norm_quantize(x, ones, fmt))):
+        with pytest.raises(ValueError, match=" on "):
+            m(v)
+    if fmt != "fp8":
+        here._buffers["fp4_bytes"].data = here._buffers["fp4_bytes"].data.cpu()
+        with pytest.raises(RuntimeError, match="not in memory"):
+            here(x.cuda())
+
+
 # ------------------------------------------------------------------ adapters
 def adapters(device, n_in=256, n_out=128):
     g = torch.Generator().manual_seed(3)

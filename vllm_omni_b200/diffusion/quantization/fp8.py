@@ -106,6 +106,8 @@ def fp8_linear(x, fp8_state, bias=None, act=None, residual=None, gate=None, out=
     ready = isinstance(x, QuantRows)
     if ready and (x.fmt != "fp8" or K != w8.shape[1]):
         raise ValueError(f"fp8 layer of {tuple(w8.shape)}: rows {x!r}")
+    if w8.device != x.device or sw.device != x.device:
+        raise ValueError(f"fp8 layer: weights on {w8.device}, rows on {x.device}")
     if not x.is_cuda:
         if ready:
             y = _epi(dequantize(x, torch.float32) @ _weight_values(w8, sw).t(), bias, act, residual, gate).to(torch.bfloat16)

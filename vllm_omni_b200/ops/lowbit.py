@@ -133,7 +133,7 @@ class QuantRows:
         p = self._buf.data_ptr()
         if p != self._seen[0] or not p:
             size, scales, row = _layout(self.fmt, self.rows, self.cols, self.experts or 1)
-            if self._buf.numel() != size or p & 15:
+            if self._buf.numel() != size or p & 15 or self._buf.get_device() != self.index:
                 raise RuntimeError(f"{self!r}: its weights are not in memory (asleep or offloaded), or not on 16 bytes")
             self._seen = (p, p + scales, p + row if self.fmt == "nvfp4" else 0)
         return self._seen
