@@ -139,6 +139,22 @@ def test_rows_of_a_result_must_not_overlap(device):
     same(L.rms_norm_quantize(x, gain, "nvfp4", residual=gain.expand(6, 64)), L.rms_norm_quantize(x, gain, "nvfp4", residual=gain.repeat(6, 1)))      # read only: may
 
 
+# ------------------------------------------------------------------ choice of experts
+@pytest.mark.parametrize("device", DEVICES)
+def test_route_of_views_and_its_refusals(device):
+    from vllm_omni_b200.ops.moe import route
+    z = rows_of(24, 40, device=device)                                     # [experts, tokens], and [tokens, experts] as a view of it
+    ids, w = route(z.t(), 4)
+    want, ww = route(z.t().contiguous(), 4)
+    assert torch.equal(ids, want) and torch.equal(w, ww) and ids.shape == (40, 4)
+    assert route(z[:0], 4)[0].shape == (0, 4)
+    with pytest.raises(ValueError, match="T, E"):
+        route(z[0], 4)
+    if device == "cuda":
+        with pytest.raises(ValueError, match="bf16"):
+            route(z.float(), 4)
+
+
 # ------------------------------------------------------------------ copies
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("fmt", tuple(L.FORMATS))

@@ -200,13 +200,20 @@ def _route(logits, T, E, k, renorm, ws):
 
 def route(logits, k: int, renorm: bool = True):
     """(ids int32, weights fp32) [T, k]: the ``k`` largest of bf16 logits [T, E] and their softmax probabilities, among themselves with ``renorm``."""
+    if logits.dim() != 2:
+        raise ValueError(f"route: logits [T, E] expected, got {list(logits.shape)}")
     T, E = logits.shape
     if not 1 <= k <= min(E, 16) or E > 256:
         raise ValueError(f"route: 1 to 16 of at most 256 experts, got {k} of {E}")
     if not logits.is_cuda:
         ids, w = moe_route_reference(logits, k, renorm)
         return ids, w
-    assert logits.dtype == torch.bfloat16 and logits.stride(1) == 1
+    if logits.dtype != torch.bfloat16:
+        raise ValueError(f"route: bf16 logits expected, got {logits.dtype}")
+    if torch._C._cuda_getDevice() != logits.get_device():            # kernels go to the current device's stream
+        with torch.cuda.device(logits.get_device()):
+            return route(logits, k, renorm)
+    logits = logits if logits.stride(1) == 1 else logits.contiguous()
     ids = torch.empty(T, k, dtype=torch.int32, device=logits.device)
     w = torch.empty(T, k, dtype=torch.float32, device=logits.device)
     nv.check_rc(nv.lib("moe").omni_moe_route(nv.ptr(logits), c_int(logits.stride(0)), c_int(T), c_int(E), c_int(k), c_int(1 if renorm else 0), nv.ptr(ids), nv.ptr(w),
