@@ -10,6 +10,7 @@ from torch import nn
 
 from vllm_omni_b200.diffusion.layers.linear import FusedLinear, weight_tensors
 from vllm_omni_b200.diffusion.quantization.fp8 import quantize_layer
+from vllm_omni_b200.models.qwen_decoder import DecoderConfig, QwenDecoderModel
 from vllm_omni_b200.ops import lowbit as L
 from test_lowbit_layers import decoder, prompt
 from test_model_zoo import GPU_CASES
@@ -99,6 +100,18 @@ def test_copied_decoder(fmt, experts, device):
     for _, t in weight_tensors(m):
         t.view(torch.uint8).zero_()
     assert torch.equal(other(batch)[0], want)
+
+
+@pytest.mark.parametrize("experts", [0, 4])
+def test_decoder_is_quantised_as_a_whole_or_not_at_all(experts):
+    """A width that no kernel takes is found before the first matrix is converted."""
+    wide = dict(moe_intermediate_size=32800) if experts else dict(intermediate_size=32800)
+    m = QwenDecoderModel(DecoderConfig(vocab_size=64, hidden_size=32, num_hidden_layers=1, num_attention_heads=1, num_key_value_heads=1, head_dim=32,
+                                       num_experts=experts, num_experts_per_tok=2, **wide), dtype=BF, device="cpu")
+    before = {n: t.clone() for n, t in weight_tensors(m)}
+    with pytest.raises(ValueError, match="intermediate_size \\(32800\\)"):
+        m.quantize("nvfp4")
+    assert m.quantization is None and all(torch.equal(t, before[n]) for n, t in weight_tensors(m))
 
 
 # ------------------------------------------------------------------ operands

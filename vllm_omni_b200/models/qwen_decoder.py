@@ -221,6 +221,9 @@ class QwenDecoderModel(nn.Module):
         bad = [f"{k} ({v})" for k, v in widths.items() if v % step]
         if bad:
             raise ValueError(f"quantization={fmt!r} needs widths that are multiples of {step}: {', '.join(bad)}")
+        wide = [f"{k} ({v})" for k, v in widths.items() if v > lowbit.MAX_COLS and (fmt != "fp8" or k == "hidden_size")]     # fp8: rows of the norms only
+        if wide:
+            raise ValueError(f"quantization={fmt!r} takes widths of at most {lowbit.MAX_COLS}: {', '.join(wide)}")
         n = 0
         for layer in self.layers:
             names = ["qkv_proj", "o_proj"] + (["gate_up", "down"] if not cfg.num_experts else
