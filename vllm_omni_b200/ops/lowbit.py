@@ -184,13 +184,6 @@ class QuantRows:
         """A gated weight's rows as those of an ordinary one."""
         return QuantRows.over(self.storage(), self.fmt, self.rows, self.cols, self.experts)
 
-    @property
-    def out_features(self) -> int:
-        return self.rows // 2 if self.gated else self.rows
-
-    def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.row_scale) if t is not None)
-
     def __repr__(self):
         return f"QuantRows({self.fmt}, {list(self.shape)}{', gated' if self.gated else ''}, {self.device})"
 
