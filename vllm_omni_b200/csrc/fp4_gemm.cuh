@@ -709,7 +709,7 @@ static int launch_any(Fp4Args& a, const Fp4Operands& o, int fmt, bool gated, int
 // CTAs, 10.6 on pairs; 1000 rows 13.6 and 12.0; gated 24576 x 4096, 200 rows 19.0 and 18.0, 8192 rows 478 and 322.
 // Few tiles: a split saves blocks of K (0.28 us each) and costs an exchange of 1.4 us and 14 ns per row, 0.6 more in fours.  4096 x 12288, 33 rows: 15.9 us
 // whole, 12.3 in two, 10.0 in four; 200 rows 16.8 whole, 14.3 in two; 4096 x 1024, 33 rows: 3.9, 5.1, 5.7.  (Clusters of 8 of these CTAs, one per SM, do
-// not all find room: 22 us.)
+// not all find room: 22 us.)  The limit counts one CTA per SM for tiles of 16 rows too, of which two run; what a split up to that would give was not measured.
 static int pick_tiles(Fp4Args& a, int force_tile, int force_split) {
   const int sms = sm_count(), kb = (a.K + 255) / 256;
   int tile = force_tile ? force_tile : a.M <= 16 ? 16 : a.M <= 64 ? 64 : 128;

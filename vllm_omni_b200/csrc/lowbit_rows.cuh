@@ -178,7 +178,8 @@ template <int FMT> struct ChunkPlace {
 };
 
 // NV chunks per thread, blockDim.x threads (a multiple of 32) per row, blockDim.y rows per block.  One pass over a row, which stays in registers.  8191 x 12288 to
-// mxfp4: 44 us (254 MB, 5.8 TB/s), integer pipe 71 % busy; with a residual, the norm, its sum and fp8, 12289 x 4096: 67 us (352 MB, 5.3 TB/s)
+// mxfp4: 44 us (254 MB, 5.8 TB/s), integer pipe 71 % busy; to nvfp4 61 (4.2 TB/s): a row's warps meet between its loads and its codes, for the row's factor.
+// With a residual, the norm, its sum and fp8, 12289 x 4096: 66 us (352 MB, 5.4 TB/s), mxfp4 61, nvfp4 68.  Without a residual 8192 x 4096 34.8, 31.5, 36.4.
 template <int FMT, bool NORM, int MODE, int NV, int MOST>
 __global__ void __launch_bounds__(MOST)
 lowbit_rows_kernel(const RowsArgs a) {
@@ -316,8 +317,9 @@ struct DequantArgs {
   int K, f32;
 };
 
-// Eight elements per thread, four rows on their way at a time; blockDim.x chunks by blockDim.y rows per block.  Stores bound it: 8191 x 12288 mxfp4 to bf16
-// 65 us, to fp32 104 (201 and 402 MB written at 3.1 and 3.9 TB/s, codes read beside them; a fill of the 201 MB takes 52).
+// Eight elements per thread, four rows on their way at a time; blockDim.x chunks by blockDim.y rows per block.  8191 x 12288 mxfp4 to bf16
+// 65 to 67 us, to fp32 104: 201 and 402 MB written at 3.0 and 3.9 TB/s, codes read beside them.  A fill of the 201 MB takes 52, a copy of them 63, so that stores
+// alone do not bound the bf16 form; its 16 bytes a thread are half of what the fp32 form stores.
 template <int FMT>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const DequantArgs a) {

@@ -62,7 +62,8 @@ def _parts(fmt: str, shape: tuple, gated: bool):
 class QuantRows:
     """Rows in a low-bit format, as the tensor cores read them: a batch's activations [R, K], a weight [N, K], or the weights of experts [E, N, K].
 
-    ``codes`` uint8 [.., R, K / 2] (fp8: [R, K]), element 2 i in the low half of byte i; ``scales`` as ``scale_shape`` says; ``row_scale`` fp32
+    ``codes`` uint8 [.., R, K / 2] (fp8: [R, K]), element 2 i in the low half of byte i; ``scales`` as ``scale_shape`` says, whose bytes for blocks past K
+    (a row's last word) have to be zero: they are multiplied too, by codes of zero, and a NaN there would be one in the row's results; ``row_scale`` fp32
     [.., R] for nvfp4.  ``gated``: the rows of a SwiGLU weight, 8 gate rows, their 8 lift rows, the next 8 gate rows and so on."""
 
     __slots__ = ("fmt", "gated", "rows", "cols", "experts", "index", "_codes", "_scales", "_row", "_buf", "_ptr", "_seen")
@@ -371,7 +372,8 @@ def pack_weight(w: torch.Tensor, fmt: str, gated: bool = False) -> QuantRows:
 
 
 def dequantize(q: QuantRows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values of ``q`` as bf16 or fp32 (4-bit formats quantised here: exactly in either)."""
+    """The values of ``q`` as bf16 or fp32 (4-bit formats quantised here: exactly in either, but for rows of less than 2^-110, whose smallest values are
+    below what bf16 has)."""
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"dequantize: bf16 or fp32, got {dtype}")
     if not q.is_cuda:
