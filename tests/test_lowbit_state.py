@@ -52,6 +52,9 @@ def test_weights_are_the_module_s_state(fmt, device):
     fresh = layer(fmt, device, seed=5)
     fresh.load_state_dict(m.state_dict())
     assert torch.equal(fresh(x), y)
+    fresh = layer(fmt, device, seed=5)
+    fresh.load_state_dict({n: t.clone() for n, t in m.state_dict().items()}, assign=True)
+    assert torch.equal(fresh(x), y)
     cast = copy.deepcopy(m).to(torch.float64).to(BF)                      # (the bias survives the way there and back)
     assert torch.equal(cast(x), y)
 
@@ -68,6 +71,21 @@ def test_layers_move_between_devices(fmt):
     assert ((on_cpu.float() - y.cpu().float()).abs() <= 0.05 * y.cpu().float().abs() + 0.05).all()        # the same weights, by the restatement
     m.to("cuda")
     assert torch.equal(m(x), y)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_states_are_the_same_on_either_side(fmt):
+    """A state saved on one side is loaded on the other byte by byte."""
+    m, x = layer(fmt, "cuda"), rows(device="cuda")
+    y = m(x)
+    host = layer(fmt, "cpu", seed=5)
+    host.load_state_dict({n: t.cpu() for n, t in m.state_dict().items()})
+    back = layer(fmt, "cuda", seed=6)
+    back.load_state_dict(host.state_dict())
+    assert torch.equal(back(x), y)
+    moved = copy.deepcopy(m).to("cpu")
+    assert torch.equal(host(x.cpu()), moved(x.cpu()))
 
 
 @gpu

@@ -26,34 +26,39 @@ class QuantizedState:
         setattr(self, name, q.over(getattr(self, name + "_bytes"), *q._like))
 
     def set_fp8(self, codes: torch.Tensor, scale: torch.Tensor) -> None:
-        """``self.fp8``: block-scaled e4m3 codes (uint8 on a GPU) and their fp32 scales."""
-        self.register_buffer("fp8_codes", codes)
+        """``self.fp8``: block-scaled e4m3 codes (bytes on a GPU) and their fp32 scales."""
+        self.register_buffer("fp8_codes", codes.view(torch.uint8))
         self.register_buffer("fp8_scale", scale)
-        self.fp8 = (self.fp8_codes, self.fp8_scale)
+        self._over_buffers()
 
     def quantized_buffers(self) -> list[str]:
         return [n for n in self._buffers if n in ("fp8_codes", "fp8_scale") or n.endswith("_bytes")]
 
+    def _over_buffers(self) -> None:
+        """The attributes anew, over what the buffers are now."""
+        for n in self.quantized_buffers():
+            if n.endswith("_bytes"):
+                q = getattr(self, n.removesuffix("_bytes"))
+                setattr(self, n.removesuffix("_bytes"), q.over(self._buffers[n], *q._like))
+            elif n == "fp8_codes":
+                c = self._buffers[n]
+                self.fp8 = (c if c.is_cuda else c.view(torch.float8_e4m3fn), self.fp8_scale)
+
     def _apply(self, fn, recurse=True):
-        names = self.quantized_buffers()
-        for n in names:                                # whole numbers, which a cast to another floating-point type leaves alone
-            if self._buffers[n].is_floating_point():
-                self._buffers[n] = self._buffers[n].view(torch.int32 if n == "fp8_scale" else torch.uint8)
+        fp32 = "fp8_scale" in self._buffers                # as whole numbers, which a cast to another floating-point type leaves alone
+        if fp32:
+            self._buffers["fp8_scale"] = self._buffers["fp8_scale"].view(torch.int32)
         try:
             super()._apply(fn, recurse)
         finally:
-            for n in names:
-                t = self._buffers[n]
-                if n == "fp8_scale":
-                    self._buffers[n] = t.view(torch.float32)
-                elif n == "fp8_codes":
-                    self._buffers[n] = t if t.is_cuda else t.view(torch.float8_e4m3fn)
-                else:
-                    q = getattr(self, n.removesuffix("_bytes"))
-                    setattr(self, n.removesuffix("_bytes"), q.over(t, *q._like))
-            if "fp8_codes" in names:
-                self.fp8 = (self.fp8_codes, self.fp8_scale)
+            if fp32:
+                self._buffers["fp8_scale"] = self._buffers["fp8_scale"].view(torch.float32)
+            self._over_buffers()
         return self
+
+    def _load_from_state_dict(self, *args, **kw):
+        super()._load_from_state_dict(*args, **kw)
+        self._over_buffers()                               # (assign=True puts other tensors in their place)
 
 
 def weight_tensors(module: nn.Module):

@@ -152,7 +152,7 @@ def quantize_layer(m, fmt: str, gated: bool = False) -> None:
         m.to_fp4(fmt, gated=gated)
         return
     w8, sw = quantize_weight_blockwise(m.weight.data)
-    m.set_fp8(w8.view(torch.uint8) if w8.is_cuda else w8, sw)
+    m.set_fp8(w8, sw)
     m.weight.data = torch.empty(0, dtype=m.weight.dtype, device=m.weight.device)
 
 
