@@ -391,21 +391,22 @@ __device__ __forceinline__ void block_scan2(int& a, int& b, int& total_a, int& t
 // expert -1.  The place of a pair among its expert's rows is what its atomic add to the expert's count returns (the order
 // inside an expert does not affect results).  One cluster of CL blocks: each counts its share of the pairs, reads the others' counts where they lie and
 // numbers its own; bound by the chain of loads and
-// atomic adds of a thread.  place_of_pair (may be null): where a pair's row stands if every tile began at a multiple of `pitch` rows.
+// atomic adds of a thread.  PLACES, a form of its own (in one for both, plans without them took 0.1 of 2.3 to 5 us longer): place_of_pair, where a pair's row
+// stands if every tile began at a multiple of `pitch` rows.
 constexpr int PLAN_CLUSTER = 8;
 __device__ __forceinline__ int ld_cluster_i32(uint32_t addr) {
   int v;
   asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-template <int CL>
+template <int CL, bool PLACES>
 __global__ void __launch_bounds__(1024)
 moe_plan_tiles_kernel(const int* ids, int n_pairs, int E, int e_lo, int e_hi, int tile_cap, int max_tiles,
                         int* __restrict__ row_of_pair, int* __restrict__ tile_expert, int* __restrict__ tile_row0,
                         int* __restrict__ tile_rows, int* __restrict__ n_rows_out, int* __restrict__ place_of_pair, int pitch, MoeBounds bd) {
   __shared__ int cnt[1024];
   __shared__ int off[1024];
-  __shared__ int row0[1024], tile0[1024], tile_size[1024];         // of an expert: its first row, its first tile, rows of a tile
+  __shared__ int row0[PLACES ? 1024 : 1], tile0[PLACES ? 1024 : 1], tile_size[PLACES ? 1024 : 1];     // of an expert: its first row, its first tile, rows of a tile
   const int rank = CL > 1 ? (int)cluster_ctarank() : 0, first = rank * 1024 + threadIdx.x;
   cnt[threadIdx.x] = 0;
   __syncthreads();
@@ -433,7 +434,7 @@ moe_plan_tiles_kernel(const int* ids, int n_pairs, int E, int e_lo, int e_hi, in
   int row = mine, tile = own, rows, tiles;
   block_scan2(row, tile, rows, tiles);
   off[e] = row + before;
-  row0[e] = row; tile0[e] = tile; tile_size[e] = size;
+  if constexpr (PLACES) { row0[e] = row; tile0[e] = tile; tile_size[e] = size; }
   if (rank == 0) {
     if (e == 0) *n_rows_out = rows;
     for (int i = 0; i < own; ++i) {                     // never empty: (own - 1) * size < mine, as tile_cap is 16 (size then too) or a multiple of 64
@@ -454,7 +455,7 @@ moe_plan_tiles_kernel(const int* ids, int n_pairs, int E, int e_lo, int e_hi, in
     if (r >= 0) {
       const int x = ids[i], at = off[x] + r;
       row_of_pair[i] = at;
-      if (place_of_pair) {
+      if constexpr (PLACES) {
         const int j = at - row0[x], n = tile_size[x];
         place_of_pair[i] = (tile0[x] + j / n) * pitch + j % n;
       }
@@ -823,11 +824,12 @@ static int plan_tiles(const int* ids, int n_pairs, int E, int e_lo, int e_hi, in
   if (E > 1024 || (!(tile_cap == 16 && place_of_pair) && tile_cap != 64 && tile_cap != 128 && tile_cap != 256)) return RC_BAD_ARG;
   // 128 experts, one block against eight: 512 pairs 2.6 and 4.4 us (the cluster's barriers), 8000 4.8 and 4.9, 19704 9.3 and 6.1, 64000 29 and 7.9
   if (n_pairs > 8192)
-    launch_with(true, PLAN_CLUSTER, moe_plan_tiles_kernel<PLAN_CLUSTER>, PLAN_CLUSTER, 1024, 0, (cudaStream_t)stream, ids, n_pairs, E, e_lo, e_hi, tile_cap, max_tiles,
-                row_of_pair, tile_expert, tile_row0, tile_rows, n_rows_out, place_of_pair, pitch, g_moe_bounds);
+    launch_with(true, PLAN_CLUSTER, place_of_pair ? moe_plan_tiles_kernel<PLAN_CLUSTER, true> : moe_plan_tiles_kernel<PLAN_CLUSTER, false>, PLAN_CLUSTER, 1024, 0,
+                (cudaStream_t)stream, ids, n_pairs, E, e_lo, e_hi, tile_cap, max_tiles, row_of_pair, tile_expert, tile_row0, tile_rows, n_rows_out, place_of_pair, pitch,
+                g_moe_bounds);
   else
-    launch_overlapped(moe_plan_tiles_kernel<1>, 1, 1024, 0, (cudaStream_t)stream, ids, n_pairs, E, e_lo, e_hi, tile_cap, max_tiles, row_of_pair,
-                      tile_expert, tile_row0, tile_rows, n_rows_out, place_of_pair, pitch, g_moe_bounds);
+    launch_overlapped(place_of_pair ? moe_plan_tiles_kernel<1, true> : moe_plan_tiles_kernel<1, false>, 1, 1024, 0, (cudaStream_t)stream, ids, n_pairs, E, e_lo, e_hi,
+                      tile_cap, max_tiles, row_of_pair, tile_expert, tile_row0, tile_rows, n_rows_out, place_of_pair, pitch, g_moe_bounds);
   return (int)cudaGetLastError();
 }
 extern "C" int omni_moe_plan_tiles(const int* ids, int n_pairs, int E, int e_lo, int e_hi, int tile_cap, int max_tiles, int* row_of_pair,
