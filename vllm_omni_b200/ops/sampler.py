@@ -1,8 +1,10 @@
 """K16 — batched token sampling on the device (csrc/sampler.cu) with a PyTorch restatement
-for CPU runs.  ``sample`` takes one ``RowParams`` per sequence."""
+for CPU runs.  ``sample`` takes one ``RowParams`` per sequence.  ``sample_given`` (csrc/sample_given.cu) takes parameters and random numbers that are on the
+device, and cuts exactly: ties go to the lowest id, and neither threads nor blocks decide the order of a sum."""
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass, field
 
 import torch
@@ -184,3 +186,93 @@ def sample(logits: torch.Tensor, rows: list[RowParams]):
                                        nv.ptr(out), nv.ptr(lp), nv.stream_ptr())
     nv.check_rc(rc, "omni_sample")
     return out, lp
+
+
+MAX_VOCAB = 262144                    # csrc/sample_given.cu: a row stays in the shared memory of eight blocks
+
+
+@functools.lru_cache(maxsize=None)
+def _given_lib():
+    P, I, L, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
+    lib = nv.lib("sample_given")
+    lib._cdll.omni_sample_given.argtypes = [P, I, L, I, I, P, P, F, P, I, P, F, P, F, P, P, P]
+    return lib
+
+
+def _per_row(name, v, B, dtype, device):
+    """(address, value) of a parameter that is one number or a tensor of one per row."""
+    if not isinstance(v, torch.Tensor):
+        return None, v
+    if v.dtype is not dtype or v.shape != (B,) or not v.is_contiguous() or v.device != device:
+        raise ValueError(f"{name}: a number or contiguous {dtype} [{B}] on {device} expected, got {v.dtype} {tuple(v.shape)} on {v.device}")
+    return v.data_ptr(), 0
+
+
+def sample_given(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+    """One token per row of ``logits`` [B, V] (bf16 or fp32) from the random numbers ``u`` (fp32 [B], in [0, 1)): (ids int32 [B], log probabilities fp32 [B]),
+    into ``out``, such a pair, if given.  ``temperature``, ``top_p``, ``min_p`` (fp32 [B]) and ``top_k`` (int32 [B]) are numbers or one value per row.
+
+    Weights are exp((x - max) / temperature) as multiples of 2^-44.  In the order by logit (ties: the lower id first) the first ``top_k`` stay (0: all), of these the
+    ones of at least ``min_p`` of the largest, of these all before which less than ``top_p`` of their mass lies, and always the first.  The token is the first kept
+    id at which the running mass in the order of the ids passes ``u`` times the kept mass.  Its log probability is that of the whole row at the temperature.
+    Temperature 0 or below: the largest logit, its log probability at temperature 1.  Logits that are not numbers count as -inf; a row of nothing else
+    gives id -1 and log probability -inf.  Does no host work and, with ``out``, no allocation: it can be captured."""
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
+        raise ValueError(f"logits: bf16 or fp32 [rows, vocabulary] with a row's values side by side expected, got {logits.dtype} {tuple(logits.shape)}")
+    B, V = logits.shape
+    if not 1 <= V <= MAX_VOCAB:
+        raise ValueError(f"vocabulary of {V}: 1 to {MAX_VOCAB}")
+    dev = logits.device
+    if u.dtype is not torch.float32 or u.shape != (B,) or not u.is_contiguous() or u.device != dev:
+        raise ValueError(f"u: contiguous fp32 [{B}] on {dev} expected, got {u.dtype} {tuple(u.shape)} on {u.device}")
+    params = [_per_row("temperature", temperature, B, torch.float32, dev), _per_row("top_k", top_k, B, torch.int32, dev),
+              _per_row("top_p", top_p, B, torch.float32, dev), _per_row("min_p", min_p, B, torch.float32, dev)]
+    if out is None:
+        ids, logprob = torch.empty(B, dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.float32, device=dev)
+    else:
+        ids, logprob = out
+        if any(t.dtype is not d or t.shape != (B,) or not t.is_contiguous() or t.device != dev for t, d in ((ids, torch.int32), (logprob, torch.float32))):
+            raise ValueError(f"out: contiguous int32 [{B}] and fp32 [{B}] on {dev} expected")
+    if not logits.is_cuda:
+        for r in range(B):
+            pick = [float(v[r] if isinstance(v, torch.Tensor) else v) for v in (temperature, top_k, top_p, min_p)]
+            ids[r], logprob[r] = _given_row(logits[r].double(), float(u[r]), *pick)
+        return ids, logprob
+    if torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return sample_given(logits, u, temperature, top_k, top_p, min_p, (ids, logprob))
+    (t, tv), (k, kv), (p, pv), (m, mv) = params
+    nv.check_rc(_given_lib().omni_sample_given(logits.data_ptr(), logits.dtype is torch.bfloat16, logits.stride(0), V, B, u.data_ptr(), t, tv, k, kv, p, pv, m, mv,
+                                               ids.data_ptr(), logprob.data_ptr(), nv.stream_ptr()), "omni_sample_given")
+    return ids, logprob
+
+
+def _given_row(x, u, temperature, top_k, top_p, min_p):
+    """The definition for one row in 64 bits."""
+    x = torch.where(x.isnan(), -float("inf"), x)
+    top = x.max()
+    if top == -float("inf"):
+        return -1, -float("inf")
+    greedy = not temperature > 0
+    z = torch.where(x == top, 0.0, (x - top) / (1.0 if greedy else temperature))
+    z = torch.where(z.isnan(), -float("inf"), z)
+    e = torch.exp(z)
+    w = torch.round(e * 2.0 ** 44).long()
+    log_all = torch.log(w.sum().double() * 2.0 ** -44)
+    if greedy:
+        i = int((x == top).nonzero()[0])
+        return i, float(-log_all)
+    order = torch.sort(x, descending=True, stable=True).indices
+    if 0 < top_k < x.numel():
+        order = order[:int(top_k)]
+    order = order[e[order] >= min(min_p, 1.0)]
+    mass = torch.cumsum(w[order], 0)
+    if top_p < 1:
+        fits = (mass - w[order]).double() < top_p * mass[-1].double()
+        order = order[:max(1, int(fits.sum()))]
+    kept = torch.sort(order).values
+    mass = torch.cumsum(w[kept], 0)
+    i = int((mass.double() <= max(u, 0.0) * mass[-1].double()).sum())
+    if i == kept.numel():                                 # u = 1: the last one with mass
+        i = int((w[kept] > 0).nonzero()[-1])
+    return int(kept[i]), float(z[kept[i]] - log_all)
