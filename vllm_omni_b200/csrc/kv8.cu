@@ -238,27 +238,37 @@ kv8_read_kernel(const __grid_constant__ Kv8Read p) {
 
 // ------------------------------------------------------------------------------------------------------------------------------------ attention
 // One row of queries reads every key and value of its sequence once: a stream from HBM at half the bytes of bf16, so the arithmetic on the way has half the
-// time.  Nothing is staged: codes go from their pages into the registers of the warp that uses them, become f16 there (exact: e4m3 has three bits of mantissa)
-// and are operands of 16 x 8 x 16 products.
+// time, 23 bytes a clock and SM.  A warp that loads for itself spends it on addresses and on waiting (64 sequences of 2500 to 4096 keys, 8 KV heads of 128: 33 instructions a
+// key and head, 152 us).  Here one warp of a block fetches pages by TMA, all heads of eight to 32 rows by one copy into [head][row][channel], swizzled so that nothing below
+// meets a bank twice, through a ring of three or six stages; the others take 32 keys of one head a stage each.  Codes become f16 in registers (exact: e4m3 has three bits
+// of mantissa) and are operands of 16 x 8 x 16 products.
 //   S[row, key]    = q K^T        the heads of a group are the rows (for several rows of queries of a sequence: their heads behind one another), keys the
-//                                 columns; lane group j of a quad owns channels 16 j .. 16 j + 15 of every 64 for both operands
-//   O^T[ch, row]  += V^T P^T      lane (g, j) loads channels g D / 8 .. of keys 2 j, 2 j + 1, 2 j + 8, 2 j + 9 and pairs neighbouring keys by byte permutes;
+//                                 columns; lane group j of a quad owns channels D / 4 j .. of both operands
+//   O^T[ch, row]  += V^T P^T      lane (g, j) holds channels g D / 8 .. of keys 2 j, 2 j + 1, 2 j + 8, 2 j + 9 and pairs neighbouring keys by byte permutes;
 //                                 P^T needs no exchange, because the accumulator of S is laid out as this operand
 // q is divided by a power of two per row, so that f16 holds it.  A page's key scale multiplies its scores.  Its value scale goes into the weights of the second
-// product, w = 2^(s + e_v - m'), whose running maximum m' is apart from the softmax's m: w is at most 2^14 whatever the scales, and the mass that f16
+// product, w = 2^(s + e_v - m'), whose running maximum m' is apart from the softmax's m: w is at most 2^15 whatever the scales, and the mass that f16
 // cannot hold is below 2^-38 of the largest for each key.  The sum of weights is that of the unrounded fp32 ones.
-constexpr int K8_WARPS = 4, K8_KEYS = 32, K8_MAX_PARTS = 256;
-constexpr float K8_LIFT = 14.f;
+// Blocks are persistent, one an SM: a share (a run of keys of a row and of up to eight heads) follows another in the ring without a pause.
+constexpr int K8_MAX_PARTS = 256, K8_MAX_GROUP = 128, K8_LISTED = 512;
+constexpr float K8_LIFT = 14.f, K8_SLACK = 1.f;     // together below f16's 2^16
+// Warps that compute, and the keys of a stage that each of them takes.  (Sixteen warps of 16 keys: 96 registers, which spill, and more instructions a key.)
+// Sixteen rows of 128 channels leave registers for 16 keys at a time, and half as large stages.
+constexpr int K8_WARPS = 8;
+constexpr int k8_keys(int D, bool up) { return D == 128 && up ? 16 : 32; }
 
 struct Kv8Attn {
+  CUtensorMap mk, mv;                              // codes: {channels, slots, heads}, boxes {D, unit, heads_block}
   const __nv_bfloat16* q;
   long q_rs, q_hs;
-  const unsigned char *k, *v;
   const float *ks, *vs;
   const int *block_tables, *lens, *row_seq;        // row_seq null: row r is sequence r
   long bt_stride;
-  int page, pages, max_keys, R, S, H, Hkv, chunks; // chunks of at most 16 heads of a group
-  int pack, splits, subs;                          // rows per block; shares of the keys: blocks, and warps of a block
+  int page, shift, pages, max_keys, R, S, H, Hkv;  // shift: log2 of the page's size, -1 if it has none
+  int chunks, heads, groups;                       // chunks of at most 16 heads of a group; KV heads of a block, blocks of them
+  int pack, unit, subs;                            // rows per block; rows of a copy; warps that share a head's keys
+  int share, splits, row_blocks;                   // keys of a share, shares of a row at most; blocks of rows
+  bool listed;                                     // blocks take the shares there are; else a number stands for every share there may be
   float scale_log2;
   float *part_o, *part_lse;
   __nv_bfloat16* out;
@@ -266,277 +276,547 @@ struct Kv8Attn {
   int* status;
 };
 
-__device__ __forceinline__ uint4 ld_codes16(const unsigned char* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ld_codes8(const unsigned char* p) {
-  uint2 v;
-  asm volatile("ld.global.L1::no_allocate.L2::256B.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
 __device__ __forceinline__ void mma_f16_16x8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// Shared memory by its address, as loads that the compiler may move between barriers.
+__device__ __forceinline__ uint4 shared4(uint32_t addr) { return *reinterpret_cast<const uint4*>(__cvta_shared_to_generic(addr)); }
+__device__ __forceinline__ uint2 shared2(uint32_t addr) { return *reinterpret_cast<const uint2*>(__cvta_shared_to_generic(addr)); }
+
+// What a share is, for the warp that fetches and for those that compute alike: rows r .. rn - 1 of one sequence, its keys from `from` to `to`.
+struct Kv8Pass {
+  int seq, rn, most, from, to;
+};
+__device__ __forceinline__ Kv8Pass kv8_pass(const Kv8Attn& p, int r, int r1, int split) {
+  Kv8Pass a;
+  a.seq = r;
+  a.rn = r + 1;
+  if (p.row_seq) {
+    a.seq = p.row_seq[r];
+    while (a.rn < r1 && p.row_seq[a.rn] == a.seq) ++a.rn;
+  }
+  a.most = 0;
+  for (int i = r; i < a.rn; ++i) a.most = max(a.most, p.lens[i]);
+  a.most = min(a.most, p.max_keys);
+  if (a.seq < 0 || a.seq >= p.S) {
+    if (a.most > 0) atomicCAS(p.status, 0, ERR_BOUNDS);
+    a.most = 0;
+  }
+  a.from = min(a.most, split * p.share);
+  a.to = min(a.most, a.from + p.share);
+  return a;
+}
+// Shares that a block of rows has: one at least.
+__device__ __forceinline__ int kv8_count(const int* lens, int rb, int pack, int R, int max_keys, int share) {
+  int most = 0;
+  for (int i = rb * pack; i < min(R, (rb + 1) * pack); ++i) most = max(most, lens[i]);
+  return max(1, (min(most, max_keys) + share - 1) / share);
+}
+// The shares there are, one after another: `before` [row_blocks + 1] counts those of the blocks of rows before one.  Without it as many of every
+// block, the first ones of all first; those behind a block's end are empty.
+struct Kv8Item {
+  int rb, group, split;
+};
+__device__ __forceinline__ Kv8Item kv8_item(const Kv8Attn& p, const int* before, int item) {
+  const int k = item / p.groups, group = item - k * p.groups;
+  if (!p.listed) {
+    const int split = k / p.row_blocks;
+    return {k - split * p.row_blocks, group, split};
+  }
+  int lo = 0, hi = p.row_blocks;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (before[mid] <= k) lo = mid; else hi = mid;
+  }
+  return {lo, group, k - before[lo]};
+}
+__device__ __forceinline__ int kv8_column(const Kv8Attn& p, int key) { return p.shift >= 0 ? key >> p.shift : key / p.page; }
+__device__ __forceinline__ int kv8_page(const Kv8Attn& p, int pg) {
+  if (pg >= 0 && pg < p.pages) return pg;
+  atomicCAS(p.status, 0, ERR_BOUNDS);
+  return 0;
+}
 
 // UP: more than 8 rows of the products are live.
 template <int D, bool UP>
-__global__ void __launch_bounds__(32 * K8_WARPS, UP ? 2 : 3)
+__global__ void __launch_bounds__(32 * (K8_WARPS + 1), 1)
 kv8_attn_kernel(const __grid_constant__ Kv8Attn p) {
-  pdl_begin();
-  constexpr int NH = UP ? 2 : 1, CH = D / 64, MT = D / 16;
+  extern __shared__ __align__(1024) unsigned char ring[];
+  __shared__ __align__(8) unsigned long long bars[12];
+  __shared__ int s_abort, before[K8_LISTED + 1];
+  __shared__ float sums[K8_WARPS][UP ? 16 : 8];
+  constexpr int NH = UP ? 2 : 1, CH = D / 64, MT = D / 16, CW = K8_WARPS, KEYS = D == 128 && UP ? 16 : 32, NE = KEYS / 8, STAGES = 96 / KEYS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
-  const int VH = p.Hkv * p.chunks, per_block = min(K8_WARPS, VH), sub = warp / per_block;
-  const int vh = blockIdx.z * K8_WARPS + warp % per_block;
-  if (sub >= p.subs || vh >= VH) return;
-  const int G = p.H / p.Hkv, hk = vh / p.chunks, hc = (vh - hk * p.chunks) * 16, Gc = min(16, G - hc), h0 = hk * G + hc;
-  const int parts = p.splits * p.subs, part = blockIdx.y * p.subs + sub;
-  const long row = (long)p.Hkv * D;
-  const int r0 = blockIdx.x * p.pack, r1 = min(p.R, r0 + p.pack);
+  const int VH = p.heads * p.chunks, keys = p.subs * KEYS, half = keys * p.heads * D;     // of a stage; bytes of its K
+  const uint32_t base = smem_u32(ring), full = smem_u32(bars), empty = full + 8 * STAGES;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, VH * p.subs);
+    }
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_begin();
+  int items = p.row_blocks * p.splits;
+  if (p.listed) {
+    for (int rb = threadIdx.x; rb < p.row_blocks; rb += blockDim.x) before[rb + 1] = kv8_count(p.lens, rb, p.pack, p.R, p.max_keys, p.share);
+    if (threadIdx.x == 0) before[0] = 0;
+    __syncthreads();
+    if (warp == 0) {
+      int run = 0;
+      for (int i0 = 0; i0 < p.row_blocks; i0 += 32) {
+        int n = i0 + lane < p.row_blocks ? before[i0 + lane + 1] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const int up = __shfl_up_sync(0xffffffffu, n, o);
+          if (lane >= o) n += up;
+        }
+        if (i0 + lane < p.row_blocks) before[i0 + lane + 1] = run + n;
+        run += __shfl_sync(0xffffffffu, n, 31);
+      }
+    }
+    __syncthreads();
+    items = before[p.row_blocks];
+  }
+  items *= p.groups;
+  int c = 0;                                       // stages so far
 
-  for (int r = r0, rn; r < r1; r = rn) {           // rows r .. rn - 1 are of one sequence
-    int seq = r;
-    rn = r + 1;
-    if (p.row_seq) {
-      seq = p.row_seq[r];
-      while (rn < r1 && p.row_seq[rn] == seq) ++rn;
+  if (warp == CW) {
+    // the pages of a share, a unit a lane
+    const int units = keys / p.unit, unit_bytes = p.unit * p.heads * D;
+    const bool plain = p.pack == 1 && !p.row_seq;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+      const Kv8Item w = kv8_item(p, before, item);
+      const int rb = w.rb, group = w.group, split = w.split, r1 = min(p.R, (rb + 1) * p.pack);
+      for (int r = rb * p.pack; r < r1;) {
+        // the first pages are asked for along with the length
+        const int guess = plain && lane < units ? p.block_tables[(long)r * p.bt_stride + kv8_column(p, min(split * p.share + lane * p.unit, p.max_keys - 1))] : 0;
+        const Kv8Pass a = kv8_pass(p, r, r1, split);
+        r = a.rn;
+        const int* bt = p.block_tables + (long)a.seq * p.bt_stride;
+        auto slot_of = [&](int key) {
+          const int col = kv8_column(p, key);
+          return kv8_page(p, bt[col]) * p.page + (key - col * p.page);
+        };
+        int key = a.from + lane * p.unit, slot = 0;
+        if (lane < units && key < a.to) slot = plain ? kv8_page(p, guess) * p.page + (key - kv8_column(p, key) * p.page) : slot_of(key);
+        for (int k0 = a.from; k0 < a.to; k0 += keys, ++c) {
+          const int s = c % STAGES;
+          if (!mbar_wait(empty + 8 * s, ((c / STAGES) & 1) ^ 1, &s_abort, p.status, ERR_WAIT_EMPTY)) break;
+          const int n = min(units, (a.to - k0 + p.unit - 1) / p.unit);
+          if (lane == 0) mbar_expect_tx(full + 8 * s, 2 * n * unit_bytes);
+          __syncwarp();
+          if (lane < n) {
+            const uint32_t at = base + s * 2 * half + lane * unit_bytes;
+            tma_load_3d(at, &p.mk, full + 8 * s, 0, slot, group * p.heads);
+            tma_load_3d(at + half, &p.mv, full + 8 * s, 0, slot, group * p.heads);
+          }
+          key += keys;
+          if (lane < units && key < a.to) slot = slot_of(key);
+        }
+      }
     }
-    // head and row of this lane's rows g and g + 8 of the products
-    int len[NH], head[NH], qrow[NH], most = 0;
-    for (int i = r; i < rn; ++i) most = max(most, p.lens[i]);
-    most = min(most, p.max_keys);
-    if (seq < 0 || seq >= p.S) {
-      if (most > 0) atomicCAS(p.status, 0, ERR_BOUNDS);
-      most = 0;
+    if (*(volatile int*)&s_abort) {                // copies in flight end before the block does
+      for (int i = 0; i < STAGES; ++i) {
+        const unsigned long long t0 = globaltimer_ns();
+        const int last = c - 1 - i;
+        if (last < 0) break;
+        while (!mbar_try_wait(full + 8 * (last % STAGES), (last / STAGES) & 1) && globaltimer_ns() - t0 < WAIT_LIMIT_NS) {}
+      }
     }
+    return;
+  }
+
+  const int vh = warp % VH, sub = warp / VH;
+  if (sub >= p.subs) return;
+  const int G = p.H / p.Hkv, head_in = vh / p.chunks, hc = (vh - head_in * p.chunks) * 16, Gc = min(16, G - hc);
+  // where a lane's pieces of eight rows are, from the first of them: K rows g, V rows 2 j and 2 j + 1
+  uint32_t k_at[CH], v_at[2];
+#pragma unroll
+  for (int x = 0; x < CH; ++x) k_at[x] = D == 128 ? g * 128 + (((2 * j + x) ^ g) << 4) : g * 64 + ((j ^ ((g >> 1) & 3)) << 4);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = 2 * j + i;
+    v_at[i] = D == 128 ? row * 128 + ((g ^ row) << 4) : row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8;
+  }
+  uint32_t eight[NE];                              // this warp's eights of a stage
+#pragma unroll
+  for (int n = 0; n < NE; ++n) {
+    const int k = sub * KEYS + n * 8, u = k / p.unit;
+    eight[n] = (uint32_t)((u * p.heads + head_in) * p.unit + (k - u * p.unit)) * D;
+  }
+
+  // While the stages of a share go by, the next one's length and first pages, then its scales are fetched, and its queries before its sums are written, where a row is its
+  // own sequence (`plain`): what follows from them does not stop the ring.
+  const bool plain = p.pack == 1 && !p.row_seq;
+  const uint32_t my_q = base + STAGES * 2 * CW * KEYS * D + warp * (NH * CH * 1024) + lane * 16;      // this warp's q: words of a lane in fours
+  if ((int)blockIdx.x >= items) return;
+  Kv8Item at = kv8_item(p, before, blockIdx.x), next = at;
+  int next_len = 0, next_page = 0;
+  float next_ks = 1.f, next_vs = 1.f;
+  uint4 raw[NH][CH][2];
+  auto first_key = [&](int split) { return split * p.share + lane / NE * keys + sub * KEYS + lane % NE * 8; };
+  auto fetch_pages = [&] {
+    next_len = p.lens[next.rb];
+    next_page = p.block_tables[(long)next.rb * p.bt_stride + kv8_column(p, min(first_key(next.split), p.max_keys - 1))];
+  };
+  auto fetch_scales = [&] {
+    const int key = first_key(next.split), hn = next.group * p.heads + head_in;
+    const int pg = key < min(next_len, p.max_keys) && key < (next.split + 1) * p.share ? kv8_page(p, next_page) : 0;
+    if (hn < p.Hkv) {
+      next_ks = p.ks[(long)pg * p.Hkv + hn];
+      next_vs = p.vs[(long)pg * p.Hkv + hn];
+    }
+  };
+  // rows g and g + 8 of the products: their heads behind one another, row by row
+  auto fetch_queries = [&](int r, int rn, int h0, bool real) {
 #pragma unroll
     for (int u = 0; u < NH; ++u) {
       const int m = u * 8 + g, i = m / Gc;
-      qrow[u] = r + i < rn ? r + i : -1;
-      head[u] = h0 + m - i * Gc;
-      len[u] = qrow[u] >= 0 && most > 0 ? min(max(p.lens[qrow[u]], 0), most) : 0;
+#pragma unroll
+      for (int x = 0; x < CH; ++x)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          raw[u][x][k] = real && r + i < rn ? *reinterpret_cast<const uint4*>(p.q + (r + i) * p.q_rs + (h0 + m - i * Gc) * p.q_hs + j * (D / 4) + x * 16 + k * 8)
+                                            : make_uint4(0u, 0u, 0u, 0u);
     }
-    const int tiles = (most + K8_KEYS - 1) / K8_KEYS, per = (tiles + p.splits - 1) / p.splits;
-    const int t1 = min(tiles, (int)(blockIdx.y + 1) * per);
-    int t = blockIdx.y * per + sub;
-    const int* bt = p.block_tables + (long)seq * p.bt_stride;
-
-    uint32_t q[NH][CH][4][2];
-    float back[NH];                                // what q was divided by, times the scale
-#pragma unroll
-    for (int u = 0; u < NH; ++u) {
-      uint4 raw[CH][2];
-      uint32_t top = 0;
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          raw[c][i] = make_uint4(0u, 0u, 0u, 0u);
-          if (qrow[u] >= 0) raw[c][i] = *reinterpret_cast<const uint4*>(p.q + qrow[u] * p.q_rs + head[u] * p.q_hs + c * 64 + j * 16 + i * 8);
-          const uint32_t w[4] = {raw[c][i].x, raw[c][i].y, raw[c][i].z, raw[c][i].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) top = max(top, max((w[k] << 16) & 0x7fffffffu, w[k] & 0x7fff0000u));
-        }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = min(max((int)(top >> 23) - 127, -126), 126);
-      const float f = pow2f(-e);
-      back[u] = pow2f(e) * p.scale_log2;
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t w[4] = {raw[c][i].x, raw[c][i].y, raw[c][i].z, raw[c][i].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 x = unpack_bf16(w[k]);
-            q[u][c][i * 2 + (k >> 1)][k & 1] = pack_half(x.x * f, x.y * f);
-          }
-        }
-    }
-    float m[NH], mv[NH], l[NH], acc[NH][MT][4];
-#pragma unroll
-    for (int u = 0; u < NH; ++u) {
-      m[u] = mv[u] = -INFINITY;
-      l[u] = 0.f;
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[u][i][e] = 0.f;
-    }
-
-    // Lane n of a quad looks up the n-th eight keys of a tile: first row in the pool, exponents of the scales.  Eight keys past the end repeat the tile's first.
-    auto look = [&](int t, int& at, float& fk, float& ev) {
-      const int k0 = t * K8_KEYS + 8 * j < most ? t * K8_KEYS + 8 * j : t * K8_KEYS;
-      const int col = k0 / p.page;
-      int pg = bt[col];
-      if (pg < 0 || pg >= p.pages) {
-        atomicCAS(p.status, 0, ERR_BOUNDS);
-        pg = 0;
+  };
+  if (plain) {
+    fetch_pages();
+    if (!UP) fetch_queries(at.rb, at.rb + 1, (at.group * p.heads + head_in) * G + hc, at.group * p.heads + head_in < p.Hkv);
+    fetch_scales();
+  }
+  for (int item = blockIdx.x; item < items; item += gridDim.x, at = next) {
+    const int split = at.split, hk = at.group * p.heads + head_in, h0 = hk * G + hc, r1 = min(p.R, (at.rb + 1) * p.pack);
+    const bool real = hk < p.Hkv;                  // the last block's heads may be fewer
+    const bool more = item + (int)gridDim.x < items, fetch = plain && more;
+    if (more) next = kv8_item(p, before, item + gridDim.x);
+    for (int r = at.rb * p.pack; r < r1;) {
+      Kv8Pass a;
+      if (plain) {
+        a = {r, r + 1, min(max(next_len, 0), p.max_keys), 0, 0};
+        a.from = min(a.most, split * p.share);
+        a.to = min(a.most, a.from + p.share);
+      } else {
+        a = kv8_pass(p, r, r1, split);
       }
-      at = pg * p.page + (k0 - col * p.page);
-      fk = pow2f(scale_exp(p.ks[(long)pg * p.Hkv + hk]));
-      ev = (float)scale_exp(p.vs[(long)pg * p.Hkv + hk]);
-    };
-    // rows past the end repeat the last key: valid memory, its weight is zero
-    auto row_in = [&](int t, int n, int i) {
-      const int k0 = t * K8_KEYS + (t * K8_KEYS + 8 * n < most ? 8 * n : 0);
-      return min(i, most - 1 - k0);
-    };
-    uint4 kr[4][CH];
-    uint4 vr[8];                                   // D = 64: x and y
-    auto load_k = [&](int t, int at) {
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const unsigned char* k = p.k + (long)(__shfl_sync(0xffffffffu, at, n, 4) + row_in(t, n, g)) * row + hk * D + j * 16;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) kr[n][c] = ld_codes16(k + c * 64);
-      }
-    };
-    auto load_v = [&](int t, int at) {
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const int a = __shfl_sync(0xffffffffu, at, n, 4);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const unsigned char* v = p.v + (long)(a + row_in(t, n, 2 * j + i)) * row + hk * D + g * (D / 8);
-          if (D == 128) {
-            vr[2 * n + i] = ld_codes16(v);
-          } else {
-            const uint2 x = ld_codes8(v);
-            vr[2 * n + i].x = x.x;
-            vr[2 * n + i].y = x.y;
-          }
-        }
-      }
-    };
-    int at = 0, next_at = 0;
-    float fk = 1.f, ev = 0.f, next_fk = 1.f, next_ev = 0.f;
-    if (t < t1) {
-      look(t, at, fk, ev);
-      load_k(t, at);
-      load_v(t, at);
-      if (t + p.subs < t1) look(t + p.subs, next_at, next_fk, next_ev);
-    }
-#pragma unroll 1
-    for (; t < t1; t += p.subs) {
-      const int next = t + p.subs;
-      float s[4][4] = {};
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const uint32_t w[4] = {kr[n][c].x, kr[n][c].y, kr[n][c].z, kr[n][c].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_f16_16x8(s[n], q[0][c][k][0], UP ? q[NH - 1][c][k][0] : 0u, q[0][c][k][1], UP ? q[NH - 1][c][k][1] : 0u, halves_of(w[k]), halves_of_hi(w[k]));
-        }
-      if (next < t1) load_k(next, next_at);
-      uint32_t pw[NH][4];
+      if (UP || !plain) fetch_queries(r, a.rn, h0, real);
+      // head and row of this lane's rows g and g + 8 of the products
+      int len[NH], head[NH], qrow[NH], least = a.most;
 #pragma unroll
       for (int u = 0; u < NH; ++u) {
-        float mx = -INFINITY, mxv = -INFINITY, evn[4];
+        const int m = u * 8 + g, i = m / Gc;
+        qrow[u] = real && r + i < a.rn ? r + i : -1;
+        head[u] = h0 + m - i * Gc;
+        len[u] = qrow[u] < 0 ? 0 : (plain ? a.most : (a.most > 0 ? min(max(p.lens[qrow[u]], 0), a.most) : 0));
+        if (qrow[u] >= 0) least = min(least, len[u]);
+      }
+      least = __reduce_min_sync(0xffffffffu, least);
+      r = a.rn;
+      // Scales of eight stages at a time: lane 4 i + n has those of the n-th eight of stage i (past the end: of the last one).
+      const int* bt = p.block_tables + (long)a.seq * p.bt_stride;
+      auto page_of = [&](int batch) {
+        const int key = min(a.from + (batch * (32 / NE) + lane / NE) * keys + sub * KEYS + lane % NE * 8, (a.to - 1) & ~7);
+        return bt[kv8_column(p, key)];
+      };
+      float ks = next_ks, vs = next_vs;
+      int ahead = 0;
+      if (a.from < a.to && real) {
+        if (!plain) {
+          const int pg = kv8_page(p, page_of(0));
+          ks = p.ks[(long)pg * p.Hkv + hk];
+          vs = p.vs[(long)pg * p.Hkv + hk];
+        }
+        if (a.to - a.from > 32 / NE * keys) ahead = page_of(1);
+      }
+      float back[NH];                              // what q was divided by, times the scale
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float f = __shfl_sync(0xffffffffu, fk, n, 4) * back[u];
-          evn[n] = __shfl_sync(0xffffffffu, ev, n, 4);
+      for (int u = 0; u < NH; ++u) {
+        uint32_t top = 0;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float y = t * K8_KEYS + n * 8 + 2 * j + e < len[u] ? s[n][2 * u + e] * f : -INFINITY;
-            s[n][2 * u + e] = y;
-            mx = fmaxf(mx, y);
-            mxv = fmaxf(mxv, y + evn[n]);
+        for (int x = 0; x < CH; ++x)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t w[4] = {raw[u][x][i].x, raw[u][x][i].y, raw[u][x][i].z, raw[u][x][i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = max(top, max((w[k] << 16) & 0x7fffffffu, w[k] & 0x7fff0000u));
+          }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max((int)(top >> 23) - 127, -126), 126);
+        const float f = pow2f(-e);
+        back[u] = pow2f(e) * p.scale_log2;
+#pragma unroll
+        for (int x = 0; x < CH; ++x)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t w[4] = {raw[u][x][i].x, raw[u][x][i].y, raw[u][x][i].z, raw[u][x][i].w};
+            uint32_t packed[4];                    // two steps of the product, their two words each
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 v = unpack_bf16(w[k]);
+              packed[k] = pack_half(v.x * f, v.y * f);
+            }
+            st_shared_v4(my_q + ((u * CH + x) * 2 + i) * 512, make_uint4(packed[0], packed[1], packed[2], packed[3]));
+          }
+      }
+      float m[NH], mv[NH], l[NH], acc[NH][MT][4];
+#pragma unroll
+      for (int u = 0; u < NH; ++u) {
+        m[u] = mv[u] = -INFINITY;
+        l[u] = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[u][i][e] = 0.f;
+      }
+
+      __syncwarp();
+      float fks = 1.f, evs = 0.f, ks2 = 1.f, vs2 = 1.f;
+      int i_stage = 0;
+#pragma unroll 1
+      for (int k0 = a.from; k0 < a.to; k0 += keys, ++c, ++i_stage) {
+        if (i_stage % (32 / NE) == 0 && i_stage) {
+          ks = ks2;
+          vs = vs2;
+        }
+        if (i_stage % (32 / NE) == 2 && real && k0 + (32 / NE - 2) * keys < a.to) {
+          const int pg = kv8_page(p, ahead);
+          ks2 = p.ks[(long)pg * p.Hkv + hk];
+          vs2 = p.vs[(long)pg * p.Hkv + hk];
+          ahead = page_of(i_stage / (32 / NE) + 2);
+        }
+        if (fetch && i_stage == 1) fetch_pages();
+        if (fetch && i_stage == 5) fetch_scales();
+        if (i_stage % (32 / NE) == 0) {
+          fks = pow2f(scale_exp(ks));
+          evs = (float)scale_exp(vs);
+        }
+        const int s = c % STAGES, key = k0 + sub * KEYS;
+        if (!mbar_wait(full + 8 * s, (c / STAGES) & 1, &s_abort, p.status, ERR_WAIT_FULL)) break;      // and on to the barriers below, which others wait at
+        if (key < a.to && real) {
+          const uint32_t at = base + s * 2 * half;
+          float sc[NE][4] = {};
+#pragma unroll
+          for (int x = 0; x < CH; ++x) {
+            uint4 kr[NE];
+#pragma unroll
+            for (int n = 0; n < NE; ++n) kr[n] = shared4(at + eight[n] + k_at[x]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint4 lo = shared4(my_q + (x * 2 + i) * 512), hi = UP ? shared4(my_q + (((NH - 1) * CH + x) * 2 + i) * 512) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+              for (int n = 0; n < NE; ++n) {
+                mma_f16_16x8(sc[n], lo.x, hi.x, lo.y, hi.y, halves_of(i ? kr[n].z : kr[n].x), halves_of_hi(i ? kr[n].z : kr[n].x));
+                mma_f16_16x8(sc[n], lo.z, hi.z, lo.w, hi.w, halves_of(i ? kr[n].w : kr[n].y), halves_of_hi(i ? kr[n].w : kr[n].y));
+              }
+            }
+          }
+          const bool ends = key + KEYS > least; // keys that some row does not see
+          uint32_t pw[NH][NE];
+          const int from_lane = i_stage % (32 / NE) * NE;
+          float fk[NE], ev[NE];
+#pragma unroll
+          for (int n = 0; n < NE; ++n) {
+            fk[n] = __shfl_sync(0xffffffffu, fks, from_lane + n);
+            ev[n] = __shfl_sync(0xffffffffu, evs, from_lane + n);
+          }
+#pragma unroll
+          for (int u = 0; u < NH; ++u) {
+            float y[NE][2], mx = -INFINITY, mxv = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NE; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) y[n][e] = sc[n][2 * u + e] * (fk[n] * back[u]);
+            if (ends)
+#pragma unroll
+              for (int n = 0; n < NE; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (key + n * 8 + 2 * j + e >= len[u]) y[n][e] = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NE; ++n) {
+              const float m0 = fmaxf(y[n][0], y[n][1]);
+              mx = fmaxf(mx, m0);
+              mxv = fmaxf(mxv, m0 + ev[n]);
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, 2));
+            // The maxima are those of some tile before, as long as none since is more than 2^K8_SLACK larger: sums are seldom scaled.
+            if (__any_sync(0xffffffffu, mx > m[u] + K8_SLACK || mxv > mv[u] + K8_SLACK)) {
+              const float was = m[u], was_v = mv[u];
+              m[u] = fmaxf(was, mx);
+              mv[u] = fmaxf(was_v, mxv);
+              l[u] *= ex2_approx(was - (m[u] == -INFINITY ? 0.f : m[u]));          // only scores of -inf so far: all weights are zero
+              const float beta = ex2_approx(was_v - (mv[u] == -INFINITY ? 0.f : mv[u]));
+              const float b0 = __shfl_sync(0xffffffffu, beta, 8 * j), b1 = __shfl_sync(0xffffffffu, beta, 8 * j + 4);   // rows 2 j, 2 j + 1
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                acc[u][i][0] *= b0; acc[u][i][1] *= b1;
+                acc[u][i][2] *= b0; acc[u][i][3] *= b1;
+              }
+            }
+            const float top = m[u] == -INFINITY ? 0.f : m[u], lift = K8_LIFT - (mv[u] == -INFINITY ? 0.f : mv[u]);
+#pragma unroll
+            for (int n = 0; n < NE; ++n) {
+              l[u] += ex2_approx(y[n][0] - top) + ex2_approx(y[n][1] - top);
+              pw[u][n] = pack_half(ex2_approx(y[n][0] + (ev[n] + lift)), ex2_approx(y[n][1] + (ev[n] + lift)));
+            }
+          }
+          // channel pair (2 i, 2 i + 1) of a lane's D / 8: rows g and g + 8 of tile i
+#pragma unroll
+          for (int h = 0; h < NE / 2; ++h) {       // sixteen keys at a time
+            uint4 vr[4];                           // D = 64: x and y
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t from = at + half + eight[2 * h + (i >> 1)] + v_at[i & 1];
+              if (D == 128) {
+                vr[i] = shared4(from);
+              } else {
+                const uint2 x = shared2(from);
+                vr[i].x = x.x;
+                vr[i].y = x.y;
+              }
+            }
+            if (ends)                              // values behind the end are nobody's: what they hold may not be a number
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (key + h * 16 + (i >> 1) * 8 + 2 * j + (i & 1) >= a.to) vr[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int w = 0; w < MT / 2; ++w) {
+              auto word = [&](const uint4& x) { return w == 0 ? x.x : (w == 1 ? x.y : (w == 2 ? x.z : x.w)); };
+              const uint32_t v0 = word(vr[0]), v1 = word(vr[1]), v2 = word(vr[2]), v3 = word(vr[3]);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {        // channels 4 w + 2 i, + 1
+                const uint32_t x = __byte_perm(v0, v1, i ? 0x7362 : 0x5140), y = __byte_perm(v2, v3, i ? 0x7362 : 0x5140);
+                const uint32_t a0 = halves_of(x), a1 = halves_of_hi(x), a2 = halves_of(y), a3 = halves_of_hi(y);
+#pragma unroll
+                for (int u = 0; u < NH; ++u) mma_f16_16x8(acc[u][2 * w + i], a0, a1, a2, a3, pw[u][2 * h], pw[u][2 * h + 1]);
+              }
+            }
           }
         }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, 2));
-        const float was = m[u], was_v = mv[u];
-        m[u] = fmaxf(was, mx);
-        mv[u] = fmaxf(was_v, mxv);
-        const float top = m[u] == -INFINITY ? 0.f : m[u], top_v = mv[u] == -INFINITY ? 0.f : mv[u];      // only scores of -inf so far: all weights are zero
-        l[u] *= ex2_approx(was - top);
-        const float beta = ex2_approx(was_v - top_v);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float y0 = s[n][2 * u], y1 = s[n][2 * u + 1], lift = evn[n] - top_v + K8_LIFT;
-          l[u] += ex2_approx(y0 - top) + ex2_approx(y1 - top);
-          pw[u][n] = pack_half(ex2_approx(y0 + lift), ex2_approx(y1 + lift));
-        }
-        const float b0 = __shfl_sync(0xffffffffu, beta, 8 * j), b1 = __shfl_sync(0xffffffffu, beta, 8 * j + 4);   // rows 2 j, 2 j + 1
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          acc[u][i][0] *= b0; acc[u][i][1] *= b1;
-          acc[u][i][2] *= b0; acc[u][i][3] *= b1;
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + 8 * s);
       }
-      // channel pair (2 i, 2 i + 1) of a lane's D / 8: rows g and g + 8 of tile i
+
+      if (fetch) {
+        if (i_stage < 2) fetch_pages();
+        const int hn = next.group * p.heads + head_in;
+        if (!UP) fetch_queries(next.rb, next.rb + 1, hn * G + hc, hn < p.Hkv);        // sixteen rows have no registers for it
+        if (i_stage < 6) fetch_scales();
+      }
+      float lse[NH];
+      bool none[NH];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)                  // keys 0 .. 15 and 16 .. 31
+      for (int u = 0; u < NH; ++u) {
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+        // O / l = acc 2^-14 / l 2^(m' - m), the two factors apart because their product may be too small for a float; a row without keys: zeros
+        none[u] = l[u] == 0.f;
+        lse[u] = none[u] ? -INFINITY : m[u] + log2f(l[u]);
+        const float inv = none[u] ? 0.f : 0x1p-14f / l[u], level = none[u] ? 0.f : ex2_approx(mv[u] - m[u]);
 #pragma unroll
-        for (int w = 0; w < MT / 2; ++w) {
-          auto word = [&](const uint4& x) { return w == 0 ? x.x : (w == 1 ? x.y : (w == 2 ? x.z : x.w)); };
-          const uint32_t a = word(vr[4 * h]), b = word(vr[4 * h + 1]), c = word(vr[4 * h + 2]), d = word(vr[4 * h + 3]);
+        for (int hh = 0; hh < 2; ++hh) {           // rows 2 j, 2 j + 1 of the products
+          const int src = 8 * j + 4 * hh;
+          const float f = __shfl_sync(0xffffffffu, inv, src), f2 = __shfl_sync(0xffffffffu, level, src);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {            // channels 4 w + 2 i, + 1
-            const uint32_t x = __byte_perm(a, b, i ? 0x7362 : 0x5140), y = __byte_perm(c, d, i ? 0x7362 : 0x5140);
-            const uint32_t a0 = halves_of(x), a1 = halves_of_hi(x), a2 = halves_of(y), a3 = halves_of_hi(y);
-#pragma unroll
-            for (int u = 0; u < NH; ++u) mma_f16_16x8(acc[u][2 * w + i], a0, a1, a2, a3, pw[u][2 * h], pw[u][2 * h + 1]);
+          for (int i = 0; i < MT; ++i) {
+            acc[u][i][hh] = acc[u][i][hh] * f * f2;
+            acc[u][i][2 + hh] = acc[u][i][2 + hh] * f * f2;
           }
         }
-      if (next < t1) {
-        load_v(next, next_at);
-        fk = next_fk;
-        ev = next_ev;
-        if (next + p.subs < t1) look(next + p.subs, next_at, next_fk, next_ev);
       }
-    }
+      // The sums of the warps of a head become one, two by two, through the memory of the giver's queries, which it needs no longer, in halves of its channels.  A lane
+      // of either warp holds the same rows and channels.
+      for (int step = 1; step < p.subs; step *= 2) {
+        const int role = sub & (2 * step - 1);     // 0 takes, `step` gives
+        float w0[NH][2], w1[NH][2];
 #pragma unroll
-    for (int u = 0; u < NH; ++u) {
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-      // O / l = acc 2^-14 / l 2^(m' - m), the two factors apart because their product may be too small for a float; a row without keys: zeros
-      const bool none = l[u] == 0.f;
-      const float inv = none ? 0.f : 0x1p-14f / l[u], level = none ? 0.f : ex2_approx(mv[u] - m[u]);
-      if (parts > 1 && j == 0 && qrow[u] >= 0) p.part_lse[((long)qrow[u] * p.H + head[u]) * parts + part] = none ? -INFINITY : m[u] + log2f(l[u]);
+        for (int side = 0; side < 2; ++side) {
+          if (role == step) {
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {             // rows 2 j, 2 j + 1 of the products
-        const int src = 8 * j + 4 * hh;
-        const float f = __shfl_sync(0xffffffffu, inv, src), f2 = __shfl_sync(0xffffffffu, level, src);
-        const int qr = __shfl_sync(0xffffffffu, qrow[u], src), hd = __shfl_sync(0xffffffffu, head[u], src);
-        const bool no = __shfl_sync(0xffffffffu, none, src);
-        if (qr < 0 || (parts > 1 && no)) continue;
+            for (int u = 0; u < NH; ++u) {
+              if (side == 0 && j == 0) sums[warp][u * 8 + g] = lse[u];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          acc[u][i][hh] *= f;
-          acc[u][i][hh] *= f2;
-          acc[u][i][2 + hh] *= f;
-          acc[u][i][2 + hh] *= f2;
+              for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int i = 0; i < MT / 2; i += 2) {
+                  const int f = side * (MT / 2) + i;
+                  st_shared_v4(my_q + ((u * 2 + hh) * (MT / 4) + i / 2) * 512,
+                               make_uint4(__float_as_uint(acc[u][f][hh]), __float_as_uint(acc[u][f][2 + hh]), __float_as_uint(acc[u][f + 1][hh]), __float_as_uint(acc[u][f + 1][2 + hh])));
+                }
+            }
+          }
+          asm volatile("bar.sync %0, %1;" ::"r"(1 + vh), "r"(32 * p.subs) : "memory");
+          if (role == 0) {
+            const uint32_t from = my_q + step * VH * (NH * CH * 1024);
+#pragma unroll
+            for (int u = 0; u < NH; ++u) {
+              if (side == 0) {
+                const float other = sums[warp + step * VH][u * 8 + g], top = fmaxf(lse[u], other), at = top == -INFINITY ? 0.f : top;
+                const float a0 = ex2_approx(lse[u] - at), a1 = ex2_approx(other - at), den = a0 + a1, inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                  w0[u][hh] = __shfl_sync(0xffffffffu, a0 * inv, 8 * j + 4 * hh);
+                  w1[u][hh] = __shfl_sync(0xffffffffu, a1 * inv, 8 * j + 4 * hh);
+                }
+                none[u] = den == 0.f;
+                lse[u] = none[u] ? -INFINITY : at + log2f(den);
+              }
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int i = 0; i < MT / 2; i += 2) {
+                  const int f = side * (MT / 2) + i;
+                  const uint4 x = shared4(from + ((u * 2 + hh) * (MT / 4) + i / 2) * 512);
+                  acc[u][f][hh] = acc[u][f][hh] * w0[u][hh] + __uint_as_float(x.x) * w1[u][hh];
+                  acc[u][f][2 + hh] = acc[u][f][2 + hh] * w0[u][hh] + __uint_as_float(x.y) * w1[u][hh];
+                  acc[u][f + 1][hh] = acc[u][f + 1][hh] * w0[u][hh] + __uint_as_float(x.z) * w1[u][hh];
+                  acc[u][f + 1][2 + hh] = acc[u][f + 1][2 + hh] * w0[u][hh] + __uint_as_float(x.w) * w1[u][hh];
+                }
+            }
+          }
+          asm volatile("bar.sync %0, %1;" ::"r"(1 + vh), "r"(32 * p.subs) : "memory");
         }
-        // a lane's channels are g D / 8 + 2 i + (0, 1), i < MT
-        if (parts > 1) {
-          float* o = p.part_o + (((long)qr * p.H + hd) * parts + part) * D + g * (D / 8);
+      }
+      if (sub) continue;
+      const int parts = p.splits, part = split;
 #pragma unroll
-          for (int i = 0; i < MT; i += 2)
-            *reinterpret_cast<float4*>(o + 2 * i) = make_float4(acc[u][i][hh], acc[u][i][2 + hh], acc[u][i + 1][hh], acc[u][i + 1][2 + hh]);
-        } else {
-          __nv_bfloat16* o = p.out + qr * p.o_rs + hd * p.o_hs + g * (D / 8);
+      for (int u = 0; u < NH; ++u) {
+        if (parts > 1 && j == 0 && qrow[u] >= 0) p.part_lse[((long)qrow[u] * p.H + head[u]) * parts + part] = lse[u];
 #pragma unroll
-          for (int i = 0; i < MT; i += 4) {
-            uint4 w;
-            w.x = pack_bf16(acc[u][i][hh], acc[u][i][2 + hh]);
-            w.y = pack_bf16(acc[u][i + 1][hh], acc[u][i + 1][2 + hh]);
-            w.z = pack_bf16(acc[u][i + 2][hh], acc[u][i + 2][2 + hh]);
-            w.w = pack_bf16(acc[u][i + 3][hh], acc[u][i + 3][2 + hh]);
-            *reinterpret_cast<uint4*>(o + 2 * i) = w;
+        for (int hh = 0; hh < 2; ++hh) {
+          const int src = 8 * j + 4 * hh;
+          const int qr = __shfl_sync(0xffffffffu, qrow[u], src), hd = __shfl_sync(0xffffffffu, head[u], src);
+          const bool no = __shfl_sync(0xffffffffu, none[u], src);
+          if (qr < 0 || (parts > 1 && no)) continue;
+          // a lane's channels are g D / 8 + 2 i + (0, 1), i < MT
+          if (parts > 1) {
+            float* o = p.part_o + (((long)qr * p.H + hd) * parts + part) * D + g * (D / 8);
+#pragma unroll
+            for (int i = 0; i < MT; i += 2)
+              *reinterpret_cast<float4*>(o + 2 * i) = make_float4(acc[u][i][hh], acc[u][i][2 + hh], acc[u][i + 1][hh], acc[u][i + 1][2 + hh]);
+          } else {
+            __nv_bfloat16* o = p.out + qr * p.o_rs + hd * p.o_hs + g * (D / 8);
+#pragma unroll
+            for (int i = 0; i < MT; i += 4) {
+              uint4 w;
+              w.x = pack_bf16(acc[u][i][hh], acc[u][i][2 + hh]);
+              w.y = pack_bf16(acc[u][i + 1][hh], acc[u][i + 1][2 + hh]);
+              w.z = pack_bf16(acc[u][i + 2][hh], acc[u][i + 2][2 + hh]);
+              w.w = pack_bf16(acc[u][i + 3][hh], acc[u][i + 3][2 + hh]);
+              *reinterpret_cast<uint4*>(o + 2 * i) = w;
+            }
           }
         }
       }
@@ -544,77 +824,166 @@ kv8_attn_kernel(const __grid_constant__ Kv8Attn p) {
   }
 }
 
-// out[row, head] = sum_s 2^(lse_s - top) o_s / sum_s 2^(lse_s - top) over the shares (at most 256): a block per (row, head), its warps take every fourth share.
+// out[row, head] = sum_s 2^(lse_s - top) o_s / sum_s 2^(lse_s - top) over the shares (at most 256): a block per (row, head), its sixteen warps take every sixteenth share.
 template <int D>
-__global__ void __launch_bounds__(128)
-kv8_merge_kernel(const float* part_o, const float* part_lse, int parts, int H, __nv_bfloat16* out, long o_rs, long o_hs) {
+__global__ void __launch_bounds__(512)
+kv8_merge_kernel(const float* part_o, const float* part_lse, const int* lens, int pack, int R, int max_keys, int share, int splits, int H, __nv_bfloat16* out, long o_rs, long o_hs) {
   pdl_begin();
-  constexpr int PER = D / 32;
-  __shared__ float weight[K8_MAX_PARTS], sums[4][D], red[4];
+  constexpr int PER = D / 32, WARPS = 16;
+  __shared__ float sums[WARPS][D];
   const long r = blockIdx.x;
+  const int parts = kv8_count(lens, (int)(r / H) / pack, pack, R, max_keys, share);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float* lse = part_lse + r * parts;
-  const float a = threadIdx.x < parts ? lse[threadIdx.x] : -INFINITY, b = threadIdx.x + 128 < parts ? lse[threadIdx.x + 128] : -INFINITY;
-  float top = fmaxf(a, b);
+  // every warp: the weights of all shares
+  float w[K8_MAX_PARTS / 32], top = -INFINITY, den = 0.f;
+#pragma unroll
+  for (int i = 0; i < K8_MAX_PARTS / 32; ++i) {
+    w[i] = lane + i * 32 < parts ? part_lse[r * splits + lane + i * 32] : -INFINITY;
+    top = fmaxf(top, w[i]);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) red[warp] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  __syncthreads();
-  const float wa = a == -INFINITY ? 0.f : ex2_approx(a - top), wb = b == -INFINITY ? 0.f : ex2_approx(b - top);
-  weight[threadIdx.x] = wa;
-  weight[threadIdx.x + 128] = wb;
-  float den = wa + wb;
+#pragma unroll
+  for (int i = 0; i < K8_MAX_PARTS / 32; ++i) {
+    w[i] = w[i] == -INFINITY ? 0.f : ex2_approx(w[i] - top);
+    den += w[i];
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
-  if (lane == 0) red[warp] = den;
-  __syncthreads();
-  den = (red[0] + red[1]) + (red[2] + red[3]);
-  const float* po = part_o + r * parts * D + lane * PER;
   float acc[PER] = {};
-#pragma unroll 4
-  for (int s = warp; s < parts; s += 4) {
-    const float w = weight[s];
-    if (w == 0.f) continue;                        // a share without keys has written no sum
-    float x[PER];
-    if (PER == 4) {
-      const float4 y = *reinterpret_cast<const float4*>(po + (long)s * D);
-      x[0] = y.x; x[1] = y.y; x[PER - 2] = y.z; x[PER - 1] = y.w;
-    } else {
-      const float2 y = *reinterpret_cast<const float2*>(po + (long)s * D);
-      x[0] = y.x; x[1] = y.y;
-    }
+  const float* po = part_o + r * splits * D + lane * PER;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = fmaf(x[i], w, acc[i]);
+  for (int i = 0; i < K8_MAX_PARTS / 32; ++i) {
+    if (i * 32 >= parts) break;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int s = i * 32 + h * WARPS + warp;
+      const float ws = __shfl_sync(0xffffffffu, w[i], h * WARPS + warp);
+      if (ws != 0.f) {                             // a share without keys has written no sum
+        float x[PER];
+        if (PER == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(po + (long)s * D);
+          x[0] = y.x; x[1] = y.y; x[PER - 2] = y.z; x[PER - 1] = y.w;
+        } else {
+          const float2 y = *reinterpret_cast<const float2*>(po + (long)s * D);
+          x[0] = y.x; x[1] = y.y;
+        }
+#pragma unroll
+        for (int k = 0; k < PER; ++k) acc[k] = fmaf(x[k], ws, acc[k]);
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) sums[warp][lane * PER + i] = acc[i];
   __syncthreads();
   const float f = den != 0.f ? 1.0f / den : 0.f;   // not a number stays one
   const long row = r / H, head = r - row * H;
-  for (int c = threadIdx.x * 2; c < D; c += 256) {
-    const float x = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]), y = (sums[0][c + 1] + sums[1][c + 1]) + (sums[2][c + 1] + sums[3][c + 1]);
+  for (int c = threadIdx.x * 2; c < D; c += 1024) {
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      x += sums[i][c];
+      y += sums[i][c + 1];
+    }
     *reinterpret_cast<uint32_t*>(out + row * o_rs + head * o_hs + c) = pack_bf16(x * f, y * f);
   }
 }
 
-// Shares of a row's keys: about 24 warps per SM in all, two rounds of the twelve that fit it, at least two tiles of 32 keys each.  The number depends on the
-// rows, the heads and the tables' width, never on lengths: a row's result is the same whatever its neighbours hold.
-static void kv8_shares(int blocks_of_rows, int VH, int max_keys, int& splits, int& subs) {
-  subs = VH < K8_WARPS ? K8_WARPS / VH : 1;
-  const long warps = (long)blocks_of_rows * VH, target = 24L * sm_count();
-  const int tiles = (max_keys + K8_KEYS - 1) / K8_KEYS;
-  long parts = (target + warps - 1) / warps;
-  if (parts > tiles / 2) parts = tiles / 2;
-  if (parts > K8_MAX_PARTS) parts = K8_MAX_PARTS;
-  if (parts < 1) parts = 1;
-  if (subs > parts) subs = (int)parts;
-  splits = (int)(parts + subs - 1) / subs;
-  if (splits * subs > K8_MAX_PARTS) splits = K8_MAX_PARTS / subs;
+// The same for many rows of up to 32 shares, a warp per (row, head): 256 rows of 32 heads and three shares 102 us in all in place of 140; 256 heads of 22 shares 23 in place of 17.
+template <int D>
+__global__ void __launch_bounds__(128)
+kv8_merge_few_kernel(const float* part_o, const float* part_lse, const int* lens, int pack, int R, int max_keys, int share, int splits, int H, __nv_bfloat16* out, long o_rs, long o_hs) {
+  pdl_begin();
+  constexpr int PER = D / 32;
+  const long r = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (r >= (long)R * H) return;
+  const long row = r / H, head = r - row * H;
+  const int parts = kv8_count(lens, (int)row / pack, pack, R, max_keys, share);
+  float w = lane < parts ? part_lse[r * splits + lane] : -INFINITY, top = w;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  w = w == -INFINITY ? 0.f : ex2_approx(w - top);
+  float den = w, acc[PER] = {};
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+  const float* po = part_o + r * splits * D + lane * PER;
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float ws = __shfl_sync(0xffffffffu, w, s);
+    if (ws != 0.f) {                               // a share without keys has written no sum
+      float x[PER];
+      if (PER == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(po + (long)s * D);
+        x[0] = y.x; x[1] = y.y; x[PER - 2] = y.z; x[PER - 1] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(po + (long)s * D);
+        x[0] = y.x; x[1] = y.y;
+      }
+#pragma unroll
+      for (int k = 0; k < PER; ++k) acc[k] = fmaf(x[k], ws, acc[k]);
+    }
+  }
+  const float f = den != 0.f ? 1.0f / den : 0.f;   // not a number stays one
+  uint32_t* o = reinterpret_cast<uint32_t*>(out + row * o_rs + head * o_hs + lane * PER);
+#pragma unroll
+  for (int k = 0; k < PER / 2; ++k) o[k] = pack_bf16(acc[2 * k] * f, acc[2 * k + 1] * f);
 }
-// Rows that share a block: as many as fill the products' sixteen rows, where rows share sequences at all.
-static int kv8_pack(int R, int S, int G, bool mapped) { return mapped && R > S && G <= 8 ? 16 / G : 1; }
+
+// How a call is dealt out.  Rows that share a block: as many as fill the products' sixteen rows, where rows share sequences at all.  A row's keys are cut into shares of the same
+// number of keys, so that about as many shares as SMs, or a small multiple, follow from the rows, the heads and the tables' width, never from lengths: a row's result is the same
+// whatever its neighbours hold.
+struct Kv8Deal {
+  int pack, chunks, heads, groups, subs, unit, share, splits, grid;
+  bool up;
+};
+static bool kv8_deal(int R, int S, int H, int Hkv, int D, bool mapped, int page, int max_keys, Kv8Deal& d) {
+  const int G = H / Hkv;
+  if (G > K8_MAX_GROUP) return false;
+  d.pack = mapped && R > S && G <= 8 ? 16 / G : 1;
+  d.chunks = (G + 15) / 16;
+  d.up = (d.chunks > 1 ? 16 : G) * d.pack > 8;
+  const int warps = K8_WARPS, most = warps / d.chunks;
+  d.groups = (Hkv + most - 1) / most;
+  d.heads = (Hkv + d.groups - 1) / d.groups;
+  d.subs = 1;
+  while (d.subs * 2 * d.heads * d.chunks <= warps) d.subs *= 2;
+  const int keys = d.subs * k8_keys(D, d.up);      // at most 256: 32 copies of eight rows
+  d.unit = page % 32 == 0 && keys % 32 == 0 ? 32 : (page % 16 == 0 ? 16 : 8);
+  const long blocks = (long)((R + d.pack - 1) / d.pack) * d.groups;
+  const int sms = sm_count();
+  // The number of shares.  Few rows: rounds of blocks times a share's keys and what it costs beside them (its queries and the way of its sums, some 64 keys' time).
+  // Many: blocks take the shares there are in turn; a row is taken to have four fifths of the table's keys.
+  double best = 1e30;
+  d.splits = 1;
+  const int stages = (max_keys + keys - 1) / keys;
+  for (int n = 1; n <= K8_MAX_PARTS && n <= stages; ++n) {
+    const int share = (stages + n - 1) / n * keys;
+    if ((max_keys + share - 1) / share != n) continue;
+    const double items = R > d.pack ? blocks * (0.8 * max_keys / share + 0.5) : (double)blocks * n, rounds = (double)((long)(items / sms) + 1);
+    const double cost = (items == (rounds - 1.0) * sms ? rounds - 1.0 : rounds) * (share + 64) + 0.25 * n;
+    if (cost < best) {
+      best = cost;
+      d.splits = n;
+      d.share = share;
+    }
+  }
+  if (d.splits == 1) d.share = stages * keys;
+  if (blocks * d.splits > 0x7fffffffL) return false;
+  d.grid = blocks * d.splits < sms ? (int)(blocks * d.splits) : sms;
+  return true;
+}
+
+// Codes as {channels, slots, heads}, boxes of `unit` slots and `heads` heads
+static int kv8_tmap(CUtensorMap* out, const void* ptr, long slots, int Hkv, int D, int unit, int heads) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) return RC_NO_DRIVER;
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)slots, (cuuint64_t)Hkv}, strides[2] = {(cuuint64_t)Hkv * D, (cuuint64_t)D};
+  const cuuint32_t box[3] = {(cuuint32_t)D, (cuuint32_t)unit, (cuuint32_t)heads}, each[3] = {1, 1, 1};
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? RC_OK : RC_TMAP;
+}
 
 }  // namespace omni
 
@@ -665,13 +1034,20 @@ extern "C" int omni_kv8_read(const void* kc, const void* vc, const float* ks, co
   return RC_OK;
 }
 
-// Shares per (row, head) that omni_kv8_attn will write: sizes its scratch (fp32, shares x D and shares x 1).
-extern "C" int omni_kv8_attn_shares(int R, int S, int H, int Hkv, int mapped, int max_keys) {
-  if (R < 1 || Hkv < 1 || H < Hkv) return 1;
-  const int G = H / Hkv, pack = kv8_pack(R, S, G, mapped != 0);
-  int splits, subs;
-  kv8_shares((R + pack - 1) / pack, Hkv * ((G + 15) / 16), max_keys, splits, subs);
-  return splits * subs;
+// Shares per (row, head) that omni_kv8_attn will write: sizes its scratch (fp32, shares x D and shares x 1); -1: sizes that it does not take.
+extern "C" int omni_kv8_attn_shares(int R, int S, int H, int Hkv, int D, int mapped, int page, int max_keys) {
+  Kv8Deal d;
+  if (R < 1 || Hkv < 1 || H < Hkv || page < 8 || max_keys < 1 || !kv8_deal(R, S, H, Hkv, D, mapped != 0, page, max_keys, d)) return -1;
+  return d.splits;
+}
+
+template <int D, bool UP>
+static int launch_kv8_attn(const Kv8Attn& p, int grid, cudaStream_t st) {
+  static unsigned long long ready = 0;
+  constexpr int warps = K8_WARPS, ring = 96 * 2 * warps * D, q = warps * (UP ? 2 : 1) * D * 16;       // a stage; queries
+  if (int e = ensure_dynamic_smem((const void*)kv8_attn_kernel<D, UP>, ring + q, ready)) return e;
+  launch_overlapped(kv8_attn_kernel<D, UP>, grid, 32 * (warps + 1), ring + q, st, p);
+  return (int)cudaGetLastError();
 }
 
 // q, out bf16 [R, H, D] at the given pitches (multiples of 8); pages as above, their size a multiple of 8; block_tables int32 [S, max_keys / page] at bt_stride;
@@ -683,27 +1059,25 @@ extern "C" int omni_kv8_attn(const void* q, long q_rs, long q_hs, const void* kc
   if (Hkv < 1 || H < 1 || H % Hkv || (D != 64 && D != 128) || page < 8 || (page & 7) || max_keys < 1 || pages < 1 || (long)pages * page > 0x7fffffffL ||
       (!row_seq && R != S) || ((q_rs | q_hs | o_rs | o_hs) & 7) || misaligned(q, kc, vc, out))
     return RC_BAD_ARG;
-  Kv8Attn p = {};
-  const int G = H / Hkv;
-  p.chunks = (G + 15) / 16;
-  const int VH = Hkv * p.chunks;
-  if ((VH + K8_WARPS - 1) / K8_WARPS > 65535) return RC_BAD_ARG;
-  p.pack = kv8_pack(R, S, G, row_seq != nullptr);
-  const int blocks = (R + p.pack - 1) / p.pack;
-  kv8_shares(blocks, VH, max_keys, p.splits, p.subs);
-  const int parts = p.splits * p.subs;
+  Kv8Deal d;
+  if (!kv8_deal(R, S, H, Hkv, D, row_seq != nullptr, page, max_keys, d)) return RC_TOO_LARGE;
+  const int parts = d.splits;
   if (parts > 1 && (!part_o || !part_lse)) return RC_BAD_ARG;
-  p.q = (const __nv_bfloat16*)q; p.q_rs = q_rs; p.q_hs = q_hs; p.k = (const unsigned char*)kc; p.v = (const unsigned char*)vc; p.ks = ks; p.vs = vs;
-  p.block_tables = block_tables; p.lens = lens; p.row_seq = row_seq; p.bt_stride = bt_stride; p.page = page; p.pages = pages; p.max_keys = max_keys;
-  p.R = R; p.S = S; p.H = H; p.Hkv = Hkv; p.scale_log2 = scale * 1.4426950408889634f; p.part_o = part_o; p.part_lse = part_lse;
+  Kv8Attn p = {};
+  if (int e = kv8_tmap(&p.mk, kc, (long)pages * page, Hkv, D, d.unit, d.heads)) return e;
+  if (int e = kv8_tmap(&p.mv, vc, (long)pages * page, Hkv, D, d.unit, d.heads)) return e;
+  p.q = (const __nv_bfloat16*)q; p.q_rs = q_rs; p.q_hs = q_hs; p.ks = ks; p.vs = vs; p.block_tables = block_tables; p.lens = lens; p.row_seq = row_seq;
+  p.bt_stride = bt_stride; p.page = page; p.shift = page & (page - 1) ? -1 : __builtin_ctz((unsigned)page); p.pages = pages; p.max_keys = max_keys; p.R = R; p.S = S; p.H = H;
+  p.Hkv = Hkv; p.chunks = d.chunks; p.heads = d.heads; p.groups = d.groups; p.pack = d.pack; p.unit = d.unit; p.subs = d.subs; p.share = d.share; p.splits = d.splits;
+  p.row_blocks = (R + d.pack - 1) / d.pack; p.listed = d.splits > 1 && p.row_blocks <= K8_LISTED && (long)p.row_blocks * d.groups * d.splits > d.grid; p.scale_log2 = scale * 1.4426950408889634f; p.part_o = part_o; p.part_lse = part_lse;
   p.out = (__nv_bfloat16*)out; p.o_rs = o_rs; p.o_hs = o_hs; p.status = status;
-  const dim3 grid((unsigned)blocks, (unsigned)p.splits, (unsigned)((VH + K8_WARPS - 1) / K8_WARPS));
   cudaStream_t st = (cudaStream_t)stream;
-  const bool up = (p.chunks > 1 ? 16 : G) * p.pack > 8;
-  launch_with(R <= 16, 1, D == 64 ? (up ? kv8_attn_kernel<64, true> : kv8_attn_kernel<64, false>) : (up ? kv8_attn_kernel<128, true> : kv8_attn_kernel<128, false>), grid,
-              32 * K8_WARPS, 0, st, p);
-  if (cudaError_t e = cudaGetLastError()) return (int)e;
+  if (int e = D == 64 ? (d.up ? launch_kv8_attn<64, true>(p, d.grid, st) : launch_kv8_attn<64, false>(p, d.grid, st))
+                      : (d.up ? launch_kv8_attn<128, true>(p, d.grid, st) : launch_kv8_attn<128, false>(p, d.grid, st)))
+    return e;
   if (parts == 1) return RC_OK;
-  launch_overlapped(D == 64 ? kv8_merge_kernel<64> : kv8_merge_kernel<128>, (unsigned)((long)R * H), 128, 0, st, part_o, part_lse, parts, H, (__nv_bfloat16*)out, o_rs, o_hs);
+  const bool few = d.splits <= 32 && (long)R * H >= 1024;
+  launch_overlapped(few ? (D == 64 ? kv8_merge_few_kernel<64> : kv8_merge_few_kernel<128>) : (D == 64 ? kv8_merge_kernel<64> : kv8_merge_kernel<128>),
+                    (unsigned)(few ? ((long)R * H + 3) / 4 : (long)R * H), few ? 128 : 512, 0, st, part_o, part_lse, lens, d.pack, R, max_keys, d.share, d.splits, H, (__nv_bfloat16*)out, o_rs, o_hs);
   return (int)cudaGetLastError();
 }

@@ -30,14 +30,17 @@ def _lib():
     c = lib._cdll
     c.omni_kv8_write.argtypes = [_P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _P]
     c.omni_kv8_read.argtypes = [_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _L, _I, _I, _I, _P, _P]
-    c.omni_kv8_attn_shares.argtypes = [_I] * 6
+    c.omni_kv8_attn_shares.argtypes = [_I] * 8
     c.omni_kv8_attn.argtypes = [_P, _L, _L, _P, _P, _P, _P, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _L, _L, _P, _P]
     return lib
 
 
 @functools.lru_cache(maxsize=4096)
-def _shares(R, S, H, Hkv, mapped, max_keys, device):
-    return _lib().omni_kv8_attn_shares(R, S, H, Hkv, mapped, max_keys)
+def _shares(R, S, H, Hkv, D, mapped, page, max_keys, device):
+    n = _lib().omni_kv8_attn_shares(R, S, H, Hkv, D, mapped, page, max_keys)
+    if n < 1:
+        raise ValueError(f"{H} heads on {Hkv} KV heads: at most 128 to one")
+    return n
 
 
 class Kv8Cache:
@@ -194,7 +197,7 @@ def kv8_decode(q, cache: Kv8Cache, block_tables, lens, row_seq=None, scale=None,
         return out
     q = _readable(q)
     S, mapped, max_keys = block_tables.shape[0], row_seq is not None, block_tables.shape[1] * cache.block_size
-    shares = _shares(R, S, H, cache.heads, mapped, max_keys, cache.device.index)
+    shares = _shares(R, S, H, cache.heads, D, mapped, cache.block_size, max_keys, cache.device.index)
     part = torch.empty(R * H * shares * (D + 1), dtype=torch.float32, device=cache.device) if shares > 1 else None
     at = 0 if part is None else part.data_ptr()
     nv.check_rc(_lib().omni_kv8_attn(
