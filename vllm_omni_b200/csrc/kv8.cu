@@ -50,55 +50,68 @@ struct Kv8Write {
   int* status;
 };
 
-// A run is the rows of one page, with fewer than 128 rows that are not written between two of them; the warp of its first row takes one head of it: largest magnitude, scale, rounding again of the rows before the
-// first written one where the scale grows, codes.  A block looks for the runs that begin among `chunk` rows and deals out (run, keys or values).  Eight
-// channels per lane: D / 8 lanes are a row, the warp takes 256 / D rows at a time.  The second pass over a run's rows finds them in L1.
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {       // of both halves
+  uint32_t m;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
+__device__ __forceinline__ uint32_t largest_of(uint4 u) {                // magnitudes of eight bf16, of those in even and in odd places
+  return max2(max2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu), max2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
+}
+__device__ __forceinline__ uint32_t finite_of(uint32_t w) {
+  return ((w & 0x7fffu) < 0x7f80u ? w & 0x7fffu : 0u) | ((w & 0x7fff0000u) < 0x7f800000u ? w & 0x7fff0000u : 0u);
+}
+__device__ __forceinline__ uint32_t largest_finite(uint4 u) { return largest_of(make_uint4(finite_of(u.x), finite_of(u.y), finite_of(u.z), finite_of(u.w))); }
+
+struct Kv8Run {
+  int t, end, low, page;                 // first row and behind the last one, lowest row of the page that is written
+  int slot;                              // of the first row, if every next row is in the next slot; -1 otherwise
+};
+
+// A run is the rows of one page, with fewer than 128 rows that are not written between two of them.  A block finds the runs that begin among `chunk` rows and deals out
+// one head of each (keys or values) to its warps: one warp where there are many (decoded tokens, small pages), up to four where there are few.  Largest magnitude, scale,
+// rounding again of the rows before the first written one where the scale grows, codes.  Eight channels per lane: D / 8 lanes are a row, a warp takes 2048 / D rows at
+// a time, in registers from the first look to the codes unless the run is longer.  16435 rows of 8 heads of 128 in pages of 64 (101 MB, 15 us at the rate of memory)
+// take 28.6 us: 23 instructions a lane for 16 bytes in each pass, and a third of the time a block looks for its runs.  One warp per run with two looks at memory took
+// 58; four heads a block, so that the runs are looked for less often, the same 28.6.  Seven rows take 3.5 us, a launch.
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
 kv8_write_kernel(const __grid_constant__ Kv8Write p) {
   pdl_begin();
-  constexpr int LANES = D / 8, ROWS = 32 / LANES;
-  __shared__ int runs[64], n_runs;
-  const int t0 = blockIdx.x * p.chunk, h = blockIdx.y;
-  if (threadIdx.x < 32) {                // `chunk` is at most 64: two rows a lane
-    int n = 0;
-    for (int i0 = 0; i0 < p.chunk; i0 += 32) {
-      const int t = t0 + i0 + threadIdx.x;
-      bool first = false;
-      if (i0 + threadIdx.x < p.chunk && t < p.T) {
-        const int s = p.slots[t];
-        if (s >= p.n_slots) atomicCAS(p.status, 0, ERR_BOUNDS);
-        first = s >= 0 && s < p.n_slots;
-        for (int b = t - 1; first && b >= 0 && b >= t - K8_GAP; --b) {
-          const int before = p.slots[b];
-          if (before < 0 || before >= p.n_slots) continue;
-          first = before / p.page != s / p.page;
-          break;
-        }
+  constexpr int LANES = D / 8, ROWS = 32 / LANES, HELD = 8;
+  __shared__ Kv8Run runs[64];
+  __shared__ int begins[64], n_begin[2];
+  __shared__ uint32_t largest[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t0 = blockIdx.x / p.Hkv * p.chunk, h = blockIdx.x % p.Hkv;
+  if (threadIdx.x < 8) largest[threadIdx.x] = 0;
+  if (threadIdx.x < 64) {                // `chunk` is at most 64
+    const int t = t0 + threadIdx.x;
+    bool first = false;
+    if ((int)threadIdx.x < p.chunk && t < p.T) {
+      const int s = p.slots[t];
+      if (s >= p.n_slots) atomicCAS(p.status, 0, ERR_BOUNDS);
+      first = s >= 0 && s < p.n_slots;
+      for (int b = t - 1; first && b >= 0 && b >= t - K8_GAP; --b) {
+        const int before = p.slots[b];
+        if (before < 0 || before >= p.n_slots) continue;
+        first = before / p.page != s / p.page;
+        break;
       }
-      const unsigned m = __ballot_sync(0xffffffffu, first);
-      if (first) runs[n + __popc(m & ((1u << threadIdx.x) - 1))] = t;
-      n += __popc(m);
     }
-    if (threadIdx.x == 0) n_runs = n;
+    const unsigned m = __ballot_sync(0xffffffffu, first);
+    if (first) begins[warp * 32 + __popc(m & ((1u << lane) - 1))] = t;
+    if (lane == 0) n_begin[warp] = __popc(m);
   }
   __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, ch = lane % LANES * 8;
-  for (int item = warp; item < 2 * n_runs; item += 8) {
-    const int t1 = runs[item >> 1];
-    const bool val = item & 1;
-    const __nv_bfloat16* x = val ? p.v + h * p.v_hs : p.k + h * p.k_hs;
-    const long rs = val ? p.v_rs : p.k_rs;
-    unsigned char* cache = val ? p.vc : p.kc;
-    float* scale = val ? p.vs : p.ks;
-    const int at = p.slots[t1] / p.page;
-    const long base = (long)at * p.page;
-    // lowest row written, end of the run, largest magnitude (as bits: magnitudes of floats are ordered like integers)
-    int low = p.page, t = t1;
-    uint32_t most = 0;
-    for (int skipped = 0, from = t1;;) {                                   // 32 rows from behind the last ones; t: behind the last one of the run
+  const int n_front = n_begin[0], n_runs = n_front + n_begin[1];
+  for (int i = warp; i < n_runs; i += 8) {
+    const int t1 = begins[i < n_front ? i : i - n_front + 32];
+    const int first = p.slots[t1], at = first / p.page, base = at * p.page;
+    int low = p.page, end = t1;
+    bool next = true;
+    for (int skipped = 0, from = t1;;) {                                   // 32 rows from behind the last ones
       const int s = from + lane < p.T ? p.slots[from + lane] : -1;
-      const bool ok = s >= 0 && s < p.n_slots, mine = ok && s / p.page == at;
+      const bool ok = s >= 0 && s < p.n_slots, mine = ok && s >= base && s - base < p.page;
       const unsigned others = __ballot_sync(0xffffffffu, ok && !mine);
       const unsigned ours = __ballot_sync(0xffffffffu, mine) & (others ? (others & -others) - 1 : 0xffffffffu);
       if (!ours) {
@@ -108,71 +121,125 @@ kv8_write_kernel(const __grid_constant__ Kv8Write p) {
         continue;
       }
       const int rows = 32 - __clz(ours);
+      next = next && __all_sync(0xffffffffu, lane >= rows || s == first + (from + lane - t1));
       low = min(low, (int)__reduce_min_sync(0xffffffffu, ours >> lane & 1 ? (unsigned)(s - base) : (unsigned)p.page));
-#pragma unroll 4
-      for (int r = sub; r < rows; r += ROWS) {
-        if (!(ours >> r & 1)) continue;
-        const uint4 u = *reinterpret_cast<const uint4*>(x + (from + r) * rs + ch);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t a = (w[i] << 16) & 0x7fffffffu, b = w[i] & 0x7fff0000u;
-          most = max(most, a < 0x7f800000u ? a : 0u);
-          most = max(most, b < 0x7f800000u ? b : 0u);
-        }
-      }
       from += rows;
-      t = from;
+      end = from;
       skipped = 0;
       if (others) break;
     }
-    most = __reduce_max_sync(0xffffffffu, most);
-    // least e with most <= 1.75 * 2^(8 + e)
-    const int need = max((int)(most >> 23) - 127 - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0), K8_LEAST);
-    float* my_scale = scale + (long)at * p.Hkv + h;
-    int e = need;
-    if (low > 0) {
-      const int old = scale_exp(*my_scale);
-      e = max(need, old);
-      if (e > old) {
-        const float f = pow2f(max(old - e, -126));                         // at 2^-126 every code becomes zero, as it would below
-        for (int r = sub; r < low; r += ROWS) {
-          unsigned char* c = cache + ((base + r) * p.Hkv + h) * D + ch;
-          uint2 u = *reinterpret_cast<const uint2*>(c);
-          uint32_t w[2] = {u.x, u.y};
+    if (lane == 0) runs[i] = {t1, end, low, at, next ? first : -1};
+  }
+  __syncthreads();
+  const int sub = lane / LANES, ch = lane % LANES * 8;
+  const int team = n_runs <= 1 ? 4 : (n_runs == 2 ? 2 : 1), teams = 8 / team, mate = warp % team, step = team * ROWS;      // warps of an item, rows they take at once
+  for (int round = 0; round < 2 * n_runs; round += teams) {
+    const int item = round + warp / team;
+    const bool live = item < 2 * n_runs, val = item & 1;
+    Kv8Run run = {0, 0, 0, 0, 0};
+    if (live) run = runs[item >> 1];
+    const __nv_bfloat16* x = (val ? p.v + h * p.v_hs : p.k + h * p.k_hs) + ch;
+    const long rs = val ? p.v_rs : p.k_rs;
+    unsigned char* cache = (val ? p.vc : p.kc) + h * D + ch;
+    float* my_scale = (val ? p.vs : p.ks) + (long)run.page * p.Hkv + h;
+    const int old = run.low > 0 ? scale_exp(*my_scale) : K8_LEAST, pitch = p.Hkv * D;
+    const int row = run.t + mate * ROWS, batch = HELD * step, rows = run.end - run.t;         // the warp's first rows, rows of a team's registers
+    uint4 u[HELD];
+    auto load = [&](int t) {             // rows t, t + step, .. of a run without gaps
+      const __nv_bfloat16* from = x + (t + sub) * rs;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float2 a = floats_of(halves_of(w[i])), b = floats_of(halves_of_hi(w[i]));
-            w[i] = codes_of(a.x * f, a.y * f, b.x * f, b.y * f);
-          }
-          *reinterpret_cast<uint2*>(c) = make_uint2(w[0], w[1]);
-        }
+      for (int i = 0; i < HELD; ++i, t += step, from += step * rs) {
+        if (t >= run.end) break;
+        u[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (t + sub < run.end) u[i] = *reinterpret_cast<const uint4*>(from);
       }
+    };
+    // largest magnitudes: of floats, they are ordered like integers.  A run's first rows are looked at last, and stay.
+    uint32_t pair = 0;
+    if (run.slot >= 0) {
+      for (int b = (rows - 1) / batch; b >= 0; --b) {
+        load(row + b * batch);
+        uint32_t here = 0;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+          if (row + b * batch + i * step >= run.end) break;
+          here = max2(here, largest_of(u[i]));
+        }
+        if ((here & 0xffffu) >= 0x7f80u || here >= 0x7f800000u) {          // infinities and NaN set no scale
+          here = 0;
+#pragma unroll
+          for (int i = 0; i < HELD; ++i) {
+            if (row + b * batch + i * step >= run.end) break;
+            here = max2(here, largest_finite(u[i]));
+          }
+        }
+        pair = max2(pair, here);
+      }
+    } else {
+      for (int t = row + sub; t < run.end; t += step)
+        if (p.slots[t] >= 0 && p.slots[t] < p.n_slots) pair = max2(pair, largest_finite(*reinterpret_cast<const uint4*>(x + t * rs)));
     }
-    __syncwarp();                                                          // the scale has been read
-    if (lane == 0) *my_scale = pow2f(e);
-    const float f = pow2f(-e);
-    const int end = t;
-    // the same slot twice in a run: later rows win, since a slot's writer is the lane group of its row and rows go in order within `r`
-    for (t = t1; t < end; t += ROWS) {
-      const int r = t + sub;
-      const int s = r < end ? p.slots[r] : -1;
-      if (s >= 0 && s < p.n_slots) {
-        const uint4 u = *reinterpret_cast<const uint4*>(x + r * rs + ch);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-        uint32_t c[2];
+    uint32_t most = __reduce_max_sync(0xffffffffu, max(pair << 16, pair & 0xffff0000u));
+    if (team > 1) {
+      if (lane == 0) atomicMax(&largest[warp / team], most);
+      __syncthreads();                                                     // the scale has been read, too
+      most = largest[warp / team];
+    }
+    // least e with most <= 1.75 * 2^(8 + e)
+    const int need = max((int)(most >> 23) - 127 - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0), K8_LEAST), e = max(need, old);
+    if (run.low > 0 && e > old) {
+      const float f = pow2f(max(old - e, -126));                           // at 2^-126 every code becomes zero, as it would below
+      for (int r = mate * ROWS + sub; r < run.low; r += step) {
+        unsigned char* c = cache + ((long)run.page * p.page + r) * pitch;
+        uint2 o = *reinterpret_cast<const uint2*>(c);
+        uint32_t w[2] = {o.x, o.y};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float2 a = unpack_bf16(w[2 * i]), b = unpack_bf16(w[2 * i + 1]);
-          c[i] = codes_of(a.x * f, a.y * f, b.x * f, b.y * f);
+          const float2 a = floats_of(halves_of(w[i])), b = floats_of(halves_of_hi(w[i]));
+          w[i] = codes_of(a.x * f, a.y * f, b.x * f, b.y * f);
         }
-        bool last = true;                                                  // of the rows of this round with this slot
-#pragma unroll
-        for (int o = 1; o < ROWS; ++o) last &= !(sub + o < ROWS && r + o < end && p.slots[r + o] == s);
-        if (last) *reinterpret_cast<uint2*>(cache + ((long)s * p.Hkv + h) * D + ch) = make_uint2(c[0], c[1]);
+        *reinterpret_cast<uint2*>(c) = make_uint2(w[0], w[1]);
       }
-      __syncwarp();
     }
+    __syncwarp();                                                          // all lanes have read the scale
+    if (live && mate == 0 && lane == 0) *my_scale = pow2f(e);
+    // A power of two of a bf16 is one: exact, but for what is below every code.
+    const __nv_bfloat162 f = __bfloat162bfloat162(__float2bfloat16(pow2f(-e)));
+    auto store = [&](uint4 r, int slot) {
+      uint32_t w[4] = {r.x, r.y, r.z, r.w}, c[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&w[j]), f);
+        w[j] = *reinterpret_cast<const uint32_t*>(&y);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2 lo = unpack_bf16(w[2 * j]), hi = unpack_bf16(w[2 * j + 1]);
+        c[j] = codes_of(lo.x, lo.y, hi.x, hi.y);
+      }
+      *reinterpret_cast<uint2*>(cache + (long)slot * pitch) = make_uint2(c[0], c[1]);
+    };
+    if (run.slot >= 0) {
+      for (int t0 = row; t0 < run.end; t0 += batch) {
+        if (t0 != row) load(t0);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+          const int t = t0 + i * step;
+          if (t >= run.end) break;
+          if (t + sub < run.end) store(u[i], run.slot + (t + sub - run.t));
+        }
+      }
+    } else {
+      for (int t = row + sub; t < run.end; t += step) {
+        int slot = p.slots[t];
+        if (slot >= p.n_slots) slot = -1;
+        if (slot >= 0)                   // the same slot twice: the last row is written
+          for (int o = t + 1; o < run.end; ++o)
+            if (p.slots[o] == slot) slot = -1;
+        if (slot >= 0) store(*reinterpret_cast<const uint4*>(x + t * rs), slot);
+      }
+    }
+    if (team > 1) break;                 // all items had a team
   }
 }
 
@@ -182,56 +249,74 @@ struct Kv8Read {
   const unsigned char *kc, *vc;
   const float *ks, *vs;
   const int* index[K8_TABLES];           // slots of the rows, or block tables
-  long row0[K8_TABLES], rows[K8_TABLES]; // first row written, rows
+  long row0[K8_TABLES];                  // first row written
+  int rows[K8_TABLES];
   __nv_bfloat16 *k, *v;                  // [.., Hkv, D]
   long n_slots;
-  int Hkv, D, page, tables;              // tables: index is block tables
+  int Hkv, D, page, shift, tables;       // tables: index is block tables; shift: log2 of the page's size, -1 if it has none
   int* status;
 };
 
+// Eight codes of a row per thread, keys and values, four rows at once: 16-byte stores side by side.  What a thread's place in a row says is worked out once.
+// Bound by memory: 18185 rows of 8 heads of 128 (112 MB) take 18.7 us, 5985 GB/s; 128 x 350 rows 46.0 us, 5996 GB/s.
 __global__ void __launch_bounds__(256)
 kv8_read_kernel(const __grid_constant__ Kv8Read p) {
   pdl_begin();
-  const int seg = blockIdx.y, vecs = p.Hkv * p.D / 16;
-  const long n = p.rows[seg] * vecs;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
-    const long t = i / vecs;
-    const int c = (int)(i - t * vecs) * 16;
-    long slot;
-    if (p.tables) {
-      const long at = t / p.page;
-      const long pg = p.index[seg][at];
-      slot = pg < 0 ? p.n_slots : pg * p.page + (t - at * p.page);
-    } else {
-      slot = p.index[seg][t];
-    }
-    uint4 out[2][2] = {};
-    if (slot >= 0 && slot < p.n_slots) {
-      const long scale_at = slot / p.page * p.Hkv + c / p.D, from = slot * p.Hkv * p.D + c;
-      const uint4 code[2] = {*reinterpret_cast<const uint4*>(p.kc + from), *reinterpret_cast<const uint4*>(p.vc + from)};
-      const float f[2] = {pow2f(scale_exp(p.ks[scale_at])), pow2f(scale_exp(p.vs[scale_at]))};
+  const int seg = blockIdx.y, vecs = p.Hkv * p.D / 8, rows = p.rows[seg], width = vecs < 256 ? vecs : 256, lines = 256 / width;
+  const int* index = p.index[seg];
+  if ((int)threadIdx.x >= lines * width) return;
+  const int line = threadIdx.x / width;
+  const long row_elems = (long)p.Hkv * p.D;
+  for (int vec = threadIdx.x - line * width; vec < vecs; vec += width) {
+    const int c = vec * 8, head = c / p.D;
+    for (int t0 = (blockIdx.x * lines + line) * 4; t0 < rows; t0 += gridDim.x * lines * 4) {
+      long slot[4];
+      uint2 code[4][2];
+      float f[4][2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const uint32_t w[4] = {code[b].x, code[b].y, code[b].z, code[b].w};
-        uint32_t o[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 lo = floats_of(halves_of(w[j])), hi = floats_of(halves_of_hi(w[j]));
-          o[2 * j] = pack_bf16(lo.x * f[b], lo.y * f[b]);
-          o[2 * j + 1] = pack_bf16(hi.x * f[b], hi.y * f[b]);
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + i;
+        slot[i] = -1;
+        if (t >= rows) continue;
+        if (p.tables) {
+          const int at = p.shift >= 0 ? t >> p.shift : t / p.page, pg = index[at];
+          slot[i] = pg < 0 ? p.n_slots : (long)pg * p.page + (t - at * p.page);
+        } else {
+          slot[i] = index[t];
         }
-        out[b][0] = make_uint4(o[0], o[1], o[2], o[3]);
-        out[b][1] = make_uint4(o[4], o[5], o[6], o[7]);
+        if (slot[i] >= p.n_slots) {
+          atomicCAS(p.status, 0, ERR_BOUNDS);
+          slot[i] = -1;
+        }
       }
-    } else if (slot >= p.n_slots) {
-      atomicCAS(p.status, 0, ERR_BOUNDS);
-    }
-    const long to = (p.row0[seg] + t) * p.Hkv * p.D + c;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      uint4* dst = reinterpret_cast<uint4*>((b ? p.v : p.k) + to);
-      dst[0] = out[b][0];
-      dst[1] = out[b][1];
+      for (int i = 0; i < 4; ++i) {
+        code[i][0] = code[i][1] = make_uint2(0u, 0u);
+        f[i][0] = f[i][1] = 0.f;
+        if (slot[i] < 0) continue;
+        const long scale_at = (long)(p.shift >= 0 ? (int)slot[i] >> p.shift : (int)slot[i] / p.page) * p.Hkv + head, from = slot[i] * row_elems + c;
+        code[i][0] = *reinterpret_cast<const uint2*>(p.kc + from);
+        code[i][1] = *reinterpret_cast<const uint2*>(p.vc + from);
+        f[i][0] = pow2f(scale_exp(p.ks[scale_at]));
+        f[i][1] = pow2f(scale_exp(p.vs[scale_at]));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (t0 + i >= rows) break;
+        const long to = (p.row0[seg] + t0 + i) * row_elems + c;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const uint32_t w[2] = {code[i][b].x, code[i][b].y};
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 lo = floats_of(halves_of(w[j])), hi = floats_of(halves_of_hi(w[j]));
+            o[2 * j] = pack_bf16(lo.x * f[i][b], lo.y * f[i][b]);
+            o[2 * j + 1] = pack_bf16(hi.x * f[i][b], hi.y * f[i][b]);
+          }
+          *reinterpret_cast<uint4*>((b ? p.v : p.k) + to) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
     }
   }
 }
@@ -1004,8 +1089,9 @@ extern "C" int omni_kv8_write(const void* k, const void* v, long k_rs, long k_hs
   while (chunk > 4 && (long)((T + chunk - 1) / chunk) * Hkv < 4L * sm_count()) chunk /= 2;
   const Kv8Write p = {(const __nv_bfloat16*)k, (const __nv_bfloat16*)v, k_rs, k_hs, v_rs, v_hs, (unsigned char*)kc, (unsigned char*)vc, ks, vs, slots, n_slots, T, Hkv, page,
                       chunk, status};
-  const dim3 grid((unsigned)((T + chunk - 1) / chunk), (unsigned)Hkv);
-  launch_overlapped(D == 64 ? kv8_write_kernel<64> : kv8_write_kernel<128>, grid, 256, 0, (cudaStream_t)stream, p);
+  const long grid = (long)((T + chunk - 1) / chunk) * Hkv;              // a chunk's heads side by side: their rows are
+  if (grid > 0x7fffffffL) return RC_TOO_LARGE;
+  launch_overlapped(D == 64 ? kv8_write_kernel<64> : kv8_write_kernel<128>, dim3((unsigned)grid), 256, 0, (cudaStream_t)stream, p);
   return (int)cudaGetLastError();
 }
 
@@ -1017,16 +1103,18 @@ extern "C" int omni_kv8_read(const void* kc, const void* vc, const float* ks, co
     const int m = n - i0 < K8_TABLES ? n - i0 : K8_TABLES;
     Kv8Read p = {};
     p.kc = (const unsigned char*)kc; p.vc = (const unsigned char*)vc; p.ks = ks; p.vs = vs; p.k = (__nv_bfloat16*)k; p.v = (__nv_bfloat16*)v;
-    p.n_slots = n_slots; p.Hkv = Hkv; p.D = D; p.page = page; p.tables = tables; p.status = status;
+    p.n_slots = n_slots; p.Hkv = Hkv; p.D = D; p.page = page; p.shift = page & (page - 1) ? -1 : __builtin_ctz((unsigned)page); p.tables = tables; p.status = status;
     long most = 0;
     for (int i = 0; i < m; ++i) {
       p.index[i] = (const int*)index[i0 + i];
       p.row0[i] = row0[i0 + i];
-      p.rows[i] = rows[i0 + i];
+      p.rows[i] = (int)rows[i0 + i];
+      if (rows[i0 + i] > 0x7fffffffL - 65536) return RC_TOO_LARGE;
       if (rows[i0 + i] > most) most = rows[i0 + i];
     }
     if (most <= 0) continue;
-    long blocks = (most * (Hkv * D / 16) + 255) / 256;
+    const int vecs = Hkv * D / 8, lines = 4 * (vecs < 256 ? 256 / vecs : 1);          // rows a block takes at once
+    long blocks = (most + lines - 1) / lines;
     if (blocks > 16L * sm_count()) blocks = 16L * sm_count();
     launch_overlapped(kv8_read_kernel, dim3((unsigned)blocks, (unsigned)m), 256, 0, (cudaStream_t)stream, p);
     if (cudaError_t e = cudaGetLastError()) return (int)e;
