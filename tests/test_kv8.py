@@ -403,6 +403,28 @@ def test_portions_against_64_bits(dev, H, Hkv, D, page, segs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,D,page", [(4, 2, 128, 16), (3, 1, 64, 24)])
+def test_more_portions_than_a_launch_takes(H, Hkv, D, page):
+    segs, at = [], 1
+    for i in range(35):
+        n = (1, 7, 30, 65)[i % 4]
+        segs.append((at, n, (0, 0, 131, 16)[(i * 5 + i // 4) % 4]))
+        at += n + i % 2
+    test_portions_against_64_bits("cuda", H, Hkv, D, page, segs[::-1])
+
+
+def test_portions_and_heads_that_are_refused():
+    c, t = cache_of(2, 16, 1, 64, "cpu"), torch.arange(2, dtype=torch.int32)
+    q = torch.zeros(8, 129, 64, dtype=BF)
+    ok = q[:, :128]
+    for bad in (lambda: kv8.kv8_prefill(ok, c, [(4, 4, 0, t), (0, 5, 0, t)]), lambda: kv8.kv8_prefill(ok, c, [(0, 8, 0, t), (2, 1, 0, t)]),
+                lambda: kv8.kv8_prefill(q, c, [(0, 8, 0, t)]), lambda: kv8.kv8_decode(q, c, t[None], torch.ones(8, dtype=torch.int32), torch.zeros(8, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            bad()
+    kv8.kv8_prefill(ok, c, [(4, 4, 0, t), (0, 4, 0, t), (2, 0, 0, t)])
+
+
+@pytest.mark.gpu
 def test_captured_and_on_another_stream():
     g = torch.Generator().manual_seed(3)
     lens = [500, 3, 70]

@@ -732,16 +732,11 @@ static int launch_segs(const CUtensorMap& tq, AttnOut& out, int H, int Hkv, cons
   return (int)cudaGetLastError();
 }
 
-}  // namespace omni
-
-// Causal attention of the prompt segments of one step.  q, k, v: bf16 [rows, heads, D], rows of the step's projections; segment i has rows
-// [start[i], start[i] + len[i]) and, before them, context[i] tokens that are in the cache.  A segment without context reads its keys from k and v; another reads
-// all of them, its own included, from the pages (head size 128 only) that table[i] (int32 page ids) names.
-extern "C" int omni_attn_prefill_segs(const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v, long v_rs, long v_hs,
-                                      const void* k_pool, const void* v_pool, int num_blocks, int block_size, void* o, long o_rs, long o_hs, int rows,
-                                      int H, int Hkv, int D, int n, const int* start, const int* len, const int* context, const void* const* table,
-                                      float scale, int* status, void* stream) {
-  using namespace omni;
+// `first_key` (may be null): where in k and v the keys of each segment begin, its context's among them; without it segments with a context read theirs from pages
+static int prefill_segs(const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v, long v_rs, long v_hs, const void* k_pool,
+                        const void* v_pool, int num_blocks, int block_size, void* o, long o_rs, long o_hs, int rows, int H, int Hkv, int D, int n,
+                        const int* start, const int* len, const int* context, const void* const* table, const long* first_key, float scale, int* status,
+                        void* stream) {
   if ((D != 64 && D != 128) || H <= 0 || Hkv <= 0 || (H % Hkv) || (o_rs & 7) || (o_hs & 7) || (reinterpret_cast<uintptr_t>(o) & 15)) return RC_BAD_ARG;
   CUtensorMap tq, pk, pv;
   if (rows <= 0 || n <= 0) return RC_OK;
@@ -750,7 +745,7 @@ extern "C" int omni_attn_prefill_segs(const void* q, long q_rs, long q_hs, const
   for (int i = 0; i < n; ++i) {
     if (len[i] < 0 || start[i] < 0 || context[i] < 0 || (long)start[i] + len[i] > rows) return RC_BAD_ARG;
     if (len[i] > 4096 * 2 * ATT_BM) return RC_TOO_LARGE;
-    if (context[i] > 0) {
+    if (context[i] > 0 && !first_key) {
       if (D != 128 || table[i] == nullptr || block_size < 8 || (block_size & 7) || (ATT_BN % block_size) || num_blocks <= 0) return RC_BAD_ARG;
       paged = true;
     }
@@ -770,15 +765,17 @@ extern "C" int omni_attn_prefill_segs(const void* q, long q_rs, long q_hs, const
   if (n == 1 && D == 128 && len[0] > 0 && len[0] + context[0] >= 1000 && (long)((len[0] + 2 * ATT_BM - 1) / (2 * ATT_BM)) * H <= sm_count()) {
     const int a = start[0], m = len[0], c = context[0];
     if (int rc = make_qkv_tmap(&tq, (const __nv_bfloat16*)q + a * q_rs, m, H, 1, q_rs, q_hs, m * q_rs)) return rc;
-    if (c == 0) {
-      if (int rc = make_qkv_tmap(&pk, (const __nv_bfloat16*)k + a * k_rs, m, Hkv, 1, k_rs, k_hs, m * k_rs)) return rc;
-      if (int rc = make_qkv_tmap(&pv, (const __nv_bfloat16*)v + a * v_rs, m, Hkv, 1, v_rs, v_hs, m * v_rs)) return rc;
+    const bool pages = c > 0 && !first_key;
+    if (!pages) {
+      const long at = first_key ? first_key[0] : a;
+      if (int rc = make_qkv_tmap(&pk, (const __nv_bfloat16*)k + at * k_rs, m + c, Hkv, 1, k_rs, k_hs, (m + c) * k_rs)) return rc;
+      if (int rc = make_qkv_tmap(&pv, (const __nv_bfloat16*)v + at * v_rs, m + c, Hkv, 1, v_rs, v_hs, (m + c) * v_rs)) return rc;
     }
     out.o += a * o_rs;
     out.rows_per_rank = out.rows_per_rank2 = 1;
     out.kv_splits = 1;
     out.split = m;
-    return launch_attn(tq, pk, pv, out, 1, H, Hkv, m, m + c, nullptr, scale, 1, c, {c > 0 ? static_cast<const int*>(table[0]) : nullptr, 0, block_size}, status,
+    return launch_attn(tq, pk, pv, out, 1, H, Hkv, m, m + c, nullptr, scale, 1, c, {pages ? static_cast<const int*>(table[0]) : nullptr, 0, block_size}, status,
                        (cudaStream_t)stream);
   }
   AttnSegs segs;
@@ -788,14 +785,16 @@ extern "C" int omni_attn_prefill_segs(const void* q, long q_rs, long q_hs, const
     for (int i = 0; i < m; ++i) {
       AttnSegs::Seg& g = segs.s[i];
       const int a = start[i0 + i], c = context[i0 + i];
+      const bool pages = c > 0 && !first_key;
       g.row0 = a; g.len = len[i0 + i]; g.kv_len = g.len + c;
-      g.block_table = c > 0 ? static_cast<const int*>(table[i0 + i]) : nullptr;
+      g.block_table = pages ? static_cast<const int*>(table[i0 + i]) : nullptr;
       left[i] = (g.len + 2 * ATT_BM - 1) / (2 * ATT_BM);
-      if (c > 0) {
+      if (pages) {
         g.tmK = pk; g.tmV = pv;
       } else if (g.len > 0) {
-        if (int rc = make_qkv_tmap(&g.tmK, (const __nv_bfloat16*)k + a * k_rs, g.len, Hkv, 1, k_rs, k_hs, g.len * k_rs, ATT_BM, D)) return rc;
-        if (int rc = make_qkv_tmap(&g.tmV, (const __nv_bfloat16*)v + a * v_rs, g.len, Hkv, 1, v_rs, v_hs, g.len * v_rs, ATT_BM, D)) return rc;
+        const long at = first_key ? first_key[i0 + i] : a;
+        if (int rc = make_qkv_tmap(&g.tmK, (const __nv_bfloat16*)k + at * k_rs, g.kv_len, Hkv, 1, k_rs, k_hs, g.kv_len * k_rs, ATT_BM, D)) return rc;
+        if (int rc = make_qkv_tmap(&g.tmV, (const __nv_bfloat16*)v + at * v_rs, g.kv_len, Hkv, 1, v_rs, v_hs, g.kv_len * v_rs, ATT_BM, D)) return rc;
       }
     }
     for (int i = m; i < AttnSegs::MAX; ++i) segs.s[i] = segs.s[0];
@@ -818,6 +817,27 @@ extern "C" int omni_attn_prefill_segs(const void* q, long q_rs, long q_hs, const
     }
   }
   return RC_OK;
+}
+
+}  // namespace omni
+
+// Causal attention of the prompt segments of one step.  q, k, v: bf16 [rows, heads, D], rows of the step's projections; segment i has rows
+// [start[i], start[i] + len[i]) and, before them, context[i] tokens that are in the cache.  A segment without context reads its keys from k and v; another reads
+// all of them, its own included, from the pages (head size 128 only) that table[i] (int32 page ids) names.
+extern "C" int omni_attn_prefill_segs(const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v, long v_rs, long v_hs,
+                                      const void* k_pool, const void* v_pool, int num_blocks, int block_size, void* o, long o_rs, long o_hs, int rows,
+                                      int H, int Hkv, int D, int n, const int* start, const int* len, const int* context, const void* const* table,
+                                      float scale, int* status, void* stream) {
+  return omni::prefill_segs(q, q_rs, q_hs, k, k_rs, k_hs, v, v_rs, v_hs, k_pool, v_pool, num_blocks, block_size, o, o_rs, o_hs, rows, H, Hkv, D, n, start, len,
+                            context, table, nullptr, scale, status, stream);
+}
+
+// The same with the keys of segment i, context[i] + len[i] of them, in rows first_key[i] .. of k and v.
+extern "C" int omni_attn_prefill_keys(const void* q, long q_rs, long q_hs, const void* k, long k_rs, long k_hs, const void* v, long v_rs, long v_hs, void* o,
+                                      long o_rs, long o_hs, int rows, int H, int Hkv, int D, int n, const int* start, const int* len, const int* context,
+                                      const long* first_key, float scale, int* status, void* stream) {
+  return omni::prefill_segs(q, q_rs, q_hs, k, k_rs, k_hs, v, v_rs, v_hs, nullptr, nullptr, 0, 0, o, o_rs, o_hs, rows, H, Hkv, D, n, start, len, context, nullptr,
+                            first_key, scale, status, stream);
 }
 
 // Strides are in elements: *_rs between consecutive sequence positions, *_hs between heads,

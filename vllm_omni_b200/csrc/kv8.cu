@@ -72,8 +72,8 @@ struct Kv8Run {
 // one head of each (keys or values) to its warps: one warp where there are many (decoded tokens, small pages), up to four where there are few.  Largest magnitude, scale,
 // rounding again of the rows before the first written one where the scale grows, codes.  Eight channels per lane: D / 8 lanes are a row, a warp takes 2048 / D rows at
 // a time, in registers from the first look to the codes unless the run is longer.  16435 rows of 8 heads of 128 in pages of 64 (101 MB, 15 us at the rate of memory)
-// take 28.6 us: 23 instructions a lane for 16 bytes in each pass, and a third of the time a block looks for its runs.  One warp per run with two looks at memory took
-// 58; four heads a block, so that the runs are looked for less often, the same 28.6.  Seven rows take 3.5 us, a launch.
+// take 28.6 us: 109 instructions a warp for 512 bytes, the search for runs and both passes among them, and warps that wait while a block looks for its runs.  One
+// warp per run with two looks at memory took 58; four heads a block, so that the runs are looked for less often, the same 28.6.  Seven rows take 3.5 us, a launch.
 template <int D>
 __global__ void __launch_bounds__(256, 3)
 kv8_write_kernel(const __grid_constant__ Kv8Write p) {
@@ -1022,7 +1022,8 @@ struct Kv8Deal {
   int pack, chunks, heads, groups, subs, unit, share, splits, grid;
   bool up;
 };
-static bool kv8_deal(int R, int S, int H, int Hkv, int D, bool mapped, int page, int max_keys, Kv8Deal& d) {
+// `splits`: the number of shares as it was worked out before for the same sizes (0: it is now, which takes as long as a launch does).
+static bool kv8_deal(int R, int S, int H, int Hkv, int D, bool mapped, int page, int max_keys, int splits, Kv8Deal& d) {
   const int G = H / Hkv;
   if (G > K8_MAX_GROUP) return false;
   d.pack = mapped && R > S && G <= 8 ? 16 / G : 1;
@@ -1041,8 +1042,9 @@ static bool kv8_deal(int R, int S, int H, int Hkv, int D, bool mapped, int page,
   // Many: blocks take the shares there are in turn; a row is taken to have four fifths of the table's keys.
   double best = 1e30;
   d.splits = 1;
+  if (splits < 0 || splits > K8_MAX_PARTS) return false;
   const int stages = (max_keys + keys - 1) / keys;
-  for (int n = 1; n <= K8_MAX_PARTS && n <= stages; ++n) {
+  for (int n = splits ? splits : 1; n <= (splits ? splits : K8_MAX_PARTS) && n <= stages; ++n) {
     const int share = (stages + n - 1) / n * keys;
     if ((max_keys + share - 1) / share != n) continue;
     const double items = R > d.pack ? blocks * (0.8 * max_keys / share + 0.5) : (double)blocks * n, rounds = (double)((long)(items / sms) + 1);
@@ -1054,6 +1056,7 @@ static bool kv8_deal(int R, int S, int H, int Hkv, int D, bool mapped, int page,
     }
   }
   if (d.splits == 1) d.share = stages * keys;
+  if (splits && d.splits != splits) return false;
   if (blocks * d.splits > 0x7fffffffL) return false;
   d.grid = blocks * d.splits < sms ? (int)(blocks * d.splits) : sms;
   return true;
@@ -1074,36 +1077,48 @@ static int kv8_tmap(CUtensorMap* out, const void* ptr, long slots, int Hkv, int 
 
 using namespace omni;
 
+static int shift_of(int page) { return page & (page - 1) ? -1 : __builtin_ctz((unsigned)page); }       // log2, -1 if it has none
 static bool misaligned(const void* a, const void* b, const void* c, const void* d) {
   return (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(d)) & 15;
 }
 
-// k, v bf16 [T, Hkv, D] at the given pitches (multiples of 8); pages uint8 [n_slots / page, page, Hkv, D], scales fp32 [n_slots / page, Hkv]; slots int32 [T],
-// below zero: not written.  The rows of a page follow one another, with fewer than 128 others that are not written between two of them.
-extern "C" int omni_kv8_write(const void* k, const void* v, long k_rs, long k_hs, long v_rs, long v_hs, void* kc, void* vc, float* ks, float* vs,
-                              const int* slots, long n_slots, int T, int Hkv, int D, int page, int* status, void* stream) {
+// A cache as the entry points take it: pages uint8 [pages, page, Hkv, D], scales fp32 [pages, Hkv]; set up once by who owns it.
+struct Kv8Cache {
+  void *kc, *vc;
+  float *ks, *vs;
+  int* status;
+  int pages, page, Hkv, D;
+};
+static bool bad_cache(const Kv8Cache& c) {
+  return c.Hkv < 1 || (c.D != 64 && c.D != 128) || c.page < 8 || (c.page & 7) || c.pages < 1 || (long)c.pages * c.page > 0x7fffffffL || misaligned(c.kc, c.vc, c.kc, c.vc);
+}
+
+// k, v bf16 [T, Hkv, D] at the given pitches (multiples of 8); slots int32 [T], below zero: not written.  The rows of a page follow one another, with fewer
+// than 128 others that are not written between two of them.
+extern "C" int omni_kv8_write(const Kv8Cache* cache, const void* k, const void* v, long k_rs, long k_hs, long v_rs, long v_hs, const int* slots, int T, void* stream) {
   if (T <= 0) return RC_OK;
-  if (Hkv < 1 || Hkv > 65535 || (D != 64 && D != 128) || page < 1 || ((k_rs | k_hs | v_rs | v_hs) & 7) || misaligned(k, v, kc, vc) || n_slots > 0x7fffffffL) return RC_BAD_ARG;
+  const Kv8Cache& c = *cache;
+  if (bad_cache(c) || ((k_rs | k_hs | v_rs | v_hs) & 7) || misaligned(k, v, k, v)) return RC_BAD_ARG;
   // rows per block: 64, or fewer where that leaves SMs without blocks
   int chunk = 64;
-  while (chunk > 4 && (long)((T + chunk - 1) / chunk) * Hkv < 4L * sm_count()) chunk /= 2;
-  const Kv8Write p = {(const __nv_bfloat16*)k, (const __nv_bfloat16*)v, k_rs, k_hs, v_rs, v_hs, (unsigned char*)kc, (unsigned char*)vc, ks, vs, slots, n_slots, T, Hkv, page,
-                      chunk, status};
-  const long grid = (long)((T + chunk - 1) / chunk) * Hkv;              // a chunk's heads side by side: their rows are
+  while (chunk > 4 && (long)((T + chunk - 1) / chunk) * c.Hkv < 4L * sm_count()) chunk /= 2;
+  const Kv8Write p = {(const __nv_bfloat16*)k, (const __nv_bfloat16*)v, k_rs, k_hs, v_rs, v_hs, (unsigned char*)c.kc, (unsigned char*)c.vc, c.ks, c.vs, slots,
+                      (long)c.pages * c.page, T, c.Hkv, c.page, chunk, c.status};
+  const long grid = (long)((T + chunk - 1) / chunk) * c.Hkv;              // a chunk's heads side by side: their rows are
   if (grid > 0x7fffffffL) return RC_TOO_LARGE;
-  launch_overlapped(D == 64 ? kv8_write_kernel<64> : kv8_write_kernel<128>, dim3((unsigned)grid), 256, 0, (cudaStream_t)stream, p);
+  launch_overlapped(c.D == 64 ? kv8_write_kernel<64> : kv8_write_kernel<128>, dim3((unsigned)grid), 256, 0, (cudaStream_t)stream, p);
   return (int)cudaGetLastError();
 }
 
 // n lists: index[i] int32 slots of rows[i] rows (tables = 0; below zero: zeros), or a block table of rows[i] tokens, to rows row0[i] .. of k, v bf16 [.., Hkv, D].
-extern "C" int omni_kv8_read(const void* kc, const void* vc, const float* ks, const float* vs, int n, const void* const* index, const long* row0, const long* rows,
-                             int tables, void* k, void* v, long n_slots, int Hkv, int D, int page, int* status, void* stream) {
-  if (Hkv < 1 || (D != 64 && D != 128) || page < 1 || misaligned(kc, vc, k, v) || n_slots > 0x7fffffffL) return RC_BAD_ARG;
+extern "C" int omni_kv8_read(const Kv8Cache* cache, int n, const void* const* index, const long* row0, const long* rows, int tables, void* k, void* v, void* stream) {
+  const Kv8Cache& c = *cache;
+  if (bad_cache(c) || misaligned(k, v, k, v)) return RC_BAD_ARG;
   for (int i0 = 0; i0 < n; i0 += K8_TABLES) {
     const int m = n - i0 < K8_TABLES ? n - i0 : K8_TABLES;
     Kv8Read p = {};
-    p.kc = (const unsigned char*)kc; p.vc = (const unsigned char*)vc; p.ks = ks; p.vs = vs; p.k = (__nv_bfloat16*)k; p.v = (__nv_bfloat16*)v;
-    p.n_slots = n_slots; p.Hkv = Hkv; p.D = D; p.page = page; p.shift = page & (page - 1) ? -1 : __builtin_ctz((unsigned)page); p.tables = tables; p.status = status;
+    p.kc = (const unsigned char*)c.kc; p.vc = (const unsigned char*)c.vc; p.ks = c.ks; p.vs = c.vs; p.k = (__nv_bfloat16*)k; p.v = (__nv_bfloat16*)v;
+    p.n_slots = (long)c.pages * c.page; p.Hkv = c.Hkv; p.D = c.D; p.page = c.page; p.shift = shift_of(c.page); p.tables = tables; p.status = c.status;
     long most = 0;
     for (int i = 0; i < m; ++i) {
       p.index[i] = (const int*)index[i0 + i];
@@ -1113,7 +1128,7 @@ extern "C" int omni_kv8_read(const void* kc, const void* vc, const float* ks, co
       if (rows[i0 + i] > most) most = rows[i0 + i];
     }
     if (most <= 0) continue;
-    const int vecs = Hkv * D / 8, lines = 4 * (vecs < 256 ? 256 / vecs : 1);          // rows a block takes at once
+    const int vecs = c.Hkv * c.D / 8, lines = 4 * (vecs < 256 ? 256 / vecs : 1);          // rows a block takes at once
     long blocks = (most + lines - 1) / lines;
     if (blocks > 16L * sm_count()) blocks = 16L * sm_count();
     launch_overlapped(kv8_read_kernel, dim3((unsigned)blocks, (unsigned)m), 256, 0, (cudaStream_t)stream, p);
@@ -1125,7 +1140,7 @@ extern "C" int omni_kv8_read(const void* kc, const void* vc, const float* ks, co
 // Shares per (row, head) that omni_kv8_attn will write: sizes its scratch (fp32, shares x D and shares x 1); -1: sizes that it does not take.
 extern "C" int omni_kv8_attn_shares(int R, int S, int H, int Hkv, int D, int mapped, int page, int max_keys) {
   Kv8Deal d;
-  if (R < 1 || Hkv < 1 || H < Hkv || page < 8 || max_keys < 1 || !kv8_deal(R, S, H, Hkv, D, mapped != 0, page, max_keys, d)) return -1;
+  if (R < 1 || Hkv < 1 || H < Hkv || page < 8 || max_keys < 1 || !kv8_deal(R, S, H, Hkv, D, mapped != 0, page, max_keys, 0, d)) return -1;
   return d.splits;
 }
 
@@ -1138,34 +1153,35 @@ static int launch_kv8_attn(const Kv8Attn& p, int grid, cudaStream_t st) {
   return (int)cudaGetLastError();
 }
 
-// q, out bf16 [R, H, D] at the given pitches (multiples of 8); pages as above, their size a multiple of 8; block_tables int32 [S, max_keys / page] at bt_stride;
-// lens int32 [R]: keys that a row sees; row_seq int32 [R] or null (R = S).
-extern "C" int omni_kv8_attn(const void* q, long q_rs, long q_hs, const void* kc, const void* vc, const float* ks, const float* vs, int pages, int page,
-                             const int* block_tables, long bt_stride, const int* lens, const int* row_seq, int R, int S, int H, int Hkv, int D, int max_keys,
-                             float scale, float* part_o, float* part_lse, void* out, long o_rs, long o_hs, int* status, void* stream) {
+// q, out bf16 [R, H, D] at the given pitches (multiples of 8); block_tables int32 [S, max_keys / page] at bt_stride; lens int32 [R]: keys that a row sees;
+// row_seq int32 [R] or null (R = S).  `part`: fp32 [R, H, shares, D + 1] where there are several shares.
+extern "C" int omni_kv8_attn(const Kv8Cache* cache, const void* q, long q_rs, long q_hs, const int* block_tables, long bt_stride, const int* lens, const int* row_seq,
+                             int R, int S, int H, int max_keys, float scale, int shares, float* part, void* out, long o_rs, long o_hs, void* stream) {
   if (R <= 0) return RC_OK;
-  if (Hkv < 1 || H < 1 || H % Hkv || (D != 64 && D != 128) || page < 8 || (page & 7) || max_keys < 1 || pages < 1 || (long)pages * page > 0x7fffffffL ||
-      (!row_seq && R != S) || ((q_rs | q_hs | o_rs | o_hs) & 7) || misaligned(q, kc, vc, out))
+  const Kv8Cache& c = *cache;
+  const int Hkv = c.Hkv, D = c.D, page = c.page;
+  if (bad_cache(c) || H < 1 || H % Hkv || max_keys < 1 || (!row_seq && R != S) || ((q_rs | q_hs | o_rs | o_hs) & 7) || misaligned(q, out, q, out) || shares < 1 ||
+      (shares > 1 && !part))
     return RC_BAD_ARG;
   Kv8Deal d;
-  if (!kv8_deal(R, S, H, Hkv, D, row_seq != nullptr, page, max_keys, d)) return RC_TOO_LARGE;
-  const int parts = d.splits;
-  if (parts > 1 && (!part_o || !part_lse)) return RC_BAD_ARG;
+  if (!kv8_deal(R, S, H, Hkv, D, row_seq != nullptr, page, max_keys, shares, d)) return RC_TOO_LARGE;
+  float* part_lse = part + (long)R * H * shares * D;
   Kv8Attn p = {};
-  if (int e = kv8_tmap(&p.mk, kc, (long)pages * page, Hkv, D, d.unit, d.heads)) return e;
-  if (int e = kv8_tmap(&p.mv, vc, (long)pages * page, Hkv, D, d.unit, d.heads)) return e;
-  p.q = (const __nv_bfloat16*)q; p.q_rs = q_rs; p.q_hs = q_hs; p.ks = ks; p.vs = vs; p.block_tables = block_tables; p.lens = lens; p.row_seq = row_seq;
-  p.bt_stride = bt_stride; p.page = page; p.shift = page & (page - 1) ? -1 : __builtin_ctz((unsigned)page); p.pages = pages; p.max_keys = max_keys; p.R = R; p.S = S; p.H = H;
+  if (int e = kv8_tmap(&p.mk, c.kc, (long)c.pages * page, Hkv, D, d.unit, d.heads)) return e;
+  if (int e = kv8_tmap(&p.mv, c.vc, (long)c.pages * page, Hkv, D, d.unit, d.heads)) return e;
+  p.q = (const __nv_bfloat16*)q; p.q_rs = q_rs; p.q_hs = q_hs; p.ks = c.ks; p.vs = c.vs; p.block_tables = block_tables; p.lens = lens; p.row_seq = row_seq;
+  p.bt_stride = bt_stride; p.page = page; p.shift = shift_of(page); p.pages = c.pages; p.max_keys = max_keys; p.R = R; p.S = S; p.H = H;
   p.Hkv = Hkv; p.chunks = d.chunks; p.heads = d.heads; p.groups = d.groups; p.pack = d.pack; p.unit = d.unit; p.subs = d.subs; p.share = d.share; p.splits = d.splits;
-  p.row_blocks = (R + d.pack - 1) / d.pack; p.listed = d.splits > 1 && p.row_blocks <= K8_LISTED && (long)p.row_blocks * d.groups * d.splits > d.grid; p.scale_log2 = scale * 1.4426950408889634f; p.part_o = part_o; p.part_lse = part_lse;
-  p.out = (__nv_bfloat16*)out; p.o_rs = o_rs; p.o_hs = o_hs; p.status = status;
+  p.row_blocks = (R + d.pack - 1) / d.pack; p.listed = d.splits > 1 && p.row_blocks <= K8_LISTED && (long)p.row_blocks * d.groups * d.splits > d.grid;
+  p.scale_log2 = scale * 1.4426950408889634f; p.part_o = part; p.part_lse = part_lse; p.out = (__nv_bfloat16*)out; p.o_rs = o_rs; p.o_hs = o_hs; p.status = c.status;
   cudaStream_t st = (cudaStream_t)stream;
   if (int e = D == 64 ? (d.up ? launch_kv8_attn<64, true>(p, d.grid, st) : launch_kv8_attn<64, false>(p, d.grid, st))
                       : (d.up ? launch_kv8_attn<128, true>(p, d.grid, st) : launch_kv8_attn<128, false>(p, d.grid, st)))
     return e;
-  if (parts == 1) return RC_OK;
+  if (shares == 1) return RC_OK;
   const bool few = d.splits <= 32 && (long)R * H >= 1024;
   launch_overlapped(few ? (D == 64 ? kv8_merge_few_kernel<64> : kv8_merge_few_kernel<128>) : (D == 64 ? kv8_merge_kernel<64> : kv8_merge_kernel<128>),
-                    (unsigned)(few ? ((long)R * H + 3) / 4 : (long)R * H), few ? 128 : 512, 0, st, part_o, part_lse, lens, d.pack, R, max_keys, d.share, d.splits, H, (__nv_bfloat16*)out, o_rs, o_hs);
+                    (unsigned)(few ? ((long)R * H + 3) / 4 : (long)R * H), few ? 128 : 512, 0, st, part, part_lse, lens, d.pack, R,
+                    max_keys, d.share, d.splits, H, (__nv_bfloat16*)out, o_rs, o_hs);
   return (int)cudaGetLastError();
 }

@@ -20,6 +20,7 @@ from . import _native as nv
 
 LEAST, MOST = -120, 120               # exponents of scales
 HEAD_SIZES = (64, 128)
+MAX_GROUP = 128                       # heads on one KV head
 CODES = torch.float8_e4m3fn
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
 
@@ -28,24 +29,32 @@ _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
 def _lib():
     lib = nv.lib("kv8")
     c = lib._cdll
-    c.omni_kv8_write.argtypes = [_P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _P]
-    c.omni_kv8_read.argtypes = [_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _L, _I, _I, _I, _P, _P]
+    c.omni_kv8_write.argtypes = [_P, _P, _P, _L, _L, _L, _L, _P, _I, _P]
+    c.omni_kv8_read.argtypes = [_P, _I, _P, _P, _P, _I, _P, _P, _P]
     c.omni_kv8_attn_shares.argtypes = [_I] * 8
-    c.omni_kv8_attn.argtypes = [_P, _L, _L, _P, _P, _P, _P, _I, _I, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _L, _L, _P, _P]
+    c.omni_kv8_attn.argtypes = [_P, _P, _L, _L, _P, _L, _P, _P, _I, _I, _I, _I, _F, _I, _P, _P, _L, _L, _P]
+    return lib
+
+
+@functools.lru_cache(maxsize=None)
+def _prefill_lib():
+    lib = nv.lib("attention_sm100")
+    lib._cdll.omni_attn_prefill_keys.argtypes = [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _I, _I, _I, _P, _P, _P, _P, _F, _P, _P]
     return lib
 
 
 @functools.lru_cache(maxsize=4096)
 def _shares(R, S, H, Hkv, D, mapped, page, max_keys, device):
-    n = _lib().omni_kv8_attn_shares(R, S, H, Hkv, D, mapped, page, max_keys)
-    if n < 1:
-        raise ValueError(f"{H} heads on {Hkv} KV heads: at most 128 to one")
-    return n
+    return _lib().omni_kv8_attn_shares(R, S, H, Hkv, D, mapped, page, max_keys)
+
+
+class _Fields(ctypes.Structure):      # Kv8Cache of csrc/kv8.cu
+    _fields_ = [(n, _P) for n in ("k", "v", "k_scale", "v_scale", "status")] + [(n, _I) for n in ("pages", "page", "heads", "channels")]
 
 
 class Kv8Cache:
     """``k``, ``v``: float8_e4m3fn [pages, page size, Hkv, D]; ``k_scale``, ``v_scale``: fp32 powers of two [pages, Hkv]."""
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "block_size", "heads", "head_size", "device")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "block_size", "heads", "head_size", "device", "_fields", "_at")
 
     def __init__(self, k, v, k_scale, v_scale):
         if k.dim() != 4 or any(t.dtype is not CODES or t.shape != k.shape or not t.is_contiguous() or t.device != k.device for t in (k, v)):
@@ -62,6 +71,9 @@ class Kv8Cache:
         if k.is_cuda and (k.data_ptr() | v.data_ptr()) & 15:
             raise ValueError("k and v must begin on 16 bytes")
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
+        if k.is_cuda:                                    # what the kernels take of it, once
+            self._fields = _Fields(*(t.data_ptr() for t in (k, v, k_scale, v_scale, nv.status_word(k.device))), *k.shape)
+            self._at = ctypes.addressof(self._fields)
 
     @classmethod
     def empty(cls, pages: int, block_size: int, heads: int, head_size: int, device) -> "Kv8Cache":
@@ -94,6 +106,10 @@ def _elsewhere(device) -> bool:
     return torch._C._cuda_getDevice() != device.index
 
 
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def kv8_write(k, v, cache: Kv8Cache, slots) -> None:
     """k, v: bf16 [T, Hkv, D]; slots int32 [T] (page * page size + row, below zero: not written)."""
     T = k.shape[0]
@@ -109,10 +125,8 @@ def kv8_write(k, v, cache: Kv8Cache, slots) -> None:
         with torch.cuda.device(cache.device):
             return kv8_write(k, v, cache, slots)
     k, v = _readable(k), _readable(v)
-    nv.check_rc(_lib().omni_kv8_write(
-        k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-        cache.v_scale.data_ptr(), slots.data_ptr(), cache.pages * cache.block_size, T, cache.heads, cache.head_size, cache.block_size,
-        nv.status_word(cache.device).data_ptr(), nv.stream_ptr()), "omni_kv8_write")
+    ks, vs = k.stride(), v.stride()
+    nv.check_rc(_lib().omni_kv8_write(cache._at, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), T, _stream(cache.device)), "omni_kv8_write")
 
 
 def _out_pair(cache, rows, out_k, out_v):
@@ -120,7 +134,7 @@ def _out_pair(cache, rows, out_k, out_v):
     if (out_k is None) != (out_v is None):
         raise ValueError("out_k and out_v: both or neither")
     if out_k is None:
-        return torch.empty(shape, dtype=torch.bfloat16, device=cache.device), torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+        return cache.k_scale.new_empty(shape, dtype=torch.bfloat16), cache.k_scale.new_empty(shape, dtype=torch.bfloat16)
     for name, t in (("out_k", out_k), ("out_v", out_v)):
         _check_rows(name, t, shape, cache.device)
         if not t.is_contiguous() or (t.is_cuda and t.data_ptr() & 15):
@@ -129,10 +143,8 @@ def _out_pair(cache, rows, out_k, out_v):
 
 
 def _read(cache, n, index, row0, rows, tables, k, v):
-    nv.check_rc(_lib().omni_kv8_read(
-        cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n, (_P * n)(*index), (_L * n)(*row0), (_L * n)(*rows), tables,
-        k.data_ptr(), v.data_ptr(), cache.pages * cache.block_size, cache.heads, cache.head_size, cache.block_size, nv.status_word(cache.device).data_ptr(),
-        nv.stream_ptr()), "omni_kv8_read")
+    nv.check_rc(_lib().omni_kv8_read(cache._at, n, (_P * n)(*index), (_L * n)(*row0), (_L * n)(*rows), tables, k.data_ptr(), v.data_ptr(), _stream(cache.device)),
+                "omni_kv8_read")
 
 
 def kv8_read(cache: Kv8Cache, slots, out_k=None, out_v=None):
@@ -164,6 +176,8 @@ def _check_tables(tables, S, cache):
 def _check_queries(q, cache, out):
     if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % cache.heads:
         raise ValueError(f"q: [rows, heads, {cache.head_size}] with heads a multiple of {cache.heads} expected, got {tuple(q.shape)}")
+    if q.shape[1] > MAX_GROUP * cache.heads:
+        raise ValueError(f"{q.shape[1]} heads on {cache.heads} KV heads: at most {MAX_GROUP} to one")
     _check_rows("q", q, (q.shape[0], q.shape[1], cache.head_size), cache.device)
     if out is not None:
         _check_rows("out", out, q.shape, cache.device)
@@ -183,7 +197,7 @@ def kv8_decode(q, cache: Kv8Cache, block_tables, lens, row_seq=None, scale=None,
         _check_index("row_seq", row_seq, R, cache.device)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if out is None:
-        out = torch.empty(R, H, D, dtype=torch.bfloat16, device=cache.device)
+        out = q.new_empty((R, H, D))
     if not q.is_cuda:
         for r in range(R):
             s = r if row_seq is None else int(row_seq[r])
@@ -198,13 +212,11 @@ def kv8_decode(q, cache: Kv8Cache, block_tables, lens, row_seq=None, scale=None,
     q = _readable(q)
     S, mapped, max_keys = block_tables.shape[0], row_seq is not None, block_tables.shape[1] * cache.block_size
     shares = _shares(R, S, H, cache.heads, D, mapped, cache.block_size, max_keys, cache.device.index)
-    part = torch.empty(R * H * shares * (D + 1), dtype=torch.float32, device=cache.device) if shares > 1 else None
-    at = 0 if part is None else part.data_ptr()
+    part = cache.k_scale.new_empty(R * H * shares * (D + 1)) if shares > 1 else None
+    qs, outs = q.stride(), out.stride()
     nv.check_rc(_lib().omni_kv8_attn(
-        q.data_ptr(), q.stride(0), q.stride(1), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.pages,
-        cache.block_size, block_tables.data_ptr(), block_tables.stride(0), lens.data_ptr(), row_seq.data_ptr() if mapped else None, R, S, H, cache.heads, D, max_keys,
-        scale, at, at + 4 * R * H * shares * D, out.data_ptr(), out.stride(0), out.stride(1), nv.status_word(cache.device).data_ptr(), nv.stream_ptr()),
-        "omni_kv8_attn")
+        cache._at, q.data_ptr(), qs[0], qs[1], block_tables.data_ptr(), block_tables.stride(0), lens.data_ptr(), row_seq.data_ptr() if mapped else None, R, S, H,
+        max_keys, scale, shares, None if part is None else part.data_ptr(), out.data_ptr(), outs[0], outs[1], _stream(cache.device)), "omni_kv8_attn")
     if part is not None:
         nv.count_launches(1)
     return out
@@ -225,9 +237,13 @@ def kv8_prefill(q, cache: Kv8Cache, segs, scale=None, out=None):
             raise ValueError(f"block table: contiguous int32 [columns] on {cache.device} expected, got {table.dtype} {tuple(table.shape)}")
         if table.numel() * cache.block_size < context + rows:
             raise ValueError(f"block table of {table.numel()} pages of {cache.block_size}: {context + rows} tokens")
+    if len(segs) > 1:
+        order = sorted((s[0], s[1]) for s in segs)
+        if any(a + n > b for (a, n), (b, _) in zip(order, order[1:])):
+            raise ValueError("portions that share rows")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if out is None:
-        out = torch.empty(T, H, D, dtype=torch.bfloat16, device=cache.device)
+        out = q.new_empty((T, H, D))
     if not q.is_cuda:
         for first, rows, context, table in segs:
             out[first:first + rows] = _attend_torch(q[first:first + rows], cache, table, context + rows, scale, context)
@@ -237,17 +253,21 @@ def kv8_prefill(q, cache: Kv8Cache, segs, scale=None, out=None):
             return kv8_prefill(q, cache, segs, scale, out)
     if not segs:
         return out
-    from .attention import attention
-    q = _readable(q)
+    q, n = _readable(q), len(segs)
     total, row0 = 0, []
     for _, rows, context, _ in segs:
         row0.append(total)
         total += context + rows
-    k, v = (torch.empty(total, cache.heads, D, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
-    _read(cache, len(segs), [s[3].data_ptr() for s in segs], row0, [s[2] + s[1] for s in segs], 1, k, v)
-    for (first, rows, context, _), at in zip(segs, row0):
-        keys = slice(at, at + context + rows)
-        attention(q[None, first:first + rows], k[None, keys], v[None, keys], scale=scale, causal=True, q_offset=context, out=out[None, first:first + rows])
+    k, v = q.new_empty((2, total, cache.heads, D))
+    _read(cache, n, [s[3].data_ptr() for s in segs], row0, [s[2] + s[1] for s in segs], 1, k, v)
+    first, rows, context = ((_I * n)(*(s[i] for s in segs)) for i in range(3))
+    rs = cache.heads * D
+    nv.check_rc(_prefill_lib().omni_attn_prefill_keys(
+        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), rs, D, v.data_ptr(), rs, D, out.data_ptr(), out.stride(0), out.stride(1), T, H, cache.heads, D, n,
+        first, rows, context, (_L * n)(*row0), scale, cache._fields.status, _stream(cache.device)), "omni_attn_prefill_keys")
+    nv.count_launches((n - 1) // 16)                         # of the pages, sixteen segments at a time
+    if n > 8 or T > 248 * 256:                               # of the attention, eight segments and 256 blocks of 256 rows at a time
+        nv.count_launches(sum(-(-sum(-(-s[1] // 256) for s in segs[i:i + 8]) // 256) for i in range(0, n, 8)) - 1)
     return out
 
 
