@@ -762,7 +762,10 @@ static int prefill_segs(const void* q, long q_rs, long q_hs, const void* k, long
   // One segment in a round of blocks has no order to gain from, and its softmax warps are 3 to 7 % faster with its numbers in the constant bank: 1000 tokens, 32 heads
   // 21.0 us (21.6 below), 6000 tokens, 4 heads 79 (85), 1 head 77 (82).  Short ones are over before that shows: 130 tokens, 32 heads 9.5
   // (9.3); heads of 64 channels leave registers enough: 1000 tokens, 16 heads 18.0 (17.4).
-  if (n == 1 && D == 128 && len[0] > 0 && len[0] + context[0] >= 1000 && (long)((len[0] + 2 * ATT_BM - 1) / (2 * ATT_BM)) * H <= sm_count()) {
+  // Where the context is most of what every row sees, no block has much more to do than another (keys side by side, 32 heads: 2039 tokens on 14345 424 us, 440 below;
+  // 2048 on 8192 272 and 270, on 4096 176 and 160).
+  if (n == 1 && D == 128 && len[0] > 0 && len[0] + context[0] >= 1000 &&
+      ((long)((len[0] + 2 * ATT_BM - 1) / (2 * ATT_BM)) * H <= sm_count() || (first_key && context[0] / 6 >= len[0]))) {
     const int a = start[0], m = len[0], c = context[0];
     if (int rc = make_qkv_tmap(&tq, (const __nv_bfloat16*)q + a * q_rs, m, H, 1, q_rs, q_hs, m * q_rs)) return rc;
     const bool pages = c > 0 && !first_key;
