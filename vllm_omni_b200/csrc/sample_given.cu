@@ -74,8 +74,9 @@ struct SgShared {
   u64 scan[SG_WARPS];
   float scan_f[SG_WARPS];
   u64 found[4];
-  uint32_t n_list, n_cand, base;
+  uint32_t n_list, base;
   int mode, lo, hi;
+  float first[2];                                       // least logits in front of the window, and in it
 };
 
 template <typename T>
@@ -231,7 +232,7 @@ struct SgRow {
   float mx, to_bin, log2_t;                             // bins and powers of two per unit of x
   double mx_d, to_64, inv_t, least;                     // 64ths of powers of two per unit; min_p 2^44
   const double* table;
-  __device__ __forceinline__ float place(float x) const { return (mx - x) * to_bin; }       // in bins behind the largest, which is finite; monotone
+  __device__ __forceinline__ float place(float x) const { return __fmul_rn(__fsub_rn(mx, x), to_bin); }       // in bins behind the largest, which is finite; monotone
   // 2^44 exp((x - m) / T) before it is rounded, within some 2^-50 of itself; 0 beyond the range.  2^(y / 64) = 2^(n / 64) e^(r ln 2 / 64), n the whole number next to y, |r| <= 1/2:
   // 2^(j / 64) from a table, e^.. by its series to the fifth power (the sixth is below 2^-54), the exponent added to the table's.
   // Every copy of this has to give the same bits: no products and sums that a compiler may fuse in one place and not in another.
@@ -336,7 +337,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
     sh.frac[b] = 0;
   }
   if (tid < 64) sh.table[tid] = exp2((double)tid * (1.0 / 64)) * SG_ONE;
-  if (tid == 0) sh.n_list = sh.n_cand = 0;
+  if (tid == 0) sh.n_list = 0;
   const T* x0 = reinterpret_cast<const T*>(p.logits) + (long)row * p.ld;
   const int off = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
   const int vecs = (V + off + 7) / 8, tiles = (vecs + SG_THREADS - 1) / SG_THREADS, per = (tiles + nc - 1) / nc, pieces = tiles * SG_WARPS;
@@ -373,7 +374,17 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
       if (top < INFINITY) {
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += ex2_approx(fmaxf((x[j] - base) * r.log2_t, -200.f));       // not a number: nothing
+        for (int j = 0; j < 8; ++j) sum += ex2_approx((x[j] - base) * r.log2_t);
+        if (sum != sum) {                                                // not a number: nothing
+          sum = 0.f;
+#pragma unroll 1
+          for (int j = 0; j < 8; ++j) {
+            float y = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) y = i == j ? x[i] : y;
+            sum += ex2_approx(fmaxf((y - base) * r.log2_t, -200.f));
+          }
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += x[j] == INFINITY ? 1.f : 0.f;
@@ -446,7 +457,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
 
   // The bound: what is below it is not kept (and -inf never).  SG_ALL: no bound and no list.
   float bound = -FLT_MAX;
-  int mode = SG_ALL, lo = SG_BINS, hi = -1;
+  int mode = SG_ALL;
   if (by_k && V > SG_LIST) {
     // the k-th largest of the pieces' maxima, rounded down to its upper 16 bits: two histograms of 256 bins
     uint32_t got = 0;
@@ -501,7 +512,6 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
     const float below = log2f(share) / r.log2_t;
     bound = fmaxf(bound, share > 0.f ? r.mx + below - 1e-5f * (fabsf(r.mx) + fabsf(below)) : bound);
   }
-  const unsigned below = (1u << lane) - 1;
   auto piece_top = [&](int t) { return sh.top[t * SG_WARPS + warp]; };
   if (by_k) {
     // 2, top-k
@@ -527,7 +537,6 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
   if (mode == SG_WINDOW && r.mx == INFINITY) mode = SG_SLOW;
   if (mode == SG_WINDOW) {
     // 2, histogram of what reaches the bound
-    uint32_t far = 0, cand = 0;
 #pragma unroll 1
     for (int t = tile0; t < tile1; ++t) {
       if (piece_top(t) < bound) continue;
@@ -535,22 +544,16 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
       raw8(load8(x0, off, V, t * SG_THREADS + tid), x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const bool in = x[j] >= bound;
-        const float y = r.place(x[j]);
-        const bool near = in && y < (float)(SG_BINS - 1);
-        cand += in;
-        far += in && !near;
-        const int b = near ? (int)y : 0;
-        if (near) {
+        // 2^23 and what is below it, rounded down: whole numbers in the low bits.  What is far beyond the range counts into the last bin.
+        const float y = fminf(r.place(x[j]), (float)SG_BINS - 0.001f), whole = __fadd_rd(y, 8388608.f);
+        const uint32_t b = __float_as_uint(whole) & (SG_BINS - 1);
+        const float part = __fsub_rn(y, __fsub_rn(whole, 8388608.f));
+        if (x[j] >= bound) {
           atomicAdd(&sh.count[b], 1u);
-          if (by_p) atomicAdd(&sh.frac[b], (uint32_t)((y - (float)b) * 8192.f));
+          if (by_p) atomicAdd(&sh.frac[b], __float_as_uint(__fmaf_rn(part, 8192.f, 8388608.f)) & 0x3fffu);
         }
       }
     }
-    cand = __reduce_add_sync(0xffffffffu, cand);
-    far = __reduce_add_sync(0xffffffffu, far);
-    if (lane == 0 && far) atomicAdd(&sh.count[SG_BINS - 1], far);
-    if (lane == 0 && cand) atomicAdd(at_rank(&sh.n_cand, 0), cand);
     __syncthreads();
     if (rank)
       for (int b = tid; b < SG_BINS; b += SG_THREADS)
@@ -586,7 +589,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
           b += n[i];
         }
         if (tid == 0 && all < (u64)k_in) sh.mode = SG_SLOW;
-      } else if (sh.n_cand <= SG_LIST) {
+      } else if (all <= SG_LIST) {
         if (tid == 0) {
           sh.lo = 0;
           sh.hi = SG_BINS;
@@ -628,16 +631,29 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
         if (tid == 0 && (listed > SG_LIST || sh.hi < sh.lo)) sh.mode = SG_SLOW;
       }
       __syncthreads();
+      // The least logits whose place is in front of the window, and in front of its end: five bits of their keys at a time, a lane for each of 32 values.
+      if (warp < 2) {
+        const float end = warp == 0 ? (float)sh.lo : (sh.hi >= SG_BINS - 1 ? INFINITY : (float)sh.hi + 1.f);
+        const uint32_t most = key_of(r.mx);
+        uint32_t key = 0;
+#pragma unroll 1
+        for (int shift = 27; shift > -5; shift -= 5) {
+          const int by = max(shift, 0);
+          const uint32_t last = min(key + ((uint32_t)lane << by) + ((1u << by) - 1), most);
+          const unsigned m = __ballot_sync(0xffffffffu, r.place(of_key(last)) < end);
+          key += m ? (uint32_t)(__ffs(m) - 1) << by : 0;
+        }
+        if (lane == 0) sh.first[warp] = end > 0.f ? of_key(key) : INFINITY;
+      }
+      __syncthreads();
       if (tid > 0 && tid < nc) {
         *at_rank(&sh.mode, tid) = sh.mode;
-        *at_rank(&sh.lo, tid) = sh.lo;
-        *at_rank(&sh.hi, tid) = sh.hi;
+        *at_rank(&sh.first[0], tid) = sh.first[0];
+        *at_rank(&sh.first[1], tid) = sh.first[1];
       }
     }
     cluster_barrier();
     mode = sh.mode;
-    lo = sh.lo;
-    hi = sh.hi;
   }
 
   // 3
@@ -665,50 +681,62 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
   } else if (mode == SG_WINDOW) {
     // Few of a piece's elements are surely kept: they are pushed together before their weights are computed.  The list's weights are the first block's.  What lies behind
     // the window counts by its fp32 weight.
-    const float from = (float)lo, to = hi >= SG_BINS - 1 ? INFINITY : (float)hi + 1.f;
     const bool by_both = by_p && min_p > 0.f;                             // S is what min-p leaves: 64-bit weights behind the window, too
-    auto wanted = [&](float top) { return top >= bound && (by_both || r.place(top) < to); };
+    const float front = fmaxf(sh.first[0], bound), inside = fmaxf(sh.first[1], bound), need = by_both ? bound : inside;
     u64 rest = 0;
-    unsigned behind = 0;
+    float least = INFINITY;
     float* q = sh.queue[warp];
 #pragma unroll 1
     for (int t = tile0; t < tile1; ++t) {
       const float top = piece_top(t);
       u64 sure = 0;
-      if (wanted(top)) {
+      if (top >= need) {
         float x[8];
         raw8(load8(x0, off, V, t * SG_THREADS + tid), x);
-        int n = 0;
-        unsigned marks = 0, other = 0;
+        unsigned listed = 0, mine = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float y = r.place(x[j]);
-          const bool in = x[j] >= bound, before = in && y < from, listed = in && y >= from && y < to;
-          marks |= (unsigned)listed << j;
-          other |= (unsigned)!(before || listed) << j;
-          const bool mine = before || (by_both && in && y >= to);
-          const unsigned m = __ballot_sync(0xffffffffu, mine);
-          if (mine) q[n + __popc(m & below)] = x[j];
-          n += __popc(m);
+          mine |= (unsigned)(x[j] >= front) << j;
+          listed |= (unsigned)(x[j] >= inside) << j;
+          least = fminf(least, x[j]);
         }
-        behind |= other;
-        append(sh, marks, x, (t * SG_THREADS + tid) * 8 - off);
-        __syncwarp();
+        listed &= ~mine;
+        append(sh, listed, x, (t * SG_THREADS + tid) * 8 - off);
+        if (by_both) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mine |= (unsigned)(x[j] >= bound && x[j] < inside) << j;
+        }
+        if (__any_sync(0xffffffffu, mine)) {
+          const int has = __popc(mine);
+          int run = has;
+#pragma unroll
+          for (int o = 1; o < 32; o *= 2) {
+            const int up = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += up;
+          }
+          const int n = __shfl_sync(0xffffffffu, run, 31);
+          float* to = q + run - has;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (mine >> j & 1) *to++ = x[j];
+          __syncwarp();
 #pragma unroll 1
-        for (int i = lane; i < n; i += 32) {
-          const u64 w = r.kept(q[i]);
-          if (r.place(q[i]) < from) sure += w;
-          else rest += w;
+          for (int i = lane; i < n; i += 32) {
+            const u64 w = r.kept(q[i]);
+            if (q[i] >= front) sure += w;
+            else rest += w;
+          }
+          __syncwarp();
+          sure = warp_sum(sure);
         }
-        __syncwarp();
-        sure = warp_sum(sure);
       } else {
-        behind = 1;
+        least = -INFINITY;
       }
       if (lane == 0) *at_rank(&sh.tile[t * SG_WARPS + warp], 0) = sure;
     }
+    const bool behind = least < inside;
     u64 a;
-    block_prefix(by_both ? rest : (u64)(behind != 0), a, sh.scan);
+    block_prefix(by_both ? rest : (u64)behind, a, sh.scan);
     if (tid == 0) *at_rank(&sh.whole[rank], 0) = a;
     join_lists(sh, rank);
     cluster_barrier();
