@@ -184,24 +184,24 @@ release_pages_kernel(const __grid_constant__ ReleasePages p) {
 #pragma unroll
   for (int i = 0; i < PP_PER; ++i) {
     const int s = s0 + i;
-    v[i] = s < p.S && p.done[s] ? min(p.W, pages_of(p.lens[s], p.page)) : 0;
+    const bool done = s < p.S && p.done[s];
+    v[i] = done ? min(p.W, pages_of(p.lens[s], p.page)) : 0;
     if (s < p.S) count[s] = (int)v[i];
+    if (done) p.lens[s] = 0;
   }
   block_scan(v, total, sh);
   const int room = p.capacity - height;
 #pragma unroll
   for (int i = 0; i < PP_PER; ++i)
     if (s0 + i < p.S) at[s0 + i] = (int)min(v[i], (long long)room);
-  __syncthreads();                       // every thread has read the height and its lengths
+  __syncthreads();                       // every thread has read the height
   if (threadIdx.x == 0) {
     *p.n_free = height + (int)min(total, (long long)room);
     if (total > room) atomicCAS(p.status, 0, ERR_BOUNDS);
   }
   const int lane = threadIdx.x & 31;
-  for (int s = threadIdx.x >> 5; s < p.S; s += PP_THREADS / 32) {
+  for (int s = threadIdx.x >> 5; s < p.S; s += PP_THREADS / 32)
     for (int i = lane; i < count[s] && at[s] + i < room; i += 32) p.free_pages[height + at[s] + i] = p.tables[(long)s * p.table_stride + i];
-    if (lane == 0 && p.done[s]) p.lens[s] = 0;
-  }
 }
 
 }  // namespace omni
