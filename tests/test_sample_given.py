@@ -111,6 +111,18 @@ def test_kernel(V, kind, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["normal", "ties", "odd"])
+@pytest.mark.parametrize("V", [3000, 40000, 152064])
+def test_more_kept_by_top_k_than_there_are_pieces(V, kind):
+    filters = [(1.0, 600, 0.9, 0.0), (0.7, 1000, 0.9, 0.01), (1.0, 2047, 0.99, 0.0), (1.3, 2048, 0.5, 0.001), (1.0, 2900, 0.9, 0.0), (0.9, 2950, 1.0, 0.0),
+               (0.05, 1000, 0.999, 0.0)]
+    g = torch.Generator().manual_seed(V)
+    x = rows_of(kind, V, len(filters), g)
+    for dtype in (torch.float32, torch.bfloat16):
+        check(x.to(dtype), filters, "cuda", torch.rand(len(filters), generator=g))
+
+
+@pytest.mark.gpu
 def test_one_value_for_all_rows_and_pitches():
     g = torch.Generator().manual_seed(3)
     for odd in (0, 1, 3, 8):
@@ -119,7 +131,13 @@ def test_one_value_for_all_rows_and_pitches():
         ids, lp = sample_given(x, u, 0.8, 40, 0.9, 0.01)
         full = lambda v, d: torch.full((9,), v, dtype=d, device="cuda")
         want = sample_given(x.contiguous(), u, full(0.8, torch.float32), full(40, torch.int32), full(0.9, torch.float32), full(0.01, torch.float32))
-        assert torch.equal(ids, want[0]) and torch.equal(lp, want[1])
+        assert torch.equal(ids, want[0])
+        # A row's pieces of 256 begin on 16 bytes, so a pitch moves their borders and with them the order of its fp32 sum: either is within `off` of the definition, by what is
+        # counted there.
+        t, p, m = (float(torch.tensor(f)) for f in (0.8, 0.9, 0.01))
+        for r in range(9):
+            i, ref, off = definition(x[r].cpu(), float(u[r]), t, 40, p, m)
+            assert int(ids[r]) == i and close(float(lp[r]), ref, off) and close(float(want[1][r]), ref, off)
         h = store.bfloat16()[:, odd // 2:5000]
         assert torch.equal(sample_given(h, u, 0.8, 40, 0.9, 0.01)[0], sample_given(h.contiguous(), u, 0.8, 40, 0.9, 0.01)[0])
 

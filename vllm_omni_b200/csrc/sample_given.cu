@@ -571,7 +571,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
       }
       const u64 before = block_prefix(mine, all, sh.scan);
       if (tid == 0) {
-        sh.mode = by_k && by_p ? SG_SLOW : SG_WINDOW;
+        sh.mode = SG_WINDOW;
         sh.lo = SG_BINS;
         sh.hi = 0;
       }
@@ -583,7 +583,8 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
         for (int i = 0; i < SG_PER; ++i) {
           if (b < (u64)k_in && b + n[i] >= (u64)k_in) {
             sh.hi = sh.lo = tid * SG_PER + i;
-            if (n[i] > SG_LIST) sh.mode = SG_SLOW;
+            if (by_p) sh.lo = 0;                                          // the list is what top-p chooses from: all of it
+            if ((by_p ? b : 0) + n[i] > SG_LIST) sh.mode = SG_SLOW;
             sh.found[0] = b;                                              // elements before the window
           }
           b += n[i];
@@ -681,7 +682,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
   } else if (mode == SG_WINDOW) {
     // Few of a piece's elements are surely kept: they are pushed together before their weights are computed.  The list's weights are the first block's.  What lies behind
     // the window counts by its fp32 weight.
-    const bool by_both = by_p && min_p > 0.f;                             // S is what min-p leaves: 64-bit weights behind the window, too
+    const bool by_both = by_p && !by_k && min_p > 0.f;                    // S is what min-p leaves: 64-bit weights behind the window, too
     const float front = fmaxf(sh.first[0], bound), inside = fmaxf(sh.first[1], bound), need = by_both ? bound : inside;
     u64 rest = 0;
     float least = INFINITY;
@@ -740,6 +741,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
     if (tid == 0) *at_rank(&sh.whole[rank], 0) = a;
     join_lists(sh, rank);
     cluster_barrier();
+    if (by_k && by_p) mode = SG_TOP;
   }
   if (rank) return;
 
