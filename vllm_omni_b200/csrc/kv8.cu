@@ -335,6 +335,9 @@ kv8_read_kernel(const __grid_constant__ Kv8Read p) {
 // product, w = 2^(s + e_v - m'), whose running maximum m' is apart from the softmax's m: w is at most 2^15 whatever the scales, and the mass that f16
 // cannot hold is below 2^-38 of the largest for each key.  The sum of weights is that of the unrounded fp32 ones.
 // Blocks are persistent, one an SM: a share (a run of keys of a row and of up to eight heads) follows another in the ring without a pause.
+// 64 sequences of 2458 to 4096 keys, 32 heads on 8 of 128 (430 MB) 88 us with the joining of shares, 4.9 TB/s; one of 131071, 64 heads on 8, 53 us, 5.1 TB/s; one of 100 8 us.
+// What is left: a share's beginning and end, some 4000 clocks in which the ring does not run full; shares that do not divide among the SMs; 650 instructions a warp
+// for 32 keys, which keep a scheduler's two warps two thirds busy.
 constexpr int K8_MAX_PARTS = 256, K8_MAX_GROUP = 128, K8_LISTED = 512;
 constexpr float K8_LIFT = 14.f, K8_SLACK = 1.f;     // together below f16's 2^16
 // Warps that compute, and the keys of a stage that each of them takes.  (Sixteen warps of 16 keys: 96 registers, which spill, and more instructions a key.)

@@ -7,7 +7,8 @@
 // A step moves 24 bytes a row, so a call is a launch and the latency of two dependent scans.  One cluster does it all: every block repeats the scans over
 // at most 4096 sequences in its own shared memory (less than a barrier across the grid would take) and then writes its share of the rows, each of which
 // finds its sequence by bisection of the starts.  The lengths and the stack's height may be written in place: a barrier of the cluster lies between the
-// blocks' reads and the first block's writes.
+// blocks' reads and the first block's writes.  One sequence and row 5.3 us, where a launch that does nothing takes 2.4; 256 6.3; 12289 rows 8.2; 4096 sequences of four
+// rows 10.6, released 12.
 #include "host_util.h"
 #include "ptx_sm100.cuh"
 

@@ -18,6 +18,9 @@
 //      sum of 1, off by some 2^-22: the cut may be one element off where top_p S is that near to an element's border.  Without a cut: 64-bit weights of every element once.
 // The first block then sorts the list, finds the cut exactly, the tile that the random number falls into and the element in it.  Rows whose lists would be longer
 // (thousands of equal logits) take histograms over keys, in the end over the indexes of ties, in the first block alone.
+//
+// Bound by instructions: of the 78 MB of 256 bf16 rows of 152064 a pass takes 12 us from memory; the largest alone takes 34 us, no cut 102 (13 fp64 instructions an element), k 50 57, p 0.9
+// 176 (two more passes of some 35 instructions an element, DRAM 5 %, 2.6 instructions a clock).  One row: 5.6 us, 13, 13, 30: steps one after another in one cluster.
 #include <cfloat>
 #include <cuda_bf16.h>
 

@@ -213,7 +213,8 @@ def sample_given(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0
     into ``out``, such a pair, if given.  ``temperature``, ``top_p``, ``min_p`` (fp32 [B]) and ``top_k`` (int32 [B]) are numbers or one value per row.
 
     Weights are exp((x - max) / temperature) as multiples of 2^-44.  In the order by logit (ties: the lower id first) the first ``top_k`` stay (0: all), of these the
-    ones of at least ``min_p`` of the largest, of these all before which less than ``top_p`` of their mass lies, and always the first.  The token is the first kept
+    ones of at least ``min_p`` of the largest, of these all before which less than ``top_p`` of their mass lies, and always the first (of a whole row without the other two
+cuts the mass is a sum in fp32, so that this border is exact to some 2^-22 of it).  The token is the first kept
     id at which the running mass in the order of the ids passes ``u`` times the kept mass.  Its log probability is that of the whole row at the temperature.
     Temperature 0 or below: the largest logit, its log probability at temperature 1.  Logits that are not numbers count as -inf; a row of nothing else
     gives id -1 and log probability -inf.  Does no host work and, with ``out``, no allocation: it can be captured."""
