@@ -1,5 +1,6 @@
 """The 8-bit key/value cache (ops/kv8.py): codes and scales bit for bit against a restatement of the definition in 64 bits, attention against 64 bits over pages whose
 rows past a sequence's end hold NaN, and what is refused."""
+import copy
 import math
 
 import pytest
@@ -411,6 +412,29 @@ def test_more_portions_than_a_launch_takes(H, Hkv, D, page):
         segs.append((at, n, (0, 0, 131, 16)[(i * 5 + i // 4) % 4]))
         at += n + i % 2
     test_portions_against_64_bits("cuda", H, Hkv, D, page, segs[::-1])
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_a_cache_keeps_its_tensors_wherever_they_move(dev):
+    g = torch.Generator().manual_seed(8)
+    c = cache_of(3, 16, 2, 64, dev)
+    k, v = (rows_for(20, 2, 64, g, "normal").to(dev) for _ in range(2))
+    slots = torch.arange(20, dtype=torch.int32, device=dev)
+    kv8.kv8_write(k, v, c, slots)
+    want = kv8.kv8_read(c, slots)
+    with pytest.raises(AttributeError):
+        c.k = torch.zeros_like(c.k)
+    twin = copy.deepcopy(c)
+    kv8.kv8_write(-k, -v, twin, slots)
+    assert all(same(a, b) for a, b in zip(kv8.kv8_read(c, slots), want))
+    assert all(same(a, -b) for a, b in zip(kv8.kv8_read(twin, slots), want))
+    old = [t.data for t in (c.k, c.v, c.k_scale, c.v_scale)]               # other memory behind the same tensors, the old filled with something else
+    for t, o in zip((c.k, c.v, c.k_scale, c.v_scale), old):
+        t.data = o.clone()
+        o.view(torch.uint8).fill_(64)
+    assert all(same(a, b) for a, b in zip(kv8.kv8_read(c, slots), want))
+    with pytest.raises(ValueError):
+        kv8.kv8_write(k[0, 0, 0], v, c, slots)
 
 
 def test_portions_and_heads_that_are_refused():

@@ -54,7 +54,7 @@ class _Fields(ctypes.Structure):      # Kv8Cache of csrc/kv8.cu
 
 class Kv8Cache:
     """``k``, ``v``: float8_e4m3fn [pages, page size, Hkv, D]; ``k_scale``, ``v_scale``: fp32 powers of two [pages, Hkv]."""
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "block_size", "heads", "head_size", "device", "_fields", "_at")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "block_size", "heads", "head_size", "device", "_fields", "_address")
 
     def __init__(self, k, v, k_scale, v_scale):
         if k.dim() != 4 or any(t.dtype is not CODES or t.shape != k.shape or not t.is_contiguous() or t.device != k.device for t in (k, v)):
@@ -71,9 +71,22 @@ class Kv8Cache:
         if k.is_cuda and (k.data_ptr() | v.data_ptr()) & 15:
             raise ValueError("k and v must begin on 16 bytes")
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
-        if k.is_cuda:                                    # what the kernels take of it, once
-            self._fields = _Fields(*(t.data_ptr() for t in (k, v, k_scale, v_scale, nv.status_word(k.device))), *k.shape)
-            self._at = ctypes.addressof(self._fields)
+        self._fields = _Fields(0, 0, 0, 0, nv.status_word(k.device).data_ptr() if k.is_cuda else 0, *k.shape)
+        self._address = ctypes.addressof(self._fields)       # the last: nothing can be set from here on
+
+    def __setattr__(self, name, value):
+        if hasattr(self, "_address"):
+            raise AttributeError(f"{name}: a cache keeps its tensors")
+        object.__setattr__(self, name, value)
+
+    def __reduce__(self):                                    # copies and pickles
+        return Kv8Cache, (self.k, self.v, self.k_scale, self.v_scale)
+
+    def _at(self) -> int:
+        """Address of what the kernels take of it; the tensors' own addresses as they are now."""
+        f = self._fields
+        f.k, f.v, f.k_scale, f.v_scale = self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
+        return self._address
 
     @classmethod
     def empty(cls, pages: int, block_size: int, heads: int, head_size: int, device) -> "Kv8Cache":
@@ -112,7 +125,7 @@ def _stream(device):
 
 def kv8_write(k, v, cache: Kv8Cache, slots) -> None:
     """k, v: bf16 [T, Hkv, D]; slots int32 [T] (page * page size + row, below zero: not written)."""
-    T = k.shape[0]
+    T = slots.numel()
     shape = (T, cache.heads, cache.head_size)
     _check_rows("k", k, shape, cache.device)
     _check_rows("v", v, shape, cache.device)
@@ -126,7 +139,7 @@ def kv8_write(k, v, cache: Kv8Cache, slots) -> None:
             return kv8_write(k, v, cache, slots)
     k, v = _readable(k), _readable(v)
     ks, vs = k.stride(), v.stride()
-    nv.check_rc(_lib().omni_kv8_write(cache._at, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), T, _stream(cache.device)), "omni_kv8_write")
+    nv.check_rc(_lib().omni_kv8_write(cache._at(), k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), T, _stream(cache.device)), "omni_kv8_write")
 
 
 def _out_pair(cache, rows, out_k, out_v):
@@ -143,7 +156,7 @@ def _out_pair(cache, rows, out_k, out_v):
 
 
 def _read(cache, n, index, row0, rows, tables, k, v):
-    nv.check_rc(_lib().omni_kv8_read(cache._at, n, (_P * n)(*index), (_L * n)(*row0), (_L * n)(*rows), tables, k.data_ptr(), v.data_ptr(), _stream(cache.device)),
+    nv.check_rc(_lib().omni_kv8_read(cache._at(), n, (_P * n)(*index), (_L * n)(*row0), (_L * n)(*rows), tables, k.data_ptr(), v.data_ptr(), _stream(cache.device)),
                 "omni_kv8_read")
 
 
@@ -215,7 +228,7 @@ def kv8_decode(q, cache: Kv8Cache, block_tables, lens, row_seq=None, scale=None,
     part = cache.k_scale.new_empty(R * H * shares * (D + 1)) if shares > 1 else None
     qs, outs = q.stride(), out.stride()
     nv.check_rc(_lib().omni_kv8_attn(
-        cache._at, q.data_ptr(), qs[0], qs[1], block_tables.data_ptr(), block_tables.stride(0), lens.data_ptr(), row_seq.data_ptr() if mapped else None, R, S, H,
+        cache._at(), q.data_ptr(), qs[0], qs[1], block_tables.data_ptr(), block_tables.stride(0), lens.data_ptr(), row_seq.data_ptr() if mapped else None, R, S, H,
         max_keys, scale, shares, None if part is None else part.data_ptr(), out.data_ptr(), outs[0], outs[1], _stream(cache.device)), "omni_kv8_attn")
     if part is not None:
         nv.count_launches(1)
