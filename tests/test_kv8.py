@@ -415,6 +415,42 @@ def test_more_portions_than_a_launch_takes(H, Hkv, D, page):
 
 
 @pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("H,Hkv,D", [(8, 2, 128), (4, 4, 64), (8, 1, 64), (16, 1, 128), (6, 3, 128)])
+def test_what_is_not_a_number_is_its_own_rows(H, Hkv, D, dev):
+    """Rows of a sequence that see different numbers of keys: a key or value that is not a number reaches those that see it, and leaves the others the same bits."""
+    g = torch.Generator().manual_seed(H + D)
+    n, per, page = 130, 5, 16
+    q = torch.randn(2 * per, H, D, generator=g).to(BF).to(dev)
+    lens = torch.tensor([n - per + 1 + i for i in range(per)] * 2, dtype=torch.int32, device=dev)
+    seq = torch.arange(2, dtype=torch.int32, device=dev).repeat_interleave(per)
+    tables = torch.arange(18, dtype=torch.int32, device=dev).view(2, 9)
+    slots = torch.cat([torch.arange(n), torch.arange(n) + 144]).to(torch.int32).to(dev)
+    k, v = (rows_for(2 * n, Hkv, D, g, "normal") for _ in range(2))
+    for what in range(3):
+        x, y = k.clone(), v.clone()
+        if what == 1:
+            y[n - 2, 0, D // 2 + 3] = math.nan                         # seen by the first sequence's last two rows
+        elif what == 2:
+            x[n - 1, Hkv - 1, 5] = math.nan                            # by its last one
+            y[2 * n - 3, Hkv - 1, 1] = math.nan                        # by the second one's last three
+        c = cache_of(18, page, Hkv, D, dev)
+        kv8.kv8_write(x.to(dev), y.to(dev), c, slots)
+        out = kv8.kv8_decode(q, c, tables, lens, row_seq=seq).view(2, per, Hkv, H // Hkv, D).cpu()
+        if what == 0:
+            want = out
+            assert bool(out.isfinite().all())
+            continue
+        odd = torch.zeros_like(out, dtype=torch.bool)
+        if what == 1:
+            odd[0, -2:, 0, :, D // 2 + 3] = True
+        else:
+            odd[0, -1:, -1] = True
+            odd[1, -3:, -1, :, 1] = True
+        assert torch.equal(out.isnan(), odd)
+        assert same(torch.where(odd, 0, out), torch.where(odd, 0, want))
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 def test_a_cache_keeps_its_tensors_wherever_they_move(dev):
     g = torch.Generator().manual_seed(8)
     c = cache_of(3, 16, 2, 64, dev)

@@ -430,8 +430,8 @@ __device__ __forceinline__ int kv8_page(const Kv8Attn& p, int pg) {
   return 0;
 }
 
-// UP: more than 8 rows of the products are live.
-template <int D, bool UP>
+// UP: more than 8 rows of the products are live.  MANY: they may be of several rows of queries.
+template <int D, bool UP, bool MANY>
 __global__ void __launch_bounds__(32 * (K8_WARPS + 1), 1)
 kv8_attn_kernel(const __grid_constant__ Kv8Attn p) {
   extern __shared__ __align__(1024) unsigned char ring[];
@@ -779,6 +779,45 @@ kv8_attn_kernel(const __grid_constant__ Kv8Attn p) {
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 if (key + h * 16 + (i >> 1) * 8 + 2 * j + (i & 1) >= a.to) vr[i] = make_uint4(0u, 0u, 0u, 0u);
+            // Nor is what some rows do not see theirs: a product apart counts what is not a number for those that do.  (Code that others do not need would cost them
+            // registers: 64 on 4 heads 85 -> 91 us.)
+            if (MANY && ends && least < a.to) {
+              auto odd_of = [](uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); };
+              uint32_t odd = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) odd |= odd_of(vr[i].x) | odd_of(vr[i].y) | (D == 128 ? odd_of(vr[i].z) | odd_of(vr[i].w) : 0u);
+              if (__any_sync(0xffffffffu, odd)) {
+                uint4 one[4];                      // codes of 1
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  one[i] = make_uint4(odd_of(vr[i].x), odd_of(vr[i].y), D == 128 ? odd_of(vr[i].z) : 0u, D == 128 ? odd_of(vr[i].w) : 0u);
+                  vr[i] = make_uint4(vr[i].x & ~one[i].x, vr[i].y & ~one[i].y, vr[i].z & ~one[i].z, vr[i].w & ~one[i].w);
+                  one[i] = make_uint4(one[i].x & 0x38383838u, one[i].y & 0x38383838u, one[i].z & 0x38383838u, one[i].w & 0x38383838u);
+                }
+#pragma unroll
+                for (int u = 0; u < NH; ++u) {
+                  uint32_t sees[2];
+#pragma unroll
+                  for (int n = 0; n < 2; ++n) {
+                    const int at = key + (2 * h + n) * 8 + 2 * j;
+                    sees[n] = pack_half(at < len[u] ? 1.f : 0.f, at + 1 < len[u] ? 1.f : 0.f);
+                  }
+#pragma unroll
+                  for (int w = 0; w < MT / 2; ++w) {
+                    auto word = [&](const uint4& x) { return w == 0 ? x.x : (w == 1 ? x.y : (w == 2 ? x.z : x.w)); };
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                      const uint32_t x = __byte_perm(word(one[0]), word(one[1]), i ? 0x7362 : 0x5140), y = __byte_perm(word(one[2]), word(one[3]), i ? 0x7362 : 0x5140);
+                      float n[4] = {};
+                      mma_f16_16x8(n, halves_of(x), halves_of_hi(x), halves_of(y), halves_of_hi(y), sees[0], sees[1]);
+#pragma unroll
+                      for (int k = 0; k < 4; ++k)
+                        if (n[k] != 0.f) acc[u][2 * w + i][k] = NAN;
+                    }
+                  }
+                }
+              }
+            }
 #pragma unroll
             for (int w = 0; w < MT / 2; ++w) {
               auto word = [&](const uint4& x) { return w == 0 ? x.x : (w == 1 ? x.y : (w == 2 ? x.z : x.w)); };
@@ -933,8 +972,8 @@ kv8_merge_kernel(const float* part_o, const float* part_lse, const int* lens, in
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
   for (int i = 0; i < K8_MAX_PARTS / 32; ++i) {
-    w[i] = w[i] == -INFINITY ? 0.f : ex2_approx(w[i] - top);
-    den += w[i];
+    w[i] = w[i] == -INFINITY ? -1.f : ex2_approx(w[i] - top);             // below zero: a share without keys, which has written no sum
+    den += w[i] < 0.f ? 0.f : w[i];
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
@@ -947,7 +986,7 @@ kv8_merge_kernel(const float* part_o, const float* part_lse, const int* lens, in
     for (int h = 0; h < 2; ++h) {
       const int s = i * 32 + h * WARPS + warp;
       const float ws = __shfl_sync(0xffffffffu, w[i], h * WARPS + warp);
-      if (ws != 0.f) {                             // a share without keys has written no sum
+      if (!(ws < 0.f)) {
         float x[PER];
         if (PER == 4) {
           const float4 y = *reinterpret_cast<const float4*>(po + (long)s * D);
@@ -991,15 +1030,15 @@ kv8_merge_few_kernel(const float* part_o, const float* part_lse, const int* lens
   float w = lane < parts ? part_lse[r * splits + lane] : -INFINITY, top = w;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  w = w == -INFINITY ? 0.f : ex2_approx(w - top);
-  float den = w, acc[PER] = {};
+  w = w == -INFINITY ? -1.f : ex2_approx(w - top);                         // below zero: a share without keys, which has written no sum
+  float den = w < 0.f ? 0.f : w, acc[PER] = {};
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
   const float* po = part_o + r * splits * D + lane * PER;
 #pragma unroll 4
   for (int s = 0; s < parts; ++s) {
     const float ws = __shfl_sync(0xffffffffu, w, s);
-    if (ws != 0.f) {                               // a share without keys has written no sum
+    if (!(ws < 0.f)) {
       float x[PER];
       if (PER == 4) {
         const float4 y = *reinterpret_cast<const float4*>(po + (long)s * D);
@@ -1147,12 +1186,12 @@ extern "C" int omni_kv8_attn_shares(int R, int S, int H, int Hkv, int D, int map
   return d.splits;
 }
 
-template <int D, bool UP>
+template <int D, bool UP, bool MANY>
 static int launch_kv8_attn(const Kv8Attn& p, int grid, cudaStream_t st) {
   static unsigned long long ready = 0;
   constexpr int warps = K8_WARPS, ring = 96 * 2 * warps * D, q = warps * (UP ? 2 : 1) * D * 16;       // a stage; queries
-  if (int e = ensure_dynamic_smem((const void*)kv8_attn_kernel<D, UP>, ring + q, ready)) return e;
-  launch_overlapped(kv8_attn_kernel<D, UP>, grid, 32 * (warps + 1), ring + q, st, p);
+  if (int e = ensure_dynamic_smem((const void*)kv8_attn_kernel<D, UP, MANY>, ring + q, ready)) return e;
+  launch_overlapped(kv8_attn_kernel<D, UP, MANY>, grid, 32 * (warps + 1), ring + q, st, p);
   return (int)cudaGetLastError();
 }
 
@@ -1178,8 +1217,10 @@ extern "C" int omni_kv8_attn(const Kv8Cache* cache, const void* q, long q_rs, lo
   p.row_blocks = (R + d.pack - 1) / d.pack; p.listed = d.splits > 1 && p.row_blocks <= K8_LISTED && (long)p.row_blocks * d.groups * d.splits > d.grid;
   p.scale_log2 = scale * 1.4426950408889634f; p.part_o = part; p.part_lse = part_lse; p.out = (__nv_bfloat16*)out; p.o_rs = o_rs; p.o_hs = o_hs; p.status = c.status;
   cudaStream_t st = (cudaStream_t)stream;
-  if (int e = D == 64 ? (d.up ? launch_kv8_attn<64, true>(p, d.grid, st) : launch_kv8_attn<64, false>(p, d.grid, st))
-                      : (d.up ? launch_kv8_attn<128, true>(p, d.grid, st) : launch_kv8_attn<128, false>(p, d.grid, st)))
+  const auto launch = d.pack > 1 ? (D == 64 ? launch_kv8_attn<64, true, true> : launch_kv8_attn<128, true, true>)      // 16 / G rows of G heads: more than 8
+                      : d.up     ? (D == 64 ? launch_kv8_attn<64, true, false> : launch_kv8_attn<128, true, false>)
+                                 : (D == 64 ? launch_kv8_attn<64, false, false> : launch_kv8_attn<128, false, false>);
+  if (int e = launch(p, d.grid, st))
     return e;
   if (shares == 1) return RC_OK;
   const bool few = d.splits <= 32 && (long)R * H >= 1024;

@@ -239,7 +239,8 @@ def kv8_prefill(q, cache: Kv8Cache, segs, scale=None, out=None):
     """Causal attention of the prompt portions of a step to the cache, into which their keys and values are written already.
 
     q bf16 [T, H, D]; ``segs``: (first row, rows, context, block table int32 [columns]) each, as in ``kv_cache.prefill_segments``: row i of a portion sees
-    context + i + 1 keys.  Rows of no portion stay as they are in ``out``."""
+    context + i + 1 keys.  Rows of no portion stay as they are in ``out``.  A value that is not a number may reach rows of its portion that do not see it, as in the
+    attention to bf16 pages (not those of ``kv8_decode``)."""
     _check_queries(q, cache, out)
     T, H, D = q.shape
     segs = [s for s in segs if s[1] > 0]
