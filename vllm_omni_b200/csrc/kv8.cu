@@ -335,7 +335,7 @@ kv8_read_kernel(const __grid_constant__ Kv8Read p) {
 // product, w = 2^(s + e_v - m'), whose running maximum m' is apart from the softmax's m: w is at most 2^15 whatever the scales, and the mass that f16
 // cannot hold is below 2^-38 of the largest for each key.  The sum of weights is that of the unrounded fp32 ones.
 // Blocks are persistent, one an SM: a share (a run of keys of a row and of up to eight heads) follows another in the ring without a pause.
-// 64 sequences of 2458 to 4096 keys, 32 heads on 8 of 128 (430 MB) 88 us with the joining of shares, 4.9 TB/s; one of 131071, 64 heads on 8, 53 us, 5.1 TB/s; one of 100 8 us.
+// 64 sequences of 2458 to 4096 keys, 32 heads on 8 of 128 (430 MB) 88 us with the joining of shares, 4.9 TB/s; one of 131071, 64 heads on 8, 51 us, 5.3 TB/s; one of 100 6 us.
 // What is left: a share's beginning and end, some 4000 clocks in which the ring does not run full; shares that do not divide among the SMs; 650 instructions a warp
 // for 32 keys, which keep a scheduler's two warps two thirds busy.
 constexpr int K8_MAX_PARTS = 256, K8_MAX_GROUP = 128, K8_LISTED = 512;
@@ -1071,34 +1071,41 @@ static bool kv8_deal(int R, int S, int H, int Hkv, int D, bool mapped, int page,
   d.pack = mapped && R > S && G <= 8 ? 16 / G : 1;
   d.chunks = (G + 15) / 16;
   d.up = (d.chunks > 1 ? 16 : G) * d.pack > 8;
-  const int warps = K8_WARPS, most = warps / d.chunks;
-  d.groups = (Hkv + most - 1) / most;
-  d.heads = (Hkv + d.groups - 1) / d.groups;
-  d.subs = 1;
-  while (d.subs * 2 * d.heads * d.chunks <= warps) d.subs *= 2;
-  const int keys = d.subs * k8_keys(D, d.up);      // at most 256: 32 copies of eight rows
-  d.unit = page % 32 == 0 && keys % 32 == 0 ? 32 : (page % 16 == 0 ? 16 : 8);
-  const long blocks = (long)((R + d.pack - 1) / d.pack) * d.groups;
-  const int sms = sm_count();
-  // The number of shares.  Few rows: rounds of blocks times a share's keys and what it costs beside them (its queries and the way of its sums, some 64 keys' time).
-  // Many: blocks take the shares there are in turn; a row is taken to have four fifths of the table's keys.
-  double best = 1e30;
-  d.splits = 1;
   if (splits < 0 || splits > K8_MAX_PARTS) return false;
-  const int stages = (max_keys + keys - 1) / keys;
-  for (int n = splits ? splits : 1; n <= (splits ? splits : K8_MAX_PARTS) && n <= stages; ++n) {
-    const int share = (stages + n - 1) / n * keys;
-    if ((max_keys + share - 1) / share != n) continue;
-    const double items = R > d.pack ? blocks * (0.8 * max_keys / share + 0.5) : (double)blocks * n, rounds = (double)((long)(items / sms) + 1);
-    const double cost = (items == (rounds - 1.0) * sms ? rounds - 1.0 : rounds) * (share + 64) + 0.25 * n;
-    if (cost < best) {
-      best = cost;
-      d.splits = n;
-      d.share = share;
+  const int warps = K8_WARPS, sms = sm_count(), fewest = (Hkv + warps / d.chunks - 1) / (warps / d.chunks);
+  const long row_blocks = (R + d.pack - 1) / d.pack;
+  // The heads of a block and the number of shares.  Few rows: rounds of blocks times the stages of a share and what it costs beside them (its queries and the way of its sums, some
+  // two stages' time), and as much once more where shares are joined.  Many: blocks take the shares there are in turn; a row is taken to have four fifths of the table's keys.
+  // Blocks of fewer heads, whose warps share the keys of one, are for calls that leave SMs without a block: a copy brings fewer bytes there.  32 heads on 8 of 128, 112 keys: 5.9 us
+  // by a head a block, 7.9 by four shares of all heads; 640 keys 9.6 and, of 20 shares, 8.5, with a launch more; one of 131071 keys, 64 heads, 51 in 37 shares, 53 in 147.
+  double best = 1e30;
+  d.splits = 0;
+  for (int heads = (Hkv + fewest - 1) / fewest;; heads = (heads + 1) / 2) {
+    Kv8Deal t = d;
+    t.heads = heads;
+    t.groups = (Hkv + heads - 1) / heads;
+    t.subs = 1;
+    while (t.subs * 2 * t.heads * t.chunks <= warps) t.subs *= 2;
+    const int keys = t.subs * k8_keys(D, t.up), stages = (max_keys + keys - 1) / keys;       // at most 256: 32 copies of eight rows
+    t.unit = page % 32 == 0 && keys % 32 == 0 ? 32 : (page % 16 == 0 ? 16 : 8);
+    const long blocks = row_blocks * t.groups;
+    for (int n = splits ? splits : 1; n <= (splits ? splits : K8_MAX_PARTS) && n <= stages; ++n) {
+      if (t.groups > fewest && blocks * n > sms) break;
+      const int share = (stages + n - 1) / n * keys;
+      if ((max_keys + share - 1) / share != n) continue;
+      const double items = R > d.pack ? blocks * (0.8 * max_keys / share + 0.5) : (double)blocks * n, rounds = (double)((long)(items / sms) + 1);
+      const double cost = (items == (rounds - 1.0) * sms ? rounds - 1.0 : rounds) * (share / keys + 2) + (n > 1 ? 2 + 0.008 * n : 0.0);
+      if (cost < best) {
+        best = cost;
+        t.splits = n;
+        t.share = share;
+        d = t;
+      }
     }
+    if (heads == 1) break;
   }
-  if (d.splits == 1) d.share = stages * keys;
-  if (splits && d.splits != splits) return false;
+  if (d.splits < 1) return false;
+  const long blocks = row_blocks * d.groups;
   if (blocks * d.splits > 0x7fffffffL) return false;
   d.grid = blocks * d.splits < sms ? (int)(blocks * d.splits) : sms;
   return true;
