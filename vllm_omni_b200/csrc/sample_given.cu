@@ -88,9 +88,12 @@ __device__ __forceinline__ T* at_rank(T* p, uint32_t rank) {            // the s
   asm("mapa.u64 %0, %1, %2;" : "=l"(out) : "l"(reinterpret_cast<u64>(p)), "r"(rank));
   return reinterpret_cast<T*>(out);
 }
-// Barrier of the cluster, for warps whose threads may have left a loop at different times.
+// Barrier of the cluster, for warps whose threads may have left a loop at different times; its halves.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 
 // Sum over the warp of values below 2^59: three additions of 22 bits each.
@@ -341,6 +344,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
   }
   if (tid < 64) sh.table[tid] = exp2((double)tid * (1.0 / 64)) * SG_ONE;
   if (tid == 0) sh.n_list = 0;
+  cluster_arrive();                                     // this block has started: its shared memory may be written
   const T* x0 = reinterpret_cast<const T*>(p.logits) + (long)row * p.ld;
   const int off = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
   const int vecs = (V + off + 7) / 8, tiles = (vecs + SG_THREADS - 1) / SG_THREADS, per = (tiles + nc - 1) / nc, pieces = tiles * SG_WARPS;
@@ -362,6 +366,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
 
   // 1.  The next tile's elements are on their way while this one's are worked on.
   const bool need_sum = (int)greedy + (int)by_k + (int)by_p > 0;         // as `||` of the three it came out false for top-p alone (nvcc 12.9)
+  cluster_wait();                                       // and so have the others, while the first tiles were on their way
 #pragma unroll 1
   for (int t = tile0; t < tile1; ++t) {
     float x[8];
