@@ -1,0 +1,80 @@
+"""Top-p next to its border (ops/sampler.sample_given): the element that decides lies last in the vocabulary, and the random number is the largest below 1, so the
+token says whether it stays.  Probabilities are the fp32 numbers around the border: steps of some 2^-24 of the mass."""
+import numpy as np
+import pytest
+import torch
+
+from vllm_omni_b200.ops.sampler import sample_given
+
+LAST = 1 - 2.0 ** -24
+
+
+def rows_of(kind, V, B, g):
+    x = {"flat": 0.3, "normal": 1.0, "wide": 4.0, "steep": 12.0}[kind] * torch.randn(B, V, generator=g)
+    x[torch.rand(B, V, generator=g) < 0.05] = -float("inf")
+    return x
+
+
+def borders(x, t, share):
+    """For each row: its last element becomes the neighbour of the border at `share` of the mass; fp32 probabilities around that border, and what the definition keeps."""
+    ps, ids, t = [], [], float(np.float32(t))                          # as the call takes it
+    for r in range(x.shape[0]):
+        row = x[r].double()
+        order = np.lexsort((np.arange(row.numel()), -row.numpy()))
+        z = np.exp((row.numpy() - row.max().item()) / t)[order]
+        at = int((np.cumsum(z) < share * z.sum()).sum())
+        x[r, -1] = x[r, order[max(at, 1)]]                             # ties with an earlier one: the last index is behind it
+        row = x[r].double().numpy()
+        order = np.lexsort((np.arange(row.size), -row))
+        w = np.round(np.exp((row[order] - row.max()) / t) * 2.0 ** 44)
+        before = np.cumsum(w) - w
+        place = int((order == row.size - 1).nonzero()[0][0])
+        middle = np.float32(before[place] / w.sum())
+        for step in range(-3, 4):
+            p = middle
+            for _ in range(abs(step)):
+                p = np.nextafter(p, np.float32(2.0 if step > 0 else -1.0))
+            kept = (before < float(p) * w.sum()) | (np.arange(row.size) == 0)
+            mass = np.zeros(row.size)
+            mass[order[kept]] = w[kept]
+            run = np.cumsum(mass)
+            ps.append(float(p))
+            ids.append(int((run <= LAST * run[-1]).sum()))
+    return torch.tensor(ps, dtype=torch.float32), ids
+
+
+def check(kind, V, B, dtype, t, share, odd, dev):
+    g = torch.Generator().manual_seed(V + len(kind))
+    x = rows_of(kind, V, B, g).to(dtype)
+    p, want = borders(x, t, share)
+    store = torch.zeros(B, V + odd, dtype=dtype, device=dev)
+    store[:, :V] = x.to(dev)
+    rows = torch.arange(B, device=dev).repeat_interleave(7)
+    u = torch.full((7 * B,), LAST, device=dev)
+    got = []
+    for step in range(7):                                              # the same pitch for every draw
+        got.append(sample_given(store[:, :V], u[:B], t, 0, p[step::7].to(dev).contiguous())[0].cpu())
+    got = torch.stack(got, 1).flatten().tolist()
+    assert rows.numel() == len(want)
+    assert got == want
+    assert 0 < sum(i == V - 1 for i in want) < len(want)               # some probabilities keep the element, some do not
+
+
+@pytest.mark.parametrize("kind", ["flat", "normal", "wide", "steep"])
+def test_restatement(kind):
+    check(kind, 3000, 4, torch.float32, 1.0, 0.9, 0, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["flat", "normal", "wide", "steep"])
+@pytest.mark.parametrize("V,t,share", [(40000, 1.0, 0.9), (152064, 1.3, 0.95), (10007, 0.5, 0.3)])
+def test_kernel(kind, V, t, share):
+    for odd in (0, 1, 3, 8):
+        check(kind, V, 6, torch.float32, t, share, odd, "cuda")
+    check(kind, V, 6, torch.bfloat16, t, share, 1, "cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [1, 40, 300])
+def test_kernel_with_more_and_fewer_blocks_a_row(B):
+    check("normal", 33000, B, torch.float32, 1.0, 0.9, 1, "cuda")

@@ -1,4 +1,5 @@
-// Tokens drawn from given random numbers: temperature, top-k, min-p and top-p over rows of logits, exactly.
+// Tokens drawn from given random numbers: temperature, top-k, min-p and top-p over rows of logits.  The token is exactly the definition's; its log probability
+// has the row's sum of weights in fp32, but for rows whose mass is summed in whole numbers for the token (no cut; top-p alone).
 //
 // For a row x with maximum m and temperature T, weights are whole numbers w_i = round(2^44 exp((x_i - m) / T)), so that sums of them have no order: blocks,
 // threads and lists may add them as they come, and the plain definition in 64 bits gives the same token.  The order of a row is (x down, index up).  A cut is the
@@ -14,13 +15,15 @@
 //      top-p's cut, since all such elements together are no more than what top-p drops.  Pieces whose maximum is below the bound are not read again.
 //   2  top-k: what reaches the bound is a list.  top-p: a histogram of it, 2048 bins of (m - x) / T, 1/64 wide, with what a bin's mass needs beside its count (the sum of
 //      positions in the bin: a chord through exp is off by at most 2^-15).
-//   3  top-p: 64-bit weights of what is surely kept, as sums per piece, and a list of the few bins that the cut can lie in.  Where something lies behind them S is the
-//      sum of 1, off by some 2^-22: the cut may be one element off where top_p S is that near to an element's border.  Without a cut: 64-bit weights of every element once.
+//   3  top-p: 64-bit weights of what is surely kept, as sums per piece, a list of the few bins that the cut can lie in, and 64-bit weights of what lies behind them: the border at
+//      top_p S is compared with masses that differ by one element's, in flat rows a few millionths of S, and a sum in fp32 may be off by as much (2^-19 for
+//      a sum of such depth).  Without a cut: 64-bit weights of every element once.
 // The first block then sorts the list, finds the cut exactly, the tile that the random number falls into and the element in it.  Rows whose lists would be longer
 // (thousands of equal logits) take histograms over keys, in the end over the indexes of ties, in the first block alone.
 //
-// Bound by instructions: of the 78 MB of 256 bf16 rows of 152064 a pass takes 12 us from memory; the largest alone takes 34 us, no cut 102 (13 fp64 instructions an element), k 50 57, p 0.9
-// 176 (two more passes of some 35 instructions an element, DRAM 5 %, 2.6 instructions a clock).  One row: 5.6 us, 13, 13, 30: steps one after another in one cluster.
+// Bound by instructions: of the 78 MB of 256 bf16 rows of 152064 a pass takes 12 us from memory; the largest alone takes 34 us, no cut 101 (13 fp64 instructions an element), k 50 58, p 0.9
+// 206 (two more passes of some 35 instructions an element, 13 fp64 ones among those of the last; with S in fp32 it took 176).  One row: 5.6 us, 13, 12, 31: steps one after another
+// in one cluster.
 #include <cfloat>
 #include <cuda_bf16.h>
 
@@ -666,6 +669,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
   }
 
   // 3
+  const bool whole_row = by_p && !by_k && !(min_p > 0.f);                 // S is the mass of the row
   if (mode == SG_ALL) {
     u64 whole = 0;
 #pragma unroll 1
@@ -688,18 +692,17 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
     if (tid == 0) *at_rank(&sh.whole[rank], 0) = a;
     cluster_barrier();
   } else if (mode == SG_WINDOW) {
-    // Few of a piece's elements are surely kept: they are pushed together before their weights are computed.  The list's weights are the first block's.  What lies behind
-    // the window counts by its fp32 weight.
-    const bool by_both = by_p && !by_k && min_p > 0.f;                    // S is what min-p leaves: 64-bit weights behind the window, too
+    // 64-bit weights of what is in front of the window and, for top-p's mass S, of what lies behind it: down to min-p's bound, or of the whole row.  The list's are the first block's.
+    // Where few of a piece's elements count they are pushed together before their weights are computed.
+    const bool by_both = by_p && !by_k && !whole_row;                     // S is what min-p leaves
     const float front = fmaxf(sh.first[0], bound), inside = fmaxf(sh.first[1], bound), need = by_both ? bound : inside;
     u64 rest = 0;
-    float least = INFINITY;
     float* q = sh.queue[warp];
 #pragma unroll 1
     for (int t = tile0; t < tile1; ++t) {
       const float top = piece_top(t);
       u64 sure = 0;
-      if (top >= need) {
+      if (whole_row ? !(r.place(top) >= (float)SG_BINS) : top >= need) {  // beyond the range there is no mass
         float x[8];
         raw8(load8(x0, off, V, t * SG_THREADS + tid), x);
         unsigned listed = 0, mine = 0;
@@ -707,45 +710,51 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
         for (int j = 0; j < 8; ++j) {
           mine |= (unsigned)(x[j] >= front) << j;
           listed |= (unsigned)(x[j] >= inside) << j;
-          least = fminf(least, x[j]);
         }
         listed &= ~mine;
         append(sh, listed, x, (t * SG_THREADS + tid) * 8 - off);
-        if (by_both) {
+        if (whole_row) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) mine |= (unsigned)(x[j] >= bound && x[j] < inside) << j;
-        }
-        if (__any_sync(0xffffffffu, mine)) {
-          const int has = __popc(mine);
-          int run = has;
-#pragma unroll
-          for (int o = 1; o < 32; o *= 2) {
-            const int up = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += up;
+          for (int j = 0; j < 8; ++j) {
+            const u64 w = SgRow::rounded(r.weight(x[j]));                 // not a number: 0
+            if (x[j] >= front) sure += w;
+            else if (!(listed >> j & 1)) rest += w;
           }
-          const int n = __shfl_sync(0xffffffffu, run, 31);
-          float* to = q + run - has;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (mine >> j & 1) *to++ = x[j];
-          __syncwarp();
-#pragma unroll 1
-          for (int i = lane; i < n; i += 32) {
-            const u64 w = r.kept(q[i]);
-            if (q[i] >= front) sure += w;
-            else rest += w;
-          }
-          __syncwarp();
           sure = warp_sum(sure);
+        } else {
+          if (by_both) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mine |= (unsigned)(x[j] >= bound && x[j] < inside) << j;
+          }
+          if (__any_sync(0xffffffffu, mine)) {
+            const int has = __popc(mine);
+            int run = has;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+              const int up = __shfl_up_sync(0xffffffffu, run, o);
+              if (lane >= o) run += up;
+            }
+            const int n = __shfl_sync(0xffffffffu, run, 31);
+            float* to = q + run - has;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (mine >> j & 1) *to++ = x[j];
+            __syncwarp();
+#pragma unroll 1
+            for (int i = lane; i < n; i += 32) {
+              const u64 w = r.kept(q[i]);
+              if (q[i] >= front) sure += w;
+              else rest += w;
+            }
+            __syncwarp();
+            sure = warp_sum(sure);
+          }
         }
-      } else {
-        least = -INFINITY;
       }
       if (lane == 0) *at_rank(&sh.tile[t * SG_WARPS + warp], 0) = sure;
     }
-    const bool behind = least < inside;
     u64 a;
-    block_prefix(by_both ? rest : (u64)behind, a, sh.scan);
+    block_prefix(rest, a, sh.scan);
     if (tid == 0) *at_rank(&sh.whole[rank], 0) = a;
     join_lists(sh, rank);
     cluster_barrier();
@@ -856,10 +865,8 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
       mine += w;
     }
     u64 before = block_prefix(mine, listed, sh.scan);
-    // S: 64-bit weights alone where nothing lies behind the window, and with min-p; else the sum of 1, which is off by some 2^-22 of itself
     const u64 behind = whole;
-    whole = sure + listed + (min_p > 0.f ? behind : 0);
-    if (behind && !(min_p > 0.f)) whole = max(whole, (u64)(approx * SG_ONE));
+    whole = sure + listed + behind;
     const double limit = (double)top_p * (double)whole;
     const u64 front = by_k ? sh.found[0] : 0;
     // The last one that stays.
@@ -973,7 +980,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
     if (passed) {
       if (lane == __ffs(passed) - 1) {
         p.ids[row] = i;
-        if (p.logprob) p.logprob[row] = (float)(r.scaled(x) - log(mode == SG_WINDOW ? approx : (double)whole * (1.0 / SG_ONE)));
+        if (p.logprob) p.logprob[row] = (float)(r.scaled(x) - log(mode == SG_WINDOW && !whole_row ? approx : (double)whole * (1.0 / SG_ONE)));
       }
       break;
     }

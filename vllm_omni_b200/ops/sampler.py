@@ -1,6 +1,6 @@
 """K16 — batched token sampling on the device (csrc/sampler.cu) with a PyTorch restatement
 for CPU runs.  ``sample`` takes one ``RowParams`` per sequence.  ``sample_given`` (csrc/sample_given.cu) takes parameters and random numbers that are on the
-device, and cuts exactly: ties go to the lowest id, and neither threads nor blocks decide the order of a sum."""
+device, and gives exactly the token of its definition: ties go to the lowest id, and masses are sums of whole numbers, which have no order."""
 from __future__ import annotations
 
 import ctypes
@@ -188,7 +188,7 @@ def sample(logits: torch.Tensor, rows: list[RowParams]):
     return out, lp
 
 
-MAX_VOCAB = 262144                    # csrc/sample_given.cu: a row stays in the shared memory of eight blocks
+MAX_VOCAB = 262144                    # csrc/sample_given.cu: maxima and sums of a row's pieces of 256 lie in every block's shared memory
 
 
 @functools.lru_cache(maxsize=None)
@@ -213,9 +213,9 @@ def sample_given(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0
     into ``out``, such a pair, if given.  ``temperature``, ``top_p``, ``min_p`` (fp32 [B]) and ``top_k`` (int32 [B]) are numbers or one value per row.
 
     Weights are exp((x - max) / temperature) as multiples of 2^-44.  In the order by logit (ties: the lower id first) the first ``top_k`` stay (0: all), of these the
-    ones of at least ``min_p`` of the largest, of these all before which less than ``top_p`` of their mass lies, and always the first (of a whole row without the other two
-cuts the mass is a sum in fp32, so that this border is exact to some 2^-22 of it).  The token is the first kept
-    id at which the running mass in the order of the ids passes ``u`` times the kept mass.  Its log probability is that of the whole row at the temperature.
+    ones of at least ``min_p`` of the largest, of these all before which less than ``top_p`` of their mass lies, and always the first.  The token is the
+    first kept id at which the running mass in the order of the ids passes ``u`` times the kept mass.  Its log probability is that of the whole row at the temperature; the
+    row's sum in it may be one in fp32, whose last bits depend on where the row begins against 16 bytes.
     Temperature 0 or below: the largest logit, its log probability at temperature 1.  Logits that are not numbers count as -inf; a row of nothing else
     gives id -1 and log probability -inf.  Does no host work and, with ``out``, no allocation: it can be captured."""
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
