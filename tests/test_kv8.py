@@ -533,3 +533,24 @@ def test_refusals():
             bad()
     kv8.kv8_write(x[:0], x[:0], c, s[:0])
     assert kv8.kv8_decode(q[:0], c, t[:0] if False else t, s[:0], s[:0]).shape == (0, 4, 64) and kv8.kv8_prefill(q, c, []).shape == q.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,D", [(16, 4, 64), (32, 4, 128), (4, 4, 128), (12, 4, 64), (8, 1, 128)])
+@pytest.mark.parametrize("seqs,per,length", [(3, 4, 2000), (2, 16, 300), (20, 5, 900)])
+def test_rows_of_a_sequence_leave_each_other_alone(H, Hkv, D, seqs, per, length):
+    """Proposed tokens share products: queries and lengths of the others leave a row's bits as they are, whatever scale its neighbours' scores are of."""
+    g = torch.Generator().manual_seed(seqs * per + D)
+    c, tables, _, _ = filled([length] * seqs, 16, Hkv, D, g)
+    n = seqs * per
+    q = 0.1 * torch.randn(n, H, D, generator=g)                        # many keys count, and with them the roundings of their weights
+    lens = torch.tensor([length - per + 1 + r % per for r in range(n)], dtype=torch.int32)
+    seq = torch.arange(seqs, dtype=torch.int32, device="cuda").repeat_interleave(per)
+    want = kv8.kv8_decode(q.to(BF).cuda(), c, tables, lens.cuda(), row_seq=seq)
+    for turn in range(4):
+        stays = torch.rand(n, generator=g) < 0.3
+        other, short = q * torch.exp2(torch.randint(-2, 8, (n, 1, 1), generator=g).float()) + turn, torch.randint(0, length + 1, (n,), generator=g, dtype=torch.int32)
+        x, m = torch.where(stays[:, None, None], q, other), torch.where(stays, lens, short if turn % 2 else lens)
+        got = kv8.kv8_decode(x.to(BF).cuda(), c, tables, m.cuda(), row_seq=seq)
+        assert same(got.cpu()[stays], want.cpu()[stays]), turn
+    assert nv.check_status(c.device) == 0

@@ -739,11 +739,13 @@ kv8_attn_kernel(const __grid_constant__ Kv8Attn p) {
             mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             mxv = fmaxf(mxv, __shfl_xor_sync(0xffffffffu, mxv, 2));
-            // The maxima are those of some tile before, as long as none since is more than 2^K8_SLACK larger: sums are seldom scaled.
-            if (__any_sync(0xffffffffu, mx > m[u] + K8_SLACK || mxv > mv[u] + K8_SLACK)) {
+            // The maxima are those of some tile before, as long as none since is more than 2^K8_SLACK larger: sums are seldom scaled.  A row moves by its own scores alone, so that
+            // its weights are rounded the same whatever rows are beside it; the others' sums are multiplied by one.
+            const bool moves = mx > m[u] + K8_SLACK || mxv > mv[u] + K8_SLACK;
+            if (__any_sync(0xffffffffu, moves)) {
               const float was = m[u], was_v = mv[u];
-              m[u] = fmaxf(was, mx);
-              mv[u] = fmaxf(was_v, mxv);
+              m[u] = moves ? fmaxf(was, mx) : was;
+              mv[u] = moves ? fmaxf(was_v, mxv) : was_v;
               l[u] *= ex2_approx(was - (m[u] == -INFINITY ? 0.f : m[u]));          // only scores of -inf so far: all weights are zero
               const float beta = ex2_approx(was_v - (mv[u] == -INFINITY ? 0.f : mv[u]));
               const float b0 = __shfl_sync(0xffffffffu, beta, 8 * j), b1 = __shfl_sync(0xffffffffu, beta, 8 * j + 4);   // rows 2 j, 2 j + 1
