@@ -368,7 +368,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
   r.table = sh.table;
 
   // 1.  The next tile's elements are on their way while this one's are worked on.
-  const bool need_sum = (int)greedy + (int)by_k + (int)by_p > 0;         // as `||` of the three it came out false for top-p alone (nvcc 12.9)
+  const bool need_sum = greedy || by_k || by_p;
   cluster_wait();                                       // and so have the others, while the first tiles were on their way
 #pragma unroll 1
   for (int t = tile0; t < tile1; ++t) {
