@@ -184,3 +184,21 @@ def test_refusals():
                 lambda: PP.release_pages(PP.PagePool.full(2, 16, "cpu"), tables, torch.full((2,), 40, dtype=torch.int32), torch.ones(2, dtype=torch.bool))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("S,W,bad", [(1, 1, [(0, 0, -1)]), (3, 4, [(0, 1, 99), (2, 3, -7)]), (60, 9, [(s, s % 9, 540 + s) for s in range(0, 60, 7)]),
+                                     (2000, 2, [(s, 0, -2 ** 31) for s in range(1, 2000, 3)])])
+def test_ids_outside_the_pool_do_not_come_back(device, S, W, bad):
+    page = 8
+    tables = torch.arange(S * W, dtype=torch.int32).view(S, W)
+    for s, col, page_id in bad:
+        tables[s, col] = page_id
+    pool = PP.PagePool(torch.full((S * W + 5,), -3, dtype=torch.int32, device=device), torch.tensor([2], dtype=torch.int32, device=device), page, S * W)
+    lens, done = torch.full((S,), W * page, dtype=torch.int32, device=device), torch.ones(S, dtype=torch.bool, device=device)
+    with pytest.raises((ValueError, nv.NativeError)):
+        PP.release_pages(pool, tables.to(device), lens, done)
+        nv.check_status(pool.device)
+    back = [p for p in tables.flatten().tolist() if 0 <= p < S * W]
+    assert int(pool.n_free) == 2 + len(back) and pool.free[:2 + len(back)].tolist() == [-3, -3] + back
+    assert not lens.any()

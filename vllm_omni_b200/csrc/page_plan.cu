@@ -170,14 +170,16 @@ struct ReleasePages {
   const int* tables;
   int *free_pages, *n_free, *status;
   long table_stride;
-  int S, W, page, capacity;              // entries of free_pages
+  int S, W, page, pages, capacity;       // ids lie below `pages`; entries of free_pages
 };
 
 __global__ void __launch_bounds__(PP_THREADS)
 release_pages_kernel(const __grid_constant__ ReleasePages p) {
   extern __shared__ int sm[];
   __shared__ long long sh[32];
+  __shared__ int bad;
   int *at = sm, *count = sm + p.S;
+  if (threadIdx.x == 0) bad = 0;
   pdl_begin();
   const int height = min(max(0, *p.n_free), p.capacity);
   long long v[PP_PER], total;
@@ -196,13 +198,37 @@ release_pages_kernel(const __grid_constant__ ReleasePages p) {
   for (int i = 0; i < PP_PER; ++i)
     if (s0 + i < p.S) at[s0 + i] = (int)min(v[i], (long long)room);
   __syncthreads();                       // every thread has read the height
+  const int back = (int)min(total, (long long)room);
   if (threadIdx.x == 0) {
-    *p.n_free = height + (int)min(total, (long long)room);
+    *p.n_free = height + back;
     if (total > room) atomicCAS(p.status, 0, ERR_BOUNDS);
   }
   const int lane = threadIdx.x & 31;
+  int* stack = p.free_pages + height;
+  bool odd = false;
   for (int s = threadIdx.x >> 5; s < p.S; s += PP_THREADS / 32)
-    for (int i = lane; i < count[s] && at[s] + i < room; i += 32) p.free_pages[height + at[s] + i] = p.tables[(long)s * p.table_stride + i];
+    for (int i = lane; i < count[s] && at[s] + i < room; i += 32) {
+      const int id = p.tables[(long)s * p.table_stride + i];
+      odd |= id < 0 || id >= p.pages;
+      stack[at[s] + i] = id;
+    }
+  if (odd) bad = 1;
+  __syncthreads();
+  if (!bad || threadIdx.x >= 32) return;
+  // Ids that no page has are reported, and the others move up: no entry is written before it has been read.
+  int to = 0;
+  for (int i0 = 0; i0 < back; i0 += 32) {
+    const int id = i0 + lane < back ? stack[i0 + lane] : -1;
+    const bool ok = id >= 0 && id < p.pages;
+    const unsigned m = __ballot_sync(0xffffffffu, ok);
+    if (ok) stack[to + __popc(m & ((1u << lane) - 1))] = id;
+    to += __popc(m);
+    __syncwarp();
+  }
+  if (lane == 0) {
+    *p.n_free = height + to;
+    atomicCAS(p.status, 0, ERR_BOUNDS);
+  }
 }
 
 }  // namespace omni
@@ -227,10 +253,10 @@ extern "C" int omni_plan_step(const int* context, const int* fresh, int* tables,
 }
 
 extern "C" int omni_release_pages(int* lens, const unsigned char* done, const int* tables, long table_stride, int* free_pages, int* n_free, int S, int W, int page,
-                                  int capacity, int* status, void* stream) {
+                                  int pages, int capacity, int* status, void* stream) {
   if (S <= 0) return RC_OK;
-  if (S > PP_MAX_SEQS || W < 1 || page < 1 || capacity < 0) return RC_BAD_ARG;
-  ReleasePages p = {lens, done, tables, free_pages, n_free, status, table_stride, S, W, page, capacity};
+  if (S > PP_MAX_SEQS || W < 1 || page < 1 || pages < 1 || capacity < 0) return RC_BAD_ARG;
+  ReleasePages p = {lens, done, tables, free_pages, n_free, status, table_stride, S, W, page, pages, capacity};
   launch_overlapped(release_pages_kernel, 1, PP_THREADS, 2 * S * 4, (cudaStream_t)stream, p);
   return (int)cudaGetLastError();
 }

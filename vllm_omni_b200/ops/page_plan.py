@@ -5,7 +5,8 @@ A ``PagePool`` is a stack of free pages.  ``plan_step`` hands them out in the or
 its keys and values go to, its position, its sequence and the keys it sees: the operands of ``kv8.kv8_write`` and ``kv8.kv8_decode`` (and of ``kv_cache.kv_write``
 and ``paged_decode``).  ``release_pages`` puts the pages of finished sequences back.  The CPU paths restate the same semantics in PyTorch.
 
-A page belongs to one sequence.  A page id outside the pool is reported through the status word (``_native.check_status``), its rows get no slot."""
+A page belongs to one sequence.  A page id outside the pool is reported, its rows get no slot, and it does not come back to the pool: on the GPU through the status
+word (``_native.check_status``); on the CPU ``release_pages`` raises when it is done."""
 from __future__ import annotations
 
 import ctypes
@@ -23,7 +24,7 @@ _P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
 def _lib():
     lib = nv.lib("page_plan")
     lib._cdll.omni_plan_step.argtypes = [_P] * 3 + [_L, _P, _P] + [_I] * 6 + [_P] * 11
-    lib._cdll.omni_release_pages.argtypes = [_P] * 3 + [_L, _P, _P] + [_I] * 4 + [_P] * 2
+    lib._cdll.omni_release_pages.argtypes = [_P] * 3 + [_L, _P, _P] + [_I] * 5 + [_P] * 2
     return lib
 
 
@@ -130,15 +131,18 @@ def release_pages(pool: PagePool, tables: torch.Tensor, lens: torch.Tensor, done
         back = [p for s in range(S) if done[s] for p in tables[s, :min(tables.shape[1], -(-max(int(lens[s]), 0) // pool.block_size))].tolist()]
         if len(back) > cap - height:
             raise ValueError(f"{len(back)} pages come back to a pool with room for {cap - height}")
-        pool.free[height:height + len(back)] = torch.tensor(back, dtype=torch.int32)
-        pool.n_free.fill_(height + len(back))
+        good = [p for p in back if 0 <= p < pool.num_blocks]
+        pool.free[height:height + len(good)] = torch.tensor(good, dtype=torch.int32)
+        pool.n_free.fill_(height + len(good))
         lens.masked_fill_(done, 0)
+        if len(good) < len(back):
+            raise ValueError(f"{len(back) - len(good)} page ids outside the pool's {pool.num_blocks}")
         return
     if torch._C._cuda_getDevice() != pool.device.index:
         with torch.cuda.device(pool.device):
             return release_pages(pool, tables, lens, done)
     nv.check_rc(_lib().omni_release_pages(lens.data_ptr(), done.data_ptr(), tables.data_ptr(), tables.stride(0), pool.free.data_ptr(), pool.n_free.data_ptr(), S,
-                                          tables.shape[1], pool.block_size, pool.free.numel(), nv.status_word(pool.device).data_ptr(), nv.stream_ptr()),
+                                          tables.shape[1], pool.block_size, pool.num_blocks, pool.free.numel(), nv.status_word(pool.device).data_ptr(), nv.stream_ptr()),
                 "omni_release_pages")
 
 
