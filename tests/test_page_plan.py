@@ -202,3 +202,15 @@ def test_ids_outside_the_pool_do_not_come_back(device, S, W, bad):
     back = [p for p in tables.flatten().tolist() if 0 <= p < S * W]
     assert int(pool.n_free) == 2 + len(back) and pool.free[:2 + len(back)].tolist() == [-3, -3] + back
     assert not lens.any()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_sequences_whose_pages_do_not_fit_keep_them(device):
+    lens = [17, 16, 0, 40, 5, 0]                          # pages of 8: 3, 2, none, 5 that do not fit, 1 behind them, none
+    pool = PP.PagePool(torch.full((9,), -3, dtype=torch.int32, device=device), torch.tensor([1], dtype=torch.int32, device=device), 8, 100)
+    tables, context = torch.arange(30, dtype=torch.int32, device=device).view(6, 5), torch.tensor(lens, dtype=torch.int32, device=device)
+    with pytest.raises((ValueError, nv.NativeError)):
+        PP.release_pages(pool, tables, context, torch.ones(6, dtype=torch.bool, device=device))
+        nv.check_status(pool.device)
+    assert context.tolist() == [0, 0, 0, 40, 5, 0]
+    assert int(pool.n_free) == 6 and pool.free.tolist() == [-3, 0, 1, 2, 5, 6, -3, -3, -3]

@@ -177,28 +177,39 @@ __global__ void __launch_bounds__(PP_THREADS)
 release_pages_kernel(const __grid_constant__ ReleasePages p) {
   extern __shared__ int sm[];
   __shared__ long long sh[32];
-  __shared__ int bad;
+  __shared__ int bad, fits;
   int *at = sm, *count = sm + p.S;
-  if (threadIdx.x == 0) bad = 0;
+  if (threadIdx.x == 0) bad = fits = 0;
   pdl_begin();
   const int height = min(max(0, *p.n_free), p.capacity);
   long long v[PP_PER], total;
+  int n[PP_PER];                         // pages of a sequence that is done, else -1
   const int s0 = threadIdx.x * PP_PER;
 #pragma unroll
   for (int i = 0; i < PP_PER; ++i) {
     const int s = s0 + i;
     const bool done = s < p.S && p.done[s];
     v[i] = done ? min(p.W, pages_of(p.lens[s], p.page)) : 0;
-    if (s < p.S) count[s] = (int)v[i];
-    if (done) p.lens[s] = 0;
+    n[i] = done ? (int)v[i] : -1;
   }
   block_scan(v, total, sh);
   const int room = p.capacity - height;
+  int end = 0;                           // of the thread's last sequence that fits
 #pragma unroll
-  for (int i = 0; i < PP_PER; ++i)
-    if (s0 + i < p.S) at[s0 + i] = (int)min(v[i], (long long)room);
+  for (int i = 0; i < PP_PER; ++i) {
+    const int s = s0 + i;
+    const bool whole = n[i] <= 0 || v[i] + n[i] <= room;  // else it keeps its pages and its length, and so do those behind it
+    if (s < p.S) {
+      at[s] = (int)min(v[i], (long long)room);
+      count[s] = whole ? max(n[i], 0) : 0;
+      if (n[i] >= 0 && whole) p.lens[s] = 0;
+      if (count[s]) end = at[s] + n[i];
+    }
+  }
+  end = __reduce_max_sync(0xffffffffu, end);
+  if ((threadIdx.x & 31) == 0 && end) atomicMax(&fits, end);
   __syncthreads();                       // every thread has read the height
-  const int back = (int)min(total, (long long)room);
+  const int back = fits;
   if (threadIdx.x == 0) {
     *p.n_free = height + back;
     if (total > room) atomicCAS(p.status, 0, ERR_BOUNDS);
@@ -207,7 +218,7 @@ release_pages_kernel(const __grid_constant__ ReleasePages p) {
   int* stack = p.free_pages + height;
   bool odd = false;
   for (int s = threadIdx.x >> 5; s < p.S; s += PP_THREADS / 32)
-    for (int i = lane; i < count[s] && at[s] + i < room; i += 32) {
+    for (int i = lane; i < count[s]; i += 32) {
       const int id = p.tables[(long)s * p.table_stride + i];
       odd |= id < 0 || id >= p.pages;
       stack[at[s] + i] = id;

@@ -5,8 +5,8 @@ A ``PagePool`` is a stack of free pages.  ``plan_step`` hands them out in the or
 its keys and values go to, its position, its sequence and the keys it sees: the operands of ``kv8.kv8_write`` and ``kv8.kv8_decode`` (and of ``kv_cache.kv_write``
 and ``paged_decode``).  ``release_pages`` puts the pages of finished sequences back.  The CPU paths restate the same semantics in PyTorch.
 
-A page belongs to one sequence.  A page id outside the pool is reported, its rows get no slot, and it does not come back to the pool: on the GPU through the status
-word (``_native.check_status``); on the CPU ``release_pages`` raises when it is done."""
+A page belongs to one sequence.  A page id outside the pool is reported, its rows get no slot, and it does not come back to the pool.
+The GPU reports through the status word (``_native.check_status``); on the CPU ``release_pages`` raises when it is done."""
 from __future__ import annotations
 
 import ctypes
@@ -120,7 +120,8 @@ def plan_step(pool: PagePool, tables: torch.Tensor, context: torch.Tensor, new: 
 
 
 def release_pages(pool: PagePool, tables: torch.Tensor, lens: torch.Tensor, done: torch.Tensor) -> None:
-    """The pages that hold the ``lens[s]`` tokens (int32 [S]) of every sequence with ``done[s]`` (bool [S]) go back to the pool, and its length becomes 0."""
+    """The pages that hold the ``lens[s]`` tokens (int32 [S]) of every sequence with ``done[s]`` (bool [S]) go back to the pool, and its length becomes 0.
+    Where the pool has no room for all of a sequence's pages, that is reported; the sequence and those behind it keep their pages and their lengths."""
     S = lens.numel()
     _check_ints("lens", lens, (S,), pool.device)
     _check_tables(tables, S, pool)
@@ -128,15 +129,19 @@ def release_pages(pool: PagePool, tables: torch.Tensor, lens: torch.Tensor, done
         raise ValueError(f"done: contiguous bool [{S}] on {pool.device} expected, got {done.dtype} {tuple(done.shape)}")
     if pool.device.type != "cuda":
         height, cap = min(max(int(pool.n_free), 0), pool.free.numel()), pool.free.numel()
-        back = [p for s in range(S) if done[s] for p in tables[s, :min(tables.shape[1], -(-max(int(lens[s]), 0) // pool.block_size))].tolist()]
-        if len(back) > cap - height:
-            raise ValueError(f"{len(back)} pages come back to a pool with room for {cap - height}")
-        good = [p for p in back if 0 <= p < pool.num_blocks]
-        pool.free[height:height + len(good)] = torch.tensor(good, dtype=torch.int32)
-        pool.n_free.fill_(height + len(good))
-        lens.masked_fill_(done, 0)
-        if len(good) < len(back):
-            raise ValueError(f"{len(back) - len(good)} page ids outside the pool's {pool.num_blocks}")
+        back, bad, full = [], 0, False
+        for s in (s for s in range(S) if done[s]):
+            pages = tables[s, :min(tables.shape[1], -(-max(int(lens[s]), 0) // pool.block_size))].tolist()
+            full |= len(back) + bad + len(pages) > cap - height
+            if not full or not pages:
+                lens[s] = 0
+                good = [p for p in pages if 0 <= p < pool.num_blocks]
+                back, bad = back + good, bad + len(pages) - len(good)
+        pool.free[height:height + len(back)] = torch.tensor(back, dtype=torch.int32)
+        pool.n_free.fill_(height + len(back))
+        if full or bad:
+            raise ValueError(f"pages of finished sequences: {bad} ids outside the pool's {pool.num_blocks}"
+                             + (f", and more than there is room for ({cap - height})" if full else ""))
         return
     if torch._C._cuda_getDevice() != pool.device.index:
         with torch.cuda.device(pool.device):
