@@ -554,3 +554,17 @@ def test_rows_of_a_sequence_leave_each_other_alone(H, Hkv, D, seqs, per, length)
         got = kv8.kv8_decode(x.to(BF).cuda(), c, tables, m.cuda(), row_seq=seq)
         assert same(got.cpu()[stays], want.cpu()[stays]), turn
     assert nv.check_status(c.device) == 0
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_rows_of_a_result_must_not_overlap(dev):
+    c, t = cache_of(8, 16, 2, 64, dev), torch.arange(8, dtype=torch.int32, device=dev).view(4, 2)
+    q, n = torch.zeros(4, 6, 64, dtype=BF, device=dev), torch.ones(4, dtype=torch.int32, device=dev)
+    buf = torch.zeros(4 * 6 * 64, dtype=BF, device=dev)
+    for bad in (buf[:384].view(6, 64).expand(4, 6, 64), buf[:256].view(4, 1, 64).expand(4, 6, 64), buf.as_strided((4, 6, 64), (320, 64, 1)), buf.as_strided((4, 6, 64), (64, 192, 1)),
+                buf.as_strided((4, 6, 64), (384, 56, 1))):
+        for call in (lambda: kv8.kv8_decode(q, c, t, n, out=bad), lambda: kv8.kv8_prefill(q, c, [(0, 4, 0, t[0])], out=bad)):
+            with pytest.raises(ValueError, match="overlap"):
+                call()
+    heads_first = torch.zeros(6, 4, 64, dtype=BF, device=dev).transpose(0, 1)          # rows within heads: apart
+    assert kv8.kv8_decode(q, c, t, n, out=heads_first) is heads_first

@@ -186,6 +186,15 @@ def _check_tables(tables, S, cache):
         raise ValueError(f"block_tables of {tables.shape[0]} sequences for {S} rows: row_seq says which row is of which sequence")
 
 
+def _check_apart(out):
+    """Of the dimensions with more than one entry each step reaches over all that lies within it."""
+    reach = 1
+    for step, size in sorted((step, size) for step, size in zip(out.stride(), out.shape) if size > 1):
+        if step < reach:
+            raise ValueError(f"out: rows or heads overlap (strides {out.stride()} of {tuple(out.shape)})")
+        reach += step * (size - 1)
+
+
 def _check_queries(q, cache, out):
     if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % cache.heads:
         raise ValueError(f"q: [rows, heads, {cache.head_size}] with heads a multiple of {cache.heads} expected, got {tuple(q.shape)}")
@@ -194,6 +203,8 @@ def _check_queries(q, cache, out):
     _check_rows("q", q, (q.shape[0], q.shape[1], cache.head_size), cache.device)
     if out is not None:
         _check_rows("out", out, q.shape, cache.device)
+        if not out.is_contiguous():
+            _check_apart(out)
         if out.is_cuda and not _fits(out):
             raise ValueError("out: channels side by side, rows and heads on 16 bytes")
 
