@@ -568,3 +568,24 @@ def test_rows_of_a_result_must_not_overlap(dev):
                 call()
     heads_first = torch.zeros(6, 4, 64, dtype=BF, device=dev).transpose(0, 1)          # rows within heads: apart
     assert kv8.kv8_decode(q, c, t, n, out=heads_first) is heads_first
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_a_single_row_or_head_of_any_pitch_and_queries_that_are_the_same(dev):
+    """A dimension of one entry has no pitch, and queries may be one row for all."""
+    g = torch.Generator().manual_seed(9)
+    c, t = cache_of(8, 16, 1, 64, dev), torch.arange(8, dtype=torch.int32, device=dev).view(1, 8)
+    k, v = (rows_for(100, 1, 64, g, "normal").to(dev) for _ in range(2))
+    kv8.kv8_write(k, v, c, torch.arange(100, dtype=torch.int32, device=dev))
+    q = torch.randn(1, 3, 64, generator=g).to(BF).to(dev)
+    n, seq = torch.tensor([100], dtype=torch.int32, device=dev), torch.zeros(5, dtype=torch.int32, device=dev)
+    out = torch.zeros(500, dtype=BF, device=dev).as_strided((1, 3, 64), (3, 64, 1))
+    assert same(kv8.kv8_decode(q, c, t, n, out=out), kv8.kv8_decode(q, c, t, n))
+    assert same(kv8.kv8_prefill(q, c, [(0, 1, 99, t[0])], out=out), kv8.kv8_prefill(q, c, [(0, 1, 99, t[0])]))
+    one = torch.randn(5, 1, 64, generator=g).to(BF).to(dev)
+    out = torch.zeros(500, dtype=BF, device=dev).as_strided((5, 1, 64), (64, 11, 1))
+    assert same(kv8.kv8_decode(one, c, t, n.repeat(5), seq, out=out), kv8.kv8_decode(one, c, t, n.repeat(5), seq))
+    assert same(kv8.kv8_prefill(one, c, [(0, 5, 95, t[0])], out=out), kv8.kv8_prefill(one, c, [(0, 5, 95, t[0])]))
+    wide = q.expand(5, 3, 64)
+    assert same(kv8.kv8_decode(wide, c, t, n.repeat(5), seq), kv8.kv8_decode(wide.contiguous(), c, t, n.repeat(5), seq))
+    assert same(kv8.kv8_prefill(wide, c, [(0, 5, 95, t[0])]), kv8.kv8_prefill(wide.contiguous(), c, [(0, 5, 95, t[0])]))

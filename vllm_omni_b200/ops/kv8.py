@@ -107,8 +107,16 @@ def _check_rows(name, t, shape, device):
 
 def _fits(t) -> bool:
     """Rows that the kernels take where they are: channels side by side, everything on 16 bytes."""
-    a, b, c = t.stride()
-    return c == 1 and not (a | b) & 7 and not t.data_ptr() & 15
+    a, b = _pitches(t)
+    return t.stride(2) == 1 and not (a | b) & 7 and not t.data_ptr() & 15
+
+
+def _pitches(t):
+    """Of rows and heads; a single one has none of its own."""
+    a, b, _ = t.stride()
+    if t.shape[1] == 1:
+        b = t.shape[2]
+    return (a if t.shape[0] > 1 else t.shape[1] * b), b
 
 
 def _readable(t):
@@ -138,7 +146,7 @@ def kv8_write(k, v, cache: Kv8Cache, slots) -> None:
         with torch.cuda.device(cache.device):
             return kv8_write(k, v, cache, slots)
     k, v = _readable(k), _readable(v)
-    ks, vs = k.stride(), v.stride()
+    ks, vs = _pitches(k), _pitches(v)
     nv.check_rc(_lib().omni_kv8_write(cache._at(), k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), T, _stream(cache.device)), "omni_kv8_write")
 
 
@@ -237,7 +245,7 @@ def kv8_decode(q, cache: Kv8Cache, block_tables, lens, row_seq=None, scale=None,
     S, mapped, max_keys = block_tables.shape[0], row_seq is not None, block_tables.shape[1] * cache.block_size
     shares = _shares(R, S, H, cache.heads, D, mapped, cache.block_size, max_keys, cache.device.index)
     part = cache.k_scale.new_empty(R * H * shares * (D + 1)) if shares > 1 else None
-    qs, outs = q.stride(), out.stride()
+    qs, outs = _pitches(q), _pitches(out)
     nv.check_rc(_lib().omni_kv8_attn(
         cache._at(), q.data_ptr(), qs[0], qs[1], block_tables.data_ptr(), block_tables.stride(0), lens.data_ptr(), row_seq.data_ptr() if mapped else None, R, S, H,
         max_keys, scale, shares, None if part is None else part.data_ptr(), out.data_ptr(), outs[0], outs[1], _stream(cache.device)), "omni_kv8_attn")
@@ -279,6 +287,10 @@ def kv8_prefill(q, cache: Kv8Cache, segs, scale=None, out=None):
     if not segs:
         return out
     q, n = _readable(q), len(segs)
+    qs, outs = _pitches(q), _pitches(out)
+    if 0 in qs:                                              # one row or head for all: tensor maps want pitches
+        q = q.contiguous()
+        qs = _pitches(q)
     total, row0 = 0, []
     for _, rows, context, _ in segs:
         row0.append(total)
@@ -288,7 +300,7 @@ def kv8_prefill(q, cache: Kv8Cache, segs, scale=None, out=None):
     first, rows, context = ((_I * n)(*(s[i] for s in segs)) for i in range(3))
     rs = cache.heads * D
     nv.check_rc(_prefill_lib().omni_attn_prefill_keys(
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), rs, D, v.data_ptr(), rs, D, out.data_ptr(), out.stride(0), out.stride(1), T, H, cache.heads, D, n,
+        q.data_ptr(), *qs, k.data_ptr(), rs, D, v.data_ptr(), rs, D, out.data_ptr(), *outs, T, H, cache.heads, D, n,
         first, rows, context, (_L * n)(*row0), scale, cache._fields.status, _stream(cache.device)), "omni_attn_prefill_keys")
     nv.count_launches((n - 1) // 16)                         # of the pages, sixteen segments at a time
     if n > 8 or T > 248 * 256:                               # of the attention, eight segments and 256 blocks of 256 rows at a time
