@@ -98,3 +98,25 @@ def test_too_few_pages():
     held = [p for s in range(S) for p in loop.tables[s, :-(-int(loop.context[s]) // PAGE)].tolist()]
     assert sorted(held + loop.pool.free[:int(loop.pool.n_free)].tolist()) == list(range(9))
     assert nv.check_status(loop.pool.device) == 0
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_sequences_wait_for_pages_and_go_on(dev):
+    """Fewer pages than the sequences want: who gets none stands still, with no slot and its length as it was, and goes on when others have given theirs back.  They want 5, 1, 5,
+    2, 1 and 3 pages, and sequences that all wait hold one less each, 11 in all: with 12 one of them has all it wants, ends and gives back."""
+    loop = Loop(dev, pages=12)
+    limits, before, waited, went_on = loop.limits.tolist(), [0] * S, set(), set()
+    for i, (ids, ctx, n_free, slots, out) in enumerate(loop.run(200, loop.step)):
+        ctx, slots = ctx.tolist(), slots.tolist()
+        for s in range(S):
+            context = 0 if before[s] >= limits[s] else before[s]       # those that were done began again
+            assert ctx[s] == context + (slots[s] >= 0)
+            if slots[s] < 0:
+                assert context % PAGE == 0                             # only a new page can be missing
+                if i < 150:                                            # the others have steps left to go on in
+                    waited.add(s)
+            elif s in waited:
+                went_on.add(s)
+        assert int(n_free) == 12 - sum(-(-c // PAGE) for c in ctx)
+        before = ctx
+    assert waited and went_on == waited

@@ -589,3 +589,40 @@ def test_a_single_row_or_head_of_any_pitch_and_queries_that_are_the_same(dev):
     wide = q.expand(5, 3, 64)
     assert same(kv8.kv8_decode(wide, c, t, n.repeat(5), seq), kv8.kv8_decode(wide.contiguous(), c, t, n.repeat(5), seq))
     assert same(kv8.kv8_prefill(wide, c, [(0, 5, 95, t[0])]), kv8.kv8_prefill(wide.contiguous(), c, [(0, 5, 95, t[0])]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,D", [(48, 1, 64), (64, 1, 128), (200, 2, 64), (128, 1, 128), (128, 1, 64), (82, 2, 128)])
+@pytest.mark.parametrize("page,lens", [(8, [1]), (16, [7, 0, 65]), (48, [1500, 1, 333])])
+def test_large_groups_against_64_bits(H, Hkv, D, page, lens):
+    g = torch.Generator().manual_seed(H + page)
+    c, tables, ks, vs = filled(lens, page, Hkv, D, g)
+    q = torch.randn(len(lens), H, D, generator=g).to(BF).cuda()
+    out = kv8.kv8_decode(q, c, tables, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    for s in range(len(lens)):
+        ref, bound = reference(q[s], ks[s], vs[s], D ** -0.5)
+        assert ((out[s].double() - ref).abs() <= bound).all(), s
+    assert nv.check_status(c.device) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,D,seqs,per", [(4, 1, 64, 620, 1), (8, 1, 128, 560, 2)])
+def test_many_rows_of_several_shares(H, Hkv, D, seqs, per):
+    """More blocks of rows than have a list of their shares: those behind a row's end are empty."""
+    g = torch.Generator().manual_seed(seqs)
+    width, page = 512, 8
+    lens = [int(torch.randint(0, 300, (1,), generator=g)) for _ in range(seqs)]
+    lens[3], lens[seqs - 1], lens[200] = 4096, 3000, 0
+    c, narrow, ks, vs = filled(lens, page, Hkv, D, g)
+    tables = torch.full((seqs, width), -9, dtype=torch.int32, device="cuda")
+    tables[:, :min(width, narrow.shape[1])] = narrow[:, :width]
+    assert kv8._lib().omni_kv8_attn_shares(seqs * per, seqs, H, Hkv, D, per > 1, page, width * page) > 1
+    q = torch.randn(seqs * per, H, D, generator=g).to(BF).cuda()
+    n = torch.tensor(lens, dtype=torch.int32).repeat_interleave(per)
+    n[per - 1::per] = (n[per - 1::per] - (per - 1)).clamp(min=0)       # the last of a sequence's rows sees less
+    seq = torch.arange(seqs, dtype=torch.int32, device="cuda").repeat_interleave(per) if per > 1 else None
+    out = kv8.kv8_decode(q, c, tables, n.cuda(), row_seq=seq)
+    for r in range(seqs * per):
+        ref, bound = reference(q[r], ks[r // per][:int(n[r])], vs[r // per][:int(n[r])], D ** -0.5)
+        assert ((out[r].double() - ref).abs() <= bound).all(), r
+    assert nv.check_status(c.device) == 0
