@@ -78,3 +78,24 @@ def test_kernel(kind, V, t, share):
 @pytest.mark.parametrize("B", [1, 40, 300])
 def test_kernel_with_more_and_fewer_blocks_a_row(B):
     check("normal", 33000, B, torch.float32, 1.0, 0.9, 1, "cuda")
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_numbers_are_what_a_tensor_of_them_is(dev):
+    """A number counts as the fp32 or int32 that a row's value would be; what is no such integer is refused and does not wrap."""
+    x, t = torch.tensor([[0.0, -1.0, -2.0, -3.0]], device=dev), 1.3
+    z = np.exp(-np.arange(4) / float(np.float32(t)))
+    share = np.float32(z[0] / z.sum())                                 # between the fp32 and the 64-bit temperature's border
+    assert float(share) != np.exp(0) / np.exp(-np.arange(4) / t).sum()
+    u = torch.tensor([LAST], device=dev)
+    full = lambda v: torch.full((1,), v, device=dev)
+    for p in (float(np.nextafter(share, np.float32(0))), float(share), float(np.nextafter(share, np.float32(1)))):
+        ids, lp = sample_given(x, u, t, 0, p)
+        want = sample_given(x, u, full(t), 0, full(p))
+        assert int(ids[0]) == int(want[0][0]) and float(lp[0]) == float(want[1][0])
+    a, b = float(np.float64(share) * (1 - 2.0 ** -40)), float(np.float64(share) * (1 + 2.0 ** -40))      # the same fp32 number
+    assert int(sample_given(x, u, t, 0, a)[0]) == int(sample_given(x, u, t, 0, b)[0])
+    for k in (2 ** 32 + 1, 2 ** 31, -2 ** 40, 1.5):
+        with pytest.raises((ValueError, TypeError)):
+            sample_given(x, u, 1.0, k)
+    assert int(sample_given(x, u, 1.0, 2 ** 31 - 1)[0]) == 3 and int(sample_given(x, u, 1.0, 1)[0]) == 0

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 from dataclasses import dataclass, field
 
 import torch
@@ -202,6 +203,8 @@ def _given_lib():
 def _per_row(name, v, B, dtype, device):
     """(address, value) of a parameter that is one number or a tensor of one per row."""
     if not isinstance(v, torch.Tensor):
+        if dtype is torch.int32 and not -1 << 31 <= operator.index(v) < 1 << 31:
+            raise ValueError(f"{name} {v}: an int32 expected")
         return None, v
     if v.dtype is not dtype or v.shape != (B,) or not v.is_contiguous() or v.device != device:
         raise ValueError(f"{name}: a number or contiguous {dtype} [{B}] on {device} expected, got {v.dtype} {tuple(v.shape)} on {v.device}")
@@ -236,8 +239,9 @@ def sample_given(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0
             raise ValueError(f"out: contiguous int32 [{B}] and fp32 [{B}] on {dev} expected")
     if not logits.is_cuda:
         for r in range(B):
-            pick = [float(v[r] if isinstance(v, torch.Tensor) else v) for v in (temperature, top_k, top_p, min_p)]
-            ids[r], logprob[r] = _given_row(logits[r].double(), float(u[r]), *pick)
+            pick = [float(v[r]) if isinstance(v, torch.Tensor) else ctypes.c_float(v).value for v in (temperature, top_p, min_p)]     # numbers are fp32, too
+            k = int(top_k[r]) if isinstance(top_k, torch.Tensor) else int(top_k)
+            ids[r], logprob[r] = _given_row(logits[r].double(), float(u[r]), pick[0], k, *pick[1:])
         return ids, logprob
     if torch._C._cuda_getDevice() != dev.index:
         with torch.cuda.device(dev):
