@@ -99,3 +99,17 @@ def test_numbers_are_what_a_tensor_of_them_is(dev):
         with pytest.raises((ValueError, TypeError)):
             sample_given(x, u, 1.0, k)
     assert int(sample_given(x, u, 1.0, 2 ** 31 - 1)[0]) == 3 and int(sample_given(x, u, 1.0, 1)[0]) == 0
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("V", [5, 3000, 20000])
+def test_parameters_that_are_not_numbers_cut_nothing(dev, V):
+    g = torch.Generator().manual_seed(V)
+    x, nan = torch.randn(3, V, generator=g).to(dev), float("nan")
+    u = torch.tensor([0.0, 0.5, LAST], device=dev)
+    for t, k, p, m, like in ((1.0, 0, nan, 0.0, (1.0, 0, 1.0, 0.0)), (1.0, 0, 1.0, nan, (1.0, 0, 1.0, 0.0)), (0.8, 3, 0.9, nan, (0.8, 3, 0.9, 0.0)), (0.8, 0, 0.9, nan, (0.8, 0, 0.9, 0.0)),
+                             (nan, 3, 0.9, 0.1, (0.0, 3, 0.9, 0.1)), (0.8, 4, 0.9, -nan, (0.8, 4, 0.9, -1.0))):
+        got, want = sample_given(x, u, t, k, p, m), sample_given(x, u, *like)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (t, k, p, m)
+    got, want = sample_given(x, torch.full((3,), nan, device=dev), 0.8, 50, 0.9), sample_given(x, torch.zeros(3, device=dev), 0.8, 50, 0.9)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

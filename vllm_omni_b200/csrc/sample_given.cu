@@ -356,7 +356,8 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
   SgVec<T> ahead = load8(x0, off, V, tile0 * SG_THREADS + tid), ahead2 = load8(x0, off, V, (tile0 + 1) * SG_THREADS + tid);
   const float T_in = p.temperature ? p.temperature[row] : p.temperature_v;
   const bool greedy = !(T_in > 0.f);
-  const float top_p = p.top_p ? p.top_p[row] : p.top_p_v, min_p = fminf(p.min_p ? p.min_p[row] : p.min_p_v, 1.f);
+  const float top_p = p.top_p ? p.top_p[row] : p.top_p_v;
+  const float min_in = p.min_p ? p.min_p[row] : p.min_p_v, min_p = min_in > 0.f ? fminf(min_in, 1.f) : 0.f;         // not a number: no cut
   const int k_in = p.top_k ? p.top_k[row] : p.top_k_v;
   const bool by_k = !greedy && k_in > 0 && k_in < V, by_p = !greedy && top_p < 1.f;
   SgRow r;

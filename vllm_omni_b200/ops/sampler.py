@@ -219,7 +219,7 @@ def sample_given(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0
     ones of at least ``min_p`` of the largest, of these all before which less than ``top_p`` of their mass lies, and always the first.  The token is the
     first kept id at which the running mass in the order of the ids passes ``u`` times the kept mass.  Its log probability is that of the whole row at the temperature; the
     row's sum in it may be one in fp32, whose last bits depend on where the row begins against 16 bytes.
-    Temperature 0 or below: the largest logit, its log probability at temperature 1.  Logits that are not numbers count as -inf; a row of nothing else
+    Temperature 0 or below, or not a number: the largest logit, its log probability at temperature 1.  Cuts that are not numbers cut nothing.  Logits that are not numbers count as -inf; a row of nothing else
     gives id -1 and log probability -inf.  Does no host work and, with ``out``, no allocation: it can be captured."""
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
         raise ValueError(f"logits: bf16 or fp32 [rows, vocabulary] with a row's values side by side expected, got {logits.dtype} {tuple(logits.shape)}")
@@ -270,14 +270,14 @@ def _given_row(x, u, temperature, top_k, top_p, min_p):
     order = torch.sort(x, descending=True, stable=True).indices
     if 0 < top_k < x.numel():
         order = order[:int(top_k)]
-    order = order[e[order] >= min(min_p, 1.0)]
+    order = order[e[order] >= (min(min_p, 1.0) if min_p > 0 else 0.0)]
     mass = torch.cumsum(w[order], 0)
     if top_p < 1:
         fits = (mass - w[order]).double() < top_p * mass[-1].double()
         order = order[:max(1, int(fits.sum()))]
     kept = torch.sort(order).values
     mass = torch.cumsum(w[kept], 0)
-    i = int((mass.double() <= max(u, 0.0) * mass[-1].double()).sum())
+    i = int((mass.double() <= (u if u > 0 else 0.0) * mass[-1].double()).sum())
     if i == kept.numel():                                 # u = 1: the last one with mass
         i = int((w[kept] > 0).nonzero()[-1])
     return int(kept[i]), float(z[kept[i]] - log_all)
