@@ -105,22 +105,25 @@ def _check_rows(name, t, shape, device):
         raise ValueError(f"{name}: bf16 {tuple(shape)} on {device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _fits(t) -> bool:
-    """Rows that the kernels take where they are: channels side by side, everything on 16 bytes."""
-    a, b = _pitches(t)
-    return t.stride(2) == 1 and not (a | b) & 7 and not t.data_ptr() & 15
-
-
 def _pitches(t):
-    """Of rows and heads; a single one has none of its own."""
-    a, b, _ = t.stride()
-    if t.shape[1] == 1:
-        b = t.shape[2]
-    return (a if t.shape[0] > 1 else t.shape[1] * b), b
+    """(of rows, of heads, whether the kernels take the tensor where it is: channels side by side, everything on 16 bytes).  A single row or head has no pitch of its own."""
+    (R, H, D), (a, b, c) = t.shape, t.stride()
+    if H == 1:
+        b = D
+    if R <= 1:
+        a = H * b
+    return a, b, c == 1 and not (a | b) & 7 and not t.data_ptr() & 15
 
 
-def _readable(t):
-    return t if _fits(t) else torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+def _readable(t, H, D):
+    """[rows, H, D] as the kernels take it, pitches of its rows and heads."""
+    if not t.is_contiguous():
+        a, b, fits = _pitches(t)
+        if fits:
+            return t, a, b
+    elif not t.data_ptr() & 15:
+        return t, H * D, D
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t), H * D, D
 
 
 def _elsewhere(device) -> bool:
@@ -145,9 +148,9 @@ def kv8_write(k, v, cache: Kv8Cache, slots) -> None:
     if _elsewhere(cache.device):
         with torch.cuda.device(cache.device):
             return kv8_write(k, v, cache, slots)
-    k, v = _readable(k), _readable(v)
-    ks, vs = _pitches(k), _pitches(v)
-    nv.check_rc(_lib().omni_kv8_write(cache._at(), k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), T, _stream(cache.device)), "omni_kv8_write")
+    k, kr, kh = _readable(k, cache.heads, cache.head_size)
+    v, vr, vh = _readable(v, cache.heads, cache.head_size)
+    nv.check_rc(_lib().omni_kv8_write(cache._at(), k.data_ptr(), v.data_ptr(), kr, kh, vr, vh, slots.data_ptr(), T, _stream(cache.device)), "omni_kv8_write")
 
 
 def _out_pair(cache, rows, out_k, out_v):
@@ -213,7 +216,7 @@ def _check_queries(q, cache, out):
         _check_rows("out", out, q.shape, cache.device)
         if not out.is_contiguous():
             _check_apart(out)
-        if out.is_cuda and not _fits(out):
+        if out.is_cuda and not _pitches(out)[2]:
             raise ValueError("out: channels side by side, rows and heads on 16 bytes")
 
 
@@ -241,14 +244,14 @@ def kv8_decode(q, cache: Kv8Cache, block_tables, lens, row_seq=None, scale=None,
             return kv8_decode(q, cache, block_tables, lens, row_seq, scale, out)
     if R == 0:
         return out
-    q = _readable(q)
+    q, qr, qh = _readable(q, H, D)
     S, mapped, max_keys = block_tables.shape[0], row_seq is not None, block_tables.shape[1] * cache.block_size
     shares = _shares(R, S, H, cache.heads, D, mapped, cache.block_size, max_keys, cache.device.index)
     part = cache.k_scale.new_empty(R * H * shares * (D + 1)) if shares > 1 else None
-    qs, outs = _pitches(q), _pitches(out)
+    _, outr, outh = _readable(out, H, D)
     nv.check_rc(_lib().omni_kv8_attn(
-        cache._at(), q.data_ptr(), qs[0], qs[1], block_tables.data_ptr(), block_tables.stride(0), lens.data_ptr(), row_seq.data_ptr() if mapped else None, R, S, H,
-        max_keys, scale, shares, None if part is None else part.data_ptr(), out.data_ptr(), outs[0], outs[1], _stream(cache.device)), "omni_kv8_attn")
+        cache._at(), q.data_ptr(), qr, qh, block_tables.data_ptr(), block_tables.stride(0), lens.data_ptr(), row_seq.data_ptr() if mapped else None, R, S, H,
+        max_keys, scale, shares, None if part is None else part.data_ptr(), out.data_ptr(), outr, outh, _stream(cache.device)), "omni_kv8_attn")
     if part is not None:
         nv.count_launches(1)
     return out
@@ -286,11 +289,9 @@ def kv8_prefill(q, cache: Kv8Cache, segs, scale=None, out=None):
             return kv8_prefill(q, cache, segs, scale, out)
     if not segs:
         return out
-    q, n = _readable(q), len(segs)
-    qs, outs = _pitches(q), _pitches(out)
-    if 0 in qs:                                              # one row or head for all: tensor maps want pitches
+    if 0 in q.stride():                                      # one row or head for all: tensor maps want pitches
         q = q.contiguous()
-        qs = _pitches(q)
+    (q, qr, qh), (_, outr, outh), n = _readable(q, H, D), _readable(out, H, D), len(segs)
     total, row0 = 0, []
     for _, rows, context, _ in segs:
         row0.append(total)
@@ -300,7 +301,7 @@ def kv8_prefill(q, cache: Kv8Cache, segs, scale=None, out=None):
     first, rows, context = ((_I * n)(*(s[i] for s in segs)) for i in range(3))
     rs = cache.heads * D
     nv.check_rc(_prefill_lib().omni_attn_prefill_keys(
-        q.data_ptr(), *qs, k.data_ptr(), rs, D, v.data_ptr(), rs, D, out.data_ptr(), *outs, T, H, cache.heads, D, n,
+        q.data_ptr(), qr, qh, k.data_ptr(), rs, D, v.data_ptr(), rs, D, out.data_ptr(), outr, outh, T, H, cache.heads, D, n,
         first, rows, context, (_L * n)(*row0), scale, cache._fields.status, _stream(cache.device)), "omni_attn_prefill_keys")
     nv.count_launches((n - 1) // 16)                         # of the pages, sixteen segments at a time
     if n > 8 or T > 248 * 256:                               # of the attention, eight segments and 256 blocks of 256 rows at a time
