@@ -762,8 +762,10 @@ static int prefill_segs(const void* q, long q_rs, long q_hs, const void* k, long
   // One segment in a round of blocks has no order to gain from, and its softmax warps are 3 to 7 % faster with its numbers in the constant bank: 1000 tokens, 32 heads
   // 21.0 us (21.6 below), 6000 tokens, 4 heads 79 (85), 1 head 77 (82).  Short ones are over before that shows: 130 tokens, 32 heads 9.5
   // (9.3); heads of 64 channels leave registers enough: 1000 tokens, 16 heads 18.0 (17.4).
-  // Where the context is most of what every row sees, no block has much more to do than another (keys side by side, 32 heads: 2039 tokens on 14345 424 us, 440 below;
-  // 2048 on 8192 272 and 270, on 4096 176 and 160).
+  // Where the context is most of what every row sees, no block has much more to do than another.  Keys side by side, with the way back to bf16, here and below: 32 heads, 2039 tokens on
+  // 4096 166 and 155 us, 8192 269 and 265, 12000 367 and 370, 14345 426 and 437, 30000 828 and 865; 40 heads, 1024 on 4096 143 and 139, 8192 248 and 251; 64 heads, 700 on 2000 90
+  // and 87, 4096 136 and 138, 2048 on 2000 211 and 200, 4096 305 and 304, 14345 830 and 859; 16 heads, 3000 on 12000 362 and 357, 20000 558 and 565.  They cross between
+  // a third of the tokens and five times; from six times on this was the faster one at all 41 sizes measured, by 1 to 6 %.
   if (n == 1 && D == 128 && len[0] > 0 && len[0] + context[0] >= 1000 &&
       ((long)((len[0] + 2 * ATT_BM - 1) / (2 * ATT_BM)) * H <= sm_count() || (first_key && context[0] / 6 >= len[0]))) {
     const int a = start[0], m = len[0], c = context[0];

@@ -1,8 +1,8 @@
-// Tokens drawn from given random numbers: temperature, top-k, min-p and top-p over rows of logits.  The token is exactly the definition's; its log probability
-// has the row's sum of weights in fp32, but for rows whose mass is summed in whole numbers for the token (no cut; top-p alone).
+// Tokens drawn from given random numbers: temperature, top-k, min-p and top-p over rows of logits.  All that decides the token is whole
+// numbers; its log probability has the row's sum of weights in fp32, but for rows whose mass is summed in whole numbers for the token (no cut; top-p alone).
 //
 // For a row x with maximum m and temperature T, weights are whole numbers w_i = round(2^44 exp((x_i - m) / T)), so that sums of them have no order: blocks,
-// threads and lists may add them as they come, and the plain definition in 64 bits gives the same token.  The order of a row is (x down, index up).  A cut is the
+// threads and lists may add them as they come, and the plain definition in 64 bits gives the same token (a weight is within 2^-50 of itself before it is rounded).  The order of a row is (x down, index up).  A cut is the
 // last element of that order that stays:
 //   top-k   the k-th element;
 //   min-p   elements whose weight is below min_p of the largest have no mass (they are the end of the order);
@@ -1143,8 +1143,8 @@ extern "C" int omni_sample_given(const void* logits, int is_bf16, long ld, int V
   if (B <= 0) return RC_OK;
   if (V < 1 || V > SG_MAX_V) return RC_BAD_ARG;
   const SampleGiven p = {logits, ld, V, temperature, top_p, min_p, u, top_k, temperature_v, top_p_v, min_p_v, top_k_v, ids, logprob};
-  // Two blocks fit an SM: as many a row as make two rounds of them at most, since rows differ in what they cost (256 rows of 152064, all kinds: 161 us with two blocks a row,
-  // 234 with one; 100 rows 96 with four, 123 with two), a tile each at least.
+  // Two blocks fit an SM: as many a row as make two rounds of them at most, since rows differ in what they cost (two draws of 256 rows of 152064, all kinds: 149 and 132 us with
+  // two blocks a row, 192 and 193 with one, 162 and 135 with four; of 100 rows 81 and 76 with four, 108 and 105 with two, 87 and 80 with eight), a tile each at least.
   int nc = 1;
   while (nc < SG_MAX_CLUSTER && (long)B * nc * 2 <= 4L * sm_count() && nc * 2 * SG_TILE <= V) nc *= 2;
   if ((long)B * nc > 0x7fffffffL) return RC_TOO_LARGE;

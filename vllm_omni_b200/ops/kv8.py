@@ -135,7 +135,8 @@ def _stream(device):
 
 
 def kv8_write(k, v, cache: Kv8Cache, slots) -> None:
-    """k, v: bf16 [T, Hkv, D]; slots int32 [T] (page * page size + row, below zero: not written)."""
+    """k, v: bf16 [T, Hkv, D]; slots int32 [T] (page * page size + row, below zero: not written).  A page's rows follow one another: a page that comes up again behind another one's
+    rows, or behind 128 rows that are not written, would be scaled by two blocks at once, and is not looked for."""
     T = slots.numel()
     shape = (T, cache.heads, cache.head_size)
     _check_rows("k", k, shape, cache.device)

@@ -1,6 +1,6 @@
 """K16 — batched token sampling on the device (csrc/sampler.cu) with a PyTorch restatement
 for CPU runs.  ``sample`` takes one ``RowParams`` per sequence.  ``sample_given`` (csrc/sample_given.cu) takes parameters and random numbers that are on the
-device, and gives exactly the token of its definition: ties go to the lowest id, and masses are sums of whole numbers, which have no order."""
+device, and gives the token of its definition: ties go to the lowest id, and masses are sums of whole numbers, which have no order."""
 from __future__ import annotations
 
 import ctypes
