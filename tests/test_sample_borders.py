@@ -113,3 +113,29 @@ def test_parameters_that_are_not_numbers_cut_nothing(dev, V):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (t, k, p, m)
     got, want = sample_given(x, torch.full((3,), nan, device=dev), 0.8, 50, 0.9), sample_given(x, torch.zeros(3, device=dev), 0.8, 50, 0.9)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("V,k", [(700, 0), (9000, 0), (9000, 600)])
+@pytest.mark.parametrize("apart", [False, True])
+def test_logits_further_apart_than_fp32_holds(dev, V, k, apart):
+    """At a temperature of their size the lowest of all numbers still have mass: exp(-2) here, though their difference from the largest is no fp32 number."""
+    x = torch.full((1, V), -3e38)
+    x[0, :V // 50 if apart else V:1 if apart else 100] = 3e38          # beside one another, or one among many everywhere
+    z = torch.where(x[0] > 0, 0.0, -2.0).double()
+    w = torch.exp((x[0].double() - x[0].max().double()) / float(np.float32(3e38)))
+    assert (w - torch.exp(z)).abs().max() < 1e-6
+    for p in (0.3, 0.9):
+        order = torch.sort(x[0], descending=True, stable=True).indices
+        order = order[:k] if k else order
+        n = torch.round(w * 2.0 ** 44)
+        before = torch.cumsum(n[order], 0) - n[order]
+        kept = torch.zeros(V, dtype=torch.bool)
+        kept[order[before < float(np.float32(p)) * n[order].sum()]] = True
+        mass = torch.cumsum(torch.where(kept, n, 0.0), 0)
+        for u in (0.1, 0.77, LAST):
+            u32 = torch.tensor([u], dtype=torch.float32)
+            ids, lp = sample_given(x.to(dev), u32.to(dev), 3e38, k, p)
+            i = int((mass <= float(u32) * mass[-1]).sum())
+            assert int(ids[0]) == i
+            assert abs(float(lp[0]) - float(torch.log(w[i] / w.sum()))) <= 2.0 ** -23 * 12 + 2.0 ** -20

@@ -238,10 +238,10 @@ __device__ __forceinline__ SgPlace place_of(const u64* list, const u64* mass, in
 
 // What a thread needs to turn elements into bins and weights.
 struct SgRow {
-  float mx, to_bin, log2_t;                             // bins and powers of two per unit of x
+  float mx, to_bin, log2_t;                             // bins and powers of two per two units of x: halves of any two numbers have a difference
   double mx_d, to_64, inv_t, least;                     // 64ths of powers of two per unit; min_p 2^44
   const double* table;
-  __device__ __forceinline__ float place(float x) const { return __fmul_rn(__fsub_rn(mx, x), to_bin); }       // in bins behind the largest, which is finite; monotone
+  __device__ __forceinline__ float place(float x) const { return __fmul_rn(__fmaf_rn(x, -0.5f, 0.5f * mx), to_bin); }       // in bins behind the largest, which is finite; monotone
   // 2^44 exp((x - m) / T) before it is rounded, within some 2^-50 of itself; 0 beyond the range.  2^(y / 64) = 2^(n / 64) e^(r ln 2 / 64), n the whole number next to y, |r| <= 1/2:
   // 2^(j / 64) from a table, e^.. by its series to the fifth power (the sixth is below 2^-54), the exponent added to the table's.
   // Every copy of this has to give the same bits: no products and sums that a compiler may fuse in one place and not in another.
@@ -362,8 +362,8 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
   const bool by_k = !greedy && k_in > 0 && k_in < V, by_p = !greedy && top_p < 1.f;
   SgRow r;
   r.inv_t = greedy ? 1.0 : 1.0 / (double)T_in;
-  r.to_bin = (float)fmin(SG_BINS / SG_RANGE * r.inv_t, 1e38);            // finite: times zero is zero
-  r.log2_t = (float)fmin(1.4426950408889634 * r.inv_t, 1e38);
+  r.to_bin = 2.f * (float)fmin(SG_BINS / SG_RANGE * r.inv_t, 1e38);      // finite: times zero is zero
+  r.log2_t = 2.f * (float)fmin(1.4426950408889634 * r.inv_t, 1e38);
   r.to_64 = 92.332482616893656 * r.inv_t;                                // 64 / ln 2
   r.least = (double)min_p * SG_ONE;
   r.table = sh.table;
@@ -384,9 +384,9 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
     float sum = 0.f;
     if (need_sum) {
       if (top < INFINITY) {
-        const float base = top == -INFINITY ? 0.f : top;
+        const float base = top == -INFINITY ? 0.f : 0.5f * top;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += ex2_approx((x[j] - base) * r.log2_t);
+        for (int j = 0; j < 8; ++j) sum += ex2_approx(__fmaf_rn(x[j], 0.5f, -base) * r.log2_t);
         if (sum != sum) {                                                // not a number: nothing
           sum = 0.f;
 #pragma unroll 1
@@ -394,7 +394,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
             float y = x[0];
 #pragma unroll
             for (int i = 1; i < 8; ++i) y = i == j ? x[i] : y;
-            sum += ex2_approx(fmaxf((y - base) * r.log2_t, -200.f));
+            sum += ex2_approx(fmaxf(__fmaf_rn(y, 0.5f, -base) * r.log2_t, -200.f));
           }
         }
       } else {
@@ -431,7 +431,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
     for (int i = 0; i < SG_PER_PIECE; ++i) {
       const int at = tid + i * SG_THREADS;
       if (at < pieces) {
-        const float d = sh.top[at] == r.mx ? 0.f : fmaxf((sh.top[at] - r.mx) * r.log2_t, -200.f);
+        const float d = sh.top[at] == r.mx ? 0.f : fmaxf(__fmaf_rn(sh.top[at], 0.5f, -0.5f * r.mx) * r.log2_t, -200.f);
         approx += (double)(sh.sum[at] * ex2_approx(d));
       }
     }
@@ -521,7 +521,7 @@ sample_given_kernel(const __grid_constant__ SampleGiven p) {
   if (by_p && !by_k) {
     // in units of the largest: (1 - p) Z / V, with room for what is rounded; with min-p its own bound, which S respects
     const float share = min_p > 0.f ? min_p * (1.f - 1e-5f) : (1.f - fmaxf(top_p, 0.f)) * (float)approx / (float)V * (1.f - 1e-4f);
-    const float below = log2f(share) / r.log2_t;
+    const float below = log2f(share) / (0.5f * r.log2_t);
     bound = fmaxf(bound, share > 0.f ? r.mx + below - 1e-5f * (fabsf(r.mx) + fabsf(below)) : bound);
   }
   auto piece_top = [&](int t) { return sh.top[t * SG_WARPS + warp]; };
